@@ -132,6 +132,7 @@ class ModelWeights(ctypes.Structure):
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _I32 = ctypes.c_int32
+_I64 = ctypes.c_int64
 _U32 = ctypes.c_uint32
 _U64 = ctypes.c_uint64
 _F32 = ctypes.c_float
@@ -177,6 +178,8 @@ SIGNATURES = {
     "ennx_b200_moe_layer": (_I32, [_P, _P, _P, _P, ctypes.c_int64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P,
                                    _SZ, _P]),
     "ennx_b200_gqa_attention": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _F32, _P]),
+    "ennx_b200_gqa_attention_packed": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _I64, _I32, _I32, _F32,
+                                              _P]),
     "ennx_b200_kda_workspace_size": (_SZ, [_I32, _I32, _I32]),
     "ennx_b200_kda_chunked": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _SZ, _P]),
     "ennx_b200_kda_chunked_noalloc": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P]),

@@ -1,0 +1,528 @@
+// attention_packed.cu -- causal grouped-query attention over packed prompts of
+// different lengths, on tcgen05 tensor cores.
+//
+// Sequence s of the packed rows is [cu[s], cu[s+1]); with lo(i) the first row
+// of row i's sequence and kv = h / (Hq / Hkv),
+//   o[i, h] = sum_{lo(i) <= j <= i} softmax_j(q[i, h] . k[j, kv] / sqrt(128)) v[j, kv].
+//
+// Bound: the tensor cores and, next to them, one exp2 per score.  Query tiles
+// are 128 consecutive PACKED rows whatever sequences they belong to, so a
+// sequence boundary costs no tile of its own: a tile reads the key tiles from
+// lo(its first row) to its own diagonal and every row masks the keys outside
+// [lo(i), i].  With a tile per sequence instead, prompts shorter than 128
+// tokens would each occupy a whole tile.
+//
+// One CTA = two 128-row query tiles (A: rows q0..q0+127, B: q0+128..q0+255)
+// of one query head, key/value tiles of 128 keys on the same 128-row grid,
+// shared by both.  Tensor memory: S_A | O_A | S_B | O_B, 128 fp32 columns
+// each.  Warp roles: 0 TMA producer (two-slot K/V ring, no multicast); 1 one
+// thread issues tcgen05.mma (S = Q K^T; O += P V with P from tensor memory);
+// 2..17 softmax, eight warps per query tile, two per 32 rows with 64 key
+// columns each, statistics in fp32, P rounded to bf16 (2^-9 relative, random
+// in sign, below the rounding of the bf16 output).
+//
+// Masked places may hold anything: masked scores are replaced, not added to,
+// but a masked V row still meets P = 0 in the MMA and an infinity or NaN there
+// makes 0 * inf = NaN.  A non-finite output is therefore recomputed by
+// `careful_row`, which reads visible keys only.
+#include "kernels.cuh"
+#include "serve.cuh"
+
+#include <math.h>
+
+#include <mutex>
+
+namespace ennx {
+
+const RopeTable& rope_table(float theta) {
+  static thread_local RopeTable t;
+  static thread_local float of = -1.0f;
+  if (of != theta) {
+    for (int i = 0; i < 64; ++i) t.inv[i] = pow((double)theta, -2.0 * i / 128.0) / 6.283185307179586476925;
+    of = theta;
+  }
+  return t;
+}
+
+namespace {
+
+constexpr int D = 128, BQ = 128, BKV = 128;
+constexpr int SUB = 128 * 128;  // bytes of one 128-row x 64-column bf16 sub-tile
+constexpr int TILE = 2 * SUB;   // 128 rows x 128 columns
+constexpr int SOFTMAX_WARPS = 16;
+constexpr int THREADS = 64 + 32 * SOFTMAX_WARPS;
+constexpr int SMEM = 6 * TILE /*Q_A, Q_B, 2 K, 2 V*/ + 1024 + 5120;
+constexpr uint32_t IDESC_QK = idesc_bf16_f32(128, 128);
+constexpr uint32_t IDESC_PV = idesc_bf16_f32(128, 128) | (1u << 16);  // B (V) MN-major
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the max grows by > 2^8
+
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void named_bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Packed rows: [begin, end) belong to sequences, clamped to the rows there are.
+struct Packing {
+  const int* cu;
+  int nseq, rows;
+  __device__ __forceinline__ int begin() const { return max(0, __ldg(cu)); }
+  __device__ __forceinline__ int end() const { return min(rows, __ldg(cu + nseq)); }
+  // first row of row r's sequence, r itself for a row of no sequence; in
+  // [0, r] whatever cu holds, so every index made from it stays in bounds
+  __device__ __forceinline__ int first_row(int r) const {
+    if (r >= end() || __ldg(cu) > r) return r;
+    int lo = 0, hi = nseq;  // last s with cu[s] <= r (empty sequences before it skipped)
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (__ldg(cu + mid) <= r) lo = mid;
+      else hi = mid;
+    }
+    return min(r, max(0, __ldg(cu + lo)));
+  }
+};
+
+struct Operands {
+  const uint16_t *q, *k, *v;
+  uint16_t* o;
+  long long ldq, ldk, ldv, ldo;
+};
+
+struct Bars {
+  uint64_t q_full, kv_full[2], kv_free[2], s_full[2], p_full[2], o_done[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int first[2];  // first_row of both tiles' first rows
+  // [tile][parity of the key tile][half][row]: partial row max / sum exchanged
+  // by the two warps of a row
+  float red[2][2][2][128];
+};
+static_assert(sizeof(Bars) <= 5120, "barrier block must fit the reserved 5 KB");
+
+// Output columns [c0, c0 + 64) of one (row, head), by one warp, reading
+// visible keys only; every sum in fp32.
+__device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int h, int kvh, int c0, float scale_log2,
+                                         int lane) {
+  const uint2 qw = *reinterpret_cast<const uint2*>(t.q + (long long)row * t.ldq + h * D + lane * 4);
+  const uint32_t qp[2] = {qw.x, qw.y};
+  float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+  for (int j = lo; j <= row; ++j) {
+    const uint2 kw = *reinterpret_cast<const uint2*>(t.k + (long long)j * t.ldk + kvh * D + lane * 4);
+    const uint32_t kp[2] = {kw.x, kw.y};
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s = fmaf(__uint_as_float(qp[i] << 16), __uint_as_float(kp[i] << 16), s);
+      s = fmaf(__uint_as_float(qp[i] & 0xffff0000u), __uint_as_float(kp[i] & 0xffff0000u), s);
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    s *= scale_log2;
+    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = ex2(m - ref), p = ex2(s - ref);
+    const uint32_t vw = *reinterpret_cast<const uint32_t*>(t.v + (long long)j * t.ldv + kvh * D + c0 + lane * 2);
+    l = l * alpha + p;
+    a0 = a0 * alpha + p * __uint_as_float(vw << 16);
+    a1 = a1 * alpha + p * __uint_as_float(vw & 0xffff0000u);
+    m = mn;
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  *reinterpret_cast<uint32_t*>(t.o + (long long)row * t.ldo + h * D + c0 + lane * 2) = pack_bf16x2(a0 * inv, a1 * inv);
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+    prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                            const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Operands t, Packing pk,
+                            int group, float scale_log2, int* err) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* base = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sQ = base;           // [2] tiles
+  uint8_t* sK = sQ + 2 * TILE;  // [2] ring slots
+  uint8_t* sV = sK + 2 * TILE;  // [2] ring slots
+  Bars& bar = *reinterpret_cast<Bars*>(sV + 2 * TILE);
+
+  const int qb = (int)(gridDim.x - 1 - blockIdx.x);  // later rows tend to see more keys: first
+  const int h = blockIdx.y, kvh = h / group;
+  const int q0 = qb * 2 * BQ;
+  const int end = pk.end();
+  if (q0 >= end) return;  // block-uniform: rows behind the last sequence stay as they are
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar.q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.kv_full[i], 1);
+      mbar_init(&bar.kv_free[i], 1);
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_full[i], 8);
+      mbar_init(&bar.o_done[i], 1);
+    }
+    bar.abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 1) { tmem_alloc(&bar.tmem_base, 512); tmem_relinquish(); }
+  if (threadIdx.x >= 64 && threadIdx.x < 66) bar.first[threadIdx.x - 64] = pk.first_row(q0 + ((int)threadIdx.x - 64) * BQ);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem_base;  // S_A: 0, O_A: 128, S_B: 256, O_B: 384
+  volatile int* abort_flag = &bar.abort_flag;
+  // key tiles on the 128-row grid, numbered from the one that holds A's first
+  // key: tile x uses [js[x], je[x]), its diagonal tile last; B may be empty
+  const int kt0 = bar.first[0] / BKV;
+  const bool two = q0 + BQ < end;
+  const int js[2] = {0, two ? max(0, bar.first[1] / BKV - kt0) : 0};
+  const int je[2] = {q0 / BKV + 1 - kt0, two ? q0 / BKV + 2 - kt0 : 0};
+  const int nt = two ? je[1] : je[0];
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+      const int nq = two ? 2 : 1;
+      mbar_arrive_expect_tx(&bar.q_full, nq * TILE);
+      for (int x = 0; x < nq; ++x) {
+        tma_load_2d(sQ + x * TILE, &tmQ, &bar.q_full, h * D, q0 + x * BQ);
+        tma_load_2d(sQ + x * TILE + SUB, &tmQ, &bar.q_full, h * D + 64, q0 + x * BQ);
+      }
+      int issued = 0;
+      for (int j = 0; j < nt && !*abort_flag; ++j) {
+        const int s = j & 1;
+        if (!mbar_wait(&bar.kv_free[s], ((j >> 1) & 1) ^ 1u, err)) { *abort_flag = 1; break; }
+        mbar_arrive_expect_tx(&bar.kv_full[s], 2 * TILE);
+        const int krow = (kt0 + j) * BKV;
+        uint8_t* k = sK + s * TILE;
+        uint8_t* v = sV + s * TILE;
+        tma_load_2d(k, &tmK, &bar.kv_full[s], kvh * D, krow);
+        tma_load_2d(k + SUB, &tmK, &bar.kv_full[s], kvh * D + 64, krow);
+        tma_load_2d(v, &tmV, &bar.kv_full[s], kvh * D, krow);
+        tma_load_2d(v + SUB, &tmV, &bar.kv_full[s], kvh * D + 64, krow);
+        issued = j + 1;
+      }
+      if (issued < nt) {  // giving up: no copy may land after the block has gone
+        mbar_wait(&bar.q_full, 0, err);
+        for (int j = max(0, issued - 2); j < issued; ++j) mbar_wait(&bar.kv_full[j & 1], (j >> 1) & 1, err);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      auto s_mma = [&](int x, int j) -> bool {  // S_X = Q_X K(j)^T
+        if (!mbar_wait(&bar.kv_full[j & 1], (j >> 1) & 1, err)) return false;
+        tc_fence_after();
+        const uint32_t qa = smem_u32(sQ + x * TILE), ka = smem_u32(sK + (j & 1) * TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem + x * 256, smem_desc_sw128(qa + (kk >> 2) * SUB + (kk & 3) * 32),
+                   smem_desc_sw128(ka + (kk >> 2) * SUB + (kk & 3) * 32), IDESC_QK, kk != 0);
+        umma_commit(&bar.s_full[x]);
+        return true;
+      };
+      bool ok = mbar_wait(&bar.q_full, 0, err);
+      for (int x = 0; ok && x < 2; ++x)
+        if (je[x] > 0 && js[x] == 0) ok = s_mma(x, 0);
+      for (int j = 0; ok && j < nt && !*abort_flag; ++j) {
+        const int last_user = j < je[1] && j >= js[1] ? 1 : 0;
+        for (int x = 0; x < 2; ++x) {
+          if (j >= je[x]) continue;
+          if (j >= js[x]) {
+            // O_X += P_X(j) V(j), P_X in tensor memory over the first 64 columns of S_X
+            if (!mbar_wait(&bar.p_full[x], (j - js[x]) & 1, err)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t va = smem_u32(sV + (j & 1) * TILE);
+#pragma unroll
+            for (int kk = 0; kk < BKV / 16; ++kk)
+              umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, smem_desc_sw128_mn(va + kk * 2048, SUB),
+                          IDESC_PV, j != js[x] || kk != 0);
+            umma_commit(&bar.o_done[x]);
+            if (x == last_user) umma_commit(&bar.kv_free[j & 1]);
+          }
+          if (j + 1 >= js[x] && j + 1 < je[x] && !s_mma(x, j + 1)) { ok = false; break; }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    // softmax: tile x, TMEM lane quarter q = warp % 4, key-column half `half`
+    const int x = (warp - 2) >> 3;
+    const int q = warp & 3;
+    const int half = ((warp - 2) >> 2) & 1;
+    const int r = q * 32 + lane;
+    const int qx0 = q0 + x * BQ;
+    const int qpos = qx0 + r;
+    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    const uint32_t s_col = tmem + lane_off + x * 256;  // S_X (P_X over its first 64 columns)
+    const uint32_t o_col = s_col + 128;                 // O_X
+    const int pair_bar = 1 + 4 * x + q;                 // shared with the warp owning the other half of these rows
+    const int steps = je[x] - js[x];
+    const int lo = pk.first_row(qpos);
+    const int max_lo = __reduce_max_sync(0xffffffffu, lo);
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      // A failed (timed-out) wait does not leave the loop: the warp keeps
+      // meeting its partner at the named barrier, which has no timeout, and
+      // skips the work; the abort flag stops every other wait early.
+      if (ok) ok = !*abort_flag && mbar_wait(&bar.s_full[x], j & 1, err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) *abort_flag = 1;
+      tc_fence_after();
+      const int k0 = (kt0 + js[x] + j) * BKV + half * 64;
+      uint32_t v0[32], v1[32];
+      if (ok) {
+        tmem_ld32(s_col + half * 64, v0);
+        tmem_ld32(s_col + half * 64 + 32, v1);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v0[i] = v1[i] = 0xff800000u;
+      }
+      if (k0 + 63 > qx0 + q * 32 || k0 < max_lo) {  // warp-uniform: some key lies outside some row's [lo, row]
+        const int a = lo - k0, b = qpos - k0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (i < a || i > b) v0[i] = 0xff800000u;  // -inf
+          if (32 + i < a || 32 + i > b) v1[i] = 0xff800000u;
+        }
+      }
+      // row max of the raw scores (the positive scale commutes with max)
+      float mt = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) mt = fmaxf(mt, fmaxf(__uint_as_float(v0[i]), __uint_as_float(v1[i])));
+      mt *= scale_log2;
+      // buffer j & 1: the partner's read of this slot two tiles ago preceded
+      // its arrival at the barrier of the tile in between
+      bar.red[x][j & 1][half][r] = mt;
+      named_bar_sync(pair_bar, 64);  // also: both halves have read S before P overwrites it
+      mt = fmaxf(mt, bar.red[x][j & 1][half ^ 1][r]);
+      if (!ok) continue;  // after the barrier: nothing below waits on the partner
+      const float m_new = fmaxf(m, mt);
+      const bool rescale = m == -INFINITY ? true : (m_new > m + kRescaleThreshold);
+      const float m_use = rescale ? m_new : m;
+      const float alpha = (rescale && m != -INFINITY) ? ex2(m - m_use) : 1.0f;
+      // P = exp2(s * scale - m) as one packed fma per pair of scores; a row
+      // with no visible score so far uses m = 0 (every exp2 argument is -inf)
+      const float nm = m_use == -INFINITY ? 0.0f : -m_use;
+      const uint64_t c2 = pack_f32x2(scale_log2, scale_log2), nm2 = pack_f32x2(nm, nm);
+      uint64_t ls2 = 0ull;
+      uint32_t pk2[32];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint64_t t01 = fma_f32x2(((uint64_t)v0[2 * i + 1] << 32) | v0[2 * i], c2, nm2);
+        const uint64_t t23 = fma_f32x2(((uint64_t)v1[2 * i + 1] << 32) | v1[2 * i], c2, nm2);
+        const float p0 = ex2(__uint_as_float((uint32_t)t01)), p1 = ex2(__uint_as_float((uint32_t)(t01 >> 32)));
+        const float p2 = ex2(__uint_as_float((uint32_t)t23)), p3 = ex2(__uint_as_float((uint32_t)(t23 >> 32)));
+        ls2 = add_f32x2(ls2, add_f32x2(pack_f32x2(p0, p1), pack_f32x2(p2, p3)));
+        pk2[i] = pack_bf16x2(p0, p1);
+        pk2[16 + i] = pack_bf16x2(p2, p3);
+      }
+      const float ls = __uint_as_float((uint32_t)ls2) + __uint_as_float((uint32_t)(ls2 >> 32));
+      tmem_st32(s_col + half * 32, pk2);
+      l = l * alpha + ls;
+      m = m_use;
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+        // the s_full wait above proves O_X += P_X(j-1) V(j-1) complete
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t ov[32];
+          tmem_ld32(o_col + half * 64 + cc * 32, ov);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+          tmem_st32(o_col + half * 64 + cc * 32, ov);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.p_full[x]);
+    }
+    if (steps > 0) {
+      // row sum over both halves
+      bar.red[x][steps & 1][half][r] = l;
+      named_bar_sync(pair_bar, 64);
+      const float l_tot = l + bar.red[x][steps & 1][half ^ 1][r];
+      if (ok && mbar_wait(&bar.o_done[x], (steps - 1) & 1, err)) {
+        tc_fence_after();
+        const float inv = l_tot > 0.0f || l_tot != l_tot ? 1.0f / l_tot : 0.0f;
+        const bool mine = qpos >= pk.begin() && qpos < end;
+        uint16_t* orow = t.o + (long long)qpos * t.ldo + h * D + half * 64;
+        float worst = 0.0f;  // NaN or 0 * inf = NaN where an output is not finite
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t ov[32];
+          tmem_ld32(o_col + half * 64 + cc * 32, ov);
+          tmem_ld_wait();
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            f[i] = __uint_as_float(ov[i]) * inv;
+            worst = fmaf(f[i], 0.0f, worst);
+          }
+          if (mine) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              st_global_v4(orow + cc * 32 + g * 8, pack_bf16x2(f[8 * g], f[8 * g + 1]),
+                           pack_bf16x2(f[8 * g + 2], f[8 * g + 3]), pack_bf16x2(f[8 * g + 4], f[8 * g + 5]),
+                           pack_bf16x2(f[8 * g + 6], f[8 * g + 7]));
+          }
+        }
+        uint32_t redo = __ballot_sync(0xffffffffu, mine && worst != worst);
+        __syncwarp();
+        while (redo) {
+          const int src = __ffs(redo) - 1;
+          redo &= redo - 1;
+          careful_row(t, qx0 + q * 32 + src, __shfl_sync(0xffffffffu, lo, src), h, kvh, half * 64, scale_log2, lane);
+        }
+      } else {
+        *abort_flag = 1;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Rotate-half RoPE in place, position = row - first row of its sequence.  One
+// thread per (row, 8 pairs), the angles computed once for all heads.
+__global__ void rope_packed_kernel(uint16_t* __restrict__ x, long long ld, int heads, Packing pk,
+                                   const __grid_constant__ RopeTable table) {
+  const int begin = pk.begin(), end = pk.end();
+  const long long total = (long long)max(0, end - begin) * 8;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (long long)gridDim.x * blockDim.x) {
+    const int r = begin + (int)(i >> 3), k0 = (int)(i & 7) * 8;
+    const int pos = r - pk.first_row(r);
+    float sn[8], cs[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rope_sincos(table, k0 + e, pos, &sn[e], &cs[e]);
+    uint16_t* row = x + (long long)r * ld + k0;
+    for (int h = 0; h < heads; ++h) {
+      uint4* pa = reinterpret_cast<uint4*>(row + (long long)h * D);
+      uint4* pb = reinterpret_cast<uint4*>(row + (long long)h * D + 64);
+      const uint4 a = *pa, b = *pb;
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+      uint32_t ya[4], yb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a0 = __uint_as_float(aw[j] << 16), a1 = __uint_as_float(aw[j] & 0xffff0000u);
+        const float b0 = __uint_as_float(bw[j] << 16), b1 = __uint_as_float(bw[j] & 0xffff0000u);
+        ya[j] = pack_bf16x2(a0 * cs[2 * j] - b0 * sn[2 * j], a1 * cs[2 * j + 1] - b1 * sn[2 * j + 1]);
+        yb[j] = pack_bf16x2(b0 * cs[2 * j] + a0 * sn[2 * j], b1 * cs[2 * j + 1] + a1 * sn[2 * j + 1]);
+      }
+      *pa = make_uint4(ya[0], ya[1], ya[2], ya[3]);
+      *pb = make_uint4(yb[0], yb[1], yb[2], yb[3]);
+    }
+  }
+}
+
+constexpr int kMaxDevices = 64;
+__device__ int g_status_word;  // written where a bounded wait gave up
+
+// Per-device set-up of the first call: the shared-memory attribute and the
+// address of the status word.  Allocates nothing.
+struct Setup {
+  std::once_flag once;
+  int32_t status = ENNX_B200_OK;
+  int* word = nullptr;
+};
+Setup g_setup[kMaxDevices];
+
+int32_t device_setup(int** word) {
+  int dev = 0;
+  ENNX_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  if (dev < 0 || dev >= kMaxDevices) return set_error(ENNX_B200_UNSUPPORTED, "device index %d out of range", dev);
+  Setup& s = g_setup[dev];
+  std::call_once(s.once, [&] {
+    void* p = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&p, g_status_word);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(prompt_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) {
+      s.status = check_cuda(e, "packed attention set-up");
+      return;
+    }
+    s.word = (int*)p;
+    register_status_word(dev, s.word);
+  });
+  if (s.status != ENNX_B200_OK) return set_error(s.status, "packed attention: set-up failed on device %d", dev);
+  *word = s.word;
+  return ENNX_B200_OK;
+}
+
+}  // namespace
+}  // namespace ennx
+
+using namespace ennx;
+
+extern "C" int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uint16_t* k, int64_t ld_k,
+                                                  const uint16_t* v, int64_t ld_v, uint16_t* o, int64_t ld_o,
+                                                  const int32_t* cu_seqlens, int32_t num_seqs, int64_t rows,
+                                                  int32_t hq, int32_t hkv, float rope_theta, void* stream) {
+  cudaStream_t s = (cudaStream_t)stream;
+  if (!cu_seqlens || num_seqs <= 0) return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: no sequences");
+  if (rows < 0 || hq <= 0 || hkv <= 0 || hq % hkv)
+    return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: Hq must be a positive multiple of Hkv");
+  if (!(rope_theta >= 0.0f) || isinf(rope_theta))
+    return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: rope_theta must be finite and not negative");
+  if (rows == 0) return ENNX_B200_OK;
+  if (!q || !k || !v || !o) return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: null argument");
+  if (rows > 0x7fffff00LL || hq > 65535)
+    return set_error(ENNX_B200_UNSUPPORTED, "attention_packed: too many rows or heads");
+  if (ld_q < (int64_t)hq * D || ld_o < (int64_t)hq * D || ld_k < (int64_t)hkv * D || ld_v < (int64_t)hkv * D)
+    return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: a row stride is shorter than its heads");
+  if ((ld_q | ld_k | ld_v | ld_o) % 8 || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15u))
+    return set_error(ENNX_B200_INVALID_ARGUMENT,
+                     "attention_packed: operands must be 16-byte aligned with strides of a multiple of 8");
+  int* err = nullptr;
+  ENNX_TRY(device_setup(&err));
+  CUtensorMap tq, tk, tv;
+  ENNX_TRY(make_tmap_2d_bf16(&tq, q, (uint64_t)hq * D, (uint64_t)rows, (uint64_t)ld_q, 64, 128, true));
+  ENNX_TRY(make_tmap_2d_bf16(&tk, k, (uint64_t)hkv * D, (uint64_t)rows, (uint64_t)ld_k, 64, 128, true));
+  ENNX_TRY(make_tmap_2d_bf16(&tv, v, (uint64_t)hkv * D, (uint64_t)rows, (uint64_t)ld_v, 64, 128, true));
+  const Packing pk{cu_seqlens, num_seqs, (int)rows};
+  if (rope_theta > 0.0f) {
+    const RopeTable& table = rope_table(rope_theta);
+    const long long blocks = (rows * 8 + 127) / 128, cap = 16LL * sm_count();
+    const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
+    rope_packed_kernel<<<grid, 128, 0, s>>>(q, ld_q, hq, pk, table);
+    ENNX_LAUNCH_CHECK("rope packed q");
+    rope_packed_kernel<<<grid, 128, 0, s>>>(k, ld_k, hkv, pk, table);
+    ENNX_LAUNCH_CHECK("rope packed k");
+  }
+  const Operands t{q, k, v, o, ld_q, ld_k, ld_v, ld_o};
+  const dim3 grid((unsigned)((rows + 2 * BQ - 1) / (2 * BQ)), (unsigned)hq);
+  prompt_attention_kernel<<<grid, THREADS, SMEM, s>>>(tq, tk, tv, t, pk, hq / hkv, 1.4426950408889634f / sqrtf((float)D),
+                                                      err);
+  ENNX_LAUNCH_CHECK("packed attention");
+  return ENNX_B200_OK;
+}

@@ -39,7 +39,7 @@ int32_t check_cuda(cudaError_t e, const char* what);
 // Kernels write a nonzero code (ENNX_B200_TIMEOUT, ...) instead of trapping.
 int* device_error_word();
 // an additional per-device status word (static device memory) that
-// consume_device_error also reads and clears
+// consume_device_error also reads and clears; up to four per device
 void register_status_word(int dev, int* word);
 int32_t consume_device_error(cudaStream_t stream);  // synchronises `stream`
 

@@ -52,24 +52,29 @@ int* device_error_word() {
   return g_err_word[d];
 }
 
-static int* g_extra_word[kMaxDevices];
+static constexpr int kMaxExtraWords = 4;
+static int* g_extra_word[kMaxDevices][kMaxExtraWords];
 
 void register_status_word(int dev, int* word) {
   std::lock_guard<std::mutex> lk(g_mu);
-  if (dev >= 0 && dev < kMaxDevices) g_extra_word[dev] = word;
+  if (dev < 0 || dev >= kMaxDevices) return;
+  for (int*& w : g_extra_word[dev]) {
+    if (w == word) return;
+    if (!w) { w = word; return; }
+  }
 }
 
 // Reads and clears every status word of the current device: the shared word
 // of the regular entry points (only if it exists already: a word that was
 // never allocated was never written, so checking allocates nothing) and the
-// static word of the allocation-free entry point.
+// static words that other paths registered.
 int32_t consume_device_error(cudaStream_t stream) {
   int d = current_device();
-  int* words[2];
+  int* words[1 + kMaxExtraWords];
   {
     std::lock_guard<std::mutex> lk(g_mu);
     words[0] = g_err_word[d];
-    words[1] = g_extra_word[d];
+    for (int i = 0; i < kMaxExtraWords; ++i) words[1 + i] = g_extra_word[d][i];
   }
   ENNX_CUDA(cudaStreamSynchronize(stream), "stream synchronize");
   int worst = 0;

@@ -195,6 +195,52 @@ def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope_theta:
     return o
 
 
+def _check_here(what: str, *ts) -> None:
+    """Every tensor given lives on the current CUDA device."""
+    _check_dev(*ts)
+    here = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != here:
+            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def _head_rows(what: str, name: str, t: torch.Tensor) -> int:
+    """Row stride of bf16 [rows, heads, 128] whose heads are contiguous within a row."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != 128:
+        raise ValueError(f"{what}: {name} must be bfloat16 [rows, heads, 128]")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128):
+        raise ValueError(f"{what}: the heads of {name} must be contiguous within a row")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * 128
+
+
+def gqa_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                         rope_theta: float = 1e6, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention over packed prompts (see ``ennx_b200_gqa_attention_packed``).
+
+    q bf16 [rows, Hq, 128], k/v [rows, Hkv, 128], each with a row stride of its
+    own (columns of a fused projection are fine); cu_seqlens int32
+    [sequences + 1] on the device: sequence s owns rows cu_seqlens[s] ..
+    cu_seqlens[s+1] - 1.  q and k are rotated in place when rope_theta > 0.
+    Rows behind the last sequence are left as they are (undefined when out is
+    None)."""
+    what = "gqa_attention_packed"
+    _check_here(what, q, k, v, cu_seqlens, out)
+    ldq, ldk, ldv = _head_rows(what, "q", q), _head_rows(what, "k", k), _head_rows(what, "v", v)
+    if k.shape != v.shape or k.shape[0] != q.shape[0]:
+        raise ValueError(f"{what}: q, k and v must have the same rows, k and v the same heads")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or \
+            not cu_seqlens.is_contiguous():
+        raise ValueError(f"{what}: cu_seqlens must be contiguous int32 [sequences + 1]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"{what}: out must have the shape of q")
+    _abi.call("ennx_b200_gqa_attention_packed", _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out),
+              _head_rows(what, "out", out), _ptr(cu_seqlens), cu_seqlens.numel() - 1, q.shape[0], q.shape[1],
+              k.shape[1], rope_theta, _stream())
+    return out
+
+
 def kda_chunked(q, k, v, g, beta, state: torch.Tensor | None = None) -> torch.Tensor:
     """Chunked KDA; q,k,v bf16 [B,T,H,128], g f32 [B,T,H,128], beta f32 [B,T,H]."""
     _check_dev(q, k, v, g, beta, state)

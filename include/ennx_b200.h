@@ -229,6 +229,24 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention(uint16_t* q, uint16_t* k, const ui
                                               int32_t batch, int32_t seq, int32_t hq, int32_t hkv,
                                               float rope_theta, void* stream);
 
+/* Causal GQA attention over packed prompts: sequence s owns rows
+ * [cu_seqlens[s], cu_seqlens[s+1]) and a row sees the rows of its own sequence
+ * up to itself.  q, o bf16 rows of hq heads of 128, k, v rows of hkv heads;
+ * ld_* = elements from one row to the next (a multiple of 8, so the operands
+ * may be columns of one fused projection), 16-byte aligned.  cu_seqlens:
+ * device int32[num_seqs + 1], not decreasing, first 0, last <= rows; empty
+ * sequences are allowed.  Rows at and after cu_seqlens[num_seqs] belong to no
+ * sequence: their o, q and k are left as they are, and what q, k and v hold
+ * there reaches no output.  If rope_theta > 0, rotary embedding (rotate-half
+ * pairing, position = row within its sequence, angles reduced in 64 bits) is
+ * applied to q and k IN PLACE first.  o must not overlap q, k or v.  Softmax
+ * statistics in fp32; a non-finite key or value reaches only the rows that
+ * see it.  Allocates nothing. */
+ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uint16_t* k, int64_t ld_k,
+                                                     const uint16_t* v, int64_t ld_v, uint16_t* o, int64_t ld_o,
+                                                     const int32_t* cu_seqlens, int32_t num_seqs, int64_t rows,
+                                                     int32_t hq, int32_t hkv, float rope_theta, void* stream);
+
 /* Chunked KDA (gated delta rule, per-key-channel decay, chunk 64, d_k = d_v =
  * 128), equivalent to the serial recurrence of kda_recurrence_16k
  * (kda_moe.metal:167-225).  q, k, v bf16 [batch, seq, heads, 128]; g f32

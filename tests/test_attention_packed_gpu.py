@@ -1,0 +1,202 @@
+"""Attention over packed prompts on the GPU against its definition in 64 bits.
+
+Tolerance: the output is rounded to bf16 once (2^-8 of a value at most), and
+P is rounded to bf16 before P V (each weight off by at most 2^-8 relative, so
+the sum by at most 2^-8 * sum |p v| <= 2^-8 * max |v|).  Together
+|got - ref| <= 2^-8 |ref| + 2^-8 max|v|, and fp32 sums add far less; the test
+allows one part in a thousand more."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from ennx_b200 import ops  # noqa: E402
+
+D = 128
+
+
+def rnd(*shape, seed, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(torch.bfloat16)
+
+
+def starts(lengths):
+    return torch.tensor([0] + list(lengths), dtype=torch.int64).cumsum(0).to(torch.int32).cuda()
+
+
+def turned(x, lengths, theta):
+    """RoPE of packed x [rows, heads, 128] in 64 bits."""
+    pos = torch.cat([torch.arange(n) for n in lengths]).double().cuda()
+    inv = theta ** (-torch.arange(64, dtype=torch.float64, device="cuda") / 64)
+    a = pos[:, None] * inv
+    c, s = a.cos()[:, None], a.sin()[:, None]
+    x1, x2 = x.double()[..., :64], x.double()[..., 64:]
+    return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], -1)
+
+
+def reference(q, k, v, lengths):
+    out, at = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), 0
+    group = q.shape[1] // k.shape[1]
+    for n in lengths:
+        r = slice(at, at + n)
+        at += n
+        kk, vv = k[r].double().repeat_interleave(group, 1), v[r].double().repeat_interleave(group, 1)
+        a = torch.einsum("ihd,jhd->hij", q[r].double(), kk) / math.sqrt(D)
+        a.masked_fill_(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+        out[r] = torch.einsum("hij,jhd->ihd", a.softmax(-1), vv)
+    return out
+
+
+def close(got, ref, vmax, extra=0.0):
+    err = (got.double() - ref).abs() - (1.001 * 2.0 ** -8 * (ref.abs() + vmax) + extra)
+    assert err.max() <= 0, float(err.max())
+
+
+CASES = [
+    ([1], 1, 1), ([2, 1, 1], 2, 1), ([128], 4, 4), ([127, 129], 4, 2), ([256, 1, 255], 4, 1), ([5] * 60, 8, 2),
+    ([1] * 300, 2, 1), ([0, 7, 0, 0, 300, 0], 4, 1), ([700, 3, 40, 513], 16, 4), ([1, 1300], 3, 1),
+    ([31, 97, 1, 129, 64, 512, 2], 6, 2),
+]
+
+
+@pytest.mark.parametrize("lengths,hq,hkv", CASES)
+def test_matches_definition(lengths, hq, hkv):
+    rows = sum(lengths)
+    q, k, v = rnd(rows, hq, D, seed=1), rnd(rows, hkv, D, seed=2), rnd(rows, hkv, D, seed=3)
+    q0, k0 = q.clone(), k.clone()
+    o = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    ops.device_status()
+    assert torch.equal(q, q0) and torch.equal(k, k0)
+    close(o, reference(q, k, v, lengths), float(v.float().abs().max()))
+
+
+def test_large_scores():
+    # scores of some hundreds: the running maximum moves by more than the lazy rescale's 2^8 many times
+    lengths = [300, 900]
+    q, k, v = rnd(1200, 4, D, seed=4, std=6.0), rnd(1200, 2, D, seed=5, std=6.0), rnd(1200, 2, D, seed=6)
+    o = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    # an fp32 score of a few hundred (in units of log2) is off by up to 2^-24 * 128 * sum|q k| ~ 2e-3 at most,
+    # which moves a weight by that much relative to itself
+    close(o, reference(q, k, v, lengths), float(v.float().abs().max()), extra=4e-3 * float(v.float().abs().max()))
+
+
+def test_rope_positions_restart_with_each_sequence():
+    lengths = [200, 0, 1, 333]
+    rows = sum(lengths)
+    q, k, v = rnd(rows, 4, D, seed=7), rnd(rows, 2, D, seed=8), rnd(rows, 2, D, seed=9)
+    rq, rk = turned(q, lengths, 1e6), turned(k, lengths, 1e6)
+    o = ops.gqa_attention_packed(q, k, v, starts(lengths))
+    for got, ref in ((q, rq), (k, rk)):  # one rounding to bf16 of an fp32 rotation
+        assert ((got.double() - ref).abs() <= 1.01 * 2.0 ** -8 * ref.abs() + 1e-5).all()
+    close(o, reference(q, k, v, lengths), float(v.float().abs().max()))
+
+
+def test_columns_of_a_fused_projection_and_rows_behind_the_last_sequence():
+    lengths, spare, hq, hkv = [190, 77], 200, 4, 2
+    rows = sum(lengths) + spare
+    ld = (hq + 2 * hkv) * D + 16
+    buf = rnd(rows, ld, seed=10)
+    live = sum(lengths)
+    buf[live:] = math.nan
+    buf[live + 1:, ::3] = math.inf
+    before = buf.clone()
+    q = buf[:, :hq * D].unflatten(1, (hq, D))
+    k = buf[:, hq * D:(hq + hkv) * D].unflatten(1, (hkv, D))
+    v = buf[:, (hq + hkv) * D:(hq + 2 * hkv) * D].unflatten(1, (hkv, D))
+    out = torch.full((rows, hq * D + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    o = out[:, :hq * D].unflatten(1, (hq, D))
+    ref = reference(q[:live], k[:live], v[:live], lengths)
+    ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0, out=o)
+    close(o[:live], ref, float(v[:live].float().abs().max()))
+    assert (out[live:] == 7.0).all() and (out[:, hq * D:] == 7.0).all()
+    assert torch.equal(buf.view(torch.int16), before.view(torch.int16))
+    ops.gqa_attention_packed(q, k, v, starts(lengths), out=o)  # rotates the live rows only
+    assert torch.equal(buf[live:].view(torch.int16), before[live:].view(torch.int16))
+    assert torch.equal(buf[:, (hq + hkv) * D:].view(torch.int16), before[:, (hq + hkv) * D:].view(torch.int16))
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_non_finite_values_reach_only_the_rows_that_see_them(bad):
+    lengths = [100, 200, 60]
+    q, k, v = rnd(360, 4, D, seed=11), rnd(360, 2, D, seed=12), rnd(360, 2, D, seed=13)
+    clean = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    v[150, 1, 5] = bad      # sequence 1, its row 50
+    k[330, 0, 9] = math.nan  # sequence 2, its row 30
+    o = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    touched = torch.zeros(360, 4, D, dtype=torch.bool, device="cuda")
+    touched[150:300, 2:, 5] = True
+    touched[330:360, :2, :] = True
+    assert torch.equal(o.isfinite(), ~touched)
+    # rows that the check recomputed carry fp32 weights, the others bf16 ones: both within the bound of the definition
+    vv = v.clone()
+    vv[150, 1, 5] = 0
+    ref = reference(q[:330], k[:330], vv[:330], [100, 200, 30])
+    assert float((o[:330].double() - ref)[~touched[:330]].abs().max()) <= 2 * 2.0 ** -8 * float(vv.float().abs().max())
+    assert torch.equal(o[:100], clean[:100])
+
+
+def test_infinite_key_scores():
+    # a visible score of +inf makes its rows NaN, as softmax does; other sequences stay whole
+    q, k, v = rnd(80, 1, D, seed=14).abs(), rnd(80, 1, D, seed=15), rnd(80, 1, D, seed=16)
+    k[50, 0, 3] = math.inf
+    o = ops.gqa_attention_packed(q, k, v, starts([40, 40]), rope_theta=0.0)
+    assert o[:50].isfinite().all() and o[50:].isnan().all()
+
+
+def test_replayed_graph_with_other_lengths_and_a_side_stream():
+    rows, hq, hkv = 512, 4, 2
+    q, k, v = rnd(rows, hq, D, seed=17), rnd(rows, hkv, D, seed=18), rnd(rows, hkv, D, seed=19)
+    cu = starts([300, 212])
+    out = torch.empty(rows, hq, D, dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0, out=out)
+    torch.cuda.current_stream().wait_stream(stream)
+    vmax = float(v.float().abs().max())
+    for lengths in ([300, 212], [1, 511], [17, 200]):
+        cu.copy_(starts(lengths))
+        graph.replay()
+        n = sum(lengths)
+        close(out[:n], reference(q[:n], k[:n], v[:n], lengths), vmax)
+
+
+def test_same_inputs_same_bits():
+    lengths = [900, 124]
+    q, k, v = rnd(1024, 8, D, seed=20), rnd(1024, 2, D, seed=21), rnd(1024, 2, D, seed=22)
+    a = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    b = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    assert torch.equal(a, b)
+
+
+def test_no_rows():
+    e = torch.empty(0, 4, D, dtype=torch.bfloat16, device="cuda")
+    o = ops.gqa_attention_packed(e, e[:, :2], e[:, :2], starts([0, 0]))
+    assert o.shape == (0, 4, D)
+
+
+def test_refusals():
+    q, k, v, cu = rnd(8, 4, D, seed=23), rnd(8, 2, D, seed=24), rnd(8, 2, D, seed=25), starts([8])
+    call = ops.gqa_attention_packed
+    with pytest.raises(ValueError, match="bfloat16"):
+        call(q.half(), k, v, cu)
+    with pytest.raises(ValueError, match="same rows"):
+        call(q, k[:7], v[:7], cu)
+    with pytest.raises(ValueError, match="int32"):
+        call(q, k, v, cu.long())
+    with pytest.raises(ValueError, match="multiple of Hkv"):
+        call(q[:, :3], k, v, cu)
+    with pytest.raises(ValueError, match="contiguous within a row"):
+        call(q[:, ::2], k, v, cu)
+    with pytest.raises(ValueError, match="rope_theta"):
+        call(q, k, v, cu, rope_theta=-1.0)
+    odd = torch.zeros(8 * 4 * D + 1, dtype=torch.bfloat16, device="cuda")[1:].view(8, 4, D)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        call(odd, k, v, cu)
+    with pytest.raises(ValueError, match="CUDA"):
+        call(q.cpu(), k, v, cu)
