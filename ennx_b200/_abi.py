@@ -73,6 +73,18 @@ class GemmParams(ctypes.Structure):
                 ("lse_partial", ctypes.c_void_p), ("target_logit", ctypes.c_void_p)]
 
 
+class DecodeAttention(ctypes.Structure):
+    """ennx_b200_decode_attention."""
+    _fields_ = [("q", ctypes.c_void_p), ("ld_q", ctypes.c_int64), ("k", ctypes.c_void_p), ("ld_k", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("ld_v", ctypes.c_int64),
+                ("k_cache", ctypes.c_void_p), ("k_seq", ctypes.c_int64), ("k_token", ctypes.c_int64),
+                ("k_head", ctypes.c_int64),
+                ("v_cache", ctypes.c_void_p), ("v_seq", ctypes.c_int64), ("v_token", ctypes.c_int64),
+                ("v_head", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("o", ctypes.c_void_p), ("ld_o", ctypes.c_int64),
+                ("batch", ctypes.c_int32), ("room", ctypes.c_int32), ("hq", ctypes.c_int32), ("hkv", ctypes.c_int32)]
+
+
 class PackedLinear(ctypes.Structure):
     """ennx_b200_packed_linear: field order of KdaPackedLinear (forward_program.rs:224-235)."""
     _fields_ = [("byte_offset", ctypes.c_uint64), ("scale_offset", ctypes.c_uint64),
@@ -177,9 +189,13 @@ SIGNATURES = {
     "ennx_b200_moe_workspace_size": (_SZ, [ctypes.c_int64, _I32, _I32, _I32, _I32]),
     "ennx_b200_moe_layer": (_I32, [_P, _P, _P, _P, ctypes.c_int64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P,
                                    _SZ, _P]),
+    "ennx_b200_moe_layer_decode_workspace_size": (_SZ, [_I64, _I32, _I32, _I32]),
+    "ennx_b200_moe_layer_decode": (_I32, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P]),
     "ennx_b200_gqa_attention": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _F32, _P]),
     "ennx_b200_gqa_attention_packed": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _I64, _I32, _I32, _F32,
                                               _P]),
+    "ennx_b200_gqa_attention_decode_workspace_size": (_SZ, [_I32, _I32, _I32, _I32]),
+    "ennx_b200_gqa_attention_decode": (_I32, [_P, _F32, _P, _SZ, _P]),
     "ennx_b200_kda_workspace_size": (_SZ, [_I32, _I32, _I32]),
     "ennx_b200_kda_chunked": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _SZ, _P]),
     "ennx_b200_kda_chunked_noalloc": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P]),

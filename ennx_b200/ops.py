@@ -184,6 +184,34 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor, 
     return (y, idx, gate) if return_routing else y
 
 
+def moe_layer_decode(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
+                     top_k: int, residual: torch.Tensor | None = None, return_routing: bool = False,
+                     out: torch.Tensor | None = None):
+    """``moe_layer`` for at most 64 tokens (see ``ennx_b200_moe_layer_decode``):
+    bound by the bytes of the picked experts' weights.  x and residual bf16
+    [tokens, hidden], weights as for ``moe_layer``; all contiguous."""
+    what = "moe_layer_decode"
+    _check_here(what, x, w_router, w_gate_up, w_down, residual, out)
+    T, H = x.shape
+    E, I2, _ = w_gate_up.shape
+    if w_router.shape != (E, H) or w_gate_up.shape != (E, I2, H) or w_down.shape != (E, H, I2 // 2) or I2 % 2:
+        raise ValueError(f"{what}: weights must be [E, H], [E, 2 I, H] and [E, H, I] for x [tokens, H]")
+    if out is None:
+        out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
+    for t in (x, w_router, w_gate_up, w_down, residual, out):
+        if t is not None and (t.dtype != torch.bfloat16 or not t.is_contiguous()):
+            raise ValueError(f"{what}: operands must be contiguous bfloat16")
+    if out.shape != (T, H) or (residual is not None and residual.shape != (T, H)):
+        raise ValueError(f"{what}: residual and out must have the shape of x")
+    idx = torch.empty(T, top_k, dtype=torch.int32, device=x.device) if return_routing else None
+    gate = torch.empty(T, top_k, dtype=torch.float32, device=x.device) if return_routing else None
+    n = _abi.lib().ennx_b200_moe_layer_decode_workspace_size(T, E, top_k, I2 // 2)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _abi.call("ennx_b200_moe_layer_decode", _ptr(x), _ptr(w_router), _ptr(w_gate_up), _ptr(w_down), T, H, E, top_k,
+              I2 // 2, _ptr(residual), _ptr(out), _ptr(idx), _ptr(gate), _ptr(ws), n, _stream())
+    return (out, idx, gate) if return_routing else out
+
+
 def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope_theta: float = 1e6) -> torch.Tensor:
     """Causal GQA attention; q [B,S,Hq,128], k/v [B,S,Hkv,128] bf16.  q and k are
     rotated in place when rope_theta > 0."""
@@ -238,6 +266,56 @@ def gqa_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     _abi.call("ennx_b200_gqa_attention_packed", _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out),
               _head_rows(what, "out", out), _ptr(cu_seqlens), cu_seqlens.numel() - 1, q.shape[0], q.shape[1],
               k.shape[1], rope_theta, _stream())
+    return out
+
+
+def _cache_strides(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """(sequence, token, head) strides of a bf16 cache [batch, room, heads, 128]."""
+    if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[3] != 128 or t.stride(3) != 1:
+        raise ValueError(f"{what}: {name} must be bfloat16 [batch, room, heads, 128] with contiguous heads")
+    # the stride of a dimension of one entry is never used
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3))
+
+
+def gqa_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                         k: torch.Tensor | None = None, v: torch.Tensor | None = None, rope_theta: float = 1e6,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA attention of one new token per sequence against a cache (see
+    ``ennx_b200_gqa_attention_decode``): the single-token form of
+    ``gqa_attention_packed``.
+
+    q bf16 [batch, Hq, 128]; k_cache/v_cache bf16 [batch, room, Hkv, 128] of any
+    strides; lengths int32 [batch] on the device, tokens with the new one; k/v
+    bf16 [batch, Hkv, 128], the new token's key and value, written to cache row
+    lengths - 1 (None: the caches hold them).  rope_theta > 0 rotates q (not in
+    place) and k to position lengths - 1."""
+    what = "gqa_attention_decode"
+    _check_here(what, q, k_cache, v_cache, lengths, k, v, out)
+    ldq = _head_rows(what, "q", q)
+    ks, vs = _cache_strides(what, "k_cache", k_cache), _cache_strides(what, "v_cache", v_cache)
+    batch, room, hkv, _ = k_cache.shape
+    if v_cache.shape != k_cache.shape or q.shape[0] != batch:
+        raise ValueError(f"{what}: q and both caches must have the same batch, the caches the same shape")
+    if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
+        raise ValueError(f"{what}: lengths must be contiguous int32 [batch]")
+    if (k is None) != (v is None):
+        raise ValueError(f"{what}: k and v come together")
+    ldk = ldv = 0
+    if k is not None:
+        ldk, ldv = _head_rows(what, "k", k), _head_rows(what, "v", v)
+        if k.shape != (batch, hkv, 128) or v.shape != k.shape:
+            raise ValueError(f"{what}: k and v must be [batch, Hkv, 128]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"{what}: out must have the shape of q")
+    p = _abi.DecodeAttention(q.data_ptr(), ldq, None if k is None else k.data_ptr(), ldk,
+                             None if v is None else v.data_ptr(), ldv, k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs,
+                             lengths.data_ptr(), out.data_ptr(), _head_rows(what, "out", out), batch, room, q.shape[1],
+                             hkv)
+    n = _abi.lib().ennx_b200_gqa_attention_decode_workspace_size(batch, room, q.shape[1], hkv)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    _abi.call("ennx_b200_gqa_attention_decode", ctypes.byref(p), rope_theta, _ptr(ws), n, _stream())
     return out
 
 

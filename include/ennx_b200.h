@@ -220,6 +220,24 @@ ENNX_B200_API int32_t ennx_b200_moe_layer(const uint16_t* x, const uint16_t* w_r
                                           uint16_t* y, int32_t* index, float* gate, void* workspace,
                                           size_t workspace_bytes, void* stream);
 
+/* ennx_b200_moe_layer for a few tokens (at most 64): the same weights, layouts
+ * and outputs, bound by the bytes of the picked experts' weights (three
+ * kernels, no permuted rows).  Routing is the rule of ennx_b200_moe_route
+ * (strict '>', the lower index wins a tie) on logits summed in fp32 in another
+ * order than its serial chain, so where two logits agree to about 1e-6 the two
+ * may pick differently; a NaN logit loses against every number.  hidden %
+ * 64 == 0, expert_width % 128 == 0, experts <= 256, top_k <= 8; tokens == 0
+ * does nothing.  y may be the residual itself, but must not overlap x or the
+ * weights.  workspace: 16-byte aligned; calls that may overlap need one each. */
+ENNX_B200_API size_t ennx_b200_moe_layer_decode_workspace_size(int64_t tokens, int32_t experts, int32_t top_k,
+                                                               int32_t expert_width);
+ENNX_B200_API int32_t ennx_b200_moe_layer_decode(const uint16_t* x, const uint16_t* w_router,
+                                                 const uint16_t* w_gate_up, const uint16_t* w_down, int64_t tokens,
+                                                 int32_t hidden, int32_t experts, int32_t top_k,
+                                                 int32_t expert_width, const uint16_t* residual, uint16_t* y,
+                                                 int32_t* index, float* gate, void* workspace,
+                                                 size_t workspace_bytes, void* stream);
+
 /* Causal GQA attention, head_dim 128, softmax scale 1/sqrt(128), fp32
  * softmax statistics.  q bf16 [batch, seq, hq, 128], k/v [batch, seq, hkv,
  * 128], o [batch, seq, hq, 128].  If rope_theta > 0, rotary embedding
@@ -246,6 +264,41 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, 
                                                      const uint16_t* v, int64_t ld_v, uint16_t* o, int64_t ld_o,
                                                      const int32_t* cu_seqlens, int32_t num_seqs, int64_t rows,
                                                      int32_t hq, int32_t hkv, float rope_theta, void* stream);
+
+/* GQA attention of one new token per sequence against a key/value cache,
+ * head_dim 128.  lengths (device int32[batch]) counts the tokens of each
+ * sequence with the new one; values outside [0, room] are taken as the nearest
+ * of the two.  With p = lengths[b] - 1: k and v (the new token's, both or
+ * neither NULL) are written to row p of sequence b of the caches, k rotated to
+ * position p if rope_theta > 0; q, rotated likewise but left as it is, attends
+ * to rows 0 .. p.  Without k and v the caches already hold row p.  lengths[b]
+ * = 0: nothing is written to the caches and o is 0.  Rows behind p may hold
+ * anything; an infinity or NaN in row p or before makes the outputs it enters
+ * non-finite (NaN where their limit would be an infinity).  All bf16; strides in elements.  Cache strides (multiples of 8)
+ * are free, so [batch, room, heads, 128] and [batch, heads, room, 128] both
+ * fit; sequences given k and v must not share cache rows.  workspace (device,
+ * 16-byte aligned) >= ennx_b200_gqa_attention_decode_workspace_size(...)
+ * bytes, which is 0 for small rooms; calls that may overlap need one each. */
+typedef struct {
+    const uint16_t* q;            /* [batch][hq][128], rows ld_q apart */
+    int64_t ld_q;
+    const uint16_t* k;            /* [batch][hkv][128], nullable */
+    int64_t ld_k;
+    const uint16_t* v;            /* [batch][hkv][128], nullable */
+    int64_t ld_v;
+    uint16_t* k_cache;            /* row (b, token, head) at b*k_seq + token*k_token + head*k_head */
+    int64_t k_seq, k_token, k_head;
+    uint16_t* v_cache;
+    int64_t v_seq, v_token, v_head;
+    const int32_t* lengths;
+    uint16_t* o;                  /* [batch][hq][128], rows ld_o apart */
+    int64_t ld_o;
+    int32_t batch, room, hq, hkv; /* room: tokens a sequence of the cache can hold */
+} ennx_b200_decode_attention;
+ENNX_B200_API size_t ennx_b200_gqa_attention_decode_workspace_size(int32_t batch, int32_t room, int32_t hq,
+                                                                   int32_t hkv);
+ENNX_B200_API int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* params, float rope_theta,
+                                                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Chunked KDA (gated delta rule, per-key-channel decay, chunk 64, d_k = d_v =
  * 128), equivalent to the serial recurrence of kda_recurrence_16k

@@ -37,3 +37,56 @@ def test_packed_attention_refuses_on_the_host():
     assert "rope_theta" in refused(*call(theta=float("nan")))
     assert "too many rows" in refused(*call(rows=1 << 31), status=_abi.UNSUPPORTED)
     assert getattr(_abi.lib(), "ennx_b200_gqa_attention_packed")(*call(rows=0)[1:]) == _abi.OK
+
+
+def test_decode_attention_refuses_on_the_host():
+    def call(theta=0.0, workspace=P(256), size=1 << 30, **over):
+        f = dict(q=256, ld_q=512, k=256, ld_k=256, v=256, ld_v=256, k_cache=256, k_seq=8192, k_token=256, k_head=128,
+                 v_cache=256, v_seq=8192, v_token=256, v_head=128, lengths=256, o=256, ld_o=512, batch=2, room=2048,
+                 hq=4, hkv=2)
+        f.update(over)
+        return ("ennx_b200_gqa_attention_decode", ctypes.byref(_abi.DecodeAttention(**f)), theta, workspace, size, None)
+
+    assert "null parameters" in refused("ennx_b200_gqa_attention_decode", None, 0.0, None, 0, None)
+    assert "room" in refused(*call(room=0))
+    assert "multiple of Hkv" in refused(*call(hq=5))
+    assert "rope_theta" in refused(*call(theta=-1.0))
+    assert "null argument" in refused(*call(lengths=None))
+    assert "come together" in refused(*call(v=None))
+    assert "shorter" in refused(*call(ld_q=504))
+    assert "shorter" in refused(*call(ld_k=128))
+    assert "negative" in refused(*call(k_seq=-8192))
+    assert "multiple of 8" in refused(*call(v_token=260))
+    assert "aligned" in refused(*call(k_cache=260))
+    assert "workspace" in refused(*call(workspace=None))
+    assert "workspace" in refused(*call(size=1000))
+    assert "workspace" in refused(*call(workspace=P(260)))
+    assert getattr(_abi.lib(), "ennx_b200_gqa_attention_decode")(*call(batch=0)[1:]) == _abi.OK
+    q = torch.zeros(2, 4, 128, dtype=BF16)
+    c = torch.zeros(2, 8, 2, 128, dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.gqa_attention_decode(q, c, c, torch.zeros(2, dtype=torch.int32))
+
+
+def test_moe_layer_decode_refuses_on_the_host():
+    a = P(256)
+
+    def call(x=a, wr=a, wgu=a, wd=a, t=2, h=256, e=8, k=2, i=128, y=a, ws=a, size=1 << 30):
+        return ("ennx_b200_moe_layer_decode", x, wr, wgu, wd, t, h, e, k, i, None, y, None, None, ws, size, None)
+
+    assert "negative" in refused(*call(t=-1))
+    assert "top_k" in refused(*call(k=9))
+    assert "top_k" in refused(*call(e=1))
+    assert "at most 64 tokens" in refused(*call(t=65), status=_abi.UNSUPPORTED)
+    assert "256 experts" in refused(*call(e=257), status=_abi.UNSUPPORTED)
+    assert "multiple of 64" in refused(*call(h=96), status=_abi.UNSUPPORTED)
+    assert "multiple of 64" in refused(*call(i=192), status=_abi.UNSUPPORTED)
+    assert "null" in refused(*call(wd=None))
+    assert "aligned" in refused(*call(x=P(258)))
+    assert "workspace" in refused(*call(size=100))
+    assert "workspace" in refused(*call(ws=P(8)))
+    assert _abi.lib().ennx_b200_moe_layer_decode(*call(t=0)[1:]) == _abi.OK
+    x = torch.zeros(2, 256, dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.moe_layer_decode(x, torch.zeros(8, 256, dtype=BF16), torch.zeros(8, 256, 256, dtype=BF16),
+                             torch.zeros(8, 256, 128, dtype=BF16), 2)
