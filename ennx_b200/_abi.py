@@ -218,6 +218,7 @@ SIGNATURES = {
     "ennx_b200_packed_dequantize_f32": (_I32, [_P, _P, _P, _P, PerturbSeed, _P, _P]),
     "ennx_b200_packed_linear_workspace_size": (_SZ, [_P]),
     "ennx_b200_packed_linear_bf16": (_I32, [_P, ctypes.c_int64, _P, _P, _P, _P, PerturbSeed, _P, _P, _SZ, _P]),
+    "ennx_b200_packed_linear_decode": (_I32, [_P, _I64, _P, _P, _P, _P, PerturbSeed, _P, _P]),
     "ennx_b200_profile_begin": (_I32, []),
     "ennx_b200_profile_end": (_I32, [_P, _I32, _P]),
     "ennx_b200_launch_count": (_U64, []),

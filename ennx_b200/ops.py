@@ -154,6 +154,34 @@ def packed_linear(x: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, 
     return out
 
 
+def packed_linear_decode(x: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
+                         linear: _abi.PackedLinear, seed: tuple[int, int, int] = (0, 0, 0),
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """``packed_linear`` for at most 16 tokens, straight from the codes (see
+    ``ennx_b200_packed_linear_decode``): any widths and group size, weights not
+    rounded to bf16.  The arenas must hold the whole linear."""
+    what = "packed_linear_decode"
+    _check_here(what, x, weights, scales, biases, out)
+    inp, n = linear.input_width, linear.output_width
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != inp or not x.is_contiguous():
+        raise ValueError(f"{what}: x must be contiguous bfloat16 [tokens, input_width]")
+    if weights.dtype != torch.uint8 or scales.dtype != torch.float32 or biases.dtype != torch.float32 or \
+            not (weights.is_contiguous() and scales.is_contiguous() and biases.is_contiguous()):
+        raise ValueError(f"{what}: arenas must be contiguous uint8 codes and float32 scales and biases")
+    if linear.bits in (4, 8) and linear.group_size:
+        groups = n * -(-inp // linear.group_size)
+        if linear.byte_offset + n * ((inp * linear.bits + 7) // 8) > weights.numel() or \
+                linear.scale_offset + groups > scales.numel() or linear.bias_offset + groups > biases.numel():
+            raise ValueError(f"{what}: the linear exceeds its arenas")
+    if out is None:
+        out = torch.empty(x.shape[0], n, dtype=torch.bfloat16, device=x.device)
+    elif out.dtype != torch.bfloat16 or out.shape != (x.shape[0], n) or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous bfloat16 [tokens, output_width]")
+    _abi.call("ennx_b200_packed_linear_decode", _ptr(x), x.shape[0], _ptr(weights), _ptr(scales), _ptr(biases),
+              ctypes.byref(linear), _abi.PerturbSeed(*seed), _ptr(out), _stream())
+    return out
+
+
 def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, with_logits: bool = False):
     """Routing indices (bit-exact with the CPU oracle) and renormalised gates."""
     _check_dev(x, w_router)

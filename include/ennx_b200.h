@@ -523,6 +523,18 @@ ENNX_B200_API int32_t ennx_b200_packed_linear_bf16(const uint16_t* x, int64_t to
                                                    ennx_b200_perturb_seed seed, uint16_t* out, void* workspace,
                                                    size_t workspace_bytes, void* stream);
 
+/* The projection for at most 16 tokens, straight from the codes (no
+ * dequantised copy, no workspace): out[t, r] = sum over groups of
+ * scale * (sum of code' x) + bias * (sum of x), in fp32 and rounded to bf16
+ * once -- ennx_b200_packed_linear_bf16 rounds every weight to bf16 first.  Any
+ * widths, group size and arena alignment (x and out 2-byte, scales and biases
+ * 4-byte aligned); x bf16 [tokens, input_width] and out [tokens, output_width]
+ * contiguous.  tokens == 0 does nothing. */
+ENNX_B200_API int32_t ennx_b200_packed_linear_decode(const uint16_t* x, int64_t tokens, const uint8_t* weights,
+                                                     const float* scales, const float* biases,
+                                                     const ennx_b200_packed_linear* linear,
+                                                     ennx_b200_perturb_seed seed, uint16_t* out, void* stream);
+
 /* ---- packed KDA attention block over whole sequences (16k prefill) ------ */
 
 /* Descriptors of one layer's KDA block in a package (names as in the

@@ -1,0 +1,141 @@
+"""Few-token packed products on the GPU against their definition in 64 bits,
+the codes taken from the oracle-checked dequantisation.
+
+Tolerance: codes and activations are exact in bf16 and so are their products in
+fp32; sums are fp32.  A chain has at most K additions, each off by at most
+2^-23 of a running magnitude below A = sum |code x| |scale| + |bias x|: with the
+256 columns of a chain joined as a tree, 2^-23 * 280 * A <= 2^-14 A bounds it for
+every width here.  The result is rounded to bf16 once (2^-8 relative)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from ennx_b200 import _abi, ops  # noqa: E402
+
+
+def make(inp, out, bits, group, seed, offsets=(0, 0, 0), whole=0, threshold=0, element=0):
+    rng = np.random.default_rng(seed)
+    row_bytes, groups = (inp * bits + 7) // 8, -(-inp // group)
+    w = rng.integers(0, 256, offsets[0] + out * row_bytes, dtype=np.uint8)
+    sc = rng.uniform(0.5, 1.5, offsets[1] + out * groups).astype(np.float32) * 3.0 / ((1 << bits) * inp ** 0.5)
+    bi = -rng.uniform(0.4, 0.6, offsets[2] + out * groups).astype(np.float32) * 3.0 / inp ** 0.5
+    lin = _abi.PackedLinear(*offsets, inp, out, bits, group, element, whole, threshold)
+    return [torch.from_numpy(a).cuda() for a in (w, sc, bi)] + [lin]
+
+
+def x_of(tokens, inp, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(tokens, inp, generator=g, device="cuda").to(torch.bfloat16)
+
+
+def check(got, x, w, sc, bi, lin, seed=(0, 0, 0)):
+    inp, out, group = lin.input_width, lin.output_width, lin.group_size
+    groups = -(-inp // group)
+    # the code itself: dequantise with scale 1 and bias 0
+    codes = ops.packed_dequantize(w, torch.ones_like(sc), torch.zeros_like(bi), lin, seed, dtype=torch.float32).double()
+    column = torch.arange(inp, device="cuda") // group
+    s = sc[lin.scale_offset:lin.scale_offset + out * groups].view(out, groups).double()[:, column]
+    b = bi[lin.bias_offset:lin.bias_offset + out * groups].view(out, groups).double()[:, column]
+    ref = x.double() @ (codes * s + b).T
+    size = x.double().abs() @ (codes * s.abs() + b.abs()).T
+    err = (got.double() - ref).abs() - (1.001 * 2.0 ** -8 * ref.abs() + 2.0 ** -14 * size)
+    assert err.max() <= 0, float(err.max())
+
+
+SHAPES = [
+    (2048, 512, 64), (256, 48, 32), (64, 16, 64), (32, 1, 32), (1, 1, 1), (7, 3, 4), (200, 17, 48), (37, 9, 8), (16, 33, 16),
+    (512, 100, 128), (1024, 31, 256), (2048, 40, 2048), (96, 300, 16), (4096, 64, 64), (4160, 24, 32), (8200, 19, 64),
+    (2011, 50, 64), (255, 65, 32), (1000, 20, 1000), (2080, 16, 96), (130, 130, 160), (2304, 8, 2000),
+]
+
+
+@pytest.mark.parametrize("inp,out,group", SHAPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("tokens", [1, 3, 8, 9, 16])
+def test_matches_definition(inp, out, group, bits, tokens):
+    w, sc, bi, lin = make(inp, out, bits, group, inp + bits)
+    x = x_of(tokens, inp, tokens)
+    check(ops.packed_linear_decode(x, w, sc, bi, lin), x, w, sc, bi, lin)
+
+
+@pytest.mark.parametrize("inp,out,group", [(256, 33, 32), (2048, 64, 64), (201, 40, 32), (37, 9, 8), (96, 20, 16)])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("whole,threshold,element", [(0, 0x40000000, 5), (1, 1 << 31, 2 ** 32 - 300), (20, 0, 0), (0, 1, 0),
+                                                     (300, 0xFFFFFFFF, 7)])
+def test_moved_codes(inp, out, group, bits, whole, threshold, element):
+    w, sc, bi, lin = make(inp, out, bits, group, 3, whole=whole, threshold=threshold, element=element)
+    x, seed = x_of(5, inp, 4), (0x9E37, 0x51ED27, 1)
+    check(ops.packed_linear_decode(x, w, sc, bi, lin, seed), x, w, sc, bi, lin, seed)
+
+
+@pytest.mark.parametrize("offsets", [(1, 1, 3), (3, 2, 1), (16, 4, 4), (18, 5, 0), (7, 0, 0)])
+@pytest.mark.parametrize("inp,group", [(2048, 64), (320, 32), (99, 32)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_arena_offsets_of_any_alignment(offsets, inp, group, bits):
+    w, sc, bi, lin = make(inp, 70, bits, group, 5, offsets=offsets)
+    big = x_of(4, inp + 1, 6).flatten()
+    x = big[1:1 + 3 * inp].view(3, inp)  # two-byte aligned only
+    check(ops.packed_linear_decode(x, w, sc, bi, lin), x, w, sc, bi, lin)
+
+
+def test_same_sign_activations():
+    # every activation positive: the largest sums the codes can make
+    w, sc, bi, lin = make(4096, 32, 8, 64, 8)
+    x = x_of(16, 4096, 9).abs() + 1
+    check(ops.packed_linear_decode(x, w, sc, bi, lin), x, w, sc, bi, lin)
+
+
+def test_a_bad_token_or_row_stays_alone():
+    w, sc, bi, lin = make(512, 40, 4, 64, 10)
+    x = x_of(9, 512, 11)
+    clean = ops.packed_linear_decode(x, w, sc, bi, lin)
+    x[4, 100] = float("nan")
+    sc[3 * 8 + 2] = float("inf")
+    y = ops.packed_linear_decode(x, w, sc, bi, lin)
+    rows = [r for r in range(40) if r != 3]
+    tok = [t for t in range(9) if t != 4]
+    assert torch.equal(y[tok][:, rows], clean[tok][:, rows])
+    assert y[4].isnan().all() and not y[:, 3].isfinite().any()
+
+
+def test_graph_out_and_stream():
+    w, sc, bi, lin = make(1024, 96, 4, 64, 12)
+    x, out = x_of(2, 1024, 13), torch.empty(2, 96, dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ops.packed_linear_decode(x, w, sc, bi, lin, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ops.packed_linear_decode(x, w, sc, bi, lin, out=out)
+    torch.cuda.current_stream().wait_stream(stream)
+    for seed in (14, 15):
+        x.copy_(x_of(2, 1024, seed))
+        graph.replay()
+        check(out, x, w, sc, bi, lin)
+
+
+def test_no_tokens():
+    w, sc, bi, lin = make(64, 8, 4, 32, 16)
+    assert ops.packed_linear_decode(x_of(1, 64, 0)[:0], w, sc, bi, lin).shape == (0, 8)
+
+
+def test_refusals():
+    w, sc, bi, lin = make(64, 8, 4, 32, 17)
+    x, call = x_of(2, 64, 18), ops.packed_linear_decode
+    with pytest.raises(Exception, match="at most 16 tokens"):
+        call(x_of(17, 64, 19), w, sc, bi, lin)
+    with pytest.raises(ValueError, match="input_width"):
+        call(x[:, :32], w, sc, bi, lin)
+    with pytest.raises(ValueError, match="exceeds its arenas"):
+        call(x, w[:-1], sc, bi, lin)
+    with pytest.raises(ValueError, match="exceeds its arenas"):
+        call(x, w, sc, bi[:-1], lin)
+    with pytest.raises(ValueError, match="uint8"):
+        call(x, w.int(), sc, bi, lin)
+    with pytest.raises(ValueError, match="bits must be 4 or 8"):
+        call(x, w, sc, bi, _abi.PackedLinear(0, 0, 0, 64, 8, 5, 32, 0, 0, 0))
+    with pytest.raises(ValueError, match="out must be"):
+        call(x, w, sc, bi, lin, out=torch.empty(2, 9, dtype=torch.bfloat16, device="cuda"))

@@ -90,3 +90,26 @@ def test_moe_layer_decode_refuses_on_the_host():
     with pytest.raises(ValueError, match="CUDA"):
         ops.moe_layer_decode(x, torch.zeros(8, 256, dtype=BF16), torch.zeros(8, 256, 256, dtype=BF16),
                              torch.zeros(8, 256, 128, dtype=BF16), 2)
+
+
+def test_packed_linear_decode_refuses_on_the_host():
+    a, seed = P(256), _abi.PerturbSeed(0, 0, 0)
+    lin = _abi.PackedLinear(0, 0, 0, 64, 8, 4, 32, 0, 0, 0)
+
+    def call(x=a, t=2, w=a, sc=a, bi=a, d=lin, out=a):
+        return ("ennx_b200_packed_linear_decode", x, t, w, sc, bi, None if d is None else ctypes.byref(d), seed, out,
+                None)
+
+    assert "descriptor is null" in refused(*call(d=None))
+    assert "bits must be 4 or 8" in refused(*call(d=_abi.PackedLinear(0, 0, 0, 64, 8, 3, 32, 0, 0, 0)))
+    assert "must be positive" in refused(*call(d=_abi.PackedLinear(0, 0, 0, 64, 8, 4, 0, 0, 0, 0)))
+    assert "negative" in refused(*call(t=-1))
+    assert "at most 16 tokens" in refused(*call(t=17), status=_abi.UNSUPPORTED)
+    assert "2^31" in refused(*call(d=_abi.PackedLinear(0, 0, 0, 1 << 31, 8, 4, 32, 0, 0, 0)), status=_abi.UNSUPPORTED)
+    assert "null" in refused(*call(bi=None))
+    assert "misaligned" in refused(*call(sc=P(258)))
+    assert "misaligned" in refused(*call(x=P(257)))
+    assert _abi.lib().ennx_b200_packed_linear_decode(*call(t=0)[1:]) == _abi.OK
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.packed_linear_decode(torch.zeros(2, 64, dtype=BF16), torch.zeros(256, dtype=torch.uint8), torch.zeros(16),
+                                 torch.zeros(16), lin)
