@@ -13,7 +13,9 @@
 // rows are the 16 rows of m16n8k16, tokens the 8 columns.  A warp owns 256
 // columns of k: its activations stay in registers for all rows, its codes
 // stream through a cp.async ring; the warps of a row tile are joined through
-// shared memory.  Narrow matrices put fewer warps on k and more on rows.
+// shared memory.  Narrow matrices put fewer warps on k and more on rows.  Rows
+// may start at any byte: the ring holds the 16-byte granules that cover them
+// (each holds at least one byte of the row) and reads are shifted into place.
 #include "kernels.cuh"
 #include "packed.cuh"
 #include "serve.cuh"
@@ -72,6 +74,325 @@ __global__ void __launch_bounds__(256) packed_rows_kernel(const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------------------
+// groups of a multiple of 32 columns: tensor products of codes
+// ---------------------------------------------------------------------------
+constexpr int kSliceChunks = 8, kSlice = 32 * kSliceChunks;  // columns of k that a warp owns in a pass
+constexpr int kWarps = 8;
+
+// How a call is laid out: `along` warps side by side on k, the others on rows.
+struct Split {
+  int along, row_warps;  // along * row_warps = kWarps
+  int passes;            // slices per warp on k
+  int tiles;             // row tiles of 16
+};
+
+template <int kBits>
+struct Tile {  // one stage of a warp's ring: 16 code rows, then scales and biases
+  static constexpr int kRowBytes = kSlice * kBits / 8;
+  // a row starts anywhere in its first 16 bytes; the pitch keeps the rows of
+  // a fragment read on different banks (4-bit: 8 rows x 16 bytes, 8-bit: x 32)
+  static constexpr int kPitch = kBits == 4 ? kRowBytes + 16 : kRowBytes + 32;
+  static constexpr int kPieces = kRowBytes / 16 + 1;
+};
+template <int kBits, int kFlush>
+constexpr int stage_bytes() { return 16 * Tile<kBits>::kPitch + 16 * (16 / kFlush) * 8; }
+// ring depth: as many stages as leave two blocks on an SM (80 to 130 KB in flight)
+template <int kBits, int kFlush>
+constexpr int stages() { return kBits == 8 ? 2 : kFlush == 4 ? 4 : 3; }
+template <int kBits, int kN, int kFlush>
+constexpr int smem_bytes() {
+  return kWarps * (stages<kBits, kFlush>() * stage_bytes<kBits, kFlush>() + (16 / kFlush) * 8 * kN * 4 + 2 * kN * 32 * 16);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds32(a)); }
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 32 bits of a row at any byte address
+__device__ __forceinline__ uint32_t word_at(uint32_t a) {
+  const uint32_t lo = a & ~3u;
+  return __funnelshift_r(lds32(lo), lds32(lo + 4), (a & 3u) * 8);
+}
+// bf16 pair of two integers below 256, exact: 2^23 + n in fp32, less 2^23
+__device__ __forceinline__ uint32_t pair_of(uint32_t lo, uint32_t hi) {
+  return pack_bf16x2(__uint_as_float(0x4b000000u | lo) - 8388608.0f, __uint_as_float(0x4b000000u | hi) - 8388608.0f);
+}
+
+// Eight codes of a lane (columns 8t .. 8t+7 of a chunk) as four bf16 pairs.
+// 4 bits: pairs (j, j + 4): two nibbles 16 bits apart are or-ed under the
+// exponent of 128 (128 + n is exact) and 128 is taken off again.  8 bits:
+// pairs (0, 1), (2, 3), ...  activation_pairs orders x the same way.
+template <int kBits, bool kMoved>
+__device__ __forceinline__ void code_pairs(const uint32_t (&w)[kBits / 4], uint32_t element, const Product& p,
+                                           uint32_t (&r)[4]) {
+  if constexpr (kMoved) {
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t code = kBits == 4 ? (w[0] >> (4 * j)) & 15u : (w[j >> 2] >> (8 * (j & 3))) & 255u;
+      c[j] = moved_code(code, p, element + j, (1u << kBits) - 1u);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = kBits == 4 ? pair_of(c[j], c[j + 4]) : pair_of(c[2 * j], c[2 * j + 1]);
+  } else if constexpr (kBits == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      r[j] = bf16x2_sub(((w[0] >> (4 * j)) & 0x000f000fu) | 0x43004300u, 0x43004300u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      r[j] = pair_of(__byte_perm(w[j >> 1], 0, 0x4440 + 2 * (j & 1)), __byte_perm(w[j >> 1], 0, 0x4441 + 2 * (j & 1)));
+  }
+}
+template <int kBits>
+__device__ __forceinline__ uint4 activation_pairs(uint4 v) {  // columns (0,1) (2,3) (4,5) (6,7)
+  if constexpr (kBits == 8) return v;
+  return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                    __byte_perm(v.y, v.w, 0x7632));
+}
+
+// kN: blocks of 8 tokens; kFlush: products of 16 columns under one scale
+template <int kBits, int kN, int kFlush, bool kMoved>
+__global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __grid_constant__ Product p,
+                                                                         const __grid_constant__ Split sp) {
+  using T = Tile<kBits>;
+  constexpr int kFlushes = 16 / kFlush;  // scales per row of a slice
+  constexpr int kStage = stage_bytes<kBits, kFlush>(), kStages = stages<kBits, kFlush>();
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int wk = warp % sp.along, wr = warp / sp.along;
+  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * kStage;
+  // sums of x over each flush of this warp's slice, per token
+  float* xsum = reinterpret_cast<float*>(smem + kWarps * kStages * kStage) + warp * kFlushes * 8 * kN;
+  float4* red = reinterpret_cast<float4*>(smem + kWarps * (kStages * kStage + kFlushes * 8 * kN * 4));
+  const uint32_t width = (uint32_t)p.d.input_width, rows = (uint32_t)p.d.output_width, groups = (uint32_t)p.d.groups;
+  const bool wide_x = width % 8 == 0 && ((uintptr_t)p.x & 15u) == 0;
+
+  const int stride = (int)gridDim.x * sp.row_warps;
+  int tile = (int)blockIdx.x * sp.row_warps + wr;
+  auto slice0 = [&](int pass) { return (uint32_t)(pass * sp.along + wk) * kSlice; };
+
+  int f_tile = tile, f_pass = 0, fetched = 0;
+  auto fetch = [&] {
+    if (f_tile < sp.tiles) {
+      const uint32_t dst = ring + (fetched % kStages) * kStage, c0 = slice0(f_pass);
+      if (c0 < width) {
+        // 16-byte granules that hold a byte of the slice, none behind the row's last
+        const uint32_t first = c0 * kBits / 8, last = min((uint32_t)p.d.row_bytes, first + T::kRowBytes);
+#pragma unroll
+        for (int i = lane; i < 16 * T::kPieces; i += 32) {
+          const int r = i / T::kPieces, c = i % T::kPieces;
+          const uint32_t row = (uint32_t)f_tile * 16 + r;
+          if (row < rows) {
+            const uint8_t* start = p.w + (uint64_t)row * p.d.row_bytes + first;
+            const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
+            if (src < start + (last - first)) cp_async16(dst + r * T::kPitch + 16 * c, src);
+          }
+        }
+        const uint32_t sdst = dst + 16 * T::kPitch;
+#pragma unroll
+        for (int i = lane; i < 16 * kFlushes; i += 32) {
+          const int r = i / kFlushes, f = i % kFlushes;
+          const uint32_t row = (uint32_t)f_tile * 16 + r, col = c0 + f * kFlush * 16;
+          if (row < rows && col < width) {
+            const uint64_t at = (uint64_t)row * groups + min(col / p.d.group_size, groups - 1u);
+            cp_async4(sdst + i * 8, p.sc + at);
+            cp_async4(sdst + i * 8 + 4, p.bi + at);
+          }
+        }
+      }
+      if (++f_pass == sp.passes) {
+        f_pass = 0;
+        f_tile += stride;
+      }
+    }
+    ++fetched;
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch();
+
+  uint4 xf[kSliceChunks][kN];
+  auto load_x = [&](int pass) {  // activations of the slice, zeros behind the last column or token
+    const uint32_t c0 = slice0(pass);
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int tok = n * 8 + g;
+      const uint16_t* x = p.x + (uint64_t)(tok < p.tokens ? tok : 0) * width;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kSliceChunks; ++j) {
+        const uint32_t c = c0 + j * 32 + t * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (tok < p.tokens) {
+          if (wide_x) {
+            if (c < width) v = __ldg(reinterpret_cast<const uint4*>(x + c));
+          } else {
+            uint32_t e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = c + i < width ? __ldg(x + c + i) : 0u;
+            v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+          }
+        }
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        float s8 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s8 += __uint_as_float(u[i] << 16) + __uint_as_float(u[i] & 0xffff0000u);
+        sum += s8;
+        if ((j + 1) % (kFlush / 2) == 0) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if (t == 0) xsum[(j / (kFlush / 2) * kN + n) * 8 + g] = sum;
+          sum = 0.0f;
+        }
+        xf[j][n] = activation_pairs<kBits>(v);
+      }
+    }
+    __syncwarp();
+  };
+  if (sp.passes == 1) load_x(0);
+
+  int done = 0;
+  for (int i = 0; tile < sp.tiles; ++done) {
+    float out[kN][4] = {};
+    for (int pass = 0; pass < sp.passes; ++pass, ++i) {
+      if (sp.passes > 1) load_x(pass);
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      const uint32_t st = ring + (i % kStages) * kStage, c0 = slice0(pass);
+      if (c0 < width) {
+        uint32_t addr[2], element[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t row = (uint32_t)tile * 16 + g + 8 * h;
+          const uint32_t skew = (uint32_t)((uintptr_t)(p.w + (uint64_t)row * p.d.row_bytes) + c0 * kBits / 8) & 15u;
+          addr[h] = st + (g + 8 * h) * T::kPitch + skew + t * kBits;
+          element[h] = (uint32_t)p.d.element_offset + row * width + c0 + t * 8;
+        }
+        const bool straight = ((addr[0] | addr[1]) & 3u) == 0;  // per lane; the same for a whole aligned matrix
+#pragma unroll
+        for (int f = 0; f < kFlushes; ++f) {
+          float acc[kN][4] = {};
+#pragma unroll
+          for (int j = f * kFlush / 2; j < (f + 1) * kFlush / 2; ++j) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[kBits / 4];
+#pragma unroll
+              for (int i4 = 0; i4 < kBits / 4; ++i4) {
+                const uint32_t at = addr[h] + j * 4 * kBits + 4 * i4;
+                w[i4] = straight ? lds32(at) : word_at(at);
+              }
+              code_pairs<kBits, kMoved>(w, element[h] + j * 32, p, a[h]);
+            }
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+              mma(acc[n], a[0][0], a[1][0], a[0][1], a[1][1], xf[j][n].x, xf[j][n].y);
+              mma(acc[n], a[0][2], a[1][2], a[0][3], a[1][3], xf[j][n].z, xf[j][n].w);
+            }
+          }
+          if (c0 + f * kFlush * 16 < width) {
+            const uint32_t sa = st + 16 * T::kPitch + (g * kFlushes + f) * 8;
+            const float s0 = ldsf(sa), b0 = ldsf(sa + 4), s1 = ldsf(sa + 64 * kFlushes), b1 = ldsf(sa + 64 * kFlushes + 4);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+              const float2 xs = *reinterpret_cast<const float2*>(xsum + (f * kN + n) * 8 + 2 * t);
+              out[n][0] = fmaf(s0, acc[n][0], fmaf(b0, xs.x, out[n][0]));
+              out[n][1] = fmaf(s0, acc[n][1], fmaf(b0, xs.y, out[n][1]));
+              out[n][2] = fmaf(s1, acc[n][2], fmaf(b1, xs.x, out[n][2]));
+              out[n][3] = fmaf(s1, acc[n][3], fmaf(b1, xs.y, out[n][3]));
+            }
+          }
+        }
+      }
+      __syncwarp();
+      fetch();
+    }
+    if (sp.along > 1) {
+      // one barrier a tile: the other buffer is written again only after the
+      // next barrier, which every reader of this one reaches first
+      float4* buf = red + ((done & 1) * sp.row_warps + wr) * sp.along * kN * 32;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) buf[(wk * kN + n) * 32 + lane] = make_float4(out[n][0], out[n][1], out[n][2], out[n][3]);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + wr), "r"(32 * sp.along) : "memory");
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+        if (wk == n) {
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int w = 0; w < sp.along; ++w) {
+            const float4 u = buf[(w * kN + n) * 32 + lane];
+            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+          }
+          out[n][0] = v.x; out[n][1] = v.y; out[n][2] = v.z; out[n][3] = v.w;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+      if (sp.along == 1 || wk == n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t row = (uint32_t)tile * 16 + g + 8 * (j >> 1);
+          const int tok = n * 8 + 2 * t + (j & 1);
+          if (row < rows && tok < p.tokens) p.out[(uint64_t)tok * rows + row] = f32_to_bf16_rne(out[n][j]);
+        }
+    tile += stride;
+  }
+  cp_wait<0>();
+}
+
+template <int kBits, int kN, int kFlush, bool kMoved>
+int32_t launch_tiles(const Product& p, cudaStream_t s) {
+  const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved>;
+  Split sp;
+  const int slices = (int)((p.d.input_width + kSlice - 1) / kSlice);
+  sp.along = 1;
+  while (sp.along < slices && sp.along < kWarps) sp.along *= 2;
+  sp.row_warps = kWarps / sp.along;
+  sp.passes = (slices + sp.along - 1) / sp.along;
+  sp.tiles = (int)((p.d.output_width + 15) / 16);
+  constexpr int smem = smem_bytes<kBits, kN, kFlush>();
+  static_assert(2 * (smem + 1024) <= 228 * 1024, "two blocks on an SM");
+  static bool attr[64];
+  int dev = 0;
+  ENNX_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return set_error(ENNX_B200_UNSUPPORTED, "device index %d out of range", dev);
+  if (!attr[dev]) {
+    ENNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "packed tiles smem");
+    attr[dev] = true;
+  }
+  const int blocks = (sp.tiles + sp.row_warps - 1) / sp.row_warps, cap = 2 * sm_count();
+  kernel<<<(unsigned)(blocks < cap ? blocks : cap), 32 * kWarps, smem, s>>>(p, sp);
+  ENNX_LAUNCH_CHECK("packed tiles");
+  return ENNX_B200_OK;
+}
+template <int kBits, int kN>
+int32_t launch_tiles(const Product& p, cudaStream_t s) {
+  const bool four = p.d.group_size % 64 == 0, moved = p.seed.enabled != 0;
+  if (four) return moved ? launch_tiles<kBits, kN, 4, true>(p, s) : launch_tiles<kBits, kN, 4, false>(p, s);
+  return moved ? launch_tiles<kBits, kN, 2, true>(p, s) : launch_tiles<kBits, kN, 2, false>(p, s);
+}
+
 }  // namespace
 }  // namespace ennx
 
@@ -103,6 +424,12 @@ extern "C" int32_t ennx_b200_packed_linear_decode(const uint16_t* x, int64_t tok
   p.tokens = (int)tokens;
   // a linear that moves no code needs no hash
   if (p.d.whole == 0 && (p.d.threshold >> 1) == 0) p.seed.enabled = 0;
+  // one group over the whole row: any size that covers it says the same
+  if (p.d.groups == 1) p.d.group_size = (uint32_t)((p.d.input_width + 63) / 64 * 64);
+  if (p.d.group_size % 32 == 0) {
+    if (p.d.bits == 4) return tokens <= 8 ? launch_tiles<4, 1>(p, s) : launch_tiles<4, 2>(p, s);
+    return tokens <= 8 ? launch_tiles<8, 1>(p, s) : launch_tiles<8, 2>(p, s);
+  }
   const uint64_t blocks = (p.d.output_width + 7) / 8, cap = (uint64_t)sm_count() * 16;
   const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
   if (tokens == 1) packed_rows_kernel<1><<<grid, 256, 0, s>>>(p);
