@@ -87,22 +87,26 @@ struct Split {
   int tiles;             // row tiles of 16
 };
 
-template <int kBits>
-struct Tile {  // one stage of a warp's ring: 16 code rows, then scales and biases
+// One stage of a warp's ring: 16 code rows, then (scale, bias) pairs.  A flush
+// is kFlush products of 16 columns under one scale; lane t of a row takes
+// 4 * kFlush consecutive columns of it, one shared-memory read.
+template <int kBits, int kFlush>
+struct Stage {
   static constexpr int kRowBytes = kSlice * kBits / 8;
-  // a row starts anywhere in its first 16 bytes; the pitch keeps the rows of
-  // a fragment read on different banks (4-bit: 8 rows x 16 bytes, 8-bit: x 32)
-  static constexpr int kPitch = kBits == 4 ? kRowBytes + 16 : kRowBytes + 32;
+  // rows of a fragment read lie on different banks (an 8-lane phase covers
+  // whole rows, each kFlush * 2 * kBits bytes), and a row that starts inside
+  // a 16-byte granule still fits
+  static constexpr int kPitch = kRowBytes + kFlush * 2 * kBits;
   static constexpr int kPieces = kRowBytes / 16 + 1;
+  static constexpr int kFlushes = 16 / kFlush;
+  static constexpr int kBytes = 16 * kPitch + 16 * kFlushes * 8;
+  // depth: as many as leave two blocks on an SM (80 to 100 KB in flight)
+  static constexpr int kDepth = kBits == 8 ? 2 : 3;
 };
-template <int kBits, int kFlush>
-constexpr int stage_bytes() { return 16 * Tile<kBits>::kPitch + 16 * (16 / kFlush) * 8; }
-// ring depth: as many stages as leave two blocks on an SM (80 to 130 KB in flight)
-template <int kBits, int kFlush>
-constexpr int stages() { return kBits == 8 ? 2 : kFlush == 4 ? 4 : 3; }
 template <int kBits, int kN, int kFlush>
 constexpr int smem_bytes() {
-  return kWarps * (stages<kBits, kFlush>() * stage_bytes<kBits, kFlush>() + (16 / kFlush) * 8 * kN * 4 + 2 * kN * 32 * 16);
+  using S = Stage<kBits, kFlush>;
+  return kWarps * (S::kDepth * S::kBytes + S::kFlushes * 8 * kN * 4 + 2 * kN * 32 * 16);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -119,7 +123,13 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds32(a)); }
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
+  static_assert(N == 1 || N == 2 || N == 4, "one shared-memory read");
+  if constexpr (N == 1) w[0] = lds32(a);
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
+  else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+}
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -137,13 +147,12 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t lo, uint32_t hi) {
   return pack_bf16x2(__uint_as_float(0x4b000000u | lo) - 8388608.0f, __uint_as_float(0x4b000000u | hi) - 8388608.0f);
 }
 
-// Eight codes of a lane (columns 8t .. 8t+7 of a chunk) as four bf16 pairs.
+// Eight consecutive codes of a lane as four bf16 pairs.
 // 4 bits: pairs (j, j + 4): two nibbles 16 bits apart are or-ed under the
 // exponent of 128 (128 + n is exact) and 128 is taken off again.  8 bits:
 // pairs (0, 1), (2, 3), ...  activation_pairs orders x the same way.
 template <int kBits, bool kMoved>
-__device__ __forceinline__ void code_pairs(const uint32_t (&w)[kBits / 4], uint32_t element, const Product& p,
-                                           uint32_t (&r)[4]) {
+__device__ __forceinline__ void code_pairs(const uint32_t* w, uint32_t element, const Product& p, uint32_t (&r)[4]) {
   if constexpr (kMoved) {
     uint32_t c[8];
 #pragma unroll
@@ -170,20 +179,20 @@ __device__ __forceinline__ uint4 activation_pairs(uint4 v) {  // columns (0,1) (
                     __byte_perm(v.y, v.w, 0x7632));
 }
 
-// kN: blocks of 8 tokens; kFlush: products of 16 columns under one scale
-template <int kBits, int kN, int kFlush, bool kMoved>
+// kN: blocks of 8 tokens.  kAligned: rows start on 16 bytes and the slice ends
+// on a granule, so copies need no per-row arithmetic and reads no shifting.
+template <int kBits, int kN, int kFlush, bool kMoved, bool kAligned>
 __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __grid_constant__ Product p,
-                                                                         const __grid_constant__ Split sp) {
-  using T = Tile<kBits>;
-  constexpr int kFlushes = 16 / kFlush;  // scales per row of a slice
-  constexpr int kStage = stage_bytes<kBits, kFlush>(), kStages = stages<kBits, kFlush>();
+                                                                      const __grid_constant__ Split sp) {
+  using S = Stage<kBits, kFlush>;
+  constexpr int kFlushes = S::kFlushes, kStages = S::kDepth, kRuns = kFlush / 2;  // runs of 8 columns of a lane in a flush
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int wk = warp % sp.along, wr = warp / sp.along;
-  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * kStage;
+  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * S::kBytes;
   // sums of x over each flush of this warp's slice, per token
-  float* xsum = reinterpret_cast<float*>(smem + kWarps * kStages * kStage) + warp * kFlushes * 8 * kN;
-  float4* red = reinterpret_cast<float4*>(smem + kWarps * (kStages * kStage + kFlushes * 8 * kN * 4));
+  float* xsum = reinterpret_cast<float*>(smem + kWarps * kStages * S::kBytes) + warp * kFlushes * 8 * kN;
+  float4* red = reinterpret_cast<float4*>(smem + kWarps * (kStages * S::kBytes + kFlushes * 8 * kN * 4));
   const uint32_t width = (uint32_t)p.d.input_width, rows = (uint32_t)p.d.output_width, groups = (uint32_t)p.d.groups;
   const bool wide_x = width % 8 == 0 && ((uintptr_t)p.x & 15u) == 0;
 
@@ -191,32 +200,46 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
   int tile = (int)blockIdx.x * sp.row_warps + wr;
   auto slice0 = [&](int pass) { return (uint32_t)(pass * sp.along + wk) * kSlice; };
 
-  int f_tile = tile, f_pass = 0, fetched = 0;
+  int f_tile = tile, f_pass = 0;
+  uint32_t f_stage = ring;
   auto fetch = [&] {
     if (f_tile < sp.tiles) {
-      const uint32_t dst = ring + (fetched % kStages) * kStage, c0 = slice0(f_pass);
+      const uint32_t dst = f_stage, c0 = slice0(f_pass), row0 = (uint32_t)f_tile * 16;
       if (c0 < width) {
-        // 16-byte granules that hold a byte of the slice, none behind the row's last
-        const uint32_t first = c0 * kBits / 8, last = min((uint32_t)p.d.row_bytes, first + T::kRowBytes);
+        const uint32_t first = c0 * kBits / 8;
+        if constexpr (kAligned) {
+          constexpr int kLanes = S::kRowBytes / 16, kRows = 32 / kLanes;  // lanes of a row, rows of an instruction
+          const int r = lane / kLanes, c = lane % kLanes;
+          const uint8_t* src = p.w + (uint64_t)(row0 + r) * p.d.row_bytes + first + 16 * c;
+          const bool inside = first + 16 * c < (uint32_t)p.d.row_bytes;
 #pragma unroll
-        for (int i = lane; i < 16 * T::kPieces; i += 32) {
-          const int r = i / T::kPieces, c = i % T::kPieces;
-          const uint32_t row = (uint32_t)f_tile * 16 + r;
-          if (row < rows) {
-            const uint8_t* start = p.w + (uint64_t)row * p.d.row_bytes + first;
-            const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
-            if (src < start + (last - first)) cp_async16(dst + r * T::kPitch + 16 * c, src);
+          for (int i = 0; i < 16 / kRows; ++i)
+            if (inside && row0 + r + i * kRows < rows)
+              cp_async16(dst + (r + i * kRows) * S::kPitch + 16 * c, src + (uint64_t)(i * kRows) * p.d.row_bytes);
+        } else {
+          // 16-byte granules that hold a byte of the slice, none behind the row's last
+          const uint32_t last = min((uint32_t)p.d.row_bytes, first + S::kRowBytes);
+#pragma unroll
+          for (int i = lane; i < 16 * S::kPieces; i += 32) {
+            const int r = i / S::kPieces, c = i % S::kPieces;
+            const uint32_t row = row0 + r;
+            if (row < rows) {
+              const uint8_t* start = p.w + (uint64_t)row * p.d.row_bytes + first;
+              const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
+              if (src < start + (last - first)) cp_async16(dst + r * S::kPitch + 16 * c, src);
+            }
           }
         }
-        const uint32_t sdst = dst + 16 * T::kPitch;
+        const int r = lane / kFlushes, f = lane % kFlushes;
+        const uint32_t col = c0 + f * kFlush * 16;
+        const uint64_t at = (uint64_t)(row0 + r) * groups + min(col / p.d.group_size, groups - 1u);
+        const uint32_t sdst = dst + 16 * S::kPitch + lane * 8;
 #pragma unroll
-        for (int i = lane; i < 16 * kFlushes; i += 32) {
-          const int r = i / kFlushes, f = i % kFlushes;
-          const uint32_t row = (uint32_t)f_tile * 16 + r, col = c0 + f * kFlush * 16;
-          if (row < rows && col < width) {
-            const uint64_t at = (uint64_t)row * groups + min(col / p.d.group_size, groups - 1u);
-            cp_async4(sdst + i * 8, p.sc + at);
-            cp_async4(sdst + i * 8 + 4, p.bi + at);
+        for (int i = 0; i < kFlushes / 2; ++i) {
+          const int more = i * (32 / kFlushes);  // rows further down
+          if (col < width && row0 + r + more < rows) {
+            cp_async4(sdst + i * 256, p.sc + at + (uint64_t)more * groups);
+            cp_async4(sdst + i * 256 + 4, p.bi + at + (uint64_t)more * groups);
           }
         }
       }
@@ -225,7 +248,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
         f_tile += stride;
       }
     }
-    ++fetched;
+    f_stage = f_stage + S::kBytes == ring + kStages * S::kBytes ? ring : f_stage + S::kBytes;
     cp_commit();
   };
 #pragma unroll
@@ -242,7 +265,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < kSliceChunks; ++j) {
-        const uint32_t c = c0 + j * 32 + t * 8;
+        const uint32_t c = c0 + j / kRuns * (16 * kFlush) + t * (8 * kRuns) + j % kRuns * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (tok < p.tokens) {
           if (wide_x) {
@@ -259,10 +282,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
 #pragma unroll
         for (int i = 0; i < 4; ++i) s8 += __uint_as_float(u[i] << 16) + __uint_as_float(u[i] & 0xffff0000u);
         sum += s8;
-        if ((j + 1) % (kFlush / 2) == 0) {
+        if ((j + 1) % kRuns == 0) {
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          if (t == 0) xsum[(j / (kFlush / 2) * kN + n) * 8 + g] = sum;
+          if (t == 0) xsum[(j / kRuns * kN + n) * 8 + g] = sum;
           sum = 0.0f;
         }
         xf[j][n] = activation_pairs<kBits>(v);
@@ -272,40 +295,46 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
   };
   if (sp.passes == 1) load_x(0);
 
-  int done = 0;
-  for (int i = 0; tile < sp.tiles; ++done) {
+  uint32_t st = ring;
+  for (int done = 0; tile < sp.tiles; ++done) {
     float out[kN][4] = {};
-    for (int pass = 0; pass < sp.passes; ++pass, ++i) {
+    for (int pass = 0; pass < sp.passes; ++pass) {
       if (sp.passes > 1) load_x(pass);
       cp_wait<kStages - 2>();
       __syncwarp();
-      const uint32_t st = ring + (i % kStages) * kStage, c0 = slice0(pass);
+      const uint32_t c0 = slice0(pass);
       if (c0 < width) {
         uint32_t addr[2], element[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t row = (uint32_t)tile * 16 + g + 8 * h;
-          const uint32_t skew = (uint32_t)((uintptr_t)(p.w + (uint64_t)row * p.d.row_bytes) + c0 * kBits / 8) & 15u;
-          addr[h] = st + (g + 8 * h) * T::kPitch + skew + t * kBits;
-          element[h] = (uint32_t)p.d.element_offset + row * width + c0 + t * 8;
+          const uint32_t skew =
+              kAligned ? 0u : (uint32_t)((uintptr_t)(p.w + (uint64_t)row * p.d.row_bytes) + c0 * kBits / 8) & 15u;
+          addr[h] = st + (g + 8 * h) * S::kPitch + skew + t * (kRuns * kBits);
+          element[h] = (uint32_t)p.d.element_offset + row * width + c0 + t * (8 * kRuns);
         }
-        const bool straight = ((addr[0] | addr[1]) & 3u) == 0;  // per lane; the same for a whole aligned matrix
 #pragma unroll
         for (int f = 0; f < kFlushes; ++f) {
           float acc[kN][4] = {};
+          constexpr int kWords = kRuns * kBits / 4;  // of a lane's columns in a flush
+          uint32_t w[2][kWords];
 #pragma unroll
-          for (int j = f * kFlush / 2; j < (f + 1) * kFlush / 2; ++j) {
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t at = addr[h] + f * (4 * kRuns * kBits);
+            if constexpr (kAligned) {
+              lds_words<kWords>(at, w[h]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kWords; ++i) w[h][i] = word_at(at + 4 * i);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i) {
+            const int j = f * kRuns + i;
             uint32_t a[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t w[kBits / 4];
-#pragma unroll
-              for (int i4 = 0; i4 < kBits / 4; ++i4) {
-                const uint32_t at = addr[h] + j * 4 * kBits + 4 * i4;
-                w[i4] = straight ? lds32(at) : word_at(at);
-              }
-              code_pairs<kBits, kMoved>(w, element[h] + j * 32, p, a[h]);
-            }
+            for (int h = 0; h < 2; ++h)
+              code_pairs<kBits, kMoved>(&w[h][i * (kBits / 4)], element[h] + f * (16 * kFlush) + i * 8, p, a[h]);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
               mma(acc[n], a[0][0], a[1][0], a[0][1], a[1][1], xf[j][n].x, xf[j][n].y);
@@ -313,8 +342,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
             }
           }
           if (c0 + f * kFlush * 16 < width) {
-            const uint32_t sa = st + 16 * T::kPitch + (g * kFlushes + f) * 8;
-            const float s0 = ldsf(sa), b0 = ldsf(sa + 4), s1 = ldsf(sa + 64 * kFlushes), b1 = ldsf(sa + 64 * kFlushes + 4);
+            const uint32_t sa = st + 16 * S::kPitch + (g * kFlushes + f) * 8;
+            uint32_t u[2], v[2];  // (scale, bias) of rows g and g + 8
+            lds_words<2>(sa, u);
+            lds_words<2>(sa + 64 * kFlushes, v);
+            const float s0 = __uint_as_float(u[0]), b0 = __uint_as_float(u[1]);
+            const float s1 = __uint_as_float(v[0]), b1 = __uint_as_float(v[1]);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
               const float2 xs = *reinterpret_cast<const float2*>(xsum + (f * kN + n) * 8 + 2 * t);
@@ -326,6 +359,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
           }
         }
       }
+      st = st + S::kBytes == ring + kStages * S::kBytes ? ring : st + S::kBytes;
       __syncwarp();
       fetch();
     }
@@ -361,9 +395,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
   cp_wait<0>();
 }
 
-template <int kBits, int kN, int kFlush, bool kMoved>
+template <int kBits, int kN, int kFlush, bool kMoved, bool kAligned>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
-  const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved>;
+  const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved, kAligned>;
   Split sp;
   const int slices = (int)((p.d.input_width + kSlice - 1) / kSlice);
   sp.along = 1;
@@ -386,11 +420,16 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   ENNX_LAUNCH_CHECK("packed tiles");
   return ENNX_B200_OK;
 }
+template <int kBits, int kN, int kFlush>
+int32_t launch_tiles(const Product& p, cudaStream_t s) {
+  // moved codes spend their time on the hash: one variant for any alignment
+  if (p.seed.enabled) return launch_tiles<kBits, kN, kFlush, true, false>(p, s);
+  if (p.d.row_bytes % 16 == 0 && ((uintptr_t)p.w & 15u) == 0) return launch_tiles<kBits, kN, kFlush, false, true>(p, s);
+  return launch_tiles<kBits, kN, kFlush, false, false>(p, s);
+}
 template <int kBits, int kN>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
-  const bool four = p.d.group_size % 64 == 0, moved = p.seed.enabled != 0;
-  if (four) return moved ? launch_tiles<kBits, kN, 4, true>(p, s) : launch_tiles<kBits, kN, 4, false>(p, s);
-  return moved ? launch_tiles<kBits, kN, 2, true>(p, s) : launch_tiles<kBits, kN, 2, false>(p, s);
+  return p.d.group_size % 64 == 0 ? launch_tiles<kBits, kN, 4>(p, s) : launch_tiles<kBits, kN, 2>(p, s);
 }
 
 }  // namespace
