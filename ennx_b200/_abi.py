@@ -7,6 +7,7 @@ the device is not sm_100, every call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libennx_b200.so"
@@ -73,16 +74,9 @@ class GemmParams(ctypes.Structure):
                 ("lse_partial", ctypes.c_void_p), ("target_logit", ctypes.c_void_p)]
 
 
-class DecodeAttention(ctypes.Structure):
-    """ennx_b200_decode_attention."""
-    _fields_ = [("q", ctypes.c_void_p), ("ld_q", ctypes.c_int64), ("k", ctypes.c_void_p), ("ld_k", ctypes.c_int64),
-                ("v", ctypes.c_void_p), ("ld_v", ctypes.c_int64),
-                ("k_cache", ctypes.c_void_p), ("k_seq", ctypes.c_int64), ("k_token", ctypes.c_int64),
-                ("k_head", ctypes.c_int64),
-                ("v_cache", ctypes.c_void_p), ("v_seq", ctypes.c_int64), ("v_token", ctypes.c_int64),
-                ("v_head", ctypes.c_int64),
-                ("lengths", ctypes.c_void_p), ("o", ctypes.c_void_p), ("ld_o", ctypes.c_int64),
-                ("batch", ctypes.c_int32), ("room", ctypes.c_int32), ("hq", ctypes.c_int32), ("hkv", ctypes.c_int32)]
+# ennx_b200_decode_attention: q, ld_q, k, ld_k, v, ld_v, k_cache, k_seq, k_token, k_head, v_cache, v_seq,
+# v_token, v_head, lengths, o, ld_o, batch, room, hq, hkv
+DECODE_ATTENTION = struct.Struct("@QqQqQqQqqqQqqqQQqiiii")
 
 
 class PackedLinear(ctypes.Structure):

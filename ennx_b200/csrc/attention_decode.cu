@@ -105,9 +105,6 @@ __device__ long long scan_units(const Args& a, long long target, int* seq, long 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -117,10 +114,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-               "{%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  mma_16x8x16(c, a[0], a[1], a[2], a[3], b0, b1);
 }
 __device__ __forceinline__ void turn(float& x1, float& x2, float s, float c) {
   const float y1 = x1 * c - x2 * s;
@@ -154,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_attention_kernel(const
   int unit;  // first unit within the segment
   if constexpr (kSplit) {
     // the join kernel may start its own prologue; it waits for this grid to finish before it reads
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    launch_dependents();
     long long before, total = scan_units(a, -1, &b, &before);
     const long long per = (total + gridDim.x - 1) / gridDim.x, first = per * blockIdx.x;
     left = min(per, total - first);
@@ -440,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_const
   const int rows = min(block_rows, a.group - g0), lane = threadIdx.x & 31;
   // the partials are complete and visible; blocks without any wait too, so
   // that this grid never ends before the one it follows
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_previous();
   if (units > 0 && c0 == c1) return;
   for (int row = threadIdx.x >> 5; row < rows; row += kWarps) {
     float m = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -476,13 +470,14 @@ int block_rows(int group) { return group <= 8 ? 8 : 16; }
 int split_grid() { return kPerSm * sm_count(); }
 
 template <int kRows>
-int32_t launch(const Args& a, const RopeTable& table, bool split, int64_t segs, cudaStream_t s) {
-  if (split) token_attention_kernel<true, kRows><<<(unsigned)split_grid(), kThreads, kSmem, s>>>(a, table);
-  else token_attention_kernel<false, kRows><<<(unsigned)segs, kThreads, kSmem, s>>>(a, table);
+int32_t launch(const Args& a, const RopeTable& table, bool split, int64_t segs, int dev, cudaStream_t s) {
+  static SharedMemorySetup setup[2];
+  const auto kernel = split ? token_attention_kernel<true, kRows> : token_attention_kernel<false, kRows>;
+  ENNX_TRY(allow_shared_memory(setup[split], dev, kernel, kSmem));
+  kernel<<<split ? (unsigned)split_grid() : (unsigned)segs, kThreads, kSmem, s>>>(a, table);
   ENNX_LAUNCH_CHECK("token attention");
   return ENNX_B200_OK;
 }
-
 
 }  // namespace
 }  // namespace ennx
@@ -531,17 +526,10 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
                p->lengths, p->batch, p->room, p->hkv, group, blocks, 1.4426950408889634f / sqrtf((float)D),
                rope_theta > 0.0f, (float*)workspace};
   const RopeTable& table = rope_table(rope_theta > 0.0f ? rope_theta : 1.0f);
-  static bool attr[64];
   int dev = 0;
-  ENNX_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-  if (dev < 0 || dev >= 64) return set_error(ENNX_B200_UNSUPPORTED, "device index %d out of range", dev);
-  if (!attr[dev]) {
-    for (const void* f : {(const void*)token_attention_kernel<true, 8>, (const void*)token_attention_kernel<true, 16>,
-                          (const void*)token_attention_kernel<false, 8>, (const void*)token_attention_kernel<false, 16>})
-      ENNX_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "token attention smem");
-    attr[dev] = true;
-  }
-  ENNX_TRY(rows == 8 ? launch<8>(a, table, need != 0, segs, s) : launch<16>(a, table, need != 0, segs, s));
+  int* status = nullptr;
+  ENNX_TRY(serving_device(&dev, &status));
+  ENNX_TRY(rows == 8 ? launch<8>(a, table, need != 0, segs, dev, s) : launch<16>(a, table, need != 0, segs, dev, s));
   if (!need) return ENNX_B200_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)segs);

@@ -30,19 +30,7 @@
 
 #include <math.h>
 
-#include <mutex>
-
 namespace ennx {
-
-const RopeTable& rope_table(float theta) {
-  static thread_local RopeTable t;
-  static thread_local float of = -1.0f;
-  if (of != theta) {
-    for (int i = 0; i < 64; ++i) t.inv[i] = pow((double)theta, -2.0 * i / 128.0) / 6.283185307179586476925;
-    of = theta;
-  }
-  return t;
-}
 
 namespace {
 
@@ -445,39 +433,7 @@ __global__ void rope_packed_kernel(uint16_t* __restrict__ x, long long ld, int h
   }
 }
 
-constexpr int kMaxDevices = 64;
-__device__ int g_status_word;  // written where a bounded wait gave up
-
-// Per-device set-up of the first call: the shared-memory attribute and the
-// address of the status word.  Allocates nothing.
-struct Setup {
-  std::once_flag once;
-  int32_t status = ENNX_B200_OK;
-  int* word = nullptr;
-};
-Setup g_setup[kMaxDevices];
-
-int32_t device_setup(int** word) {
-  int dev = 0;
-  ENNX_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-  if (dev < 0 || dev >= kMaxDevices) return set_error(ENNX_B200_UNSUPPORTED, "device index %d out of range", dev);
-  Setup& s = g_setup[dev];
-  std::call_once(s.once, [&] {
-    void* p = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(&p, g_status_word);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(prompt_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-    if (e != cudaSuccess) {
-      s.status = check_cuda(e, "packed attention set-up");
-      return;
-    }
-    s.word = (int*)p;
-    register_status_word(dev, s.word);
-  });
-  if (s.status != ENNX_B200_OK) return set_error(s.status, "packed attention: set-up failed on device %d", dev);
-  *word = s.word;
-  return ENNX_B200_OK;
-}
+SharedMemorySetup g_setup;
 
 }  // namespace
 }  // namespace ennx
@@ -503,8 +459,10 @@ extern "C" int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uin
   if ((ld_q | ld_k | ld_v | ld_o) % 8 || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15u))
     return set_error(ENNX_B200_INVALID_ARGUMENT,
                      "attention_packed: operands must be 16-byte aligned with strides of a multiple of 8");
+  int dev = 0;
   int* err = nullptr;
-  ENNX_TRY(device_setup(&err));
+  ENNX_TRY(serving_device(&dev, &err));
+  ENNX_TRY(allow_shared_memory(g_setup, dev, prompt_attention_kernel, SMEM));
   CUtensorMap tq, tk, tv;
   ENNX_TRY(make_tmap_2d_bf16(&tq, q, (uint64_t)hq * D, (uint64_t)rows, (uint64_t)ld_q, 64, 128, true));
   ENNX_TRY(make_tmap_2d_bf16(&tk, k, (uint64_t)hkv * D, (uint64_t)rows, (uint64_t)ld_k, 64, 128, true));

@@ -18,9 +18,11 @@
 // routing from the logits itself, which costs less than another launch.
 //
 // Products run on m16n8k16 with weight rows as the 16 rows and tokens as the
-// 8 columns; each warp streams its own weight tiles through a cp.async ring
-// (two 8 KB tiles in flight per warp, 128 KB per SM).  k is permuted the same
-// way in both operands so that a lane's fragments are 16 contiguous bytes.
+// 8 columns; each warp streams its own weight tiles through a ring of bulk
+// copies, a row (512 bytes) each: copying with a 16-byte instruction per lane
+// instead took 6 times the instructions and was bound by them (64 tokens 212
+// us).  k is permuted the same way in both operands so that a lane's fragments
+// are 16 contiguous bytes.
 #include "kernels.cuh"
 #include "serve.cuh"
 
@@ -31,28 +33,14 @@ namespace {
 
 constexpr int kTokens = 64, kTopK = 8, kExperts = 256;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kChunk = 32;               // k of one 64-byte piece per row: two mma steps
-constexpr int kTileChunks = 8;           // chunks of a warp's tile
-constexpr int kPitch = kTileChunks * 64;  // bytes of a tile row
-constexpr int kTileBytes = 16 * kPitch;
-constexpr int kStages = 3;
-constexpr int kRing = kWarps * kStages * kTileBytes;
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-               "{%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+constexpr int kChunk = 32;       // k of one 64-byte piece per row: two products of 16
+constexpr int kTileChunks = 8;   // chunks of a warp's tile
+constexpr int kStages = 3;       // two tiles of 8 KB in flight per warp, 128 KB per SM
+// Rows of a tile in shared memory, in pairs 1088 bytes apart, the second row
+// 576 bytes behind the first: the two rows of an 8-lane phase, 64 bytes each,
+// then lie on different banks wherever the phase starts.
+__device__ __forceinline__ constexpr uint32_t row_at(int r) { return (uint32_t)((r >> 1) * 1088 + (r & 1) * 576); }
+constexpr int tile_bytes(int rows) { return (rows + 1) / 2 * 1088; }
 
 struct Layer {
   const uint16_t *x, *w_router, *w_gate_up, *w_down, *residual;
@@ -62,6 +50,37 @@ struct Layer {
   float* logits;  // [tokens][experts]
   uint16_t* act;  // [tokens * top_k][width], rows expert by expert
   int tokens, hidden, experts, top_k, width;
+  int* status;
+};
+
+// A warp's ring of weight tiles, filled by one bulk copy per row.
+struct Ring {
+  uint8_t* base;
+  uint64_t* full;
+  int stage_bytes, fetched, used;
+  bool bad;  // a wait gave up: later ones are not tried again, the results are void
+  __device__ __forceinline__ void init(uint8_t* at, uint64_t* bars, int bytes, int lane) {
+    base = at; full = bars; stage_bytes = bytes; fetched = used = 0; bad = false;
+    if (lane < kStages) mbar_init(full + lane, 1);
+    fence_barrier_init();
+    fence_proxy_async();
+    __syncwarp();
+  }
+  // lane r < 16 copies row r from `src` where `ok`; the same `bytes` per row
+  __device__ __forceinline__ void fetch(const uint16_t* src, bool ok, int bytes, int lane) {
+    const int at = fetched % kStages;
+    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, ok));
+    if (lane == 0) mbar_arrive_expect_tx(full + at, copies * bytes);
+    __syncwarp();
+    if (ok) bulk_copy(smem_u32(base) + at * stage_bytes + row_at(lane), src, bytes, full + at);
+    ++fetched;
+  }
+  __device__ __forceinline__ uint32_t wait(int* status) {  // the next tile's address
+    const int at = used % kStages;
+    if (!bad) bad = !mbar_wait(full + at, (used / kStages) & 1, status);
+    ++used;
+    return smem_u32(base) + at * stage_bytes;
+  }
 };
 
 // ---------------------------------------------------------------------------
@@ -227,27 +246,27 @@ __device__ void make_plan(const Layer& p, Plan& s) {
   __syncthreads();
 }
 
-// piece (16 bytes) c of row r of a ring tile: rows 512 bytes apart would put
-// the two rows of a quarter-warp on the same banks, so odd rows swap halves
-__device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)(r * kPitch + ((c ^ ((r & 1) << 2)) << 4)); }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-
 // ---------------------------------------------------------------------------
 // gate/up: a block takes an equal run of the (picked expert, column) list.  A
 // tile is 8 columns (8 gate rows and their 8 up rows) x all k, the k split
 // over the warps; kN blocks of 8 tokens at a time stay in registers.
 // ---------------------------------------------------------------------------
 template <int kN>
+struct GateUpShared {
+  uint8_t ring[kWarps][kStages][tile_bytes(16)];
+  float4 red[2][kWarps][kN][32];
+  uint64_t full[kWarps][kStages];
+  Plan plan;
+};
+
+template <int kN>
 __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid_constant__ Layer p) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  float4* red = reinterpret_cast<float4*>(smem + kRing);  // [2][warp][kN][lane]
-  Plan& s = *reinterpret_cast<Plan*>(smem + kRing + 2 * kWarps * kN * 32 * sizeof(float4));
+  extern __shared__ __align__(128) uint8_t smem[];
+  GateUpShared<kN>& sh = *reinterpret_cast<GateUpShared<kN>*>(smem);
+  Plan& s = sh.plan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kTileBytes;
+  Ring ring;
+  ring.init(sh.ring[warp][0], sh.full[warp], tile_bytes(16), lane);
   wait_previous();
   launch_dependents();
   make_plan(p, s);
@@ -261,67 +280,64 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
   const long long columns = (long long)s.active * p.width;
   const long long begin = columns * blockIdx.x / gridDim.x, end = columns * (blockIdx.x + 1) / gridDim.x;
   if (begin >= end) return;
+  const int a_first = (int)(begin / p.width), a_last = (int)((end - 1) / p.width);
+  const int c_first = (int)(begin - (long long)a_first * p.width), c_last = (int)(end - (long long)a_last * p.width);
   const int chunks = p.hidden / kChunk, passes = (chunks + kWarps * kTileChunks - 1) / (kWarps * kTileChunks);
   const int per = ((chunks + passes - 1) / passes + kWarps - 1) / kWarps;  // chunks of a warp in a pass
 
   // tiles in order: expert, group of kN * 8 tokens, 8 columns, k pass
-  struct Tile {
-    int a, c, pass, group;  // c: column within the expert
+  struct Walk {
+    int a, c, c_begin, c_end, group, groups, pass;
   };
-  auto last_column = [&](int a) { return (int)min((long long)p.width, end - (long long)a * p.width); };
-  auto first_column = [&](int a) { return (int)max(0LL, begin - (long long)a * p.width); };
-  auto next = [&](Tile& w) -> bool {  // false behind the last tile
+  auto enter = [&](Walk& w) {  // first tile of expert w.a
+    w.c = w.c_begin = w.a == a_first ? c_first : 0;
+    w.c_end = w.a == a_last ? c_last : p.width;
+    w.groups = (s.first[w.a + 1] - s.first[w.a] + kN * 8 - 1) / (kN * 8);
+    w.group = w.pass = 0;
+  };
+  auto next = [&](Walk& w) -> bool {  // false behind the last tile
     if (++w.pass < passes) return true;
     w.pass = 0;
     w.c += 8;
-    if (w.c < last_column(w.a)) return true;
-    w.c = first_column(w.a);
-    if (++w.group * kN * 8 < s.first[w.a + 1] - s.first[w.a]) return true;
-    w.group = 0;
-    ++w.a;
-    w.c = 0;
-    return (long long)w.a * p.width < end;
+    if (w.c < w.c_end) return true;
+    w.c = w.c_begin;
+    if (++w.group < w.groups) return true;
+    if (++w.a > a_last) return false;
+    enter(w);
+    return true;
   };
   auto chunk0 = [&](int pass) { return (pass * kWarps + warp) * per; };
+  auto valid = [&](int pass) { return max(0, min(per, chunks - chunk0(pass))); };  // chunks of this warp's tile
 
-  Tile ahead{(int)(begin / p.width), (int)(begin % p.width), 0, 0}, now = ahead;
+  Walk ahead, now;
+  ahead.a = a_first;
+  enter(ahead);
+  now = ahead;
   bool more = true;
-  int fetched = 0;
   auto fetch = [&] {
-    if (more) {
-      const uint16_t* w = p.w_gate_up + (long long)s.expert[ahead.a] * 2 * p.width * p.hidden;
-      const uint32_t dst = ring + (fetched % kStages) * kTileBytes;
-      const int c_end = last_column(ahead.a), k0 = chunk0(ahead.pass);
-      const bool k_ok = (lane >> 2) < per && k0 + (lane >> 2) < chunks;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int col = ahead.c + (r & 7), row = (col >> 7) * 256 + (r >> 3) * 128 + (col & 127);
-        const bool ok = k_ok && col < c_end;
-        cp_async16(dst + piece(r, lane), w + (ok ? (long long)row * p.hidden + k0 * kChunk + lane * 8 : 0), ok);
-      }
-      more = next(ahead);
-    }
-    ++fetched;
-    cp_commit();
+    if (!more) return;
+    const int col = ahead.c + (lane & 7), row = (col >> 7) * 256 + (lane >> 3) * 128 + (col & 127), n = valid(ahead.pass);
+    const uint16_t* w = p.w_gate_up + ((long long)s.expert[ahead.a] * 2 * p.width + row) * p.hidden + chunk0(ahead.pass) * kChunk;
+    ring.fetch(w, lane < 16 && col < ahead.c_end && n > 0, n * 64, lane);
+    more = next(ahead);
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
   uint4 xf[kTileChunks][kN];
-  int have_a = -1, have_group = -1, have_pass = -1;
+  bool reload = true;
   float acc[kN][4];
-  for (int i = 0, done = 0;; ++i) {
-    if (now.a != have_a || now.group != have_group || now.pass != have_pass) {
-      have_a = now.a; have_group = now.group; have_pass = now.pass;
+  for (int done = 0;;) {
+    const int n_chunks = valid(now.pass), first = s.first[now.a] + now.group * kN * 8, last = s.first[now.a + 1];
+    if (reload) {
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        const int slot = s.first[now.a] + (now.group * kN + n) * 8 + g;
-        const bool ok = slot < s.first[now.a + 1];
+        const int slot = first + n * 8 + g;
+        const bool ok = slot < last;
         const uint16_t* x = p.x + (ok ? (long long)s.token(slot) * p.hidden : 0) + chunk0(now.pass) * kChunk + t * 8;
 #pragma unroll
         for (int j = 0; j < kTileChunks; ++j)
-          xf[j][n] = ok && j < per && chunk0(now.pass) + j < chunks ? __ldg(reinterpret_cast<const uint4*>(x + j * kChunk))
-                                                                 : make_uint4(0, 0, 0, 0);
+          xf[j][n] = ok && j < n_chunks ? __ldg(reinterpret_cast<const uint4*>(x + j * kChunk)) : make_uint4(0, 0, 0, 0);
       }
     }
     if (now.pass == 0) {
@@ -330,28 +346,25 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
     }
-    cp_wait<kStages - 2>();
-    __syncwarp();
-    const uint32_t tile = ring + (i % kStages) * kTileBytes;
+    const uint32_t tile = ring.wait(p.status) + row_at(g) + 16 * t;  // row g + 8: row_at(8) further on
 #pragma unroll
     for (int j = 0; j < kTileChunks; ++j) {
-      if (j < per) {
-        const uint4 a = lds128(tile + piece(g, 4 * j + t)), b = lds128(tile + piece(g + 8, 4 * j + t));
+      if (j < n_chunks) {
+        const uint4 a = lds128(tile + 64 * j), b = lds128(tile + row_at(8) + 64 * j);
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-          mma(acc[n], a.x, b.x, a.y, b.y, xf[j][n].x, xf[j][n].y);
-          mma(acc[n], a.z, b.z, a.w, b.w, xf[j][n].z, xf[j][n].w);
+          mma_16x8x16(acc[n], a.x, b.x, a.y, b.y, xf[j][n].x, xf[j][n].y);
+          mma_16x8x16(acc[n], a.z, b.z, a.w, b.w, xf[j][n].z, xf[j][n].w);
         }
       }
     }
     __syncwarp();
     fetch();
     if (now.pass == passes - 1) {
-      float4* buf = red + (done & 1) * kWarps * kN * 32;
+      float4(&buf)[kWarps][kN][32] = sh.red[done & 1];
       ++done;
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
-        buf[(warp * kN + n) * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+      for (int n = 0; n < kN; ++n) buf[warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
       // one barrier a tile: the other buffer is written again only after the
       // next barrier, which every reader of this one reaches first
       __syncthreads();
@@ -359,21 +372,22 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 u = buf[(w * kN + warp) * 32 + lane];
+          const float4 u = buf[w][warp][lane];
           v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
         }
-        const int col = now.c + g, slot = s.first[now.a] + (now.group * kN + warp) * 8 + 2 * t;
-        if (col < last_column(now.a)) {
+        const int col = now.c + g, slot = first + warp * 8 + 2 * t;
+        if (col < now.c_end) {
           // rounded to bf16 for the second product: at most 2^-8 of a value
           uint16_t* h = p.act + (long long)slot * p.width + col;
-          if (slot < s.first[now.a + 1]) h[0] = f32_to_bf16_rne(v.x / (1.0f + expf(-v.x)) * v.z);
-          if (slot + 1 < s.first[now.a + 1]) h[p.width] = f32_to_bf16_rne(v.y / (1.0f + expf(-v.y)) * v.w);
+          if (slot < last) h[0] = f32_to_bf16_rne(v.x / (1.0f + expf(-v.x)) * v.z);
+          if (slot + 1 < last) h[p.width] = f32_to_bf16_rne(v.y / (1.0f + expf(-v.y)) * v.w);
         }
       }
     }
+    const int a = now.a, group = now.group;
     if (!next(now)) break;
+    reload = passes > 1 || now.a != a || now.group != group;
   }
-  cp_wait<0>();
 }
 
 // ---------------------------------------------------------------------------
@@ -383,14 +397,23 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
 // the warps, a warp's tile is kRows rows x 256 k.
 // ---------------------------------------------------------------------------
 constexpr int kRows = 14;
+struct DownShared {
+  uint8_t ring[kWarps][kStages][tile_bytes(kRows)];
+  uint64_t full[kWarps][kStages];
+  Plan plan;
+  float sums[1];  // [warp][token][kRows]
+};
+
 template <int kN>
 __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_constant__ Layer p) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  float* sums = reinterpret_cast<float*>(smem + kRing);  // [warp][token][kRows]
+  extern __shared__ __align__(128) uint8_t smem[];
+  DownShared& sh = *reinterpret_cast<DownShared*>(smem);
+  Plan& s = sh.plan;
   const int span = p.tokens * kRows;
-  Plan& s = *reinterpret_cast<Plan*>(smem + kRing + sizeof(float) * kWarps * span);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kTileBytes;
+  float* sums = sh.sums + warp * span;
+  Ring ring;
+  ring.init(sh.ring[warp][0], sh.full[warp], tile_bytes(kRows), lane);
   // the router grid has finished (every gate/up block waited for it before it
   // let this grid start), so the routing and the first weights can be fetched
   // while the gate/up products are still running
@@ -402,10 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_co
 
   for (int row0 = row_begin; row0 < row_end; row0 += kRows) {
     const int rows = min(kRows, row_end - row0);
-    struct Tile {
+    struct Walk {
       int a, group, pass;
     };
-    auto next = [&](Tile& w) -> bool {
+    auto next = [&](Walk& w) -> bool {
       if (++w.pass < passes) return true;
       w.pass = 0;
       if (++w.group * kN * 8 < s.first[w.a + 1] - s.first[w.a]) return true;
@@ -413,45 +436,35 @@ __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_co
       w.a += kWarps;
       return w.a < s.active;
     };
-    Tile ahead{warp, 0, 0}, now = ahead;
+    Walk ahead{warp, 0, 0}, now = ahead;
     bool more = warp < s.active;
-    int fetched = 0;
     auto fetch = [&] {
-      if (more) {
-        const uint16_t* w = p.w_down + ((long long)s.expert[ahead.a] * p.hidden + row0) * p.width;
-        const uint32_t dst = ring + (fetched % kStages) * kTileBytes;
-        const int k0 = ahead.pass * kTileChunks;
-        const bool k_ok = k0 + (lane >> 2) < chunks;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool ok = k_ok && r < rows;
-          cp_async16(dst + piece(r, lane), w + (ok ? (long long)r * p.width + k0 * kChunk + lane * 8 : 0), ok);
-        }
-        more = next(ahead);
-      }
-      ++fetched;
-      cp_commit();
+      if (!more) return;
+      const int k0 = ahead.pass * kTileChunks, n = min(kTileChunks, chunks - k0);
+      const uint16_t* w = p.w_down + ((long long)s.expert[ahead.a] * p.hidden + row0 + lane) * p.width + k0 * kChunk;
+      ring.fetch(w, lane < rows, n * 64, lane);
+      more = next(ahead);
     };
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) fetch();
-    for (int i = lane; i < span; i += 32) sums[warp * span + i] = 0.0f;
+    for (int i = lane; i < span; i += 32) sums[i] = 0.0f;
     if (!waited) {
       wait_previous();  // the activations are complete and visible
       waited = true;
     }
     __syncwarp();
     float acc[kN][4];
-    for (int i = 0; warp < s.active; ++i) {
+    while (warp < s.active) {
       const int first = s.first[now.a] + now.group * kN * 8, last = s.first[now.a + 1];
+      const int k0 = now.pass * kTileChunks, n_chunks = min(kTileChunks, chunks - k0);
       uint4 hf[kTileChunks][kN];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         const bool ok = first + n * 8 + g < last;
-        const uint16_t* h = p.act + (ok ? (long long)(first + n * 8 + g) * p.width : 0) + now.pass * kTileChunks * kChunk + t * 8;
+        const uint16_t* h = p.act + (ok ? (long long)(first + n * 8 + g) * p.width : 0) + k0 * kChunk + t * 8;
 #pragma unroll
         for (int j = 0; j < kTileChunks; ++j)
-          hf[j][n] = ok && now.pass * kTileChunks + j < chunks ? __ldcg(reinterpret_cast<const uint4*>(h + j * kChunk))
-                                                                : make_uint4(0, 0, 0, 0);
+          hf[j][n] = ok && j < n_chunks ? __ldcg(reinterpret_cast<const uint4*>(h + j * kChunk)) : make_uint4(0, 0, 0, 0);
       }
       if (now.pass == 0) {
 #pragma unroll
@@ -459,16 +472,18 @@ __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_co
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
       }
-      cp_wait<kStages - 2>();
-      __syncwarp();
-      const uint32_t tile = ring + (i % kStages) * kTileBytes;
+      // rows 14 and 15 of the product are not copied: whatever lies there
+      // (the next tile's first bytes) enters only their own sums
+      const uint32_t tile = ring.wait(p.status) + row_at(g) + 16 * t;
 #pragma unroll
       for (int j = 0; j < kTileChunks; ++j) {
-        const uint4 a = lds128(tile + piece(g, 4 * j + t)), b = lds128(tile + piece(g + 8, 4 * j + t));
+        if (j < n_chunks) {
+          const uint4 a = lds128(tile + 64 * j), b = lds128(tile + (g < kRows - 8 ? row_at(8) : 0u) + 64 * j);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          mma(acc[n], a.x, b.x, a.y, b.y, hf[j][n].x, hf[j][n].y);
-          mma(acc[n], a.z, b.z, a.w, b.w, hf[j][n].z, hf[j][n].w);
+          for (int n = 0; n < kN; ++n) {
+            mma_16x8x16(acc[n], a.x, b.x, a.y, b.y, hf[j][n].x, hf[j][n].y);
+            mma_16x8x16(acc[n], a.z, b.z, a.w, b.w, hf[j][n].z, hf[j][n].w);
+          }
         }
       }
       __syncwarp();
@@ -477,15 +492,19 @@ __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_co
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int slot = first + n * 8 + 2 * t + (j & 1), row = g + 8 * (j >> 1);
-            if (slot < last && row < kRows) sums[warp * span + s.token(slot) * kRows + row] += s.gate(slot) * acc[n][j];
+          for (int e = 0; e < 2; ++e) {
+            const int slot = first + n * 8 + 2 * t + e;
+            if (slot < last) {
+              float* to = sums + s.token(slot) * kRows + g;
+              const float gate = s.gate(slot);
+              to[0] += gate * acc[n][e];
+              if (g < kRows - 8) to[8] += gate * acc[n][2 + e];
+            }
           }
         __syncwarp();
       }
       if (!next(now)) break;
     }
-    cp_wait<0>();
     __syncthreads();
     for (int i = threadIdx.x; i < span; i += kThreads) {
       const int tok = i / kRows, r = i % kRows;
@@ -493,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_co
         const long long at = (long long)tok * p.hidden + row0 + r;
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += sums[w * span + i];
+        for (int w = 0; w < kWarps; ++w) v += sh.sums[w * span + i];
         if (p.residual) v += bf16_to_f32(p.residual[at]);
         p.y[at] = f32_to_bf16_rne(v);
       }
@@ -503,18 +522,16 @@ __global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_co
   if (!waited) wait_previous();  // no grid of the chain ends before the one it follows
 }
 
-template <int kN>
-constexpr size_t gate_up_smem() { return kRing + 2 * kWarps * kN * 32 * sizeof(float4) + sizeof(Plan); }
-constexpr size_t down_smem(int tokens) { return kRing + sizeof(float) * kWarps * tokens * kRows + sizeof(Plan); }
-static_assert(gate_up_smem<2>() <= 227 * 1024, "gate/up shared memory");
-static_assert(down_smem(kTokens) <= 227 * 1024, "down shared memory");
+constexpr size_t down_smem(int tokens) { return sizeof(DownShared) + sizeof(float) * kWarps * tokens * kRows; }
+static_assert(sizeof(GateUpShared<2>) <= 227 * 1024 && down_smem(kTokens) <= 227 * 1024, "shared memory of one block");
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename K>
-int32_t launch_after(K kernel, int grid, size_t smem, const Layer& p, cudaStream_t s) {
+int32_t launch_after(SharedMemorySetup& setup, int dev, K kernel, size_t smem, size_t most, const Layer& p, cudaStream_t s) {
+  ENNX_TRY(allow_shared_memory(setup, dev, kernel, (int)most));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)sm_count());
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -526,6 +543,13 @@ int32_t launch_after(K kernel, int grid, size_t smem, const Layer& p, cudaStream
   ENNX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p), "few-token moe");
   ENNX_LAUNCH_CHECK("few-token moe");
   return ENNX_B200_OK;
+}
+template <int kN>
+int32_t launch_experts(const Layer& p, int dev, cudaStream_t s) {
+  static SharedMemorySetup setup[2];
+  constexpr size_t smem = sizeof(GateUpShared<kN>);
+  ENNX_TRY(launch_after(setup[0], dev, token_gate_up_kernel<kN>, smem, smem, p, s));
+  return launch_after(setup[1], dev, token_down_kernel<kN>, down_smem(p.tokens), down_smem(kTokens), p, s);
 }
 
 }  // namespace
@@ -563,31 +587,16 @@ int32_t ennx_b200_moe_layer_decode(const uint16_t* x, const uint16_t* w_router, 
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u))
     return set_error(ENNX_B200_INVALID_ARGUMENT, "moe_layer_decode: a 16-byte aligned workspace of %zu bytes required",
                      need);
-  Layer p{x, w_router, w_gate_up, w_down, residual, y, index, gate, (float*)workspace,
-          (uint16_t*)((uint8_t*)workspace + round256(sizeof(float) * tokens * experts)),
-          (int)tokens, hidden, experts, top_k, expert_width};
-  static bool attr[64];
   int dev = 0;
-  ENNX_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-  if (dev < 0 || dev >= 64) return set_error(ENNX_B200_UNSUPPORTED, "device index %d out of range", dev);
-  if (!attr[dev]) {
-    const auto most = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    ENNX_CUDA(cudaFuncSetAttribute(token_gate_up_kernel<1>, most, (int)gate_up_smem<1>()), "few-token moe smem");
-    ENNX_CUDA(cudaFuncSetAttribute(token_gate_up_kernel<2>, most, (int)gate_up_smem<2>()), "few-token moe smem");
-    ENNX_CUDA(cudaFuncSetAttribute(token_down_kernel<1>, most, (int)down_smem(kTokens)), "few-token moe smem");
-    ENNX_CUDA(cudaFuncSetAttribute(token_down_kernel<2>, most, (int)down_smem(kTokens)), "few-token moe smem");
-    attr[dev] = true;
-  }
+  int* status = nullptr;
+  ENNX_TRY(serving_device(&dev, &status));
+  const Layer p{x, w_router, w_gate_up, w_down, residual, y, index, gate, (float*)workspace,
+                (uint16_t*)((uint8_t*)workspace + round256(sizeof(float) * tokens * experts)),
+                (int)tokens, hidden, experts, top_k, expert_width, status};
   const dim3 router((unsigned)((experts + kRE - 1) / kRE), (unsigned)((tokens + kRT - 1) / kRT));
   token_router_kernel<<<router, kThreads, 0, s>>>(p);
   ENNX_LAUNCH_CHECK("few-token router");
-  const int grid = sm_count();
-  if (tokens <= 8) {
-    ENNX_TRY(launch_after(token_gate_up_kernel<1>, grid, gate_up_smem<1>(), p, s));
-    return launch_after(token_down_kernel<1>, grid, down_smem((int)tokens), p, s);
-  }
-  ENNX_TRY(launch_after(token_gate_up_kernel<2>, grid, gate_up_smem<2>(), p, s));
-  return launch_after(token_down_kernel<2>, grid, down_smem((int)tokens), p, s);
+  return tokens <= 8 ? launch_experts<1>(p, dev, s) : launch_experts<2>(p, dev, s);
 }
 
 }  // extern "C"

@@ -115,9 +115,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -129,13 +126,6 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
   if constexpr (N == 1) w[0] = lds32(a);
   else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
   else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-               "{%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // 32 bits of a row at any byte address
 __device__ __forceinline__ uint32_t word_at(uint32_t a) {
@@ -337,8 +327,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
               code_pairs<kBits, kMoved>(&w[h][i * (kBits / 4)], element[h] + f * (16 * kFlush) + i * 8, p, a[h]);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
-              mma(acc[n], a[0][0], a[1][0], a[0][1], a[1][1], xf[j][n].x, xf[j][n].y);
-              mma(acc[n], a[0][2], a[1][2], a[0][3], a[1][3], xf[j][n].z, xf[j][n].w);
+              mma_16x8x16(acc[n], a[0][0], a[1][0], a[0][1], a[1][1], xf[j][n].x, xf[j][n].y);
+              mma_16x8x16(acc[n], a[0][2], a[1][2], a[0][3], a[1][3], xf[j][n].z, xf[j][n].w);
             }
           }
           if (c0 + f * kFlush * 16 < width) {
@@ -407,14 +397,11 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   sp.tiles = (int)((p.d.output_width + 15) / 16);
   constexpr int smem = smem_bytes<kBits, kN, kFlush>();
   static_assert(2 * (smem + 1024) <= 228 * 1024, "two blocks on an SM");
-  static bool attr[64];
+  static SharedMemorySetup setup;
   int dev = 0;
-  ENNX_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-  if (dev < 0 || dev >= 64) return set_error(ENNX_B200_UNSUPPORTED, "device index %d out of range", dev);
-  if (!attr[dev]) {
-    ENNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "packed tiles smem");
-    attr[dev] = true;
-  }
+  int* status = nullptr;
+  ENNX_TRY(serving_device(&dev, &status));
+  ENNX_TRY(allow_shared_memory(setup, dev, kernel, smem));
   const int blocks = (sp.tiles + sp.row_warps - 1) / sp.row_warps, cap = 2 * sm_count();
   kernel<<<(unsigned)(blocks < cap ? blocks : cap), 32 * kWarps, smem, s>>>(p, sp);
   ENNX_LAUNCH_CHECK("packed tiles");

@@ -154,6 +154,38 @@ def packed_linear(x: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, 
     return out
 
 
+# A serving call lasts a few microseconds on the device, so the checks below
+# read each tensor's attributes once and pass addresses as plain integers.
+
+def _here(what: str, first: torch.Tensor, *ts) -> int:
+    """The current device; every tensor given has to live on it."""
+    device = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != device:
+            _check_dev(first, t)
+            raise ValueError(f"{what}: tensors are on {first.device} and {t.device}")
+    _check_dev(first)
+    if device != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors are on {first.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return device
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _head_rows(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, heads, row stride) of bf16 [rows, heads, 128] whose heads are contiguous within a row."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[2] != 128:
+        raise ValueError(f"{what}: {name} must be bfloat16 [rows, heads, 128]")
+    rows, heads, _ = t.shape
+    ld, between, inner = t.stride()
+    if inner != 1 or (between != 128 and heads > 1):
+        raise ValueError(f"{what}: the heads of {name} must be contiguous within a row")
+    return rows, heads, ld if rows > 1 else heads * 128  # the stride of one row is never used
+
+
 def packed_linear_decode(x: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
                          linear: _abi.PackedLinear, seed: tuple[int, int, int] = (0, 0, 0),
                          out: torch.Tensor | None = None) -> torch.Tensor:
@@ -161,24 +193,27 @@ def packed_linear_decode(x: torch.Tensor, weights: torch.Tensor, scales: torch.T
     ``ennx_b200_packed_linear_decode``): any widths and group size, weights not
     rounded to bf16.  The arenas must hold the whole linear."""
     what = "packed_linear_decode"
-    _check_here(what, x, weights, scales, biases, out)
-    inp, n = linear.input_width, linear.output_width
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != inp or not x.is_contiguous():
+    device = _here(what, x, weights, scales, biases, out)
+    inp, n, bits, group = linear.input_width, linear.output_width, linear.bits, linear.group_size
+    if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != inp or not x.is_contiguous():
         raise ValueError(f"{what}: x must be contiguous bfloat16 [tokens, input_width]")
-    if weights.dtype != torch.uint8 or scales.dtype != torch.float32 or biases.dtype != torch.float32 or \
+    if weights.dtype is not torch.uint8 or scales.dtype is not torch.float32 or \
+            biases.dtype is not torch.float32 or \
             not (weights.is_contiguous() and scales.is_contiguous() and biases.is_contiguous()):
         raise ValueError(f"{what}: arenas must be contiguous uint8 codes and float32 scales and biases")
-    if linear.bits in (4, 8) and linear.group_size:
-        groups = n * -(-inp // linear.group_size)
-        if linear.byte_offset + n * ((inp * linear.bits + 7) // 8) > weights.numel() or \
+    tokens = x.shape[0]
+    if group and (bits == 4 or bits == 8):
+        groups = n * -(-inp // group)
+        if linear.byte_offset + n * ((inp * bits + 7) // 8) > weights.numel() or \
                 linear.scale_offset + groups > scales.numel() or linear.bias_offset + groups > biases.numel():
             raise ValueError(f"{what}: the linear exceeds its arenas")
     if out is None:
-        out = torch.empty(x.shape[0], n, dtype=torch.bfloat16, device=x.device)
-    elif out.dtype != torch.bfloat16 or out.shape != (x.shape[0], n) or not out.is_contiguous():
+        out = torch.empty((tokens, n), dtype=torch.bfloat16, device=x.device)
+    elif out.dtype is not torch.bfloat16 or out.shape != (tokens, n) or not out.is_contiguous():
         raise ValueError(f"{what}: out must be contiguous bfloat16 [tokens, output_width]")
-    _abi.call("ennx_b200_packed_linear_decode", _ptr(x), x.shape[0], _ptr(weights), _ptr(scales), _ptr(biases),
-              ctypes.byref(linear), _abi.PerturbSeed(*seed), _ptr(out), _stream())
+    _abi.check(_abi.lib().ennx_b200_packed_linear_decode(
+        x.data_ptr(), tokens, weights.data_ptr(), scales.data_ptr(), biases.data_ptr(), ctypes.byref(linear),
+        _abi.PerturbSeed(*seed), out.data_ptr(), _raw_stream(device)), what)
     return out
 
 
@@ -219,24 +254,32 @@ def moe_layer_decode(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.T
     bound by the bytes of the picked experts' weights.  x and residual bf16
     [tokens, hidden], weights as for ``moe_layer``; all contiguous."""
     what = "moe_layer_decode"
-    _check_here(what, x, w_router, w_gate_up, w_down, residual, out)
+    device = _here(what, x, w_router, w_gate_up, w_down, residual, out)
+    if x.dim() != 2 or w_gate_up.dim() != 3:
+        raise ValueError(f"{what}: x must be [tokens, H], w_gate_up [E, 2 I, H]")
     T, H = x.shape
     E, I2, _ = w_gate_up.shape
-    if w_router.shape != (E, H) or w_gate_up.shape != (E, I2, H) or w_down.shape != (E, H, I2 // 2) or I2 % 2:
+    if w_router.shape != (E, H) or w_gate_up.shape[2] != H or w_down.shape != (E, H, I2 // 2) or I2 % 2:
         raise ValueError(f"{what}: weights must be [E, H], [E, 2 I, H] and [E, H, I] for x [tokens, H]")
-    if out is None:
-        out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
     for t in (x, w_router, w_gate_up, w_down, residual, out):
-        if t is not None and (t.dtype != torch.bfloat16 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.bfloat16 or not t.is_contiguous()):
             raise ValueError(f"{what}: operands must be contiguous bfloat16")
-    if out.shape != (T, H) or (residual is not None and residual.shape != (T, H)):
+    if (out is not None and out.shape != (T, H)) or (residual is not None and residual.shape != (T, H)):
         raise ValueError(f"{what}: residual and out must have the shape of x")
-    idx = torch.empty(T, top_k, dtype=torch.int32, device=x.device) if return_routing else None
-    gate = torch.empty(T, top_k, dtype=torch.float32, device=x.device) if return_routing else None
-    n = _abi.lib().ennx_b200_moe_layer_decode_workspace_size(T, E, top_k, I2 // 2)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _abi.call("ennx_b200_moe_layer_decode", _ptr(x), _ptr(w_router), _ptr(w_gate_up), _ptr(w_down), T, H, E, top_k,
-              I2 // 2, _ptr(residual), _ptr(out), _ptr(idx), _ptr(gate), _ptr(ws), n, _stream())
+    where = x.device
+    if out is None:
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=where)
+    idx = gate = None
+    if return_routing:
+        idx = torch.empty((T, top_k), dtype=torch.int32, device=where)
+        gate = torch.empty((T, top_k), dtype=torch.float32, device=where)
+    lib = _abi.lib()
+    n = lib.ennx_b200_moe_layer_decode_workspace_size(T, E, top_k, I2 // 2)
+    ws = torch.empty(n, dtype=torch.uint8, device=where) if n else None
+    _abi.check(lib.ennx_b200_moe_layer_decode(
+        x.data_ptr(), w_router.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), T, H, E, top_k, I2 // 2,
+        None if residual is None else residual.data_ptr(), out.data_ptr(), idx.data_ptr() if return_routing else None,
+        gate.data_ptr() if return_routing else None, ws.data_ptr() if n else None, n, _raw_stream(device)), what)
     return (out, idx, gate) if return_routing else out
 
 
@@ -251,24 +294,6 @@ def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope_theta:
     return o
 
 
-def _check_here(what: str, *ts) -> None:
-    """Every tensor given lives on the current CUDA device."""
-    _check_dev(*ts)
-    here = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.device.index != here:
-            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
-
-
-def _head_rows(what: str, name: str, t: torch.Tensor) -> int:
-    """Row stride of bf16 [rows, heads, 128] whose heads are contiguous within a row."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != 128:
-        raise ValueError(f"{what}: {name} must be bfloat16 [rows, heads, 128]")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128):
-        raise ValueError(f"{what}: the heads of {name} must be contiguous within a row")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * 128
-
-
 def gqa_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                          rope_theta: float = 1e6, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal GQA attention over packed prompts (see ``ennx_b200_gqa_attention_packed``).
@@ -280,29 +305,35 @@ def gqa_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     Rows behind the last sequence are left as they are (undefined when out is
     None)."""
     what = "gqa_attention_packed"
-    _check_here(what, q, k, v, cu_seqlens, out)
-    ldq, ldk, ldv = _head_rows(what, "q", q), _head_rows(what, "k", k), _head_rows(what, "v", v)
-    if k.shape != v.shape or k.shape[0] != q.shape[0]:
+    device = _here(what, q, k, v, cu_seqlens, out)
+    rows, hq, ldq = _head_rows(what, "q", q)
+    krows, hkv, ldk = _head_rows(what, "k", k)
+    vrows, vheads, ldv = _head_rows(what, "v", v)
+    if krows != rows or vrows != rows or vheads != hkv:
         raise ValueError(f"{what}: q, k and v must have the same rows, k and v the same heads")
-    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or \
+    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or \
             not cu_seqlens.is_contiguous():
         raise ValueError(f"{what}: cu_seqlens must be contiguous int32 [sequences + 1]")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape:
-        raise ValueError(f"{what}: out must have the shape of q")
-    _abi.call("ennx_b200_gqa_attention_packed", _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, _ptr(out),
-              _head_rows(what, "out", out), _ptr(cu_seqlens), cu_seqlens.numel() - 1, q.shape[0], q.shape[1],
-              k.shape[1], rope_theta, _stream())
+        out, ldo = torch.empty((rows, hq, 128), dtype=torch.bfloat16, device=q.device), hq * 128
+    else:
+        orows, oheads, ldo = _head_rows(what, "out", out)
+        if orows != rows or oheads != hq:
+            raise ValueError(f"{what}: out must have the shape of q")
+    _abi.check(_abi.lib().ennx_b200_gqa_attention_packed(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, cu_seqlens.data_ptr(),
+        cu_seqlens.numel() - 1, rows, hq, hkv, rope_theta, _raw_stream(device)), what)
     return out
 
 
-def _cache_strides(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
-    """(sequence, token, head) strides of a bf16 cache [batch, room, heads, 128]."""
-    if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[3] != 128 or t.stride(3) != 1:
+def _cache(what: str, name: str, t: torch.Tensor) -> tuple[torch.Size, tuple[int, int, int]]:
+    """Shape and (sequence, token, head) strides of a bf16 cache [batch, room, heads, 128]."""
+    shape = t.shape
+    if t.dtype is not torch.bfloat16 or len(shape) != 4 or shape[3] != 128 or t.stride(3) != 1:
         raise ValueError(f"{what}: {name} must be bfloat16 [batch, room, heads, 128] with contiguous heads")
+    st = t.stride()
     # the stride of a dimension of one entry is never used
-    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3))
+    return shape, (st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0, st[2] if shape[2] > 1 else 0)
 
 
 def gqa_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -318,32 +349,39 @@ def gqa_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     lengths - 1 (None: the caches hold them).  rope_theta > 0 rotates q (not in
     place) and k to position lengths - 1."""
     what = "gqa_attention_decode"
-    _check_here(what, q, k_cache, v_cache, lengths, k, v, out)
-    ldq = _head_rows(what, "q", q)
-    ks, vs = _cache_strides(what, "k_cache", k_cache), _cache_strides(what, "v_cache", v_cache)
-    batch, room, hkv, _ = k_cache.shape
-    if v_cache.shape != k_cache.shape or q.shape[0] != batch:
+    device = _here(what, q, k_cache, v_cache, lengths, k, v, out)
+    rows, hq, ldq = _head_rows(what, "q", q)
+    shape, ks = _cache(what, "k_cache", k_cache)
+    vshape, vs = _cache(what, "v_cache", v_cache)
+    batch, room, hkv, _ = shape
+    if vshape != shape or rows != batch:
         raise ValueError(f"{what}: q and both caches must have the same batch, the caches the same shape")
-    if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.numel() != batch or \
+            not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths must be contiguous int32 [batch]")
     if (k is None) != (v is None):
         raise ValueError(f"{what}: k and v come together")
-    ldk = ldv = 0
+    kp = vp = ldk = ldv = 0
     if k is not None:
-        ldk, ldv = _head_rows(what, "k", k), _head_rows(what, "v", v)
-        if k.shape != (batch, hkv, 128) or v.shape != k.shape:
+        krows, kheads, ldk = _head_rows(what, "k", k)
+        vrows, vheads, ldv = _head_rows(what, "v", v)
+        if krows != batch or vrows != batch or kheads != hkv or vheads != hkv:
             raise ValueError(f"{what}: k and v must be [batch, Hkv, 128]")
+        kp, vp = k.data_ptr(), v.data_ptr()
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape:
-        raise ValueError(f"{what}: out must have the shape of q")
-    p = _abi.DecodeAttention(q.data_ptr(), ldq, None if k is None else k.data_ptr(), ldk,
-                             None if v is None else v.data_ptr(), ldv, k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs,
-                             lengths.data_ptr(), out.data_ptr(), _head_rows(what, "out", out), batch, room, q.shape[1],
-                             hkv)
-    n = _abi.lib().ennx_b200_gqa_attention_decode_workspace_size(batch, room, q.shape[1], hkv)
+        out, ldo = torch.empty((batch, hq, 128), dtype=torch.bfloat16, device=q.device), hq * 128
+    else:
+        orows, oheads, ldo = _head_rows(what, "out", out)
+        if orows != batch or oheads != hq:
+            raise ValueError(f"{what}: out must have the shape of q")
+    lib = _abi.lib()
+    n = lib.ennx_b200_gqa_attention_decode_workspace_size(batch, room, hq, hkv)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    _abi.call("ennx_b200_gqa_attention_decode", ctypes.byref(p), rope_theta, _ptr(ws), n, _stream())
+    params = _abi.DECODE_ATTENTION.pack(q.data_ptr(), ldq, kp, ldk, vp, ldv, k_cache.data_ptr(), *ks,
+                                        v_cache.data_ptr(), *vs, lengths.data_ptr(), out.data_ptr(), ldo, batch, room,
+                                        hq, hkv)
+    _abi.check(lib.ennx_b200_gqa_attention_decode(params, rope_theta, ws.data_ptr() if n else None, n,
+                                                  _raw_stream(device)), what)
     return out
 
 
