@@ -9,13 +9,13 @@
 // the grouped GEMM path of the full layer spends its time on permuting rows
 // and on tiles of 128 tokens instead.
 //
-// Three kernels in one programmatic-launch chain: router logits; gate/up
-// products with SwiGLU; down products with the weighted sum.  The last two
-// give every block an equal share of the weight rows whatever the routing is
-// (gate/up: an equal run of the picked experts' columns; down: an equal share
-// of the output rows over all picked experts, so a block owns its outputs and
-// sums the experts in a fixed order without atomics).  Each block derives the
-// routing from the logits itself, which costs less than another launch.
+// Three kernels in one programmatic-launch chain: router; gate/up products
+// with SwiGLU; down products with the weighted sum.  The last two give every
+// block an equal share of the weight rows whatever the routing is (gate/up: an
+// equal run of the picked experts' columns; down: an equal share of the output
+// rows over all picked experts, so a block owns its outputs and sums the
+// experts in a fixed order without atomics).  Each block sorts the picks by
+// expert for itself, about a microsecond, which costs less than another launch.
 //
 // Products run on m16n8k16 with weight rows as the 16 rows and tokens as the
 // 8 columns; each warp streams its own weight tiles through a ring of bulk
@@ -47,7 +47,8 @@ struct Layer {
   uint16_t* y;
   int* index;     // nullable
   float* gate;    // nullable
-  float* logits;  // [tokens][experts]
+  uint8_t* picks;  // [tokens][kTopK]
+  float* gates;    // [tokens][kTopK]
   uint16_t* act;  // [tokens * top_k][width], rows expert by expert
   int tokens, hidden, experts, top_k, width;
   int* status;
@@ -84,75 +85,12 @@ struct Ring {
 };
 
 // ---------------------------------------------------------------------------
-// router logits: block = 4 experts x 8 tokens, a thread 8 k at a time.  Each
-// logit is an fp32 sum over the threads' short chains (8 or 16 products at
-// hidden 2048) joined as a tree.
+// router: a cluster of 8 blocks takes 8 tokens; each block forms the logits of
+// an eighth of the experts, block r gathers those of token r over distributed
+// shared memory and picks.  A logit is an fp32 sum: a thread's chain of 8
+// products (16 at hidden 4096), joined as a tree.
 // ---------------------------------------------------------------------------
-constexpr int kRE = 4, kRT = 8;
-__global__ void __launch_bounds__(kThreads) token_router_kernel(const __grid_constant__ Layer p) {
-  launch_dependents();
-  __shared__ float part[kWarps][kRE][kRT];
-  const int e0 = blockIdx.x * kRE, t0 = blockIdx.y * kRT;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float acc[kRE][kRT] = {};
-  for (int c = threadIdx.x; c < p.hidden / 8; c += kThreads) {
-    uint4 w[kRE];
-#pragma unroll
-    for (int e = 0; e < kRE; ++e)
-      w[e] = e0 + e < p.experts ? ldg_stream_v4(p.w_router + (long long)(e0 + e) * p.hidden + c * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int t = 0; t < kRT; ++t) {
-      if (t0 + t < p.tokens) {
-        const uint4 xv = __ldg(reinterpret_cast<const uint4*>(p.x + (long long)(t0 + t) * p.hidden + c * 8));
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-        for (int e = 0; e < kRE; ++e) {
-          const uint32_t ww[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc[e][t] = fmaf(__uint_as_float(xw[j] << 16), __uint_as_float(ww[j] << 16), acc[e][t]);
-            acc[e][t] = fmaf(__uint_as_float(xw[j] & 0xffff0000u), __uint_as_float(ww[j] & 0xffff0000u), acc[e][t]);
-          }
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < kRT; ++t)
-    if (t0 + t < p.tokens) {
-#pragma unroll
-      for (int e = 0; e < kRE; ++e) {
-        float v = acc[e][t];
-#pragma unroll
-        for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-        if (lane == 0) part[warp][e][t] = v;
-      }
-    }
-  __syncthreads();
-  const int e = threadIdx.x / kRT, t = threadIdx.x % kRT;
-  if (e < kRE && e0 + e < p.experts && t0 + t < p.tokens) {
-    float v[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) v[w] = part[w][e][t];
-    p.logits[(t0 + t) * p.experts + e0 + e] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-  }
-}
-
-// ---------------------------------------------------------------------------
-// routing of all tokens, by every block for itself
-// ---------------------------------------------------------------------------
-struct Plan {
-  float gates[kTokens * kTopK];     // of pick r of token t at t * kTopK + r
-  uint8_t picks[kTokens * kTopK];
-  uint32_t takers[kExperts][2];     // tokens that picked an expert, a bit each
-  int active;                       // experts that some token picked
-  uint8_t expert[kExperts];         // active expert a
-  uint16_t first[kExperts + 1];     // its first slot; slots run expert by expert, token by token
-  uint16_t slot[kTokens * kTopK];   // t * kTopK + r of a slot
-  int scan[kWarps][2];
-  __device__ __forceinline__ int token(int i) const { return slot[i] / kTopK; }
-  __device__ __forceinline__ float gate(int i) const { return gates[slot[i]]; }
-};
+constexpr int kCluster = 8;
 
 // NaN sorts below everything, so that it never displaces a number
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -160,88 +98,190 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return v != v ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__device__ void make_plan(const Layer& p, Plan& s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kPer = kExperts / 32;
-  for (int i = threadIdx.x; i < 2 * kExperts; i += kThreads) s.takers[i >> 1][i & 1] = 0u;
-  for (int t = warp; t < p.tokens; t += kWarps) {
-    float v[kPer];
-    uint32_t key[kPer];  // 0 with `taken`: picked already or no expert
-    uint32_t taken = 0;
+// Sum of N values over the lanes, N a power of two up to 64: each exchange
+// halves the values a lane holds while it can, so lane l ends with the N / 32
+// values from l * N / 32 on (N < 32: value l * N / 32, in all its lanes).
+template <int N, int kOff = 16>
+__device__ __forceinline__ void spread_sum(float* v, int lane) {
+  if constexpr (kOff > 0) {
+    if constexpr (N > 1) {
+      const bool upper = lane & kOff;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = i * 32 + lane;
-      v[i] = e < p.experts ? __ldcg(p.logits + t * p.experts + e) : 0.0f;
-      key[i] = order_key(v[i]);
-      if (e >= p.experts) taken |= 1u << i;
+      for (int i = 0; i < N / 2; ++i) {
+        const float send = upper ? v[i] : v[i + N / 2], keep = upper ? v[i + N / 2] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, kOff);
+      }
+      spread_sum<N / 2, kOff / 2>(v, lane);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], kOff);
+      spread_sum<1, kOff / 2>(v, lane);
     }
-    float top = 0.0f, sum = 0.0f, mine = 0.0f;
-    int pick = 0;
-    for (int r = 0; r < p.top_k; ++r) {
-      uint32_t best = 0;
-      int at = 0x7fffffff;
+  }
+}
+
+template <int kT>  // tokens of a cluster
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
+    token_router_kernel(const __grid_constant__ Layer p) {
+  constexpr int kE = 8, kV = kE * kT;  // experts at a time, sums at a time
+  constexpr int kHeld = kV >= 32 ? kV / 32 : 1, kRepeat = kV >= 32 ? 1 : 32 / kV;  // values a lane ends with, lanes of a value
+  __shared__ float part[kWarps][kV];
+  __shared__ float logits[kExperts];
+  launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster_ctarank();
+  const int t0 = (int)(blockIdx.x / kCluster) * kT;
+  const int per = (p.experts + kCluster - 1) / kCluster, e_end = min(p.experts, (rank + 1) * per);
+  for (int e0 = rank * per; e0 < e_end; e0 += kE) {
+    float acc[kV] = {};
+    for (int c = threadIdx.x; c < p.hidden / 8; c += kThreads) {
+      uint4 x[kT];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i * 32 < p.experts && !(taken >> i & 1u) && (at == 0x7fffffff || key[i] > best)) {
-          best = key[i];
-          at = i * 32 + lane;
-        }
-      const uint32_t m = __reduce_max_sync(0xffffffffu, at == 0x7fffffff ? 0u : best);
-      const int e = __reduce_min_sync(0xffffffffu, at != 0x7fffffff && best == m ? at : 0x7fffffff);
-      float val = 0.0f;
+      for (int t = 0; t < kT; ++t)
+        x[t] = t0 + t < p.tokens ? __ldg(reinterpret_cast<const uint4*>(p.x + (long long)(t0 + t) * p.hidden + c * 8))
+                                 : make_uint4(0, 0, 0, 0);
+      uint4 w[kE];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (e == i * 32 + lane) {
-          taken |= 1u << i;
-          val = v[i];
+      for (int e = 0; e < kE; ++e)
+        w[e] = e0 + e < e_end ? ldg_stream_v4(p.w_router + (long long)(e0 + e) * p.hidden + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const uint32_t ww[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          const uint32_t xw[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[e * kT + t] = fmaf(__uint_as_float(xw[j] << 16), __uint_as_float(ww[j] << 16), acc[e * kT + t]);
+            acc[e * kT + t] = fmaf(__uint_as_float(xw[j] & 0xffff0000u), __uint_as_float(ww[j] & 0xffff0000u), acc[e * kT + t]);
+          }
         }
-      val = __shfl_sync(0xffffffffu, val, e & 31);
-      if (r == 0) top = val;
-      const float g = expf(val - top);
-      sum += g;
-      if (lane == r) {
-        mine = g;
-        pick = e;
       }
     }
-    if (lane < p.top_k) {
-      s.picks[t * kTopK + lane] = (uint8_t)pick;
-      s.gates[t * kTopK + lane] = mine / sum;
+    spread_sum<kV>(acc, lane);
+    __syncthreads();  // the sums of the experts before have been read
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (lane % kRepeat == 0) part[warp][lane / kRepeat * kHeld + i] = acc[i];
+    __syncthreads();
+    if (threadIdx.x < kV) {
+      float v[kWarps];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) v[w] = part[w][threadIdx.x];
+      const float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      const int e = e0 + (int)threadIdx.x / kT, t = (int)threadIdx.x % kT;
+      if (e < e_end)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(&logits[e], (uint32_t)t)), "f"(sum) : "memory");
     }
   }
+  cluster_sync();  // every block has all logits of its token; nothing remote is touched behind it
+  const int tok = t0 + rank;
+  if (rank >= kT || tok >= p.tokens || warp != 0) return;
+  constexpr int kPer = kExperts / 32;
+  float v[kPer];
+  uint32_t key[kPer], taken = 0;  // taken: picked already, or no expert
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = i * 32 + lane;
+    v[i] = e < p.experts ? logits[e] : 0.0f;
+    key[i] = order_key(v[i]);
+    if (e >= p.experts) taken |= 1u << i;
+  }
+  float top = 0.0f, mine = 0.0f;
+  int pick = 0;
+  for (int r = 0; r < p.top_k; ++r) {
+    uint32_t best = 0;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i * 32 < p.experts && !(taken >> i & 1u) && (at == 0x7fffffff || key[i] > best)) {
+        best = key[i];
+        at = i * 32 + lane;
+      }
+    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+    const int e = __reduce_min_sync(0xffffffffu, best == m ? at : 0x7fffffff);
+    if ((e & 31) == lane) taken |= 1u << (e >> 5);
+    if (lane == r) pick = e;
+  }
+  if (lane < p.top_k) mine = logits[pick];
+  top = __shfl_sync(0xffffffffu, mine, 0);
+  const float g = lane < p.top_k ? expf(mine - top) : 0.0f;
+  float sum = g;
+#pragma unroll
+  for (int off = 4; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);  // lanes 0 .. 7
+  if (lane < p.top_k) {
+    p.picks[tok * kTopK + lane] = (uint8_t)pick;
+    p.gates[tok * kTopK + lane] = g / sum;
+    if (p.index) p.index[tok * p.top_k + lane] = pick;
+    if (p.gate) p.gate[tok * p.top_k + lane] = g / sum;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// picks of all tokens sorted by expert, by every block for itself
+// ---------------------------------------------------------------------------
+struct Plan {
+  float gates[kTokens * kTopK];  // of pick r of token t at t * kTopK + r
+  uint32_t takers[kExperts][2];  // tokens that picked an expert, a bit each
+  uint16_t start[kExperts];      // first slot of an expert
+  int active;                    // experts that some token picked
+  uint8_t expert[kExperts];      // active expert a
+  uint16_t first[kExperts + 1];  // its first slot; slots run expert by expert, token by token
+  uint16_t slot[kTokens * kTopK];  // t * kTopK + r of a slot
+  int scan[kWarps][2];
+  __device__ __forceinline__ int token(int i) const { return slot[i] / kTopK; }
+  __device__ __forceinline__ float gate(int i) const { return gates[slot[i]]; }
+};
+
+// by every thread of a block; those behind the first kThreads only keep step
+__device__ __forceinline__ void make_plan(const Layer& p, Plan& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool works = threadIdx.x < kThreads;
+  constexpr int kMine = kTokens * kTopK / kThreads;
+  int pick[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {  // pick r of token t, -1 behind the last
+    const int at = threadIdx.x + i * kThreads;
+    const bool ok = works && at / kTopK < p.tokens && at % kTopK < p.top_k;
+    pick[i] = ok ? (int)__ldcg(p.picks + at) : -1;
+    if (ok) s.gates[at] = __ldcg(p.gates + at);
+  }
+  static_assert(kThreads == kExperts, "a thread per expert");
+  if (works) s.takers[threadIdx.x][0] = s.takers[threadIdx.x][1] = 0u;
   __syncthreads();
-  for (int i = threadIdx.x; i < p.tokens * p.top_k; i += kThreads) {
-    const int t = i / p.top_k, e = s.picks[t * kTopK + i % p.top_k];
-    atomicOr(&s.takers[e][t >> 5], 1u << (t & 31));
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int t = (threadIdx.x + i * kThreads) / kTopK;
+    if (pick[i] >= 0) atomicOr(&s.takers[pick[i]][t >> 5], 1u << (t & 31));
   }
   __syncthreads();
-  static_assert(kThreads == kExperts, "a thread per expert");
-  const uint32_t lo = s.takers[threadIdx.x][0], hi = s.takers[threadIdx.x][1];
-  const int n = __popc(lo) + __popc(hi);
+  const int n = works ? __popc(s.takers[threadIdx.x][0]) + __popc(s.takers[threadIdx.x][1]) : 0;
   int slots = n, actives = n > 0;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, slots, off), b = __shfl_up_sync(0xffffffffu, actives, off);
     if (lane >= off) { slots += a; actives += b; }
   }
-  if (lane == 31) { s.scan[warp][0] = slots; s.scan[warp][1] = actives; }
+  if (works && lane == 31) { s.scan[warp][0] = slots; s.scan[warp][1] = actives; }
   __syncthreads();
-  for (int w = 0; w < warp; ++w) { slots += s.scan[w][0]; actives += s.scan[w][1]; }
+#pragma unroll
+  for (int w = 0; w < kWarps - 1; ++w)
+    if (w < warp) { slots += s.scan[w][0]; actives += s.scan[w][1]; }
+  if (works) s.start[threadIdx.x] = (uint16_t)(slots - n);
   if (threadIdx.x == kThreads - 1) {
     s.active = actives;
     s.first[actives] = (uint16_t)slots;
   }
   if (n > 0) {
-    int slot = slots - n;
     s.expert[actives - 1] = (uint8_t)threadIdx.x;
-    s.first[actives - 1] = (uint16_t)slot;
-    for (int t = 0; t < p.tokens; ++t)
-      if ((t < 32 ? lo >> t : hi >> (t - 32)) & 1u) {
-        int at = t * kTopK;
-        for (int r = 0; r < p.top_k; ++r)
-          if (s.picks[t * kTopK + r] == threadIdx.x) at = t * kTopK + r;
-        s.slot[slot++] = (uint16_t)at;
-      }
+    s.first[actives - 1] = (uint16_t)(slots - n);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = threadIdx.x + i * kThreads, t = at / kTopK;
+    if (pick[i] >= 0) {
+      const uint32_t lo = s.takers[pick[i]][0], hi = s.takers[pick[i]][1], below = (1u << (t & 31)) - 1u;
+      s.slot[s.start[pick[i]] + (t < 32 ? __popc(lo & below) : __popc(lo) + __popc(hi & below))] = (uint16_t)at;
+    }
   }
   __syncthreads();
 }
@@ -270,13 +310,6 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
   wait_previous();
   launch_dependents();
   make_plan(p, s);
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < p.tokens * p.top_k; i += kThreads) {
-      const int at = i / p.top_k * kTopK + i % p.top_k;
-      if (p.index) p.index[i] = s.picks[at];
-      if (p.gate) p.gate[i] = s.gates[at];
-    }
-
   const long long columns = (long long)s.active * p.width;
   const long long begin = columns * blockIdx.x / gridDim.x, end = columns * (blockIdx.x + 1) / gridDim.x;
   if (begin >= end) return;
@@ -377,10 +410,11 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
         }
         const int col = now.c + g, slot = first + warp * 8 + 2 * t;
         if (col < now.c_end) {
-          // rounded to bf16 for the second product: at most 2^-8 of a value
+          // weighted here, so that the down products only add up, and rounded
+          // to bf16 for them: at most 2^-8 of a value
           uint16_t* h = p.act + (long long)slot * p.width + col;
-          if (slot < last) h[0] = f32_to_bf16_rne(v.x / (1.0f + expf(-v.x)) * v.z);
-          if (slot + 1 < last) h[p.width] = f32_to_bf16_rne(v.y / (1.0f + expf(-v.y)) * v.w);
+          if (slot < last) h[0] = f32_to_bf16_rne(s.gate(slot) * (v.x / (1.0f + expf(-v.x)) * v.z));
+          if (slot + 1 < last) h[p.width] = f32_to_bf16_rne(s.gate(slot + 1) * (v.y / (1.0f + expf(-v.y)) * v.w));
         }
       }
     }
@@ -393,146 +427,253 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
 // ---------------------------------------------------------------------------
 // down: a block owns an equal share of the output rows (kRows at a time: 14 of
 // the 16 of a product, 2048 rows over 148 blocks, keep the sums of 64 tokens
-// in shared memory beside the ring) over all picked experts; experts go round
-// the warps, a warp's tile is kRows rows x 256 k.
+// in shared memory beside the ring) over all picked experts.  Four warps copy
+// tiles in turn, one picked expert after the other: kRows weight rows x 768 k
+// and the activations of the expert's tokens (at expert width 768 both are
+// contiguous runs).  A warp issues a copy in 30 ns, so one warp alone would
+// hold the 15 copies of a tile to 1 us, twice their time on the bus.  The
+// eight others work in two teams that take every second tile: a tile's chain of
+// lookups, products and sums lasts longer than its bytes (0.74 us against 0.49
+// with one team of eight), so two are under way at a time.  A team splits its
+// tile's k and each warp keeps its own sums of all tokens, so nothing is joined
+// before the end.
+//
+// kDirect (at most kN * 8 tokens): the columns of a product are the tokens, an
+// expert's other columns are zero, and the sums stay in the accumulators over
+// all experts.  Otherwise the columns are the tokens that picked the expert and
+// are added to sums in shared memory, all of a lane's old values read before
+// the first is written.
 // ---------------------------------------------------------------------------
-constexpr int kRows = 14;
+constexpr int kRows = 14, kPassChunks = 24, kWeightPitch = kPassChunks * 64 + 64, kActPitch = kPassChunks * 64;
+constexpr int kTeams = 2, kTeam = kWarps / kTeams;
+constexpr int kMine = kPassChunks / kTeam;  // chunks of a warp in a tile
+constexpr int kCopyWarps = 4, kDownThreads = kThreads + 32 * kCopyWarps;
+template <int kN>
 struct DownShared {
-  uint8_t ring[kWarps][kStages][tile_bytes(kRows)];
-  uint64_t full[kWarps][kStages];
+  // Tiles in the ring.  A waiter tells two phases of a barrier apart only by
+  // parity, so the same copying warp and the same team have to serve a stage
+  // every time: the depth is a multiple of both numbers.
+  static constexpr int kDepth = 4;
+  static_assert(kDepth % kCopyWarps == 0 && kDepth % kTeams == 0, "every phase of a stage is seen by its waiters");
+  struct Tile {
+    uint8_t weights[kRows * kWeightPitch];
+    uint8_t act[kN * 8 * kActPitch];
+  } ring[kDepth];
+  uint64_t full[kDepth], free[kDepth];
   Plan plan;
   float sums[1];  // [warp][token][kRows]
 };
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
 
-template <int kN>
-__global__ void __launch_bounds__(kThreads, 1) token_down_kernel(const __grid_constant__ Layer p) {
+template <int kN, bool kDirect>
+__global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __grid_constant__ Layer p) {
+  using Shared = DownShared<kN>;
+  constexpr int kDepth = Shared::kDepth;
   extern __shared__ __align__(128) uint8_t smem[];
-  DownShared& sh = *reinterpret_cast<DownShared*>(smem);
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
   Plan& s = sh.plan;
-  const int span = p.tokens * kRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  float* sums = sh.sums + warp * span;
-  Ring ring;
-  ring.init(sh.ring[warp][0], sh.full[warp], tile_bytes(kRows), lane);
+  if (threadIdx.x < kDepth) {
+    mbar_init(&sh.full[threadIdx.x], 2);  // the weights' bytes and the activations'
+    mbar_init(&sh.free[threadIdx.x], kTeam);
+    fence_barrier_init();
+    fence_proxy_async();
+  }
   // the router grid has finished (every gate/up block waited for it before it
   // let this grid start), so the routing and the first weights can be fetched
   // while the gate/up products are still running
   make_plan(p, s);
-  const int chunks = p.width / kChunk, passes = (chunks + kTileChunks - 1) / kTileChunks;
+  const int chunks = p.width / kChunk, passes = (chunks + kPassChunks - 1) / kPassChunks;
   const int row_begin = (int)((long long)p.hidden * blockIdx.x / gridDim.x);
   const int row_end = (int)((long long)p.hidden * (blockIdx.x + 1) / gridDim.x);
-  bool waited = false;
 
-  for (int row0 = row_begin; row0 < row_end; row0 += kRows) {
-    const int rows = min(kRows, row_end - row0);
-    struct Walk {
-      int a, group, pass;
+  // tiles in order: 14 rows, expert, group of kN * 8 of its tokens, k pass
+  struct Walk {
+    int row0, a, first, pass;  // first: slot of the group's first token
+  };
+  auto next = [&](Walk& w) -> bool {  // false behind the last tile of these rows
+    if (++w.pass < passes) return true;
+    w.pass = 0;
+    w.first += kN * 8;
+    if (w.first < s.first[w.a + 1]) return true;
+    if (++w.a == s.active) return false;
+    w.first = s.first[w.a];
+    return true;
+  };
+  if (warp >= kWarps) {
+    bool waited = false;
+    auto copy_act = [&](const Walk& w, int at) {
+      const int rows = min(kN * 8, s.first[w.a + 1] - w.first), bytes = min(kPassChunks, chunks - w.pass * kPassChunks) * 64;
+      uint64_t* full = &sh.full[at % kDepth];
+      const uint32_t dst = smem_u32(sh.ring[at % kDepth].act);
+      const uint16_t* src = p.act + (long long)w.first * p.width + w.pass * kPassChunks * kChunk;
+      if (lane == 0) mbar_arrive_expect_tx(full, rows * bytes);
+      __syncwarp();
+      if (passes == 1 && bytes == kActPitch) {
+        if (lane == 0) bulk_copy(dst, src, rows * bytes, full);
+      } else if (lane < rows) {
+        bulk_copy(dst + lane * kActPitch, src + (long long)lane * p.width, bytes, full);
+      }
     };
-    auto next = [&](Walk& w) -> bool {
-      if (++w.pass < passes) return true;
-      w.pass = 0;
-      if (++w.group * kN * 8 < s.first[w.a + 1] - s.first[w.a]) return true;
-      w.group = 0;
-      w.a += kWarps;
-      return w.a < s.active;
-    };
-    Walk ahead{warp, 0, 0}, now = ahead;
-    bool more = warp < s.active;
-    auto fetch = [&] {
-      if (!more) return;
-      const int k0 = ahead.pass * kTileChunks, n = min(kTileChunks, chunks - k0);
-      const uint16_t* w = p.w_down + ((long long)s.expert[ahead.a] * p.hidden + row0 + lane) * p.width + k0 * kChunk;
-      ring.fetch(w, lane < rows, n * 64, lane);
-      more = next(ahead);
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch();
-    for (int i = lane; i < span; i += 32) sums[i] = 0.0f;
-    if (!waited) {
-      wait_previous();  // the activations are complete and visible
-      waited = true;
+    Walk held{}, w{row_begin, 0, 0, 0};
+    int held_at = -1;
+    for (int at = 0; w.row0 < row_end; ++at) {
+      if (at % kCopyWarps == warp - kWarps) {
+        const int stage = at % kDepth, bytes = min(kPassChunks, chunks - w.pass * kPassChunks) * 64;
+        const int rows = min(kRows, row_end - w.row0);
+        const uint16_t* src = p.w_down + ((long long)s.expert[w.a] * p.hidden + w.row0 + lane) * p.width + w.pass * kPassChunks * kChunk;
+        // a second tile of this warp: what the first one left is sent before it can wait for the ring
+        if (held_at >= 0) {
+          wait_previous();
+          waited = true;
+          copy_act(held, held_at);
+          held_at = -1;
+        }
+        if (!mbar_wait(&sh.free[stage], ((at / kDepth) & 1) ^ 1u, p.status)) return;
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[stage], rows * bytes);
+        __syncwarp();
+        if (lane < rows) bulk_copy(smem_u32(sh.ring[stage].weights) + lane * kWeightPitch, src, bytes, &sh.full[stage]);
+        if (waited) {
+          copy_act(w, at);
+        } else {
+          held = w;
+          held_at = at;
+        }
+      }
+      if (!next(w)) w = Walk{w.row0 + kRows, 0, 0, 0};
     }
+    if (held_at >= 0) {
+      wait_previous();
+      copy_act(held, held_at);
+    }
+    return;
+  }
+
+  const int span = p.tokens * kRows;
+  float* sums = sh.sums + warp * span;
+  const uint32_t mine = smem_u32(sums) + g * 4;
+  if constexpr (!kDirect) {
+    for (int i = lane; i < span; i += 32) sums[i] = 0.0f;
     __syncwarp();
-    float acc[kN][4];
-    while (warp < s.active) {
-      const int first = s.first[now.a] + now.group * kN * 8, last = s.first[now.a + 1];
-      const int k0 = now.pass * kTileChunks, n_chunks = min(kTileChunks, chunks - k0);
-      uint4 hf[kTileChunks][kN];
+  }
+  wait_previous();  // no grid of the chain ends before the one it follows
+  bool bad = false;  // a wait gave up: later ones are not tried again, the results are void
+  int at = 0;
+  for (int row0 = row_begin; row0 < row_end; row0 += kRows) {
+    float acc[kN][4] = {};
+    Walk w{row0, 0, 0, 0};
+    bool more = true;
+    for (; more; ++at, more = next(w)) {
+      if (at % kTeams != warp / kTeam) continue;
+      const int stage = at % kDepth, n_chunks = chunks - w.pass * kPassChunks, first = w.first, last = s.first[w.a + 1];
+      // where this lane's column of the activations lies; columns without a
+      // token read row 0 and are replaced by zeros
+      uint32_t column[kN];
+      bool live[kN], any[kN];  // any: some column of the block has a token
+      uint32_t to[kN][2];
+      float old[kN][4];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        const bool ok = first + n * 8 + g < last;
-        const uint16_t* h = p.act + (ok ? (long long)(first + n * 8 + g) * p.width : 0) + k0 * kChunk + t * 8;
+        if constexpr (kDirect) {
+          const uint32_t takers = s.takers[s.expert[w.a]][0];
+          live[n] = takers >> (n * 8 + g) & 1u;
+          any[n] = takers >> (n * 8) & 255u;
+          column[n] = live[n] ? __popc(takers & ((1u << (n * 8 + g)) - 1u)) : 0u;
+        } else {
+          live[n] = first + n * 8 + g < last;
+          any[n] = first + n * 8 < last;
+          column[n] = live[n] ? n * 8 + g : 0u;
 #pragma unroll
-        for (int j = 0; j < kTileChunks; ++j)
-          hf[j][n] = ok && j < n_chunks ? __ldcg(reinterpret_cast<const uint4*>(h + j * kChunk)) : make_uint4(0, 0, 0, 0);
+          for (int e = 0; e < 2; ++e) {
+            const int slot = first + n * 8 + 2 * t + e;
+            to[n][e] = slot < last ? mine + s.token(slot) * (kRows * 4) : 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[n][j] = old[n][j] = 0.0f;
+            if (to[n][j & 1] && (j < 2 || g < kRows - 8)) old[n][j] = lds_f32(to[n][j & 1] + 32 * (j >> 1));
+          }
+        }
       }
-      if (now.pass == 0) {
+      if (!bad) bad = !mbar_wait(&sh.full[stage], (at / kDepth) & 1, p.status);
+      // rows behind the block's last (and 14, 15) are not copied: what lies
+      // there enters only sums that are not used
+      const uint32_t tile = smem_u32(sh.ring[stage].weights) + g * kWeightPitch + 16 * t + warp % kTeam * 64;
+      const uint32_t act = smem_u32(sh.ring[stage].act) + 16 * t + warp % kTeam * 64;
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
-      }
-      // rows 14 and 15 of the product are not copied: whatever lies there
-      // (the next tile's first bytes) enters only their own sums
-      const uint32_t tile = ring.wait(p.status) + row_at(g) + 16 * t;
-#pragma unroll
-      for (int j = 0; j < kTileChunks; ++j) {
-        if (j < n_chunks) {
-          const uint4 a = lds128(tile + 64 * j), b = lds128(tile + (g < kRows - 8 ? row_at(8) : 0u) + 64 * j);
+      for (int j = 0; j < kMine; ++j) {
+        if (warp % kTeam + j * kTeam < n_chunks) {
+          const uint4 u = lds128(tile + j * kTeam * 64);
+          const uint4 v = lds128(tile + (g < kRows - 8 ? 8 * kWeightPitch : 0) + j * kTeam * 64);
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
-            mma_16x8x16(acc[n], a.x, b.x, a.y, b.y, hf[j][n].x, hf[j][n].y);
-            mma_16x8x16(acc[n], a.z, b.z, a.w, b.w, hf[j][n].z, hf[j][n].w);
+            if (!any[n]) continue;
+            uint4 h = lds128(act + column[n] * kActPitch + j * kTeam * 64);
+            if (!live[n]) h = make_uint4(0, 0, 0, 0);
+            mma_16x8x16(acc[n], u.x, v.x, u.y, v.y, h.x, h.y);
+            mma_16x8x16(acc[n], u.z, v.z, u.w, v.w, h.z, h.w);
           }
         }
       }
       __syncwarp();
-      fetch();
-      if (now.pass == passes - 1) {
+      if (lane == 0) mbar_arrive(&sh.free[stage]);
+      if constexpr (!kDirect) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int slot = first + n * 8 + 2 * t + e;
-            if (slot < last) {
-              float* to = sums + s.token(slot) * kRows + g;
-              const float gate = s.gate(slot);
-              to[0] += gate * acc[n][e];
-              if (g < kRows - 8) to[8] += gate * acc[n][2 + e];
-            }
-          }
+          for (int j = 0; j < 4; ++j)
+            if (to[n][j & 1] && (j < 2 || g < kRows - 8))
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(to[n][j & 1] + 32 * (j >> 1)), "f"(old[n][j] + acc[n][j]) : "memory");
         __syncwarp();
       }
-      if (!next(now)) break;
     }
-    __syncthreads();
+    if constexpr (kDirect) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = n * 8 + 2 * t + (j & 1), r = g + 8 * (j >> 1);
+          if (tok < p.tokens && r < kRows) sums[tok * kRows + r] = acc[n][j];
+        }
+    }
+    const int rows = min(kRows, row_end - row0);
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
     for (int i = threadIdx.x; i < span; i += kThreads) {
       const int tok = i / kRows, r = i % kRows;
       if (r < rows) {
-        const long long at = (long long)tok * p.hidden + row0 + r;
+        const long long out = (long long)tok * p.hidden + row0 + r;
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += sh.sums[w * span + i];
-        if (p.residual) v += bf16_to_f32(p.residual[at]);
-        p.y[at] = f32_to_bf16_rne(v);
+        for (int k = 0; k < kWarps; ++k) v += sh.sums[k * span + i];
+        if (p.residual) v += bf16_to_f32(p.residual[out]);
+        p.y[out] = f32_to_bf16_rne(v);
       }
     }
-    __syncthreads();
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    if constexpr (!kDirect) {
+      for (int i = lane; i < span; i += 32) sums[i] = 0.0f;
+      __syncwarp();
+    }
   }
-  if (!waited) wait_previous();  // no grid of the chain ends before the one it follows
 }
 
-constexpr size_t down_smem(int tokens) { return sizeof(DownShared) + sizeof(float) * kWarps * tokens * kRows; }
-static_assert(sizeof(GateUpShared<2>) <= 227 * 1024 && down_smem(kTokens) <= 227 * 1024, "shared memory of one block");
+template <int kN>
+constexpr size_t down_smem(int tokens) { return sizeof(DownShared<kN>) + sizeof(float) * kWarps * tokens * kRows; }
+static_assert(sizeof(GateUpShared<2>) <= 227 * 1024 && down_smem<2>(kTokens) <= 227 * 1024, "shared memory of one block");
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename K>
-int32_t launch_after(SharedMemorySetup& setup, int dev, K kernel, size_t smem, size_t most, const Layer& p, cudaStream_t s) {
+int32_t launch_after(SharedMemorySetup& setup, int dev, K kernel, int threads, size_t smem, size_t most, const Layer& p,
+                     cudaStream_t s) {
   ENNX_TRY(allow_shared_memory(setup, dev, kernel, (int)most));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)sm_count());
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute early;
@@ -544,12 +685,13 @@ int32_t launch_after(SharedMemorySetup& setup, int dev, K kernel, size_t smem, s
   ENNX_LAUNCH_CHECK("few-token moe");
   return ENNX_B200_OK;
 }
-template <int kN>
+template <int kN, bool kDirect>
 int32_t launch_experts(const Layer& p, int dev, cudaStream_t s) {
   static SharedMemorySetup setup[2];
   constexpr size_t smem = sizeof(GateUpShared<kN>);
-  ENNX_TRY(launch_after(setup[0], dev, token_gate_up_kernel<kN>, smem, smem, p, s));
-  return launch_after(setup[1], dev, token_down_kernel<kN>, down_smem(p.tokens), down_smem(kTokens), p, s);
+  ENNX_TRY(launch_after(setup[0], dev, token_gate_up_kernel<kN>, kThreads, smem, smem, p, s));
+  return launch_after(setup[1], dev, token_down_kernel<kN, kDirect>, kDownThreads, down_smem<kN>(p.tokens),
+                      down_smem<kN>(kDirect ? kN * 8 : kTokens), p, s);
 }
 
 }  // namespace
@@ -561,7 +703,7 @@ extern "C" {
 
 size_t ennx_b200_moe_layer_decode_workspace_size(int64_t tokens, int32_t experts, int32_t top_k, int32_t expert_width) {
   if (tokens <= 0 || tokens > kTokens || experts <= 0 || top_k <= 0 || expert_width <= 0) return 0;
-  return round256(sizeof(float) * tokens * experts) + round256(sizeof(uint16_t) * tokens * top_k * expert_width);
+  return round256((sizeof(float) + 1) * kTokens * kTopK) + round256(sizeof(uint16_t) * tokens * top_k * expert_width);
 }
 
 int32_t ennx_b200_moe_layer_decode(const uint16_t* x, const uint16_t* w_router, const uint16_t* w_gate_up,
@@ -590,13 +732,15 @@ int32_t ennx_b200_moe_layer_decode(const uint16_t* x, const uint16_t* w_router, 
   int dev = 0;
   int* status = nullptr;
   ENNX_TRY(serving_device(&dev, &status));
-  const Layer p{x, w_router, w_gate_up, w_down, residual, y, index, gate, (float*)workspace,
-                (uint16_t*)((uint8_t*)workspace + round256(sizeof(float) * tokens * experts)),
+  float* gates = (float*)workspace;
+  const Layer p{x, w_router, w_gate_up, w_down, residual, y, index, gate, (uint8_t*)(gates + kTokens * kTopK), gates,
+                (uint16_t*)((uint8_t*)workspace + round256((sizeof(float) + 1) * kTokens * kTopK)),
                 (int)tokens, hidden, experts, top_k, expert_width, status};
-  const dim3 router((unsigned)((experts + kRE - 1) / kRE), (unsigned)((tokens + kRT - 1) / kRT));
-  token_router_kernel<<<router, kThreads, 0, s>>>(p);
+  if (tokens == 1) token_router_kernel<1><<<kCluster, kThreads, 0, s>>>(p);
+  else token_router_kernel<8><<<(unsigned)(kCluster * ((tokens + 7) / 8)), kThreads, 0, s>>>(p);
   ENNX_LAUNCH_CHECK("few-token router");
-  return tokens <= 8 ? launch_experts<1>(p, dev, s) : launch_experts<2>(p, dev, s);
+  if (tokens <= 8) return launch_experts<1, true>(p, dev, s);
+  return tokens <= 16 ? launch_experts<2, true>(p, dev, s) : launch_experts<2, false>(p, dev, s);
 }
 
 }  // extern "C"
