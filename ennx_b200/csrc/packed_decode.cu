@@ -35,13 +35,27 @@ struct Product {
   int tokens;
 };
 
-__device__ __forceinline__ uint32_t moved_code(uint32_t code, const Product& p, uint32_t element, uint32_t max_code) {
-  const uint32_t random = packed_hash(p.seed.low, p.seed.high, element);
-  const uint32_t amount = p.d.whole + (uint32_t)((random >> 1) < (p.d.threshold >> 1));
-  if (amount == 0u) return code;
-  if ((random & 1u) == 0u) return code >= amount ? code - amount : min(code + amount, max_code);
-  return code + amount <= max_code ? code + amount : code >= amount ? code - amount : 0u;
+// The code moved by its step: down where the hash is even, up where it is odd,
+// reflected at the ends of the code range (perturb_code, kda_moe.metal:73-90,
+// without its branches; a step of 0 leaves the code).  `product` is element *
+// 0x9E3779B9, the hash's first multiplication.
+__device__ __forceinline__ uint32_t moved_code(uint32_t code, const Product& p, uint32_t product, uint32_t max_code) {
+  uint32_t v = p.seed.low ^ product;
+  v ^= v >> 16;
+  v *= 0x7FEB352Du;
+  v ^= v >> 15;
+  v *= 0x846CA68Bu;
+  v ^= v >> 15;
+  v ^= p.seed.high;
+  // (v >> 1) < (threshold >> 1) is v < threshold without its last bit
+  const uint32_t amount = p.d.whole + (v < (p.d.threshold & ~1u) ? 1u : 0u);
+  const uint32_t up = code + amount, down = code - amount;
+  const bool room_below = code >= amount;
+  const uint32_t when_even = room_below ? down : min(up, max_code);
+  const uint32_t when_odd = up <= max_code ? up : room_below ? down : 0u;
+  return (v & 1u) ? when_odd : when_even;
 }
+constexpr uint32_t kHashFactor = 0x9E3779B9u;
 
 // ---------------------------------------------------------------------------
 // any group size and width: a warp per row, a lane per column
@@ -57,7 +71,7 @@ __global__ void __launch_bounds__(256) packed_rows_kernel(const __grid_constant_
     for (uint32_t c = lane; c < p.d.input_width; c += 32) {
       uint32_t code = p.d.bits == 4 ? (__ldg(w + (c >> 1)) >> ((c & 1) * 4)) & 15u : __ldg(w + c);
       if (p.seed.enabled)
-        code = moved_code(code, p, (uint32_t)p.d.element_offset + (uint32_t)row * (uint32_t)p.d.input_width + c, max_code);
+        code = moved_code(code, p, kHashFactor * ((uint32_t)p.d.element_offset + (uint32_t)row * (uint32_t)p.d.input_width + c), max_code);
       const uint32_t group = min(c / p.d.group_size, (uint32_t)p.d.groups - 1u);
       const float v = __fmaf_rn((float)code, __ldg(sc + group), __ldg(bi + group));
 #pragma unroll
@@ -77,12 +91,17 @@ __global__ void __launch_bounds__(256) packed_rows_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------
 // groups of a multiple of 32 columns: tensor products of codes
 // ---------------------------------------------------------------------------
-constexpr int kSliceChunks = 8, kSlice = 32 * kSliceChunks;  // columns of k that a warp owns in a pass
-constexpr int kWarps = 8;
+// Columns of k that a warp owns in a pass, and warps of a block.  Moved codes
+// cost some 30 integer instructions each and are bound by them: half the
+// columns and twice the warps keep twice as many instructions ready.
+template <bool kMoved>
+struct Shape {
+  static constexpr int kChunks = kMoved ? 4 : 8, kSlice = 32 * kChunks, kWarps = kMoved ? 16 : 8, kBlocks = kMoved ? 1 : 2;
+};
 
 // How a call is laid out: `along` warps side by side on k, the others on rows.
 struct Split {
-  int along, row_warps;  // along * row_warps = kWarps
+  int along, row_warps;  // together all warps of a block
   int passes;            // slices per warp on k
   int tiles;             // row tiles of 16
 };
@@ -90,23 +109,24 @@ struct Split {
 // One stage of a warp's ring: 16 code rows, then (scale, bias) pairs.  A flush
 // is kFlush products of 16 columns under one scale; lane t of a row takes
 // 4 * kFlush consecutive columns of it, one shared-memory read.
-template <int kBits, int kFlush>
+template <int kBits, int kFlush, bool kMoved>
 struct Stage {
-  static constexpr int kRowBytes = kSlice * kBits / 8;
+  static constexpr int kSlice = Shape<kMoved>::kSlice, kRowBytes = kSlice * kBits / 8;
   // rows of a fragment read lie on different banks (an 8-lane phase covers
   // whole rows, each kFlush * 2 * kBits bytes), and a row that starts inside
   // a 16-byte granule still fits
   static constexpr int kPitch = kRowBytes + kFlush * 2 * kBits;
   static constexpr int kPieces = kRowBytes / 16 + 1;
-  static constexpr int kFlushes = 16 / kFlush;
+  static constexpr int kFlushes = kSlice / 16 / kFlush;
   static constexpr int kBytes = 16 * kPitch + 16 * kFlushes * 8;
-  // depth: as many as leave two blocks on an SM (80 to 100 KB in flight)
+  // depth: as many as leave 16 warps on an SM (80 to 100 KB in flight)
   static constexpr int kDepth = kBits == 8 ? 2 : 3;
 };
-template <int kBits, int kN, int kFlush>
+// ring, then sums of x, then the joins
+template <int kBits, int kN, int kFlush, bool kMoved>
 constexpr int smem_bytes() {
-  using S = Stage<kBits, kFlush>;
-  return kWarps * (S::kDepth * S::kBytes + S::kFlushes * 8 * kN * 4 + 2 * kN * 32 * 16);
+  using S = Stage<kBits, kFlush, kMoved>;
+  return Shape<kMoved>::kWarps * (S::kDepth * S::kBytes + S::kFlushes * 8 * kN * 4 + 2 * kN * 32 * 16);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -137,25 +157,29 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t lo, uint32_t hi) {
   return pack_bf16x2(__uint_as_float(0x4b000000u | lo) - 8388608.0f, __uint_as_float(0x4b000000u | hi) - 8388608.0f);
 }
 
-// Eight consecutive codes of a lane as four bf16 pairs.
+// Eight consecutive codes of a lane as four bf16 pairs, plus kCodeBias.
 // 4 bits: pairs (j, j + 4): two nibbles 16 bits apart are or-ed under the
-// exponent of 128 (128 + n is exact) and 128 is taken off again.  8 bits:
-// pairs (0, 1), (2, 3), ...  activation_pairs orders x the same way.
+// exponent of 128 (128 + n is exact in bf16) and left there: the 128 x that
+// come with the products are taken off once per scale.  8 bits: pairs (0, 1),
+// (2, 3), ...  activation_pairs orders x the same way.
+template <int kBits>
+constexpr float kCodeBias = kBits == 4 ? 128.0f : 0.0f;
 template <int kBits, bool kMoved>
 __device__ __forceinline__ void code_pairs(const uint32_t* w, uint32_t element, const Product& p, uint32_t (&r)[4]) {
   if constexpr (kMoved) {
+    const uint32_t product = element * kHashFactor;
     uint32_t c[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t code = kBits == 4 ? (w[0] >> (4 * j)) & 15u : (w[j >> 2] >> (8 * (j & 3))) & 255u;
-      c[j] = moved_code(code, p, element + j, (1u << kBits) - 1u);
+      c[j] = moved_code(code, p, product + (uint32_t)j * kHashFactor, (1u << kBits) - 1u);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = kBits == 4 ? pair_of(c[j], c[j + 4]) : pair_of(c[2 * j], c[2 * j + 1]);
+    for (int j = 0; j < 4; ++j)
+      r[j] = kBits == 4 ? (c[j] | c[j + 4] << 16 | 0x43004300u) : pair_of(c[2 * j], c[2 * j + 1]);
   } else if constexpr (kBits == 4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      r[j] = bf16x2_sub(((w[0] >> (4 * j)) & 0x000f000fu) | 0x43004300u, 0x43004300u);
+    for (int j = 0; j < 4; ++j) r[j] = ((w[0] >> (4 * j)) & 0x000f000fu) | 0x43004300u;
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -172,9 +196,10 @@ __device__ __forceinline__ uint4 activation_pairs(uint4 v) {  // columns (0,1) (
 // kN: blocks of 8 tokens.  kAligned: rows start on 16 bytes and the slice ends
 // on a granule, so copies need no per-row arithmetic and reads no shifting.
 template <int kBits, int kN, int kFlush, bool kMoved, bool kAligned>
-__global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __grid_constant__ Product p,
-                                                                      const __grid_constant__ Split sp) {
-  using S = Stage<kBits, kFlush>;
+__global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBlocks)
+    packed_tiles_kernel(const __grid_constant__ Product p, const __grid_constant__ Split sp) {
+  using S = Stage<kBits, kFlush, kMoved>;
+  constexpr int kSlice = S::kSlice, kSliceChunks = Shape<kMoved>::kChunks, kWarps = Shape<kMoved>::kWarps;
   constexpr int kFlushes = S::kFlushes, kStages = S::kDepth, kRuns = kFlush / 2;  // runs of 8 columns of a lane in a flush
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -184,12 +209,16 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
   float* xsum = reinterpret_cast<float*>(smem + kWarps * kStages * S::kBytes) + warp * kFlushes * 8 * kN;
   float4* red = reinterpret_cast<float4*>(smem + kWarps * (kStages * S::kBytes + kFlushes * 8 * kN * 4));
   const uint32_t width = (uint32_t)p.d.input_width, rows = (uint32_t)p.d.output_width, groups = (uint32_t)p.d.groups;
+  const uint32_t row_bytes = (uint32_t)p.d.row_bytes;
   const bool wide_x = width % 8 == 0 && ((uintptr_t)p.x & 15u) == 0;
 
   const int stride = (int)gridDim.x * sp.row_warps;
   int tile = (int)blockIdx.x * sp.row_warps + wr;
   auto slice0 = [&](int pass) { return (uint32_t)(pass * sp.along + wk) * kSlice; };
 
+  // group of this lane's scale in a fetch, the same for all tiles if there is one pass
+  auto group_of = [&](int pass) { return min((slice0(pass) + lane % kFlushes * (kFlush * 16)) / p.d.group_size, groups - 1u); };
+  uint32_t f_group = group_of(0);
   int f_tile = tile, f_pass = 0;
   uint32_t f_stage = ring;
   auto fetch = [&] {
@@ -200,21 +229,21 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
         if constexpr (kAligned) {
           constexpr int kLanes = S::kRowBytes / 16, kRows = 32 / kLanes;  // lanes of a row, rows of an instruction
           const int r = lane / kLanes, c = lane % kLanes;
-          const uint8_t* src = p.w + (uint64_t)(row0 + r) * p.d.row_bytes + first + 16 * c;
-          const bool inside = first + 16 * c < (uint32_t)p.d.row_bytes;
+          const uint8_t* src = p.w + (uint64_t)(row0 + r) * row_bytes + first + 16 * c;
+          const bool inside = first + 16 * c < row_bytes, whole = row0 + 16 <= rows;
 #pragma unroll
           for (int i = 0; i < 16 / kRows; ++i)
-            if (inside && row0 + r + i * kRows < rows)
-              cp_async16(dst + (r + i * kRows) * S::kPitch + 16 * c, src + (uint64_t)(i * kRows) * p.d.row_bytes);
+            if (inside && (whole || row0 + r + i * kRows < rows))
+              cp_async16(dst + (r + i * kRows) * S::kPitch + 16 * c, src + (uint64_t)(i * kRows) * row_bytes);
         } else {
           // 16-byte granules that hold a byte of the slice, none behind the row's last
-          const uint32_t last = min((uint32_t)p.d.row_bytes, first + S::kRowBytes);
+          const uint32_t last = min(row_bytes, first + S::kRowBytes);
 #pragma unroll
           for (int i = lane; i < 16 * S::kPieces; i += 32) {
             const int r = i / S::kPieces, c = i % S::kPieces;
             const uint32_t row = row0 + r;
             if (row < rows) {
-              const uint8_t* start = p.w + (uint64_t)row * p.d.row_bytes + first;
+              const uint8_t* start = p.w + (uint64_t)row * row_bytes + first;
               const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
               if (src < start + (last - first)) cp_async16(dst + r * S::kPitch + 16 * c, src);
             }
@@ -222,12 +251,13 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
         }
         const int r = lane / kFlushes, f = lane % kFlushes;
         const uint32_t col = c0 + f * kFlush * 16;
-        const uint64_t at = (uint64_t)(row0 + r) * groups + min(col / p.d.group_size, groups - 1u);
+        if (sp.passes > 1) f_group = group_of(f_pass);
+        const uint64_t at = (uint64_t)(row0 + r) * groups + f_group;
         const uint32_t sdst = dst + 16 * S::kPitch + lane * 8;
 #pragma unroll
-        for (int i = 0; i < kFlushes / 2; ++i) {
+        for (int i = 0; i < (kFlushes + 1) / 2; ++i) {
           const int more = i * (32 / kFlushes);  // rows further down
-          if (col < width && row0 + r + more < rows) {
+          if (col < width && r + more < 16 && row0 + r + more < rows) {
             cp_async4(sdst + i * 256, p.sc + at + (uint64_t)more * groups);
             cp_async4(sdst + i * 256 + 4, p.bi + at + (uint64_t)more * groups);
           }
@@ -245,14 +275,16 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
   uint4 xf[kSliceChunks][kN];
-  auto load_x = [&](int pass) {  // activations of the slice, zeros behind the last column or token
+  // Activations of the slice, zeros behind the last column or token, and their
+  // sums per flush: products with ones, in the order of the codes' products,
+  // so that the 128 of a 4-bit code's pair cancels to the last bit.
+  auto load_x = [&](int pass) {
     const uint32_t c0 = slice0(pass);
     __syncwarp();
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const int tok = n * 8 + g;
       const uint16_t* x = p.x + (uint64_t)(tok < p.tokens ? tok : 0) * width;
-      float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < kSliceChunks; ++j) {
         const uint32_t c = c0 + j / kRuns * (16 * kFlush) + t * (8 * kRuns) + j % kRuns * 8;
@@ -267,20 +299,22 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
             v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
           }
         }
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        float s8 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s8 += __uint_as_float(u[i] << 16) + __uint_as_float(u[i] & 0xffff0000u);
-        sum += s8;
-        if ((j + 1) % kRuns == 0) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          if (t == 0) xsum[(j / kRuns * kN + n) * 8 + g] = sum;
-          sum = 0.0f;
-        }
         xf[j][n] = activation_pairs<kBits>(v);
       }
     }
+    constexpr uint32_t kOnes = 0x3f803f80u;
+#pragma unroll
+    for (int f = 0; f < kFlushes; ++f)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        float sum[4] = {};
+#pragma unroll
+        for (int j = f * kRuns; j < (f + 1) * kRuns; ++j) {
+          mma_16x8x16(sum, kOnes, kOnes, kOnes, kOnes, xf[j][n].x, xf[j][n].y);
+          mma_16x8x16(sum, kOnes, kOnes, kOnes, kOnes, xf[j][n].z, xf[j][n].w);
+        }
+        if (g == 0) *reinterpret_cast<float2*>(xsum + (f * kN + n) * 8 + 2 * t) = make_float2(sum[0], sum[1]);
+      }
     __syncwarp();
   };
   if (sp.passes == 1) load_x(0);
@@ -299,7 +333,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
         for (int h = 0; h < 2; ++h) {
           const uint32_t row = (uint32_t)tile * 16 + g + 8 * h;
           const uint32_t skew =
-              kAligned ? 0u : (uint32_t)((uintptr_t)(p.w + (uint64_t)row * p.d.row_bytes) + c0 * kBits / 8) & 15u;
+              kAligned ? 0u : (uint32_t)((uintptr_t)(p.w + (uint64_t)row * row_bytes) + c0 * kBits / 8) & 15u;
           addr[h] = st + (g + 8 * h) * S::kPitch + skew + t * (kRuns * kBits);
           element[h] = (uint32_t)p.d.element_offset + row * width + c0 + t * (8 * kRuns);
         }
@@ -341,10 +375,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) packed_tiles_kernel(const __gr
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
               const float2 xs = *reinterpret_cast<const float2*>(xsum + (f * kN + n) * 8 + 2 * t);
-              out[n][0] = fmaf(s0, acc[n][0], fmaf(b0, xs.x, out[n][0]));
-              out[n][1] = fmaf(s0, acc[n][1], fmaf(b0, xs.y, out[n][1]));
-              out[n][2] = fmaf(s1, acc[n][2], fmaf(b1, xs.x, out[n][2]));
-              out[n][3] = fmaf(s1, acc[n][3], fmaf(b1, xs.y, out[n][3]));
+              // exact where all codes are 0: acc is 128 xs then, sum by sum (see load_x)
+              constexpr float kBias = kCodeBias<kBits>;
+              out[n][0] = fmaf(s0, fmaf(-kBias, xs.x, acc[n][0]), fmaf(b0, xs.x, out[n][0]));
+              out[n][1] = fmaf(s0, fmaf(-kBias, xs.y, acc[n][1]), fmaf(b0, xs.y, out[n][1]));
+              out[n][2] = fmaf(s1, fmaf(-kBias, xs.x, acc[n][2]), fmaf(b1, xs.x, out[n][2]));
+              out[n][3] = fmaf(s1, fmaf(-kBias, xs.y, acc[n][3]), fmaf(b1, xs.y, out[n][3]));
             }
           }
         }
@@ -389,20 +425,21 @@ template <int kBits, int kN, int kFlush, bool kMoved, bool kAligned>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
   const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved, kAligned>;
   Split sp;
+  constexpr int kSlice = Shape<kMoved>::kSlice, kWarps = Shape<kMoved>::kWarps;
   const int slices = (int)((p.d.input_width + kSlice - 1) / kSlice);
   sp.along = 1;
   while (sp.along < slices && sp.along < kWarps) sp.along *= 2;
   sp.row_warps = kWarps / sp.along;
   sp.passes = (slices + sp.along - 1) / sp.along;
   sp.tiles = (int)((p.d.output_width + 15) / 16);
-  constexpr int smem = smem_bytes<kBits, kN, kFlush>();
-  static_assert(2 * (smem + 1024) <= 228 * 1024, "two blocks on an SM");
+  constexpr int smem = smem_bytes<kBits, kN, kFlush, kMoved>();
+  static_assert(Shape<kMoved>::kBlocks * (smem + 1024) <= 228 * 1024 && smem <= 227 * 1024, "blocks of an SM");
   static SharedMemorySetup setup;
   int dev = 0;
   int* status = nullptr;
   ENNX_TRY(serving_device(&dev, &status));
   ENNX_TRY(allow_shared_memory(setup, dev, kernel, smem));
-  const int blocks = (sp.tiles + sp.row_warps - 1) / sp.row_warps, cap = 2 * sm_count();
+  const int blocks = (sp.tiles + sp.row_warps - 1) / sp.row_warps, cap = Shape<kMoved>::kBlocks * sm_count();
   kernel<<<(unsigned)(blocks < cap ? blocks : cap), 32 * kWarps, smem, s>>>(p, sp);
   ENNX_LAUNCH_CHECK("packed tiles");
   return ENNX_B200_OK;

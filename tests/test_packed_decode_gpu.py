@@ -139,3 +139,12 @@ def test_refusals():
         call(x, w, sc, bi, _abi.PackedLinear(0, 0, 0, 64, 8, 5, 32, 0, 0, 0))
     with pytest.raises(ValueError, match="out must be"):
         call(x, w, sc, bi, lin, out=torch.empty(2, 9, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("inp,group", [(2048, 64), (96, 32), (301, 64)])
+def test_rows_of_zero_codes_without_bias_give_zero(inp, group):
+    w, sc, bi, lin = make(inp, 48, 4, group, 20)
+    w.view(48, -1)[5:40] = 0
+    bi.view(48, -1)[5:40] = 0
+    y = ops.packed_linear_decode(x_of(11, inp, 21) * 100, w, sc, bi, lin)
+    assert (y[:, 5:40] == 0).all() and (y[:, :5] != 0).any()
