@@ -132,8 +132,8 @@ constexpr int smem_bytes() {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {  // zero where !ok
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
@@ -216,56 +216,68 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
   int tile = (int)blockIdx.x * sp.row_warps + wr;
   auto slice0 = [&](int pass) { return (uint32_t)(pass * sp.along + wk) * kSlice; };
 
-  // group of this lane's scale in a fetch, the same for all tiles if there is one pass
-  auto group_of = [&](int pass) { return min((slice0(pass) + lane % kFlushes * (kFlush * 16)) / p.d.group_size, groups - 1u); };
-  uint32_t f_group = group_of(0);
+  // What a lane copies of a tile: codes at row `code_row` (aligned rows: every
+  // kCopyRows further down), scale and bias of row `scale_row` and every
+  // kScaleRows further down.  Pointers run from tile to tile.
+  constexpr int kLanes = S::kRowBytes / 16, kCopyRows = 32 / kLanes, kScaleRows = 32 / kFlushes;
+  const uint32_t code_row = lane / kLanes, scale_row = lane / kFlushes, scale_col = lane % kFlushes * (kFlush * 16);
+  auto group_of = [&](int pass) { return min((slice0(pass) + scale_col) / p.d.group_size, groups - 1u); };
+  uint32_t f_group = group_of(0), f_row = (uint32_t)tile * 16;
+  const uint8_t* f_code = p.w + (uint64_t)(f_row + code_row) * row_bytes + 16 * (lane % kLanes);
+  uint64_t f_scale = (uint64_t)(f_row + scale_row) * groups;
+  const uint64_t code_step = (uint64_t)(16 * stride) * row_bytes, scale_step = (uint64_t)(16 * stride) * groups;
   int f_tile = tile, f_pass = 0;
   uint32_t f_stage = ring;
   auto fetch = [&] {
     if (f_tile < sp.tiles) {
-      const uint32_t dst = f_stage, c0 = slice0(f_pass), row0 = (uint32_t)f_tile * 16;
-      if (c0 < width) {
-        const uint32_t first = c0 * kBits / 8;
-        if constexpr (kAligned) {
-          constexpr int kLanes = S::kRowBytes / 16, kRows = 32 / kLanes;  // lanes of a row, rows of an instruction
-          const int r = lane / kLanes, c = lane % kLanes;
-          const uint8_t* src = p.w + (uint64_t)(row0 + r) * row_bytes + first + 16 * c;
-          const bool inside = first + 16 * c < row_bytes, whole = row0 + 16 <= rows;
+      const uint32_t dst = f_stage, c0 = slice0(f_pass), first = c0 * kBits / 8;
+      const bool whole = f_row + 16 <= rows;
+      if constexpr (kAligned) {
+        if (first + 16 * (lane % kLanes) < row_bytes) {
+          const uint8_t* src = f_code + first;
+          const uint32_t to = dst + code_row * S::kPitch + 16 * (lane % kLanes);
+          if (whole) {
 #pragma unroll
-          for (int i = 0; i < 16 / kRows; ++i)
-            if (inside && (whole || row0 + r + i * kRows < rows))
-              cp_async16(dst + (r + i * kRows) * S::kPitch + 16 * c, src + (uint64_t)(i * kRows) * row_bytes);
-        } else {
-          // 16-byte granules that hold a byte of the slice, none behind the row's last
-          const uint32_t last = min(row_bytes, first + S::kRowBytes);
-#pragma unroll
-          for (int i = lane; i < 16 * S::kPieces; i += 32) {
-            const int r = i / S::kPieces, c = i % S::kPieces;
-            const uint32_t row = row0 + r;
-            if (row < rows) {
-              const uint8_t* start = p.w + (uint64_t)row * row_bytes + first;
-              const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
-              if (src < start + (last - first)) cp_async16(dst + r * S::kPitch + 16 * c, src);
-            }
+            for (int i = 0; i < 16 / kCopyRows; ++i)
+              cp_async16(to + i * kCopyRows * S::kPitch, src + (uint64_t)(i * kCopyRows) * row_bytes);
+          } else {
+            for (int i = 0; i < 16 / kCopyRows; ++i)
+              if (f_row + code_row + i * kCopyRows < rows)
+                cp_async16(to + i * kCopyRows * S::kPitch, src + (uint64_t)(i * kCopyRows) * row_bytes);
           }
         }
-        const int r = lane / kFlushes, f = lane % kFlushes;
-        const uint32_t col = c0 + f * kFlush * 16;
-        if (sp.passes > 1) f_group = group_of(f_pass);
-        const uint64_t at = (uint64_t)(row0 + r) * groups + f_group;
-        const uint32_t sdst = dst + 16 * S::kPitch + lane * 8;
+      } else if (c0 < width) {
+        // 16-byte granules that hold a byte of the slice, none behind the row's last
+        const uint32_t last = min(row_bytes, first + S::kRowBytes);
 #pragma unroll
-        for (int i = 0; i < (kFlushes + 1) / 2; ++i) {
-          const int more = i * (32 / kFlushes);  // rows further down
-          if (col < width && r + more < 16 && row0 + r + more < rows) {
-            cp_async4(sdst + i * 256, p.sc + at + (uint64_t)more * groups);
-            cp_async4(sdst + i * 256 + 4, p.bi + at + (uint64_t)more * groups);
+        for (int i = lane; i < 16 * S::kPieces; i += 32) {
+          const int r = i / S::kPieces, c = i % S::kPieces;
+          const uint32_t row = f_row + r;
+          if (row < rows) {
+            const uint8_t* start = p.w + (uint64_t)row * row_bytes + first;
+            const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
+            if (src < start + (last - first)) cp_async16(dst + r * S::kPitch + 16 * c, src);
           }
         }
+      }
+      // scales behind the last column are 0, which takes their columns out
+      if (sp.passes > 1) f_group = group_of(f_pass);
+      const bool inside = c0 + scale_col < width;
+      const float *sc = p.sc + f_scale + f_group, *bi = p.bi + f_scale + f_group;
+      const uint32_t sdst = dst + 16 * S::kPitch + lane * 8;
+#pragma unroll
+      for (int i = 0; i < 16 / kScaleRows; ++i) {
+        const bool ok = inside && (whole || f_row + scale_row + i * kScaleRows < rows);
+        const uint64_t down = ok ? (uint64_t)(i * kScaleRows) * groups : 0;
+        cp_async4(sdst + i * 256, ok ? sc + down : p.sc, ok);
+        cp_async4(sdst + i * 256 + 4, ok ? bi + down : p.bi, ok);
       }
       if (++f_pass == sp.passes) {
         f_pass = 0;
         f_tile += stride;
+        f_row += 16 * stride;
+        f_code += code_step;
+        f_scale += scale_step;
       }
     }
     f_stage = f_stage + S::kBytes == ring + kStages * S::kBytes ? ring : f_stage + S::kBytes;
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
       cp_wait<kStages - 2>();
       __syncwarp();
       const uint32_t c0 = slice0(pass);
-      if (c0 < width) {
+      {
         uint32_t addr[2], element[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -365,7 +377,7 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
               mma_16x8x16(acc[n], a[0][2], a[1][2], a[0][3], a[1][3], xf[j][n].z, xf[j][n].w);
             }
           }
-          if (c0 + f * kFlush * 16 < width) {
+          {
             const uint32_t sa = st + 16 * S::kPitch + (g * kFlushes + f) * 8;
             uint32_t u[2], v[2];  // (scale, bias) of rows g and g + 8
             lds_words<2>(sa, u);
