@@ -157,6 +157,13 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t lo, uint32_t hi) {
   return pack_bf16x2(__uint_as_float(0x4b000000u | lo) - 8388608.0f, __uint_as_float(0x4b000000u | hi) - 8388608.0f);
 }
 
+// (v & 0x000f000f) | 0x43004300 in one logic instruction: written out, it
+// became two, and logic instructions are what the unpacking is made of
+__device__ __forceinline__ uint32_t nibbles_under_128(uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(0x000f000fu), "r"(0x43004300u));
+  return r;
+}
 // Eight consecutive codes of a lane as four bf16 pairs, plus kCodeBias.
 // 4 bits: pairs (j, j + 4): two nibbles 16 bits apart are or-ed under the
 // exponent of 128 (128 + n is exact in bf16) and left there: the 128 x that
@@ -179,7 +186,7 @@ __device__ __forceinline__ void code_pairs(const uint32_t* w, uint32_t element, 
       r[j] = kBits == 4 ? (c[j] | c[j + 4] << 16 | 0x43004300u) : pair_of(c[2 * j], c[2 * j + 1]);
   } else if constexpr (kBits == 4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = ((w[0] >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+    for (int j = 0; j < 4; ++j) r[j] = nibbles_under_128(w[0] >> (4 * j));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
