@@ -7,7 +7,6 @@ the device is not sm_100, every call raises.
 from __future__ import annotations
 
 import ctypes
-import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libennx_b200.so"
@@ -74,9 +73,16 @@ class GemmParams(ctypes.Structure):
                 ("lse_partial", ctypes.c_void_p), ("target_logit", ctypes.c_void_p)]
 
 
-# ennx_b200_decode_attention: q, ld_q, k, ld_k, v, ld_v, k_cache, k_seq, k_token, k_head, v_cache, v_seq,
-# v_token, v_head, lengths, o, ld_o, batch, room, hq, hkv
-DECODE_ATTENTION = struct.Struct("@QqQqQqQqqqQqqqQQqiiii")
+class DecodeAttention(ctypes.Structure):
+    """ennx_b200_decode_attention."""
+    _fields_ = [("q", ctypes.c_void_p), ("ld_q", ctypes.c_int64), ("k", ctypes.c_void_p), ("ld_k", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("ld_v", ctypes.c_int64),
+                ("k_cache", ctypes.c_void_p), ("k_seq", ctypes.c_int64), ("k_token", ctypes.c_int64),
+                ("k_head", ctypes.c_int64),
+                ("v_cache", ctypes.c_void_p), ("v_seq", ctypes.c_int64), ("v_token", ctypes.c_int64),
+                ("v_head", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("o", ctypes.c_void_p), ("ld_o", ctypes.c_int64),
+                ("batch", ctypes.c_int32), ("room", ctypes.c_int32), ("hq", ctypes.c_int32), ("hkv", ctypes.c_int32)]
 
 
 class PackedLinear(ctypes.Structure):
@@ -236,6 +242,28 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+_serving = None
+
+
+def serving():
+    """The extension module of the serving operators (raises if it has not been built)."""
+    global _serving
+    if _serving is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (the module links against torch's libraries)
+        path = LIB_PATH.with_name("ennx_b200_serving.so")
+        if not path.exists():
+            raise EnnxB200Error(CUDA_ERROR, f"{path} is missing: run `python -m ennx_b200.build`")
+        lib()
+        loader = importlib.machinery.ExtensionFileLoader("ennx_b200_serving", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("ennx_b200_serving", loader))
+        loader.exec_module(module)
+        _serving = module
+    return _serving
 
 
 def check(status: int, what: str = "") -> None:

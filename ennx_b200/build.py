@@ -2,7 +2,8 @@
 
 ``python -m ennx_b200.build`` (or ``__graft_entry__.build()``) compiles every
 ``csrc/*.cu`` with nvcc for ``sm_100a`` and links one shared library exporting
-the C ABI declared in ``include/ennx_b200.h``.  Objects are cached under
+the C ABI declared in ``include/ennx_b200.h``, then ``csrc/bindings.cpp`` into
+the extension module of the serving operators.  Objects are cached under
 ``_build/`` and rebuilt when a source or header is newer.
 """
 from __future__ import annotations
@@ -18,6 +19,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = ROOT / "_build" / "obj"
 LIB = PKG / "_lib" / "libennx_b200.so"
+BINDINGS = PKG / "_lib" / "ennx_b200_serving.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -44,6 +46,27 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_bindings() -> None:
+    """The torch extension module over the library (host code only)."""
+    src = CSRC / "bindings.cpp"
+    newest = max(p.stat().st_mtime for p in [src, *_headers()])
+    if BINDINGS.exists() and BINDINGS.stat().st_mtime >= newest:
+        return
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).parent
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", ROOT / "include",
+           Path(NVCC).parents[1] / "include", Path(sysconfig.get_paths()["include"])]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{p}" for p in inc],
+           str(src), "-o", str(BINDINGS), f"-L{LIB.parent}", "-lennx_b200", "-Wl,-rpath,$ORIGIN",
+           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for bindings.cpp:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     LIB.parent.mkdir(parents=True, exist_ok=True)
@@ -55,6 +78,7 @@ def build(verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_bindings()
     return LIB
 
 

@@ -154,67 +154,13 @@ def packed_linear(x: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, 
     return out
 
 
-# A serving call lasts a few microseconds on the device, so the checks below
-# read each tensor's attributes once and pass addresses as plain integers.
-
-def _here(what: str, first: torch.Tensor, *ts) -> int:
-    """The current device; every tensor given has to live on it."""
-    device = first.get_device()
-    for t in ts:
-        if t is not None and t.get_device() != device:
-            _check_dev(first, t)
-            raise ValueError(f"{what}: tensors are on {first.device} and {t.device}")
-    _check_dev(first)
-    if device != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensors are on {first.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
-    return device
-
-
-def _raw_stream(device: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-def _head_rows(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
-    """(rows, heads, row stride) of bf16 [rows, heads, 128] whose heads are contiguous within a row."""
-    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[2] != 128:
-        raise ValueError(f"{what}: {name} must be bfloat16 [rows, heads, 128]")
-    rows, heads, _ = t.shape
-    ld, between, inner = t.stride()
-    if inner != 1 or (between != 128 and heads > 1):
-        raise ValueError(f"{what}: the heads of {name} must be contiguous within a row")
-    return rows, heads, ld if rows > 1 else heads * 128  # the stride of one row is never used
-
-
 def packed_linear_decode(x: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
                          linear: _abi.PackedLinear, seed: tuple[int, int, int] = (0, 0, 0),
                          out: torch.Tensor | None = None) -> torch.Tensor:
     """``packed_linear`` for at most 16 tokens, straight from the codes (see
     ``ennx_b200_packed_linear_decode``): any widths and group size, weights not
     rounded to bf16.  The arenas must hold the whole linear."""
-    what = "packed_linear_decode"
-    device = _here(what, x, weights, scales, biases, out)
-    inp, n, bits, group = linear.input_width, linear.output_width, linear.bits, linear.group_size
-    if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != inp or not x.is_contiguous():
-        raise ValueError(f"{what}: x must be contiguous bfloat16 [tokens, input_width]")
-    if weights.dtype is not torch.uint8 or scales.dtype is not torch.float32 or \
-            biases.dtype is not torch.float32 or \
-            not (weights.is_contiguous() and scales.is_contiguous() and biases.is_contiguous()):
-        raise ValueError(f"{what}: arenas must be contiguous uint8 codes and float32 scales and biases")
-    tokens = x.shape[0]
-    if group and (bits == 4 or bits == 8):
-        groups = n * -(-inp // group)
-        if linear.byte_offset + n * ((inp * bits + 7) // 8) > weights.numel() or \
-                linear.scale_offset + groups > scales.numel() or linear.bias_offset + groups > biases.numel():
-            raise ValueError(f"{what}: the linear exceeds its arenas")
-    if out is None:
-        out = torch.empty((tokens, n), dtype=torch.bfloat16, device=x.device)
-    elif out.dtype is not torch.bfloat16 or out.shape != (tokens, n) or not out.is_contiguous():
-        raise ValueError(f"{what}: out must be contiguous bfloat16 [tokens, output_width]")
-    _abi.check(_abi.lib().ennx_b200_packed_linear_decode(
-        x.data_ptr(), tokens, weights.data_ptr(), scales.data_ptr(), biases.data_ptr(), ctypes.byref(linear),
-        _abi.PerturbSeed(*seed), out.data_ptr(), _raw_stream(device)), what)
-    return out
+    return _abi.serving().packed_linear_decode(x, weights, scales, biases, linear, seed, out)
 
 
 def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, with_logits: bool = False):
@@ -253,34 +199,7 @@ def moe_layer_decode(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.T
     """``moe_layer`` for at most 64 tokens (see ``ennx_b200_moe_layer_decode``):
     bound by the bytes of the picked experts' weights.  x and residual bf16
     [tokens, hidden], weights as for ``moe_layer``; all contiguous."""
-    what = "moe_layer_decode"
-    device = _here(what, x, w_router, w_gate_up, w_down, residual, out)
-    if x.dim() != 2 or w_gate_up.dim() != 3:
-        raise ValueError(f"{what}: x must be [tokens, H], w_gate_up [E, 2 I, H]")
-    T, H = x.shape
-    E, I2, _ = w_gate_up.shape
-    if w_router.shape != (E, H) or w_gate_up.shape[2] != H or w_down.shape != (E, H, I2 // 2) or I2 % 2:
-        raise ValueError(f"{what}: weights must be [E, H], [E, 2 I, H] and [E, H, I] for x [tokens, H]")
-    for t in (x, w_router, w_gate_up, w_down, residual, out):
-        if t is not None and (t.dtype is not torch.bfloat16 or not t.is_contiguous()):
-            raise ValueError(f"{what}: operands must be contiguous bfloat16")
-    if (out is not None and out.shape != (T, H)) or (residual is not None and residual.shape != (T, H)):
-        raise ValueError(f"{what}: residual and out must have the shape of x")
-    where = x.device
-    if out is None:
-        out = torch.empty((T, H), dtype=torch.bfloat16, device=where)
-    idx = gate = None
-    if return_routing:
-        idx = torch.empty((T, top_k), dtype=torch.int32, device=where)
-        gate = torch.empty((T, top_k), dtype=torch.float32, device=where)
-    lib = _abi.lib()
-    n = lib.ennx_b200_moe_layer_decode_workspace_size(T, E, top_k, I2 // 2)
-    ws = torch.empty(n, dtype=torch.uint8, device=where) if n else None
-    _abi.check(lib.ennx_b200_moe_layer_decode(
-        x.data_ptr(), w_router.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), T, H, E, top_k, I2 // 2,
-        None if residual is None else residual.data_ptr(), out.data_ptr(), idx.data_ptr() if return_routing else None,
-        gate.data_ptr() if return_routing else None, ws.data_ptr() if n else None, n, _raw_stream(device)), what)
-    return (out, idx, gate) if return_routing else out
+    return _abi.serving().moe_layer_decode(x, w_router, w_gate_up, w_down, top_k, residual, return_routing, out)
 
 
 def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope_theta: float = 1e6) -> torch.Tensor:
@@ -304,36 +223,7 @@ def gqa_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     cu_seqlens[s+1] - 1.  q and k are rotated in place when rope_theta > 0.
     Rows behind the last sequence are left as they are (undefined when out is
     None)."""
-    what = "gqa_attention_packed"
-    device = _here(what, q, k, v, cu_seqlens, out)
-    rows, hq, ldq = _head_rows(what, "q", q)
-    krows, hkv, ldk = _head_rows(what, "k", k)
-    vrows, vheads, ldv = _head_rows(what, "v", v)
-    if krows != rows or vrows != rows or vheads != hkv:
-        raise ValueError(f"{what}: q, k and v must have the same rows, k and v the same heads")
-    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or \
-            not cu_seqlens.is_contiguous():
-        raise ValueError(f"{what}: cu_seqlens must be contiguous int32 [sequences + 1]")
-    if out is None:
-        out, ldo = torch.empty((rows, hq, 128), dtype=torch.bfloat16, device=q.device), hq * 128
-    else:
-        orows, oheads, ldo = _head_rows(what, "out", out)
-        if orows != rows or oheads != hq:
-            raise ValueError(f"{what}: out must have the shape of q")
-    _abi.check(_abi.lib().ennx_b200_gqa_attention_packed(
-        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, cu_seqlens.data_ptr(),
-        cu_seqlens.numel() - 1, rows, hq, hkv, rope_theta, _raw_stream(device)), what)
-    return out
-
-
-def _cache(what: str, name: str, t: torch.Tensor) -> tuple[torch.Size, tuple[int, int, int]]:
-    """Shape and (sequence, token, head) strides of a bf16 cache [batch, room, heads, 128]."""
-    shape = t.shape
-    if t.dtype is not torch.bfloat16 or len(shape) != 4 or shape[3] != 128 or t.stride(3) != 1:
-        raise ValueError(f"{what}: {name} must be bfloat16 [batch, room, heads, 128] with contiguous heads")
-    st = t.stride()
-    # the stride of a dimension of one entry is never used
-    return shape, (st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0, st[2] if shape[2] > 1 else 0)
+    return _abi.serving().gqa_attention_packed(q, k, v, cu_seqlens, rope_theta, out)
 
 
 def gqa_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -348,41 +238,7 @@ def gqa_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     bf16 [batch, Hkv, 128], the new token's key and value, written to cache row
     lengths - 1 (None: the caches hold them).  rope_theta > 0 rotates q (not in
     place) and k to position lengths - 1."""
-    what = "gqa_attention_decode"
-    device = _here(what, q, k_cache, v_cache, lengths, k, v, out)
-    rows, hq, ldq = _head_rows(what, "q", q)
-    shape, ks = _cache(what, "k_cache", k_cache)
-    vshape, vs = _cache(what, "v_cache", v_cache)
-    batch, room, hkv, _ = shape
-    if vshape != shape or rows != batch:
-        raise ValueError(f"{what}: q and both caches must have the same batch, the caches the same shape")
-    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.numel() != batch or \
-            not lengths.is_contiguous():
-        raise ValueError(f"{what}: lengths must be contiguous int32 [batch]")
-    if (k is None) != (v is None):
-        raise ValueError(f"{what}: k and v come together")
-    kp = vp = ldk = ldv = 0
-    if k is not None:
-        krows, kheads, ldk = _head_rows(what, "k", k)
-        vrows, vheads, ldv = _head_rows(what, "v", v)
-        if krows != batch or vrows != batch or kheads != hkv or vheads != hkv:
-            raise ValueError(f"{what}: k and v must be [batch, Hkv, 128]")
-        kp, vp = k.data_ptr(), v.data_ptr()
-    if out is None:
-        out, ldo = torch.empty((batch, hq, 128), dtype=torch.bfloat16, device=q.device), hq * 128
-    else:
-        orows, oheads, ldo = _head_rows(what, "out", out)
-        if orows != batch or oheads != hq:
-            raise ValueError(f"{what}: out must have the shape of q")
-    lib = _abi.lib()
-    n = lib.ennx_b200_gqa_attention_decode_workspace_size(batch, room, hq, hkv)
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    params = _abi.DECODE_ATTENTION.pack(q.data_ptr(), ldq, kp, ldk, vp, ldv, k_cache.data_ptr(), *ks,
-                                        v_cache.data_ptr(), *vs, lengths.data_ptr(), out.data_ptr(), ldo, batch, room,
-                                        hq, hkv)
-    _abi.check(lib.ennx_b200_gqa_attention_decode(params, rope_theta, ws.data_ptr() if n else None, n,
-                                                  _raw_stream(device)), what)
-    return out
+    return _abi.serving().gqa_attention_decode(q, k_cache, v_cache, lengths, k, v, rope_theta, out)
 
 
 def kda_chunked(q, k, v, g, beta, state: torch.Tensor | None = None) -> torch.Tensor:

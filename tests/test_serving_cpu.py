@@ -45,7 +45,7 @@ def test_decode_attention_refuses_on_the_host():
                  v_cache=256, v_seq=8192, v_token=256, v_head=128, lengths=256, o=256, ld_o=512, batch=2, room=2048,
                  hq=4, hkv=2)
         f.update(over)
-        return ("ennx_b200_gqa_attention_decode", _abi.DECODE_ATTENTION.pack(*f.values()), theta, workspace, size, None)
+        return ("ennx_b200_gqa_attention_decode", ctypes.byref(_abi.DecodeAttention(**f)), theta, workspace, size, None)
 
     assert "null parameters" in refused("ennx_b200_gqa_attention_decode", None, 0.0, None, 0, None)
     assert "room" in refused(*call(room=0))
