@@ -17,9 +17,17 @@
 // shared by both.  Tensor memory: S_A | O_A | S_B | O_B, 128 fp32 columns
 // each.  Warp roles: 0 TMA producer (two-slot K/V ring, no multicast); 1 one
 // thread issues tcgen05.mma (S = Q K^T; O += P V with P from tensor memory);
-// 2..17 softmax, eight warps per query tile, two per 32 rows with 64 key
-// columns each, statistics in fp32, P rounded to bf16 (2^-9 relative, random
-// in sign, below the rounding of the bf16 output).
+// 4..11 softmax, four warps per query tile, a thread per row, statistics in
+// fp32, P rounded to bf16 (at most 2^-8 relative, random in sign, below the
+// rounding of the bf16 output).
+//
+// A key tile costs each query tile 1024 clocks of tensor work and, at 16 exp2 a
+// clock, 1024 clocks of the exponential unit, and with one query tile's products
+// running under the other's softmax neither may take longer.  So three eighths
+// of the exponentials are a cubic on the FMA units instead (`exp2_cubic`), P is
+// handed over in two halves so that its product starts under the second half,
+// and no two threads share a row (two per row and an exchange of maxima under
+// a barrier: 16384 tokens 1.19 ms).
 //
 // Masked places may hold anything: masked scores are replaced, not added to,
 // but a masked V row still meets P = 0 in the MMA and an infinity or NaN there
@@ -37,9 +45,14 @@ namespace {
 constexpr int D = 128, BQ = 128, BKV = 128;
 constexpr int SUB = 128 * 128;  // bytes of one 128-row x 64-column bf16 sub-tile
 constexpr int TILE = 2 * SUB;   // 128 rows x 128 columns
-constexpr int SOFTMAX_WARPS = 16;
-constexpr int THREADS = 64 + 32 * SOFTMAX_WARPS;
-constexpr int SMEM = 6 * TILE /*Q_A, Q_B, 2 K, 2 V*/ + 1024 + 5120;
+// three groups of four warps: producer and MMA (two warps idle), softmax of
+// tile A, softmax of tile B; the first gives registers to the others, whose
+// threads hold 128 scores (56 + 2 * 224 = 3 * 168, what the block starts with)
+constexpr int SOFTMAX_WARPS = 8;
+constexpr int FEW_REGS = 56, MANY_REGS = 224;
+constexpr int THREADS = 128 + 32 * SOFTMAX_WARPS;
+static_assert(FEW_REGS + 2 * MANY_REGS <= 3 * 168 && THREADS == 384, "registers of the block");
+constexpr int SMEM = 6 * TILE /*Q_A, Q_B, 2 K, 2 V*/ + 1024 + 256;
 constexpr uint32_t IDESC_QK = idesc_bf16_f32(128, 128);
 constexpr uint32_t IDESC_PV = idesc_bf16_f32(128, 128) | (1u << 16);  // B (V) MN-major
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the max grows by > 2^8
@@ -69,8 +82,29 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ void named_bar_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+__device__ __forceinline__ bool elect_one() {  // one lane of the (converged) warp
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+// 2^x of a pair on the FMA units: x = n + f with n the nearest integer (left in
+// the low bits by adding 1.5 * 2^23), |f| <= 1/2; 2^f by the cubic of least
+// largest relative error, 7.5e-5, found by the exchange algorithm (P is rounded
+// to bf16 next, 4e-3); then n is added to the exponent.  Below 2^-126 the result
+// stays there instead of going to 0, so masked scores take ex2.
+__device__ __forceinline__ uint64_t exp2_cubic(uint64_t x) {
+  const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f), minus = pack_f32x2(-12582912.0f, -12582912.0f);
+  const uint64_t negone = pack_f32x2(-1.0f, -1.0f);
+  x = pack_f32x2(fmaxf(low(x), -126.0f), fmaxf(high(x), -126.0f));
+  const uint64_t t = add_f32x2(x, magic), f = fma_f32x2(add_f32x2(t, minus), negone, x);
+  uint64_t y = fma_f32x2(f, pack_f32x2(0.05517166852951050f, 0.05517166852951050f),
+                         pack_f32x2(0.24261112511157990f, 0.24261112511157990f));
+  y = fma_f32x2(y, f, pack_f32x2(0.69326096773147583f, 0.69326096773147583f));
+  y = fma_f32x2(y, f, pack_f32x2(0.99992805719375610f, 0.99992805719375610f));
+  const uint32_t lo = ((uint32_t)t << 23) + (uint32_t)y, hi = ((uint32_t)(t >> 32) << 23) + (uint32_t)(y >> 32);
+  return ((uint64_t)hi << 32) | lo;
 }
 
 // Packed rows: [begin, end) belong to sequences, clamped to the rows there are.
@@ -100,26 +134,23 @@ struct Operands {
 };
 
 struct Bars {
-  uint64_t q_full, kv_full[2], kv_free[2], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full, kv_full[2], kv_free[2], s_full[2], p_full[2][2] /*[tile][half of the keys]*/, o_done[2];
   uint32_t tmem_base;
   int abort_flag;
   int first[2];  // first_row of both tiles' first rows
-  // [tile][parity of the key tile][half][row]: partial row max / sum exchanged
-  // by the two warps of a row
-  float red[2][2][2][128];
 };
-static_assert(sizeof(Bars) <= 5120, "barrier block must fit the reserved 5 KB");
+static_assert(sizeof(Bars) <= 256, "barrier block must fit the reserved 256 bytes");
 
-// Output columns [c0, c0 + 64) of one (row, head), by one warp, reading
-// visible keys only; every sum in fp32.
-__device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int h, int kvh, int c0, float scale_log2,
-                                         int lane) {
+// Output of one (row, head), by one warp, reading visible keys only; every sum
+// in fp32.
+__device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int h, int kvh, float scale_log2, int lane) {
   const uint2 qw = *reinterpret_cast<const uint2*>(t.q + (long long)row * t.ldq + h * D + lane * 4);
   const uint32_t qp[2] = {qw.x, qw.y};
-  float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+  float m = -INFINITY, l = 0.0f, a[4] = {};
   for (int j = lo; j <= row; ++j) {
     const uint2 kw = *reinterpret_cast<const uint2*>(t.k + (long long)j * t.ldk + kvh * D + lane * 4);
-    const uint32_t kp[2] = {kw.x, kw.y};
+    const uint2 vw = *reinterpret_cast<const uint2*>(t.v + (long long)j * t.ldv + kvh * D + lane * 4);
+    const uint32_t kp[2] = {kw.x, kw.y}, vp[2] = {vw.x, vw.y};
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -131,15 +162,22 @@ __device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int
     s *= scale_log2;
     const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
     const float alpha = ex2(m - ref), p = ex2(s - ref);
-    const uint32_t vw = *reinterpret_cast<const uint32_t*>(t.v + (long long)j * t.ldv + kvh * D + c0 + lane * 2);
     l = l * alpha + p;
-    a0 = a0 * alpha + p * __uint_as_float(vw << 16);
-    a1 = a1 * alpha + p * __uint_as_float(vw & 0xffff0000u);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      a[2 * i] = a[2 * i] * alpha + p * __uint_as_float(vp[i] << 16);
+      a[2 * i + 1] = a[2 * i + 1] * alpha + p * __uint_as_float(vp[i] & 0xffff0000u);
+    }
     m = mn;
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  *reinterpret_cast<uint32_t*>(t.o + (long long)row * t.ldo + h * D + c0 + lane * 2) = pack_bf16x2(a0 * inv, a1 * inv);
+  *reinterpret_cast<uint2*>(t.o + (long long)row * t.ldo + h * D + lane * 4) =
+      make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
 }
+
+struct True { static constexpr bool value = true; };
+struct False { static constexpr bool value = false; };
+constexpr int kCubicOf8 = 3;  // of 8 pairs of exponentials, on the FMA units
 
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -166,7 +204,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bar.kv_full[i], 1);
       mbar_init(&bar.kv_free[i], 1);
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], 8);
+      mbar_init(&bar.p_full[i][0], 4);
+      mbar_init(&bar.p_full[i][1], 4);
       mbar_init(&bar.o_done[i], 1);
     }
     bar.abort_flag = 0;
@@ -188,6 +227,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int je[2] = {q0 / BKV + 1 - kt0, two ? q0 / BKV + 2 - kt0 : 0};
   const int nt = two ? je[1] : je[0];
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS));
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&tmQ);
@@ -219,152 +260,174 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      auto s_mma = [&](int x, int j) -> bool {  // S_X = Q_X K(j)^T
-        if (!mbar_wait(&bar.kv_full[j & 1], (j >> 1) & 1, err)) return false;
-        tc_fence_after();
-        const uint32_t qa = smem_u32(sQ + x * TILE), ka = smem_u32(sK + (j & 1) * TILE);
+    // The whole warp runs the loop, one elected lane issues: descriptors then
+    // stay in uniform registers.  Built per product by a lone lane, they made
+    // an instruction every 110 clocks, which a 128 x 128 x 16 product does not
+    // last (64).
+    const bool elected = elect_one();
+    uint64_t qd[2], kd[2], vd[2];
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem + x * 256, smem_desc_sw128(qa + (kk >> 2) * SUB + (kk & 3) * 32),
-                   smem_desc_sw128(ka + (kk >> 2) * SUB + (kk & 3) * 32), IDESC_QK, kk != 0);
-        umma_commit(&bar.s_full[x]);
-        return true;
-      };
-      bool ok = mbar_wait(&bar.q_full, 0, err);
-      for (int x = 0; ok && x < 2; ++x)
-        if (je[x] > 0 && js[x] == 0) ok = s_mma(x, 0);
-      for (int j = 0; ok && j < nt && !*abort_flag; ++j) {
-        const int last_user = j < je[1] && j >= js[1] ? 1 : 0;
-        for (int x = 0; x < 2; ++x) {
-          if (j >= je[x]) continue;
-          if (j >= js[x]) {
-            // O_X += P_X(j) V(j), P_X in tensor memory over the first 64 columns of S_X
-            if (!mbar_wait(&bar.p_full[x], (j - js[x]) & 1, err)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t va = smem_u32(sV + (j & 1) * TILE);
-#pragma unroll
-            for (int kk = 0; kk < BKV / 16; ++kk)
-              umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, smem_desc_sw128_mn(va + kk * 2048, SUB),
-                          IDESC_PV, j != js[x] || kk != 0);
-            umma_commit(&bar.o_done[x]);
-            if (x == last_user) umma_commit(&bar.kv_free[j & 1]);
-          }
-          if (j + 1 >= js[x] && j + 1 < je[x] && !s_mma(x, j + 1)) { ok = false; break; }
-        }
-      }
-      if (!ok) *abort_flag = 1;
+    for (int i = 0; i < 2; ++i) {
+      qd[i] = smem_desc_sw128(smem_u32(sQ + i * TILE));
+      kd[i] = smem_desc_sw128(smem_u32(sK + i * TILE));
+      vd[i] = smem_desc_sw128_mn(smem_u32(sV + i * TILE), SUB);
     }
+    auto s_mma = [&](int x, int j) -> bool {  // S_X = Q_X K(j)^T
+      if (!mbar_wait(&bar.kv_full[j & 1], (j >> 1) & 1, err)) return false;
+      tc_fence_after();
+      const uint64_t a = x ? qd[1] : qd[0], b = j & 1 ? kd[1] : kd[0];
+      if (elected) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t off = ((kk >> 2) * SUB + (kk & 3) * 32) >> 4;
+          umma_f16(tmem + x * 256, a + off, b + off, IDESC_QK, kk != 0);
+        }
+        umma_commit(&bar.s_full[x]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = mbar_wait(&bar.q_full, 0, err);
+    for (int x = 0; ok && x < 2; ++x)
+      if (je[x] > 0 && js[x] == 0) ok = s_mma(x, 0);
+    for (int j = 0; ok && j < nt && !*abort_flag; ++j) {
+      const int last_user = j < je[1] && j >= js[1] ? 1 : 0;
+      const uint64_t b = j & 1 ? vd[1] : vd[0];
+      for (int x = 0; x < 2; ++x) {
+        if (j >= je[x]) continue;
+        if (j >= js[x]) {
+          // O_X += P_X(j) V(j), P_X in tensor memory over the first 64 columns of S_X
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!mbar_wait(&bar.p_full[x][half], (j - js[x]) & 1, err)) { ok = false; break; }
+            tc_fence_after();
+            if (elected) {
+#pragma unroll
+              for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, b + kk * 128, IDESC_PV, j != js[x] || kk != 0);
+              if (half == 1) {
+                umma_commit(&bar.o_done[x]);
+                if (x == last_user) umma_commit(&bar.kv_free[j & 1]);
+              }
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+        }
+        if (j + 1 >= js[x] && j + 1 < je[x] && !s_mma(x, j + 1)) { ok = false; break; }
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  }
   } else {
-    // softmax: tile x, TMEM lane quarter q = warp % 4, key-column half `half`
-    const int x = (warp - 2) >> 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY_REGS));
+    // softmax: tile x, TMEM lane quarter q = warp % 4, a thread per row
+    const int x = (warp - 4) >> 2;
     const int q = warp & 3;
-    const int half = ((warp - 2) >> 2) & 1;
-    const int r = q * 32 + lane;
     const int qx0 = q0 + x * BQ;
-    const int qpos = qx0 + r;
-    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t s_col = tmem + lane_off + x * 256;  // S_X (P_X over its first 64 columns)
-    const uint32_t o_col = s_col + 128;                 // O_X
-    const int pair_bar = 1 + 4 * x + q;                 // shared with the warp owning the other half of these rows
+    const int qpos = qx0 + q * 32 + lane;
+    const uint32_t s_col = tmem + ((uint32_t)(q * 32) << 16) + x * 256;  // S_X (P_X over its first 64 columns)
+    const uint32_t o_col = s_col + 128;                                   // O_X
     const int steps = je[x] - js[x];
     const int lo = pk.first_row(qpos);
     const int max_lo = __reduce_max_sync(0xffffffffu, lo);
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
-      // A failed (timed-out) wait does not leave the loop: the warp keeps
-      // meeting its partner at the named barrier, which has no timeout, and
-      // skips the work; the abort flag stops every other wait early.
-      if (ok) ok = !*abort_flag && mbar_wait(&bar.s_full[x], j & 1, err);
+      ok = !*abort_flag && mbar_wait(&bar.s_full[x], j & 1, err);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) *abort_flag = 1;
-      tc_fence_after();
-      const int k0 = (kt0 + js[x] + j) * BKV + half * 64;
-      uint32_t v0[32], v1[32];
-      if (ok) {
-        tmem_ld32(s_col + half * 64, v0);
-        tmem_ld32(s_col + half * 64 + 32, v1);
-        tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v0[i] = v1[i] = 0xff800000u;
+      if (!ok) {
+        *abort_flag = 1;
+        break;
       }
-      if (k0 + 63 > qx0 + q * 32 || k0 < max_lo) {  // warp-uniform: some key lies outside some row's [lo, row]
+      tc_fence_after();
+      const int k0 = (kt0 + js[x] + j) * BKV;
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, v[c]);
+      tmem_ld_wait();
+      // warp-uniform: some key lies outside some row's [lo, row]
+      const bool masked = k0 + BKV - 1 > qx0 + q * 32 || k0 < max_lo;
+      if (masked) {
         const int a = lo - k0, b = qpos - k0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (i < a || i > b) v0[i] = 0xff800000u;  // -inf
-          if (32 + i < a || 32 + i > b) v1[i] = 0xff800000u;
-        }
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i < a || c * 32 + i > b) v[c][i] = 0xff800000u;  // -inf
       }
       // row max of the raw scores (the positive scale commutes with max)
-      float mt = -INFINITY;
+      float top[4];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) mt = fmaxf(mt, fmaxf(__uint_as_float(v0[i]), __uint_as_float(v1[i])));
-      mt *= scale_log2;
-      // buffer j & 1: the partner's read of this slot two tiles ago preceded
-      // its arrival at the barrier of the tile in between
-      bar.red[x][j & 1][half][r] = mt;
-      named_bar_sync(pair_bar, 64);  // also: both halves have read S before P overwrites it
-      mt = fmaxf(mt, bar.red[x][j & 1][half ^ 1][r]);
-      if (!ok) continue;  // after the barrier: nothing below waits on the partner
-      const float m_new = fmaxf(m, mt);
+      for (int c = 0; c < 4; ++c) {
+        top[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+        for (int i = 1; i + 1 < 32; i += 2)
+          top[c] = fmaxf(top[c], fmaxf(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])));
+        top[c] = fmaxf(top[c], __uint_as_float(v[c][31]));
+      }
+      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale_log2);
       const bool rescale = m == -INFINITY ? true : (m_new > m + kRescaleThreshold);
       const float m_use = rescale ? m_new : m;
       const float alpha = (rescale && m != -INFINITY) ? ex2(m - m_use) : 1.0f;
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+        // the s_full wait above proves O_X += P_X(j-1) V(j-1) complete
+        for (int c = 0; c < 4; ++c) {
+          uint32_t ov[32];
+          tmem_ld32(o_col + c * 32, ov);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+          tmem_st32(o_col + c * 32, ov);
+        }
+      }
       // P = exp2(s * scale - m) as one packed fma per pair of scores; a row
       // with no visible score so far uses m = 0 (every exp2 argument is -inf)
       const float nm = m_use == -INFINITY ? 0.0f : -m_use;
       const uint64_t c2 = pack_f32x2(scale_log2, scale_log2), nm2 = pack_f32x2(nm, nm);
-      uint64_t ls2 = 0ull;
-      uint32_t pk2[32];
+      uint64_t sum[2] = {0ull, 0ull};
+      auto half_p = [&](int half, auto cubic) {
+        uint32_t pk2[32];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint64_t t01 = fma_f32x2(((uint64_t)v0[2 * i + 1] << 32) | v0[2 * i], c2, nm2);
-        const uint64_t t23 = fma_f32x2(((uint64_t)v1[2 * i + 1] << 32) | v1[2 * i], c2, nm2);
-        const float p0 = ex2(__uint_as_float((uint32_t)t01)), p1 = ex2(__uint_as_float((uint32_t)(t01 >> 32)));
-        const float p2 = ex2(__uint_as_float((uint32_t)t23)), p3 = ex2(__uint_as_float((uint32_t)(t23 >> 32)));
-        ls2 = add_f32x2(ls2, add_f32x2(pack_f32x2(p0, p1), pack_f32x2(p2, p3)));
-        pk2[i] = pack_bf16x2(p0, p1);
-        pk2[16 + i] = pack_bf16x2(p2, p3);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t* s2 = &v[2 * half + c][2 * i];
+            const uint64_t t = fma_f32x2(((uint64_t)s2[1] << 32) | s2[0], c2, nm2);
+            uint64_t e;
+            if (decltype(cubic)::value && i % 8 < kCubicOf8) e = exp2_cubic(t);
+            else e = pack_f32x2(ex2(low(t)), ex2(high(t)));
+            sum[i & 1] = add_f32x2(sum[i & 1], e);
+            pk2[16 * c + i] = pack_bf16x2(low(e), high(e));
+          }
+        tmem_st32(s_col + half * 32, pk2);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[x][half]);
+      };
+      if (masked) {
+        half_p(0, False{});
+        half_p(1, False{});
+      } else {
+        half_p(0, True{});
+        half_p(1, True{});
       }
-      const float ls = __uint_as_float((uint32_t)ls2) + __uint_as_float((uint32_t)(ls2 >> 32));
-      tmem_st32(s_col + half * 32, pk2);
-      l = l * alpha + ls;
+      const uint64_t both = add_f32x2(sum[0], sum[1]);
+      l = l * alpha + (low(both) + high(both));
       m = m_use;
-      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-        // the s_full wait above proves O_X += P_X(j-1) V(j-1) complete
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          uint32_t ov[32];
-          tmem_ld32(o_col + half * 64 + cc * 32, ov);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-          tmem_st32(o_col + half * 64 + cc * 32, ov);
-        }
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.p_full[x]);
     }
-    if (steps > 0) {
-      // row sum over both halves
-      bar.red[x][steps & 1][half][r] = l;
-      named_bar_sync(pair_bar, 64);
-      const float l_tot = l + bar.red[x][steps & 1][half ^ 1][r];
-      if (ok && mbar_wait(&bar.o_done[x], (steps - 1) & 1, err)) {
+    if (steps > 0 && ok) {
+      if (mbar_wait(&bar.o_done[x], (steps - 1) & 1, err)) {
         tc_fence_after();
-        const float inv = l_tot > 0.0f || l_tot != l_tot ? 1.0f / l_tot : 0.0f;
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const bool mine = qpos >= pk.begin() && qpos < end;
-        uint16_t* orow = t.o + (long long)qpos * t.ldo + h * D + half * 64;
+        uint16_t* orow = t.o + (long long)qpos * t.ldo + h * D;
         float worst = 0.0f;  // NaN or 0 * inf = NaN where an output is not finite
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t ov[32];
-          tmem_ld32(o_col + half * 64 + cc * 32, ov);
+          tmem_ld32(o_col + c * 32, ov);
           tmem_ld_wait();
           float f[32];
 #pragma unroll
@@ -375,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (mine) {
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-              st_global_v4(orow + cc * 32 + g * 8, pack_bf16x2(f[8 * g], f[8 * g + 1]),
+              st_global_v4(orow + c * 32 + g * 8, pack_bf16x2(f[8 * g], f[8 * g + 1]),
                            pack_bf16x2(f[8 * g + 2], f[8 * g + 3]), pack_bf16x2(f[8 * g + 4], f[8 * g + 5]),
                            pack_bf16x2(f[8 * g + 6], f[8 * g + 7]));
           }
@@ -385,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         while (redo) {
           const int src = __ffs(redo) - 1;
           redo &= redo - 1;
-          careful_row(t, qx0 + q * 32 + src, __shfl_sync(0xffffffffu, lo, src), h, kvh, half * 64, scale_log2, lane);
+          careful_row(t, qx0 + q * 32 + src, __shfl_sync(0xffffffffu, lo, src), h, kvh, scale_log2, lane);
         }
       } else {
         *abort_flag = 1;
