@@ -18,12 +18,17 @@
 // lane finds both sums in its own accumulators (rows g and g + 8): exactness
 // costs no instruction.  9 to 16 heads take a second product each.
 //
-// Work is cut into units of 64 keys, numbered over all (sequence, cache head,
-// block of kRows query heads), and every block takes an equal run of units
-// whatever the lengths are: one long sequence is split over all blocks and a
-// ragged batch is balanced.  Where a run ends inside a sequence its partial
-// (maximum, sum, output) goes to the workspace in fp32 and a second kernel
-// joins the partials in order.
+// Work is counted in steps of 16 keys, numbered over all (sequence, cache head,
+// block of kRows query heads), and every WARP takes an equal run of steps
+// whatever the lengths are: one long sequence is split over the device and a
+// ragged batch is balanced.  A warp needs nobody else: it reads and rotates its
+// own query rows, and its copies run ahead from one sequence into the next.
+// Where a run begins or ends inside a sequence its partial (maximum, sum,
+// output) goes to the workspace in fp32 and a second kernel joins the partials
+// in order.  (Runs of blocks, with a merge of their warps and an empty ring at
+// the end of each sequence, took 40 us instead of TB us on 32 ragged sequences
+// of up to 4096 keys.)  Small caches take one block per head instead, whose
+// warps share the keys and merge once, and no second kernel.
 #include "kernels.cuh"
 #include "serve.cuh"
 
@@ -34,15 +39,16 @@ namespace {
 
 constexpr int D = 128;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kStep = 16;                  // keys per warp step
-constexpr int kUnit = kStep * kWarps;      // keys per unit of work
-constexpr int kStages = 3;                 // ring depth: 2 steps (16 KB) in flight per warp, 128 KB per SM
+constexpr int kStep = 16;                       // keys of a warp's step
+constexpr int kStages = 3;                      // ring depth: 2 steps (16 KB) in flight per warp, 128 KB per SM
 constexpr int kStageBytes = 2 * kStep * D * 2;  // K and V rows of one step
-constexpr int kRing = kWarps * kStages * kStageBytes;
-constexpr int kQBytes = 16 * D * 2;
-constexpr int kSmem = kRing + 2 * kQBytes;  // the second tile: lo parts where the heads fill the first
-constexpr int kPerSm = 2;                  // blocks resident per SM (2 x 100 KB of shared memory)
-static_assert(kWarps * 16 * (D + 2) * 4 <= kRing, "the merge buffer overlays the ring");
+constexpr int kWarpRing = kStages * kStageBytes;
+constexpr int kLoBytes = 16 * D * 2;            // a warp's lo parts of 16 query rows
+constexpr int kSmem = kWarps * (kWarpRing + kLoBytes);
+constexpr int kPerSm = 2;                       // blocks resident per SM
+constexpr int kPart = D + 2;                    // floats of a partial row: output, maximum, sum
+static_assert(kPerSm * (kSmem + 1024) <= 228 * 1024, "blocks of an SM");
+static_assert(kWarps * 16 * kPart * 4 <= kWarps * kWarpRing, "the merge buffer overlays the rings");
 
 struct Cache {
   uint16_t *k, *v;
@@ -62,44 +68,13 @@ struct Args {
 };
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) { return min(a.room, max(0, __ldg(a.lengths + b))); }
-__device__ __forceinline__ long long seq_units(const Args& a, int b) {
-  return (long long)((seq_len(a, b) + kUnit - 1) / kUnit) * a.hkv * a.blocks;
-}
-
-// Sum over sequences of their units, and (target >= 0) the sequence that
-// holds unit `target` with the units before it.  By every thread of a block
-// of kThreads threads.
-__device__ long long scan_units(const Args& a, long long target, int* seq, long long* before) {
-  __shared__ long long warp_sum[kWarps];
-  __shared__ int hit_seq;
-  __shared__ long long hit_before;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long run = 0;
-  __syncthreads();  // an earlier call's results have been read
-  if (threadIdx.x == 0) { hit_seq = -1; hit_before = 0; }
-  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-    const int b = b0 + (int)threadIdx.x;
-    const long long mine = b < a.batch ? seq_units(a, b) : 0;
-    long long inc = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, off);
-      if (lane >= off) inc += up;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sum[warp] = inc;
-    __syncthreads();
-    long long first = run + inc - mine;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) first += warp_sum[w];
-      run += warp_sum[w];
-    }
-    if (mine > 0 && target >= first && target < first + mine) { hit_seq = b; hit_before = first; }
-  }
-  __syncthreads();
-  *seq = hit_seq;
-  *before = hit_before;
-  return run;
+// steps of one head of a sequence, and its weight in the division of the work:
+// a head costs the reading of its query rows beside its steps
+__device__ __forceinline__ int head_steps(int len) { return (len + kStep - 1) / kStep; }
+constexpr int kHeadCost = 2;
+__device__ __forceinline__ int head_weight(int steps) { return steps > 0 ? steps + kHeadCost : 0; }
+__device__ __forceinline__ long long seq_weight(const Args& a, int b) {
+  return (long long)head_weight(head_steps(seq_len(a, b))) * a.hkv * a.blocks;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
@@ -131,331 +106,504 @@ __device__ __forceinline__ uint32_t take_hi(float& x, float& y) {
 // 16-byte chunk `c` of row `r` in a tile of 256-byte rows
 __device__ __forceinline__ uint32_t at(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) << 4)); }
 
-// kSplit: block = an equal run of all units, partials where a run ends inside
-// a segment; otherwise block = one whole (sequence, cache head, head block).
-template <bool kSplit, int kRows>
-__global__ void __launch_bounds__(kThreads, kPerSm) token_attention_kernel(const __grid_constant__ Args a,
-                                                                           const __grid_constant__ RopeTable table) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ float rot[2][64];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
-  const uint32_t sq = smem_u32(smem) + kRing;
-  float* merge = reinterpret_cast<float*>(smem);  // [warp][16][D + 2] over the ring, used with the ring drained
+// One warp's work on one (sequence, cache head, block of query heads).
+template <int kRows>
+struct Head {
+  static constexpr int R = kRows / 8;  // rows g (and g + 8) of a lane
+  int b, h, hq0, rows, len;            // query heads hq0 .. hq0 + rows - 1
+  uint32_t qf[8][4];
+  float acc[16][4], m[R], l[R];        // l of this lane's columns
+  float sn[2], cs[2];                  // rotation of pairs lane and lane + 32 to position len - 1
 
-  int b;
-  long long seg, left;
-  int unit;  // first unit within the segment
-  if constexpr (kSplit) {
-    // the join kernel may start its own prologue; it waits for this grid to finish before it reads
-    launch_dependents();
-    long long before, total = scan_units(a, -1, &b, &before);
-    const long long per = (total + gridDim.x - 1) / gridDim.x, first = per * blockIdx.x;
-    left = min(per, total - first);
-    if (left <= 0) return;
-    scan_units(a, first, &b, &before);
-    const int n = (seq_len(a, b) + kUnit - 1) / kUnit;
-    const long long in_seq = first - before;
-    seg = (long long)b * a.hkv * a.blocks + in_seq / n;
-    unit = (int)(in_seq % n);
-  } else {
-    seg = blockIdx.x;
-    b = (int)(seg / (a.hkv * a.blocks));
-    unit = 0;
-    left = (seq_len(a, b) + kUnit - 1) / kUnit;
+  __device__ __forceinline__ void place(const Args& a, int seq, int within, int n) {
+    b = seq;
+    len = n;
+    h = within / a.blocks;
+    const int g0 = within % a.blocks * kRows;
+    rows = min(kRows, a.group - g0);
+    hq0 = h * a.group + g0;
   }
 
-  while (true) {
-    const int len = seq_len(a, b), units = (len + kUnit - 1) / kUnit;
-    const int within = (int)(seg - (long long)b * a.hkv * a.blocks);
-    const int h = within / a.blocks, g0 = (within % a.blocks) * kRows;
-    const int rows = min(kRows, a.group - g0), hq0 = h * a.group + g0;  // query heads hq0 .. hq0 + rows - 1
-    const int n = (int)min((long long)(units - unit), left);
-    const uint16_t* kbase = a.c.k + (long long)b * a.c.kb + (long long)h * a.c.kh;
-    const uint16_t* vbase = a.c.v + (long long)b * a.c.vb + (long long)h * a.c.vh;
-
-    auto fetch = [&](int i) {  // keys of step i of this warp, zeros behind the last one
-      if (i < n) {
-        const int key0 = (unit + i) * kUnit + warp * kStep;
-        const uint32_t dst = ring + (i % kStages) * kStageBytes;
+  // Query rows as fragments: rotated, split into hi and lo.  kRows 8: the lo
+  // parts are rows 8 .. 15 of the tile; kRows 16: they go to `lo_parts`.
+  // The loads come first, all of them, and the rotation's frequencies from
+  // shared memory: a load at a time between the shuffles, and frequencies
+  // indexed by lane in the parameters, took 4.4 us, a third of a short run.
+  __device__ __forceinline__ void start(const Args& a, const double* inv, uint32_t lo_parts, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    uint32_t raw[R][4][2][2];  // columns 16 kk + 8 e + 2t, + 1 and those 64 further on
 #pragma unroll
-        for (int j = 0; j < kStep / 2; ++j) {
-          const int r = 2 * j + (lane >> 4), c = lane & 15, key = key0 + r;
-          const bool ok = key < len;
-          const long long tok = ok ? key : 0;
-          cp_async16(dst + at(r, c), kbase + tok * a.c.kt + c * 8, ok);
-          cp_async16(dst + kStep * 256 + at(r, c), vbase + tok * a.c.vt + c * 8, ok);
-        }
-      }
-      cp_commit();
-    };
+    for (int r = 0; r < R; ++r) {
+      const uint16_t* q = a.q + (long long)b * a.ldq + (long long)(hq0 + (g + 8 * r < rows ? g + 8 * r : 0)) * D + 2 * t;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(i);
-
-    // the segment's query rows, rotated, to shared memory as hi and lo
-    if (a.rotate && threadIdx.x < 64) rope_sincos(table, threadIdx.x, len - 1, &rot[0][threadIdx.x], &rot[1][threadIdx.x]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kRows * 64; i += kThreads) {
-      const int r = i >> 6, d = i & 63;
-      float x[2] = {0.0f, 0.0f};
-      if (r < rows) {
-        const uint16_t* src = a.q + (long long)b * a.ldq + (hq0 + r) * D + d;
-        x[0] = bf16_to_f32(__ldg(src));
-        x[1] = bf16_to_f32(__ldg(src + 64));
-        if (a.rotate) turn(x[0], x[1], rot[0][d], rot[1][d]);
-      }
-      uint8_t* row = smem + kRing;
+      for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = (d + 64 * e) >> 3, byte = (d & 7) * 2;
-        const uint16_t hi = f32_to_bf16_rne(x[e]), lo = f32_to_bf16_rne(x[e] - bf16_to_f32(hi));
-        *reinterpret_cast<uint16_t*>(row + at(r, c) + byte) = hi;
-        *reinterpret_cast<uint16_t*>(row + (kRows == 8 ? at(r + 8, c) : kQBytes + at(r, c)) + byte) = lo;
-      }
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int far = 0; far < 2; ++far)
+            raw[r][kk][e][far] = __ldg(reinterpret_cast<const uint32_t*>(q + 16 * kk + 8 * e + 64 * far));
     }
-    __syncthreads();
-    uint32_t qf[8][4];
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) ldsm4(sq + at(lane & 15, 2 * kk + (lane >> 4)), qf[kk]);
-
-    float acc[16][4];
+    for (int e = 0; e < 2; ++e) {
+      sn[e] = 0.0f;
+      cs[e] = 1.0f;
+      if (a.rotate) rope_sincos(inv[lane + 32 * e], len - 1, &sn[e], &cs[e]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = g + 8 * r < rows;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t w1 = raw[r][kk][e][0], w2 = raw[r][kk][e][1];
+          float x[2] = {__uint_as_float(w1 << 16), __uint_as_float(w1 & 0xffff0000u)};
+          float y[2] = {__uint_as_float(w2 << 16), __uint_as_float(w2 & 0xffff0000u)};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int from = (16 * (kk & 1) + 8 * e + 2 * t + i) & 31;
+            const float s = __shfl_sync(0xffffffffu, sn[kk >> 1], from), c = __shfl_sync(0xffffffffu, cs[kk >> 1], from);
+            if (a.rotate) turn(x[i], y[i], s, c);
+            if (!live) x[i] = y[i] = 0.0f;
+          }
+          const uint32_t xh = take_hi(x[0], x[1]), yh = take_hi(y[0], y[1]);
+          const uint32_t xl = pack_bf16x2(x[0], x[1]), yl = pack_bf16x2(y[0], y[1]);
+          qf[kk][2 * e + r] = xh;
+          qf[kk + 4][2 * e + r] = yh;
+          if constexpr (kRows == 8) {
+            qf[kk][2 * e + 1] = xl;
+            qf[kk + 4][2 * e + 1] = yl;
+          } else {
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(lo_parts + at(g + 8 * r, 2 * kk + e) + 4 * t), "r"(xl) : "memory");
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(lo_parts + at(g + 8 * r, 2 * kk + 8 + e) + 4 * t), "r"(yl) : "memory");
+          }
+        }
+    }
+    if constexpr (kRows == 16) __syncwarp();
 #pragma unroll
     for (int i = 0; i < 16; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    // heads g (and g + 8); l of this lane's columns
-    constexpr int R = kRows / 8;
-    float m[R], l[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) { m[r] = -INFINITY; l[r] = 0.0f; }
+  }
 
-    for (int i = 0; i < n; ++i) {
-      cp_wait<kStages - 2>();
-      __syncwarp();
-      const uint32_t sk = ring + (i % kStages) * kStageBytes, sv = sk + kStep * 256;
-      const int key0 = (unit + i) * kUnit + warp * kStep;
-      const int p = len - 1 - key0;  // the new token's row of this step, if it is in it
-      if (a.knew && p >= 0 && p < kStep) {
-        // row p of the cache is written here and replaced in the copy just read
-        uint8_t* st = smem + warp * kStages * kStageBytes + (i % kStages) * kStageBytes;
-        uint16_t* kw = a.c.k + (long long)b * a.c.kb + (long long)h * a.c.kh + (long long)(len - 1) * a.c.kt;
-        uint16_t* vw = a.c.v + (long long)b * a.c.vb + (long long)h * a.c.vh + (long long)(len - 1) * a.c.vt;
-        const uint16_t* kn = a.knew + (long long)b * a.ldk + h * D;
-        const uint16_t* vn = a.vnew + (long long)b * a.ldv + h * D;
+  // Writes the new token's key and value to the cache and over row `p` of the stage.
+  __device__ __forceinline__ void append(const Args& a, uint8_t* st, int p, int lane) {
+    uint16_t* kw = a.c.k + (long long)b * a.c.kb + (long long)h * a.c.kh + (long long)(len - 1) * a.c.kt;
+    uint16_t* vw = a.c.v + (long long)b * a.c.vb + (long long)h * a.c.vh + (long long)(len - 1) * a.c.vt;
+    const uint16_t* kn = a.knew + (long long)b * a.ldk + h * D;
+    const uint16_t* vn = a.vnew + (long long)b * a.ldv + h * D;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = lane + 32 * e;
-          float x1 = bf16_to_f32(__ldg(kn + d)), x2 = bf16_to_f32(__ldg(kn + d + 64));
-          if (a.rotate) turn(x1, x2, rot[0][d], rot[1][d]);
-          const uint16_t b1 = f32_to_bf16_rne(x1), b2 = f32_to_bf16_rne(x2);
-          kw[d] = b1;
-          kw[d + 64] = b2;
-          *reinterpret_cast<uint16_t*>(st + at(p, d >> 3) + (d & 7) * 2) = b1;
-          *reinterpret_cast<uint16_t*>(st + at(p, (d + 64) >> 3) + (d & 7) * 2) = b2;
-          const uint16_t w1 = __ldg(vn + d), w2 = __ldg(vn + d + 64);
-          vw[d] = w1;
-          vw[d + 64] = w2;
-          *reinterpret_cast<uint16_t*>(st + kStep * 256 + at(p, d >> 3) + (d & 7) * 2) = w1;
-          *reinterpret_cast<uint16_t*>(st + kStep * 256 + at(p, (d + 64) >> 3) + (d & 7) * 2) = w2;
-        }
-        __syncwarp();
-      }
-      float s[2][4] = {};
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        uint32_t kf[4];
-        ldsm4(sk + at((lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), kf);
-        mma(s[0], qf[kk], kf[0], kf[1]);
-        mma(s[1], qf[kk], kf[2], kf[3]);
-        if (kRows == 16 && a.rotate) {
-          uint32_t ql[4];
-          ldsm4(sq + kQBytes + at(lane & 15, 2 * kk + (lane >> 4)), ql);
-          mma(s[0], ql, kf[0], kf[1]);
-          mma(s[1], ql, kf[2], kf[3]);
-        }
-      }
-      float alpha[R], ref[R], pr[R][4];  // pr[.]: keys 2t, 2t + 1 of both blocks of 8
-      bool moved = false;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int nb = j >> 1, e = j & 1;
-          const float v = kRows == 8 ? s[nb][e] + s[nb][2 + e] : s[nb][2 * r + e];
-          pr[r][j] = key0 + nb * 8 + 2 * t + e < len ? v * a.scale_log2 : -INFINITY;
-          top = fmaxf(top, pr[r][j]);
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m[r], top);
-        ref[r] = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every exponent below is -inf
-        alpha[r] = ex2(m[r] - ref[r]);
-        moved |= alpha[r] != 1.0f;
-        m[r] = mn;
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) l[r] *= alpha[r];
-#pragma unroll
-        for (int nb = 0; nb < 16; ++nb)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[nb][j] *= alpha[kRows == 8 ? 0 : j >> 1];
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          pr[r][j] = ex2(pr[r][j] - ref[r]);
-          l[r] += pr[r][j];
-        }
-      uint32_t pf[4], pl[4];
-      if constexpr (kRows == 8) {
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-          pf[2 * nb] = take_hi(pr[0][2 * nb], pr[0][2 * nb + 1]);
-          pf[2 * nb + 1] = pack_bf16x2(pr[0][2 * nb], pr[0][2 * nb + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            pf[2 * nb + r] = take_hi(pr[r][2 * nb], pr[r][2 * nb + 1]);
-            pl[2 * nb + r] = pack_bf16x2(pr[r][2 * nb], pr[r][2 * nb + 1]);
-          }
-      }
-#pragma unroll
-      for (int nb = 0; nb < 8; ++nb) {
-        uint32_t vf[4];
-        ldsm4t(sv + at(lane & 15, 2 * nb + (lane >> 4)), vf);
-        mma(acc[2 * nb], pf, vf[0], vf[1]);
-        mma(acc[2 * nb + 1], pf, vf[2], vf[3]);
-        if constexpr (kRows == 16) {
-          mma(acc[2 * nb], pl, vf[0], vf[1]);
-          mma(acc[2 * nb + 1], pl, vf[2], vf[3]);
-        }
-      }
-      __syncwarp();  // all lanes have read the stage that the next fetch overwrites
-      fetch(i + kStages - 1);
+    for (int e = 0; e < 2; ++e) {
+      const int d = lane + 32 * e;
+      float x1 = bf16_to_f32(__ldg(kn + d)), x2 = bf16_to_f32(__ldg(kn + d + 64));
+      if (a.rotate) turn(x1, x2, sn[e], cs[e]);
+      const uint16_t b1 = f32_to_bf16_rne(x1), b2 = f32_to_bf16_rne(x2);
+      kw[d] = b1;
+      kw[d + 64] = b2;
+      *reinterpret_cast<uint16_t*>(st + at(p, d >> 3) + (d & 7) * 2) = b1;
+      *reinterpret_cast<uint16_t*>(st + at(p, (d + 64) >> 3) + (d & 7) * 2) = b2;
+      const uint16_t w1 = __ldg(vn + d), w2 = __ldg(vn + d + 64);
+      vw[d] = w1;
+      vw[d + 64] = w2;
+      *reinterpret_cast<uint16_t*>(st + kStep * 256 + at(p, d >> 3) + (d & 7) * 2) = w1;
+      *reinterpret_cast<uint16_t*>(st + kStep * 256 + at(p, (d + 64) >> 3) + (d & 7) * 2) = w2;
     }
-    cp_wait<0>();
-    __syncthreads();  // every ring is drained: the merge buffer may overlay it
+    __syncwarp();
+  }
+
+  // keys key0 .. key0 + 15, of which those below len count
+  __device__ __forceinline__ void step(const Args& a, uint32_t sk, uint32_t lo_parts, int key0, int lane) {
+    const int t = lane & 3;
+    const uint32_t sv = sk + kStep * 256;
+    float s[2][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      uint32_t kf[4];
+      ldsm4(sk + at((lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), kf);
+      mma(s[0], qf[kk], kf[0], kf[1]);
+      mma(s[1], qf[kk], kf[2], kf[3]);
+      if (kRows == 16 && a.rotate) {
+        uint32_t ql[4];
+        ldsm4(lo_parts + at(lane & 15, 2 * kk + (lane >> 4)), ql);
+        mma(s[0], ql, kf[0], kf[1]);
+        mma(s[1], ql, kf[2], kf[3]);
+      }
+    }
+    float alpha[R], ref[R], pr[R][4];  // pr[.]: keys 2t, 2t + 1 of both blocks of 8
+    bool moved = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int nb = j >> 1, e = j & 1;
+        const float v = kRows == 8 ? s[nb][e] + s[nb][2 + e] : s[nb][2 * r + e];
+        pr[r][j] = key0 + nb * 8 + 2 * t + e < len ? v * a.scale_log2 : -INFINITY;
+        top = fmaxf(top, pr[r][j]);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float mn = fmaxf(m[r], top);
+      ref[r] = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every exponent below is -inf
+      alpha[r] = ex2(m[r] - ref[r]);
+      moved |= alpha[r] != 1.0f;
+      m[r] = mn;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) l[r] *= alpha[r];
+#pragma unroll
+      for (int nb = 0; nb < 16; ++nb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nb][j] *= alpha[kRows == 8 ? 0 : j >> 1];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pr[r][j] = ex2(pr[r][j] - ref[r]);
+        l[r] += pr[r][j];
+      }
+    uint32_t pf[4], pl[4];
+    if constexpr (kRows == 8) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        pf[2 * nb] = take_hi(pr[0][2 * nb], pr[0][2 * nb + 1]);
+        pf[2 * nb + 1] = pack_bf16x2(pr[0][2 * nb], pr[0][2 * nb + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          pf[2 * nb + r] = take_hi(pr[r][2 * nb], pr[r][2 * nb + 1]);
+          pl[2 * nb + r] = pack_bf16x2(pr[r][2 * nb], pr[r][2 * nb + 1]);
+        }
+    }
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) {
+      uint32_t vf[4];
+      ldsm4t(sv + at(lane & 15, 2 * nb + (lane >> 4)), vf);
+      mma(acc[2 * nb], pf, vf[0], vf[1]);
+      mma(acc[2 * nb + 1], pf, vf[2], vf[3]);
+      if constexpr (kRows == 16) {
+        mma(acc[2 * nb], pl, vf[0], vf[1]);
+        mma(acc[2 * nb + 1], pl, vf[2], vf[3]);
+      }
+    }
+  }
+
+  // the row sums over the lanes that share a row
+  __device__ __forceinline__ void close() {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      const int row = g + 8 * r;
-      float* mr = merge + (warp * 16 + row) * (D + 2);
-      if (row < rows) {
-#pragma unroll
-        for (int nb = 0; nb < 16; ++nb)
-          *reinterpret_cast<float2*>(mr + nb * 8 + 2 * t) =
-              kRows == 8 ? make_float2(acc[nb][0] + acc[nb][2], acc[nb][1] + acc[nb][3])
-                         : make_float2(acc[nb][2 * r], acc[nb][2 * r + 1]);
-        if (t == 0) { mr[D] = m[r]; mr[D + 1] = l[r]; }
-      }
-    }
-    __syncthreads();
-    const bool whole = !kSplit || n == units;
-    const int per_row = kThreads / 16;  // threads of one row
-    for (int row = threadIdx.x / per_row; row < rows; row += 16) {
-      float mx = -INFINITY, sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, merge[(w * 16 + row) * (D + 2) + D]);
-      const float ref = mx == -INFINITY ? 0.0f : mx;
-      float f[kWarps];
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float* mr = merge + (w * 16 + row) * (D + 2);
-        f[w] = ex2(mr[D] - ref);
-        sum += f[w] * mr[D + 1];
-      }
-      const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-      float* part = kSplit ? a.partial + ((long long)blockIdx.x + seg) * 16 * (D + 2) + row * (D + 2) : nullptr;
-      uint16_t* orow = a.o + (long long)b * a.ldo + (hq0 + row) * D;
-      for (int d = (threadIdx.x % per_row) * 2; d < D; d += 2 * per_row) {
-        float y0 = 0.0f, y1 = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 v = *reinterpret_cast<const float2*>(merge + (w * 16 + row) * (D + 2) + d);
-          y0 += f[w] * v.x;
-          y1 += f[w] * v.y;
-        }
-        if (whole) *reinterpret_cast<uint32_t*>(orow + d) = pack_bf16x2(y0 * inv, y1 * inv);
-        else *reinterpret_cast<float2*>(part + d) = make_float2(y0, y1);
-      }
-      if (!whole && threadIdx.x % per_row == 0) *reinterpret_cast<float2*>(part + D) = make_float2(mx, sum);
-    }
-    left -= n;
-    if (left <= 0) return;
-    __syncthreads();  // the ring and the query rows are free again
-    ++seg;
-    unit = 0;
-    if (seg == (long long)(b + 1) * a.hkv * a.blocks) {
-      do ++b;
-      while (b < a.batch && seq_len(a, b) == 0);
-      if (b >= a.batch) return;  // not reached: `left` counts the units there are
-      seg = (long long)b * a.hkv * a.blocks;
     }
   }
+  __device__ __forceinline__ float2 value(int r, int nb) const {  // columns 8 nb + 2t, + 1 of row g + 8r
+    return kRows == 8 ? make_float2(acc[nb][0] + acc[nb][2], acc[nb][1] + acc[nb][3])
+                      : make_float2(acc[nb][2 * r], acc[nb][2 * r + 1]);
+  }
+  // partial rows, kPart floats each
+  __device__ __forceinline__ void put_partial(float* to, int lane) const {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (g + 8 * r < rows) {
+        float* row = to + (g + 8 * r) * kPart;
+#pragma unroll
+        for (int nb = 0; nb < 16; ++nb) *reinterpret_cast<float2*>(row + nb * 8 + 2 * t) = value(r, nb);
+        if (t == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[r], l[r]);
+      }
+  }
+  __device__ __forceinline__ void put_output(const Args& a, int lane) const {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (g + 8 * r < rows) {
+        const float inv = l[r] > 0.0f || l[r] != l[r] ? 1.0f / l[r] : 0.0f;
+        uint16_t* o = a.o + (long long)b * a.ldo + (long long)(hq0 + g + 8 * r) * D + 2 * t;
+#pragma unroll
+        for (int nb = 0; nb < 16; ++nb) {
+          const float2 v = value(r, nb);
+          *reinterpret_cast<uint32_t*>(o + nb * 8) = pack_bf16x2(v.x * inv, v.y * inv);
+        }
+      }
+  }
+};
+
+// Keys key0 .. key0 + 15 of one cache head into a stage, zeros from `len` on.
+__device__ __forceinline__ void copy_step(const Args& a, const uint16_t* kbase, const uint16_t* vbase, int key0, int len,
+                                          uint32_t dst, int lane) {
+#pragma unroll
+  for (int j = 0; j < kStep / 2; ++j) {
+    const int r = 2 * j + (lane >> 4), c = lane & 15, key = key0 + r;
+    const bool ok = key < len;
+    const long long tok = ok ? key : 0;
+    cp_async16(dst + at(r, c), kbase + tok * a.c.kt + c * 8, ok);
+    cp_async16(dst + kStep * 256 + at(r, c), vbase + tok * a.c.vt + c * 8, ok);
+  }
+}
+__device__ __forceinline__ const uint16_t* head_base(const uint16_t* cache, long long seq_stride, long long head_stride, int b,
+                                                     int h) {
+  return cache + (long long)b * seq_stride + (long long)h * head_stride;
+}
+
+// Small caches: one block per (sequence, cache head, head block); its warps
+// take the steps in turn and are merged at the end.
+template <int kRows>
+__global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __grid_constant__ Args a,
+                                                                       const __grid_constant__ RopeTable table) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ double inv[64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = table.inv[threadIdx.x];
+  __syncthreads();
+  uint8_t* mine = smem + warp * kWarpRing;
+  const uint32_t ring = smem_u32(mine), lo_parts = smem_u32(smem) + kWarps * kWarpRing + warp * kLoBytes;
+  const int per_seq = a.hkv * a.blocks, b = blockIdx.x / per_seq, len = seq_len(a, b), steps = head_steps(len);
+  Head<kRows> s;
+  s.place(a, b, blockIdx.x % per_seq, len);
+  const uint16_t *kbase = head_base(a.c.k, a.c.kb, a.c.kh, b, s.h), *vbase = head_base(a.c.v, a.c.vb, a.c.vh, b, s.h);
+  const int n = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 4, ..
+  auto fetch = [&](int i) {
+    if (i < n) copy_step(a, kbase, vbase, (warp + i * kWarps) * kStep, len, ring + i % kStages * kStageBytes, lane);
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  s.start(a, inv, lo_parts, lane);
+  for (int i = 0; i < n; ++i) {
+    cp_wait<kStages - 2>();
+    __syncwarp();
+    const int key0 = (warp + i * kWarps) * kStep, p = len - 1 - key0;
+    if (a.knew && p >= 0 && p < kStep) s.append(a, mine + i % kStages * kStageBytes, p, lane);
+    s.step(a, ring + i % kStages * kStageBytes, lo_parts, key0, lane);
+    __syncwarp();  // all lanes have read the stage that the next fetch overwrites
+    fetch(i + kStages - 1);
+  }
+  cp_wait<0>();
+  s.close();
+  __syncthreads();  // every ring is drained: the merge buffer may overlay them
+  float* merge = reinterpret_cast<float*>(smem);  // [warp][row][kPart]
+  s.put_partial(merge + warp * 16 * kPart, lane);
+  __syncthreads();
+  for (int row = warp; row < s.rows; row += kWarps) {
+    float mx = -INFINITY, sum = 0.0f, f[kWarps], y[4] = {};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, merge[(w * 16 + row) * kPart + D]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* part = merge + (w * 16 + row) * kPart;
+      f[w] = ex2(part[D] - ref);
+      sum += f[w] * part[D + 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += f[w] * part[lane * 4 + e];
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    *reinterpret_cast<uint2*>(a.o + (long long)b * a.ldo + (long long)(s.hq0 + row) * D + lane * 4) =
+        make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
+  }
+}
+
+// Any cache: every warp an equal run of all steps.
+template <int kRows>
+__global__ void __launch_bounds__(kThreads, kPerSm) token_split_kernel(const __grid_constant__ Args a,
+                                                                       const __grid_constant__ RopeTable table) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ double inv[64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = table.inv[threadIdx.x];
+  __syncthreads();
+  uint8_t* mine = smem + warp * kWarpRing;
+  const uint32_t ring = smem_u32(mine), lo_parts = smem_u32(smem) + kWarps * kWarpRing + warp * kLoBytes;
+  // the join kernel may start its own prologue; it waits for this grid to finish before it reads
+  launch_dependents();
+  const int per_seq = a.hkv * a.blocks;
+  const long long worker = (long long)blockIdx.x * kWarps + warp, workers = (long long)gridDim.x * kWarps;
+  long long total = 0;
+  for (int i = lane; i < a.batch; i += 32) total += seq_weight(a, i);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  const long long per = (total + workers - 1) / workers, first = per * worker;
+  int left = (int)min(per, total - first);
+  if (left <= 0) return;
+  // the sequence that holds step `first`, and the steps before it
+  int b = 0;
+  long long before = 0;
+  for (int b0 = 0;; b0 += 32) {  // ends: first < total
+    const long long own = b0 + lane < a.batch ? seq_weight(a, b0 + lane) : 0;
+    long long upto = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += up;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, first < before + upto);
+    if (hit) {
+      const int at_lane = __ffs(hit) - 1;
+      b = b0 + at_lane;
+      before += __shfl_sync(0xffffffffu, upto - own, at_lane);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  // where the copies and the products stand
+  struct Walk {
+    int b, within, step, len, steps;
+  };
+  auto enter = [&](Walk& w) {
+    w.len = seq_len(a, w.b);
+    w.steps = head_steps(w.len);
+  };
+  auto next_head = [&](Walk& w) {  // the next head with keys, while there are steps left
+    w.step = 0;
+    if (++w.within < per_seq) return;
+    w.within = 0;
+    do ++w.b;
+    while (w.b < a.batch && seq_len(a, w.b) == 0);
+    if (w.b < a.batch) enter(w);
+  };
+  Walk now{b, 0, 0, 0, 0};
+  enter(now);
+  now.within = (int)((first - before) / head_weight(now.steps));
+  int weight_in = (int)((first - before) % head_weight(now.steps));  // of the head, before this run
+  now.step = max(0, weight_in - kHeadCost);
+  // steps of the run: its weight without that of the heads it opens
+  int to_copy = 0;
+  {
+    Walk w = now;
+    int in = weight_in;
+    for (int rest = left; rest > 0; in = 0) {
+      const int part = min(rest, head_weight(w.steps) - in);
+      to_copy += max(0, in + part - kHeadCost) - max(0, in - kHeadCost);
+      rest -= part;
+      if (rest > 0) next_head(w);
+    }
+  }
+  Walk ahead = now;
+  int copied = 0;
+  const uint16_t *kbase = nullptr, *vbase = nullptr;
+  auto base = [&] {
+    const int h = ahead.within / a.blocks;
+    kbase = head_base(a.c.k, a.c.kb, a.c.kh, ahead.b, h);
+    vbase = head_base(a.c.v, a.c.vb, a.c.vh, ahead.b, h);
+  };
+  base();
+  auto fetch = [&] {
+    if (to_copy > 0) {
+      copy_step(a, kbase, vbase, ahead.step * kStep, ahead.len, ring + copied % kStages * kStageBytes, lane);
+      if (--to_copy > 0 && ++ahead.step == ahead.steps) {
+        next_head(ahead);
+        base();
+      }
+    }
+    ++copied;
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch();
+
+  Head<kRows> s;
+  for (int used = 0; left > 0;) {
+    const int part = min(left, head_weight(now.steps) - weight_in);
+    const int n = max(0, weight_in + part - kHeadCost) - now.step;
+    if (n > 0) {
+    s.place(a, now.b, now.within, now.len);
+    s.start(a, inv, lo_parts, lane);
+    for (int i = 0; i < n; ++i, ++used) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      const int key0 = (now.step + i) * kStep, p = now.len - 1 - key0;
+      if (a.knew && p >= 0 && p < kStep) s.append(a, mine + used % kStages * kStageBytes, p, lane);
+      s.step(a, ring + used % kStages * kStageBytes, lo_parts, key0, lane);
+      __syncwarp();  // all lanes have read the stage that the next fetch overwrites
+      fetch();
+    }
+    s.close();
+    const long long seg = (long long)now.b * per_seq + now.within;
+    // a slot per (worker, segment): from one such pair to the next either number grows
+    if (n == now.steps) s.put_output(a, lane);
+    else s.put_partial(a.partial + (worker + seg) * kRows * kPart, lane);
+    }
+    left -= part;
+    weight_in = 0;
+    if (left > 0) next_head(now);
+  }
+  cp_wait<0>();
 }
 
 // Joins the partials of one segment (block) in the order of its keys; one
 // warp per query head.  A segment of one part was written by that part's
-// block, an empty one gets zeros here.
-__global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_constant__ Args a, int grid, int block_rows) {
+// warp, an empty one gets zeros here.
+__global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_constant__ Args a, int workers, int block_rows) {
   const int seg = blockIdx.x, per_seq = a.hkv * a.blocks, b = seg / per_seq, within = seg % per_seq;
-  const int len = seq_len(a, b), units = (len + kUnit - 1) / kUnit;
-  // the units before this sequence, and all of them
-  long long mine = 0, total;
-  {
-    __shared__ long long sums[2][kWarps];
-    long long all = 0;
-    for (int i = threadIdx.x; i < a.batch; i += kThreads) {
-      const long long u = seq_units(a, i);
-      all += u;
-      if (i < b) mine += u;
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, off);
-      mine += __shfl_xor_sync(0xffffffffu, mine, off);
-    }
-    if ((threadIdx.x & 31) == 0) { sums[0][threadIdx.x >> 5] = all; sums[1][threadIdx.x >> 5] = mine; }
-    __syncthreads();
-    total = mine = 0;
-    for (int w = 0; w < kWarps; ++w) { total += sums[0][w]; mine += sums[1][w]; }
+  const int steps = head_steps(seq_len(a, b)), lane = threadIdx.x & 31;
+  // the weight before this sequence, and all of it
+  __shared__ long long sums[2][kWarps];
+  long long before = 0, total = 0;
+  for (int i = threadIdx.x; i < a.batch; i += kThreads) {
+    const long long u = seq_weight(a, i);
+    total += u;
+    if (i < b) before += u;
   }
-  const long long first = mine + (long long)within * units;
-  const long long per = total > 0 ? (total + grid - 1) / grid : 1;
-  const long long c0 = first / per, c1 = units > 0 ? (first + units - 1) / per : c0;
-  const int h = within / a.blocks, g0 = (within % a.blocks) * block_rows;
-  const int rows = min(block_rows, a.group - g0), lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 16; off; off >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+    before += __shfl_xor_sync(0xffffffffu, before, off);
+  }
+  if (lane == 0) { sums[0][threadIdx.x >> 5] = total; sums[1][threadIdx.x >> 5] = before; }
+  __syncthreads();
+  total = before = 0;
+  for (int w = 0; w < kWarps; ++w) { total += sums[0][w]; before += sums[1][w]; }
+  const long long first = before + (long long)within * head_weight(steps) + kHeadCost;  // its first step
+  const long long per = total > 0 ? (total + workers - 1) / workers : 1;
+  const long long c0 = first / per, c1 = steps > 0 ? (first + steps - 1) / per : c0;
+  const int h = within / a.blocks, g0 = within % a.blocks * block_rows, rows = min(block_rows, a.group - g0);
   // the partials are complete and visible; blocks without any wait too, so
   // that this grid never ends before the one it follows
   wait_previous();
-  if (units > 0 && c0 == c1) return;
+  if (steps > 0 && c0 == c1) return;
   for (int row = threadIdx.x >> 5; row < rows; row += kWarps) {
     float m = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (units > 0)
-      for (long long c = c0; c <= c1; ++c) {
-        const float* part = a.partial + (c + seg) * 16 * (D + 2) + row * (D + 2);
-        const float2 ml = *reinterpret_cast<const float2*>(part + D);
-        const float2 v0 = *reinterpret_cast<const float2*>(part + lane * 4);
-        const float2 v1 = *reinterpret_cast<const float2*>(part + lane * 4 + 2);
-        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-        const float f0 = ex2(m - ref), f1 = ex2(ml.x - ref);
-        l = l * f0 + ml.y * f1;
-        y[0] = y[0] * f0 + v0.x * f1;
-        y[1] = y[1] * f0 + v0.y * f1;
-        y[2] = y[2] * f0 + v1.x * f1;
-        y[3] = y[3] * f0 + v1.y * f1;
+    if (steps > 0)
+      for (long long c = c0; c <= c1; c += 32) {
+        // 32 parts at a time: their maxima and sums first, a lane each, then
+        // the outputs, all loads independent
+        const int n = (int)min(32LL, c1 - c + 1);
+        const float* part = a.partial + ((c + seg) * block_rows + row) * kPart;
+        const long long stride = (long long)block_rows * kPart;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < n) ml = *reinterpret_cast<const float2*>(part + lane * stride + D);
+        float mn = fmaxf(m, ml.x);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+        const float ref = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - ref), f = ex2(ml.x - ref);
+        float sum = f * ml.y;
+#pragma unroll
+        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l = l * f0 + sum;
         m = mn;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= f0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const float fi = __shfl_sync(0xffffffffu, f, i);
+          const float2 u = *reinterpret_cast<const float2*>(part + i * stride + lane * 4);
+          const float2 v = *reinterpret_cast<const float2*>(part + i * stride + lane * 4 + 2);
+          y[0] += fi * u.x;
+          y[1] += fi * u.y;
+          y[2] += fi * v.x;
+          y[3] += fi * v.y;
+        }
       }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    uint16_t* orow = a.o + (long long)b * a.ldo + (h * a.group + g0 + row) * D + lane * 4;
-    *reinterpret_cast<uint2*>(orow) = make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
+    *reinterpret_cast<uint2*>(a.o + (long long)b * a.ldo + (long long)(h * a.group + g0 + row) * D + lane * 4) =
+        make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
   }
 }
 
@@ -472,7 +620,7 @@ int split_grid() { return kPerSm * sm_count(); }
 template <int kRows>
 int32_t launch(const Args& a, const RopeTable& table, bool split, int64_t segs, int dev, cudaStream_t s) {
   static SharedMemorySetup setup[2];
-  const auto kernel = split ? token_attention_kernel<true, kRows> : token_attention_kernel<false, kRows>;
+  const auto kernel = split ? token_split_kernel<kRows> : token_whole_kernel<kRows>;
   ENNX_TRY(allow_shared_memory(setup[split], dev, kernel, kSmem));
   kernel<<<split ? (unsigned)split_grid() : (unsigned)segs, kThreads, kSmem, s>>>(a, table);
   ENNX_LAUNCH_CHECK("token attention");
@@ -490,7 +638,7 @@ size_t ennx_b200_gqa_attention_decode_workspace_size(int32_t batch, int32_t room
   if (batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || room <= kWholeRoom) return 0;
   const int rows = block_rows(hq / hkv);
   const size_t segs = (size_t)batch * hkv * ((hq / hkv + rows - 1) / rows);
-  return (segs + split_grid()) * 16 * (D + 2) * sizeof(float);
+  return (segs + (size_t)split_grid() * kWarps) * rows * kPart * sizeof(float);
 }
 
 int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, float rope_theta, void* workspace,
@@ -511,9 +659,10 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: a row stride is shorter than its heads");
   const int64_t strides = p->k_seq | p->k_token | p->k_head | p->v_seq | p->v_token | p->v_head;
   if (strides < 0) return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: a cache stride is negative");
-  if ((strides | p->ld_q | p->ld_o) % 8 || (((uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->o) & 15u))
+  if ((strides | p->ld_q | p->ld_o) % 8 ||
+      (((uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->q | (uintptr_t)p->o) & 15u))
     return set_error(ENNX_B200_INVALID_ARGUMENT,
-                     "attention_decode: caches and o must be 16-byte aligned with strides of a multiple of 8");
+                     "attention_decode: caches, q and o must be 16-byte aligned with strides of a multiple of 8");
   const int group = p->hq / p->hkv, rows = block_rows(group), blocks = (group + rows - 1) / rows;
   const int64_t segs = (int64_t)p->batch * p->hkv * blocks;
   if (segs > 0x7fffffffLL - 65536) return set_error(ENNX_B200_UNSUPPORTED, "attention_decode: too many heads");
@@ -540,7 +689,7 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  ENNX_CUDA(cudaLaunchKernelEx(&cfg, token_join_kernel, a, split_grid(), rows), "token attention join");
+  ENNX_CUDA(cudaLaunchKernelEx(&cfg, token_join_kernel, a, split_grid() * kWarps, rows), "token attention join");
   ENNX_LAUNCH_CHECK("token attention join");
   return ENNX_B200_OK;
 }

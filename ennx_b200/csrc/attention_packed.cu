@@ -477,7 +477,7 @@ __global__ void rope_packed_kernel(uint16_t* __restrict__ x, long long ld, int h
     const int pos = r - pk.first_row(r);
     float sn[8], cs[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rope_sincos(table, k0 + e, pos, &sn[e], &cs[e]);
+    for (int e = 0; e < 8; ++e) rope_sincos(table.inv[k0 + e], pos, &sn[e], &cs[e]);
     uint16_t* row = x + (long long)r * ld + k0;
     for (int h = 0; h < heads; ++h) {
       uint4* pa = reinterpret_cast<uint4*>(row + (long long)h * D);

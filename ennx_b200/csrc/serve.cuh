@@ -73,8 +73,8 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
 struct RopeTable {
   double inv[64];
 };
-__device__ __forceinline__ void rope_sincos(const RopeTable& t, int i, int pos, float* s, float* c) {
-  const double turns = (double)pos * t.inv[i];
+__device__ __forceinline__ void rope_sincos(double inv, int pos, float* s, float* c) {
+  const double turns = (double)pos * inv;
   sincospif((float)(2.0 * (turns - rint(turns))), s, c);
 }
 // host: inv[i] = theta^(-2i/128) / (2*pi)

@@ -276,7 +276,8 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, 
  * anything; an infinity or NaN in row p or before makes the outputs it enters
  * non-finite (NaN where their limit would be an infinity).  All bf16; strides in elements.  Cache strides (multiples of 8)
  * are free, so [batch, room, heads, 128] and [batch, heads, room, 128] both
- * fit; sequences given k and v must not share cache rows.  workspace (device,
+ * fit; the caches, q and o are 16-byte aligned, ld_q and ld_o multiples of 8;
+ * sequences given k and v must not share cache rows.  workspace (device,
  * 16-byte aligned) >= ennx_b200_gqa_attention_decode_workspace_size(...)
  * bytes, which is 0 for small rooms; calls that may overlap need one each. */
 typedef struct {
