@@ -9,8 +9,7 @@
 // FLOP per byte pair.  The G query heads of a cache head are the rows of an
 // m16n8k16 product, so a key is read once for all of them.  Each warp streams
 // 16 keys a step through its own cp.async ring and keeps its own running
-// maximum, sum and output, so no barrier stands in the loop; warps are merged
-// once per sequence and head.
+// maximum, sum and output, so no barrier stands in the loop.
 //
 // The rotated query and the weights have more bits than bf16 holds, so both
 // enter the products as hi + lo, two bf16 numbers (2^-16 of the value left).
@@ -26,7 +25,7 @@
 // Where a run begins or ends inside a sequence its partial (maximum, sum,
 // output) goes to the workspace in fp32 and a second kernel joins the partials
 // in order.  (Runs of blocks, with a merge of their warps and an empty ring at
-// the end of each sequence, took 40 us instead of TB us on 32 ragged sequences
+// the end of each sequence, took 40 us instead of 32 on 32 ragged sequences
 // of up to 4096 keys.)  Small caches take one block per head instead, whose
 // warps share the keys and merge once, and no second kernel.
 #include "kernels.cuh"
@@ -378,12 +377,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __g
   s.start(a, inv, lo_parts, lane);
   for (int i = 0; i < n; ++i) {
     cp_wait<kStages - 2>();
-    __syncwarp();
+    __syncwarp();            // the stage is there, and all lanes have read the one before it,
+    fetch(i + kStages - 1);  // which is filled again while this one is used
     const int key0 = (warp + i * kWarps) * kStep, p = len - 1 - key0;
     if (a.knew && p >= 0 && p < kStep) s.append(a, mine + i % kStages * kStageBytes, p, lane);
     s.step(a, ring + i % kStages * kStageBytes, lo_parts, key0, lane);
-    __syncwarp();  // all lanes have read the stage that the next fetch overwrites
-    fetch(i + kStages - 1);
   }
   cp_wait<0>();
   s.close();
@@ -517,12 +515,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_split_kernel(const __g
     s.start(a, inv, lo_parts, lane);
     for (int i = 0; i < n; ++i, ++used) {
       cp_wait<kStages - 2>();
-      __syncwarp();
+      __syncwarp();  // the stage is there, and all lanes have read the one before it,
+      fetch();       // which is filled again while this one is used
       const int key0 = (now.step + i) * kStep, p = now.len - 1 - key0;
       if (a.knew && p >= 0 && p < kStep) s.append(a, mine + used % kStages * kStageBytes, p, lane);
       s.step(a, ring + used % kStages * kStageBytes, lo_parts, key0, lane);
-      __syncwarp();  // all lanes have read the stage that the next fetch overwrites
-      fetch();
     }
     s.close();
     const long long seg = (long long)now.b * per_seq + now.within;
@@ -537,14 +534,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_split_kernel(const __g
   cp_wait<0>();
 }
 
-// Joins the partials of one segment (block) in the order of its keys; one
-// warp per query head.  A segment of one part was written by that part's
-// warp, an empty one gets zeros here.
+// Joins the partials of one row of a segment (block): its warps take 32 parts
+// each at a time and are joined in order.  A segment of one part was written by
+// that part's warp, an empty one gets zeros here.  (One warp for all parts of a
+// row took 9 us for 74 of them.)
 __global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_constant__ Args a, int workers, int block_rows) {
-  const int seg = blockIdx.x, per_seq = a.hkv * a.blocks, b = seg / per_seq, within = seg % per_seq;
-  const int steps = head_steps(seq_len(a, b)), lane = threadIdx.x & 31;
+  const int seg = blockIdx.x, row = blockIdx.y, per_seq = a.hkv * a.blocks, b = seg / per_seq, within = seg % per_seq;
+  const int steps = head_steps(seq_len(a, b)), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // the weight before this sequence, and all of it
   __shared__ long long sums[2][kWarps];
+  __shared__ float joined[kWarps][kPart];
   long long before = 0, total = 0;
   for (int i = threadIdx.x; i < a.batch; i += kThreads) {
     const long long u = seq_weight(a, i);
@@ -556,55 +555,67 @@ __global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_const
     total += __shfl_xor_sync(0xffffffffu, total, off);
     before += __shfl_xor_sync(0xffffffffu, before, off);
   }
-  if (lane == 0) { sums[0][threadIdx.x >> 5] = total; sums[1][threadIdx.x >> 5] = before; }
+  if (lane == 0) { sums[0][warp] = total; sums[1][warp] = before; }
   __syncthreads();
   total = before = 0;
   for (int w = 0; w < kWarps; ++w) { total += sums[0][w]; before += sums[1][w]; }
   const long long first = before + (long long)within * head_weight(steps) + kHeadCost;  // its first step
   const long long per = total > 0 ? (total + workers - 1) / workers : 1;
-  const long long c0 = first / per, c1 = steps > 0 ? (first + steps - 1) / per : c0;
-  const int h = within / a.blocks, g0 = within % a.blocks * block_rows, rows = min(block_rows, a.group - g0);
+  const long long c0 = first / per;
+  const int parts = steps > 0 ? (int)((first + steps - 1) / per - c0) + 1 : 0;
+  const int h = within / a.blocks, g0 = within % a.blocks * block_rows;
   // the partials are complete and visible; blocks without any wait too, so
   // that this grid never ends before the one it follows
   wait_previous();
-  if (steps > 0 && c0 == c1) return;
-  for (int row = threadIdx.x >> 5; row < rows; row += kWarps) {
-    float m = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (steps > 0)
-      for (long long c = c0; c <= c1; c += 32) {
-        // 32 parts at a time: their maxima and sums first, a lane each, then
-        // the outputs, all loads independent
-        const int n = (int)min(32LL, c1 - c + 1);
-        const float* part = a.partial + ((c + seg) * block_rows + row) * kPart;
-        const long long stride = (long long)block_rows * kPart;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (lane < n) ml = *reinterpret_cast<const float2*>(part + lane * stride + D);
-        float mn = fmaxf(m, ml.x);
+  if (parts == 1 || row >= min(block_rows, a.group - g0)) return;  // block-uniform
+  float m = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = warp * 32; c < parts; c += 32 * kWarps) {
+    // maxima and sums first, a lane each, then the outputs, all loads independent
+    const int n = min(32, parts - c);
+    const float* part = a.partial + ((c0 + c + seg) * block_rows + row) * kPart;
+    const long long stride = (long long)block_rows * kPart;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(part + lane * stride + D);
+    float mn = fmaxf(m, ml.x);
 #pragma unroll
-        for (int off = 16; off; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-        const float ref = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - ref), f = ex2(ml.x - ref);
-        float sum = f * ml.y;
+    for (int off = 16; off; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+    const float ref = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - ref), f = ex2(ml.x - ref);
+    float sum = f * ml.y;
 #pragma unroll
-        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        l = l * f0 + sum;
-        m = mn;
+    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    l = l * f0 + sum;
+    m = mn;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] *= f0;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-          const float fi = __shfl_sync(0xffffffffu, f, i);
-          const float2 u = *reinterpret_cast<const float2*>(part + i * stride + lane * 4);
-          const float2 v = *reinterpret_cast<const float2*>(part + i * stride + lane * 4 + 2);
-          y[0] += fi * u.x;
-          y[1] += fi * u.y;
-          y[2] += fi * v.x;
-          y[3] += fi * v.y;
-        }
-      }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    *reinterpret_cast<uint2*>(a.o + (long long)b * a.ldo + (long long)(h * a.group + g0 + row) * D + lane * 4) =
-        make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
+    for (int e = 0; e < 4; ++e) y[e] *= f0;
+#pragma unroll 16
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const float2 u = *reinterpret_cast<const float2*>(part + i * stride + lane * 4);
+      const float2 v = *reinterpret_cast<const float2*>(part + i * stride + lane * 4 + 2);
+      y[0] += fi * u.x;
+      y[1] += fi * u.y;
+      y[2] += fi * v.x;
+      y[3] += fi * v.y;
+    }
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) joined[warp][lane * 4 + e] = y[e];
+  if (lane == 0) { joined[warp][D] = m; joined[warp][D + 1] = l; }
+  __syncthreads();
+  const int d = threadIdx.x;  // a column each
+  static_assert(kThreads == D, "a thread per column");
+  float mx = -INFINITY, sum = 0.0f, v = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, joined[w][D]);
+  const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const float f = ex2(joined[w][D] - ref);
+    sum += f * joined[w][D + 1];
+    v += f * joined[w][d];
+  }
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  a.o[(long long)b * a.ldo + (long long)(h * a.group + g0 + row) * D + d] = f32_to_bf16_rne(v * inv);
 }
 
 // Caches of up to this many tokens are not split: at 1024 keys one block per
@@ -681,7 +692,7 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
   ENNX_TRY(rows == 8 ? launch<8>(a, table, need != 0, segs, dev, s) : launch<16>(a, table, need != 0, segs, dev, s));
   if (!need) return ENNX_B200_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)segs);
+  cfg.gridDim = dim3((unsigned)segs, (unsigned)(group < rows ? group : rows));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute early;

@@ -380,6 +380,8 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
         for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
     }
     const uint32_t tile = ring.wait(p.status) + row_at(g) + 16 * t;  // row g + 8: row_at(8) further on
+    __syncwarp();  // all lanes have read the tile before this one,
+    fetch();       // whose place is filled again while this one is used
 #pragma unroll
     for (int j = 0; j < kTileChunks; ++j) {
       if (j < n_chunks) {
@@ -391,8 +393,6 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
         }
       }
     }
-    __syncwarp();
-    fetch();
     if (now.pass == passes - 1) {
       float4(&buf)[kWarps][kN][32] = sh.red[done & 1];
       ++done;

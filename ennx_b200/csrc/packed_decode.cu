@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
     for (int pass = 0; pass < sp.passes; ++pass) {
       if (sp.passes > 1) load_x(pass);
       cp_wait<kStages - 2>();
-      __syncwarp();
+      __syncwarp();  // the stage is there, and all lanes have read the one before it,
+      fetch();       // which is filled again while this one is used
       const uint32_t c0 = slice0(pass);
       {
         uint32_t addr[2], element[2];
@@ -405,8 +406,6 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
         }
       }
       st = st + S::kBytes == ring + kStages * S::kBytes ? ring : st + S::kBytes;
-      __syncwarp();
-      fetch();
     }
     if (sp.along > 1) {
       // one barrier a tile: the other buffer is written again only after the
