@@ -90,11 +90,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   mma_16x8x16(c, a[0], a[1], a[2], a[3], b0, b1);
 }
-__device__ __forceinline__ void turn(float& x1, float& x2, float s, float c) {
-  const float y1 = x1 * c - x2 * s;
-  x2 = x2 * c + x1 * s;
-  x1 = y1;
-}
 // hi parts of a pair packed, the pair replaced by what is left
 __device__ __forceinline__ uint32_t take_hi(float& x, float& y) {
   const uint32_t hi = pack_bf16x2(x, y);
@@ -162,7 +157,7 @@ struct Head {
           for (int i = 0; i < 2; ++i) {
             const int from = (16 * (kk & 1) + 8 * e + 2 * t + i) & 31;
             const float s = __shfl_sync(0xffffffffu, sn[kk >> 1], from), c = __shfl_sync(0xffffffffu, cs[kk >> 1], from);
-            if (a.rotate) turn(x[i], y[i], s, c);
+            if (a.rotate) rope_turn(x[i], y[i], s, c);
             if (!live) x[i] = y[i] = 0.0f;
           }
           const uint32_t xh = take_hi(x[0], x[1]), yh = take_hi(y[0], y[1]);
@@ -197,7 +192,7 @@ struct Head {
     for (int e = 0; e < 2; ++e) {
       const int d = lane + 32 * e;
       float x1 = bf16_to_f32(__ldg(kn + d)), x2 = bf16_to_f32(__ldg(kn + d + 64));
-      if (a.rotate) turn(x1, x2, sn[e], cs[e]);
+      if (a.rotate) rope_turn(x1, x2, sn[e], cs[e]);
       const uint16_t b1 = f32_to_bf16_rne(x1), b2 = f32_to_bf16_rne(x2);
       kw[d] = b1;
       kw[d + 64] = b2;
@@ -359,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __g
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ double inv[64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = table.inv[threadIdx.x];
+  if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = rope_inv(table, threadIdx.x);
   __syncthreads();
   uint8_t* mine = smem + warp * kWarpRing;
   const uint32_t ring = smem_u32(mine), lo_parts = smem_u32(smem) + kWarps * kWarpRing + warp * kLoBytes;
@@ -415,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_split_kernel(const __g
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ double inv[64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = table.inv[threadIdx.x];
+  if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = rope_inv(table, threadIdx.x);
   __syncthreads();
   uint8_t* mine = smem + warp * kWarpRing;
   const uint32_t ring = smem_u32(mine), lo_parts = smem_u32(smem) + kWarps * kWarpRing + warp * kLoBytes;
@@ -618,8 +613,10 @@ __global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_const
   a.o[(long long)b * a.ldo + (long long)(h * a.group + g0 + row) * D + d] = f32_to_bf16_rne(v * inv);
 }
 
-// Caches of up to this many tokens are not split: at 1024 keys one block per
-// head takes about as long as a split and its join together.
+// Caches of up to this many tokens are not split.  A block per head against a
+// split and its join (16 query heads on 4 cache heads): 64 keys 3.8 and 7.8 us,
+// 512 keys 7.8 and 11.3, 1024 keys 12.1 and 11.5; 64 sequences of 1024 keys 24
+// and 31.
 constexpr int kWholeRoom = 1024;
 
 // query heads per block of rows: 8 leave room for the lo parts in the tile,
@@ -674,6 +671,11 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
       (((uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->q | (uintptr_t)p->o) & 15u))
     return set_error(ENNX_B200_INVALID_ARGUMENT,
                      "attention_decode: caches, q and o must be 16-byte aligned with strides of a multiple of 8");
+  const auto shared = [&](int64_t seq, int64_t token, int64_t head) {
+    return (p->batch > 1 && !seq) || (p->room > 1 && !token) || (p->hkv > 1 && !head);
+  };
+  if (p->k && (shared(p->k_seq, p->k_token, p->k_head) || shared(p->v_seq, p->v_token, p->v_head)))
+    return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: a cache that takes k and v cannot have strides of 0");
   const int group = p->hq / p->hkv, rows = block_rows(group), blocks = (group + rows - 1) / rows;
   const int64_t segs = (int64_t)p->batch * p->hkv * blocks;
   if (segs > 0x7fffffffLL - 65536) return set_error(ENNX_B200_UNSUPPORTED, "attention_decode: too many heads");

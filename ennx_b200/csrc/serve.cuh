@@ -77,6 +77,20 @@ __device__ __forceinline__ void rope_sincos(double inv, int pos, float* s, float
   const double turns = (double)pos * inv;
   sincospif((float)(2.0 * (turns - rint(turns))), s, c);
 }
+// inv[i] for an i of the lane's own.  An indexed read of a parameter goes to the
+// constant cache, one lane after another; the generic address does not.
+__device__ __forceinline__ double rope_inv(const RopeTable& table, int i) {
+  double v;
+  asm("ld.f64 %0, [%1];" : "=d"(v) : "l"(table.inv + i));
+  return v;
+}
+// A pair turned.  The operations are spelled out, so that a prompt's pass and a
+// token step leave the same bits in a cache.
+__device__ __forceinline__ void rope_turn(float& x1, float& x2, float s, float c) {
+  const float y1 = fmaf(x1, c, -__fmul_rn(x2, s));
+  x2 = fmaf(x2, c, __fmul_rn(x1, s));
+  x1 = y1;
+}
 // host: inv[i] = theta^(-2i/128) / (2*pi)
 const RopeTable& rope_table(float theta);
 

@@ -257,9 +257,10 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention(uint16_t* q, uint16_t* k, const ui
  * sequence: their o, q and k are left as they are, and what q, k and v hold
  * there reaches no output.  If rope_theta > 0, rotary embedding (rotate-half
  * pairing, position = row within its sequence, angles reduced in 64 bits) is
- * applied to q and k IN PLACE first.  o must not overlap q, k or v.  Softmax
- * statistics in fp32; a non-finite key or value reaches only the rows that
- * see it.  Allocates nothing. */
+ * applied to q and k IN PLACE first, which then overlap neither one another
+ * nor v.  o must not overlap q, k or v.  Softmax statistics in fp32; a
+ * non-finite key or value reaches only the rows that see it.  Allocates
+ * nothing. */
 ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uint16_t* k, int64_t ld_k,
                                                      const uint16_t* v, int64_t ld_v, uint16_t* o, int64_t ld_o,
                                                      const int32_t* cu_seqlens, int32_t num_seqs, int64_t rows,
@@ -274,10 +275,12 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, 
  * to rows 0 .. p.  Without k and v the caches already hold row p.  lengths[b]
  * = 0: nothing is written to the caches and o is 0.  Rows behind p may hold
  * anything; an infinity or NaN in row p or before makes the outputs it enters
- * non-finite (NaN where their limit would be an infinity).  All bf16; strides in elements.  Cache strides (multiples of 8)
- * are free, so [batch, room, heads, 128] and [batch, heads, room, 128] both
- * fit; the caches, q and o are 16-byte aligned, ld_q and ld_o multiples of 8;
- * sequences given k and v must not share cache rows.  workspace (device,
+ * non-finite (NaN where their limit would be an infinity).  All bf16; strides
+ * in elements.  Cache strides (multiples of 8) are free, so [batch, room,
+ * heads, 128] and [batch, heads, room, 128] both fit; the caches, q and o are
+ * 16-byte aligned, ld_q and ld_o multiples of 8.  Caches that take k and v
+ * share no rows between sequences or heads; k and v lie outside them.  o may
+ * be q itself and overlaps nothing else.  workspace (device,
  * 16-byte aligned) >= ennx_b200_gqa_attention_decode_workspace_size(...)
  * bytes, which is 0 for small rooms; calls that may overlap need one each. */
 typedef struct {
@@ -530,7 +533,7 @@ ENNX_B200_API int32_t ennx_b200_packed_linear_bf16(const uint16_t* x, int64_t to
  * once -- ennx_b200_packed_linear_bf16 rounds every weight to bf16 first.  Any
  * widths, group size and arena alignment (x and out 2-byte, scales and biases
  * 4-byte aligned); x bf16 [tokens, input_width] and out [tokens, output_width]
- * contiguous.  tokens == 0 does nothing. */
+ * contiguous, out apart from all that is read.  tokens == 0 does nothing. */
 ENNX_B200_API int32_t ennx_b200_packed_linear_decode(const uint16_t* x, int64_t tokens, const uint8_t* weights,
                                                      const float* scales, const float* biases,
                                                      const ennx_b200_packed_linear* linear,

@@ -118,6 +118,22 @@ def test_new_token_without_rope_and_out_with_a_stride():
     assert (wide[:, 4 * D:] == 5.0).all()
 
 
+@pytest.mark.parametrize("room,hq", [(300, 4), (3000, 4), (3000, 40)])
+def test_out_may_be_the_queries(room, hq):
+    kc, vc, q = rnd(3, room, 2, D, seed=50), rnd(3, room, 2, D, seed=51), rnd(3, hq, D, seed=52)
+    want, ln = q.clone(), i32([room, 0, 77])
+    ref = ops.gqa_attention_decode(want, kc, vc, ln)
+    assert torch.equal(ops.gqa_attention_decode(want, kc, vc, ln, out=want), ref)
+
+
+def test_sequences_that_share_a_cache_they_only_read():
+    kc, vc, q = rnd(1, 2000, 2, D, seed=53), rnd(1, 2000, 2, D, seed=54), rnd(3, 4, D, seed=55)
+    kc, vc = kc.expand(3, -1, -1, -1), vc.expand(3, -1, -1, -1)
+    check(ops.gqa_attention_decode(q, kc, vc, i32([2000, 3, 1500]), rope_theta=0.0), q, kc, vc, [2000, 3, 1500])
+    with pytest.raises(ValueError, match="strides of 0"):
+        ops.gqa_attention_decode(q, kc, vc, i32([9, 3, 1]), k=rnd(3, 2, D, seed=56), v=rnd(3, 2, D, seed=57))
+
+
 def test_large_scores_and_far_positions():
     n = 100001
     kc, vc = rnd(1, n, 1, D, seed=12, std=5.0), rnd(1, n, 1, D, seed=13)

@@ -35,6 +35,7 @@ def test_packed_attention_refuses_on_the_host():
     assert "aligned" in refused(*call(ldk=260))
     assert "aligned" in refused(*call(v=P(264 + 2)))
     assert "rope_theta" in refused(*call(theta=float("nan")))
+    assert "cannot be shared" in refused(*call(ldq=512, theta=1e6))
     assert "too many rows" in refused(*call(rows=1 << 31), status=_abi.UNSUPPORTED)
     assert getattr(_abi.lib(), "ennx_b200_gqa_attention_packed")(*call(rows=0)[1:]) == _abi.OK
 
@@ -58,6 +59,10 @@ def test_decode_attention_refuses_on_the_host():
     assert "negative" in refused(*call(k_seq=-8192))
     assert "multiple of 8" in refused(*call(v_token=260))
     assert "aligned" in refused(*call(k_cache=260))
+    assert "strides of 0" in refused(*call(k_seq=0))
+    assert "strides of 0" in refused(*call(v_head=0))
+    assert "strides of 0" in refused(*call(v_token=0))
+    assert "workspace" in refused(*call(k=0, v=0, k_seq=0, workspace=None))  # caches that are only read may share
     assert "workspace" in refused(*call(workspace=None))
     assert "workspace" in refused(*call(size=1000))
     assert "workspace" in refused(*call(workspace=P(260)))
