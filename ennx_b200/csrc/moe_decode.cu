@@ -82,6 +82,10 @@ struct Ring {
     ++used;
     return smem_u32(base) + at * stage_bytes;
   }
+  __device__ __forceinline__ void drain(int* status) {  // after a wait that gave up: no copy may land behind the block
+    if (!bad) return;
+    for (int i = max(0, fetched - kStages); i < fetched; ++i) mbar_wait(full + i % kStages, (i / kStages) & 1, status);
+  }
 };
 
 // ---------------------------------------------------------------------------
@@ -422,6 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
     if (!next(now)) break;
     reload = passes > 1 || now.a != a || now.group != group;
   }
+  ring.drain(p.status);
 }
 
 // ---------------------------------------------------------------------------
@@ -439,8 +444,8 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
 // before the end.
 //
 // kDirect (at most kN * 8 tokens): the columns of a product are the tokens, an
-// expert's other columns are zero, and the sums stay in the accumulators over
-// all experts.  Otherwise the columns are the tokens that picked the expert and
+// expert's other columns are zero, and the sums stay in registers over all
+// experts.  Otherwise the columns are the tokens that picked the expert and
 // are added to sums in shared memory, all of a lane's old values read before
 // the first is written.
 // ---------------------------------------------------------------------------
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
       }
     };
     Walk held{}, w{row_begin, 0, 0, 0};
-    int held_at = -1;
+    int held_at = -1, last_at = -1;
     for (int at = 0; w.row0 < row_end; ++at) {
       if (at % kCopyWarps == warp - kWarps) {
         const int stage = at % kDepth, bytes = min(kPassChunks, chunks - w.pass * kPassChunks) * 64;
@@ -533,7 +538,8 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
           copy_act(held, held_at);
           held_at = -1;
         }
-        if (!mbar_wait(&sh.free[stage], ((at / kDepth) & 1) ^ 1u, p.status)) return;
+        if (!mbar_wait(&sh.free[stage], ((at / kDepth) & 1) ^ 1u, p.status)) break;
+        last_at = at;
         if (lane == 0) mbar_arrive_expect_tx(&sh.full[stage], rows * bytes);
         __syncwarp();
         if (lane < rows) bulk_copy(smem_u32(sh.ring[stage].weights) + lane * kWeightPitch, src, bytes, &sh.full[stage]);
@@ -550,6 +556,10 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
       wait_previous();
       copy_act(held, held_at);
     }
+    // no copy may land behind the block, whose other warps skip their waits
+    // once one has given up; the warp's earlier copies came before this one's
+    static_assert(kDepth == kCopyWarps, "a copying warp has one stage");
+    if (last_at >= 0) mbar_wait(&sh.full[last_at % kDepth], (last_at / kDepth) & 1, p.status);
     return;
   }
 
@@ -564,7 +574,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
   bool bad = false;  // a wait gave up: later ones are not tried again, the results are void
   int at = 0;
   for (int row0 = row_begin; row0 < row_end; row0 += kRows) {
-    float acc[kN][4] = {};
+    float total[kN][4] = {};  // kDirect
     Walk w{row0, 0, 0, 0};
     bool more = true;
     for (; more; ++at, more = next(w)) {
@@ -575,7 +585,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
       uint32_t column[kN];
       bool live[kN], any[kN];  // any: some column of the block has a token
       uint32_t to[kN][2];
-      float old[kN][4];
+      float acc[kN][4] = {}, old[kN][4];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         if constexpr (kDirect) {
@@ -594,7 +604,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            acc[n][j] = old[n][j] = 0.0f;
+            old[n][j] = 0.0f;
             if (to[n][j & 1] && (j < 2 || g < kRows - 8)) old[n][j] = lds_f32(to[n][j & 1] + 32 * (j >> 1));
           }
         }
@@ -621,7 +631,15 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.free[stage]);
-      if constexpr (!kDirect) {
+      if constexpr (kDirect) {
+        // only tokens of the expert: another's zeros times an infinite weight are no zeros
+        const uint32_t takers = s.takers[s.expert[w.a]][0];
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (takers >> (n * 8 + 2 * t + (j & 1)) & 1u) total[n][j] += acc[n][j];
+      } else {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -637,7 +655,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = n * 8 + 2 * t + (j & 1), r = g + 8 * (j >> 1);
-          if (tok < p.tokens && r < kRows) sums[tok * kRows + r] = acc[n][j];
+          if (tok < p.tokens && r < kRows) sums[tok * kRows + r] = total[n][j];
         }
     }
     const int rows = min(kRows, row_end - row0);

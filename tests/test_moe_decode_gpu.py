@@ -132,6 +132,20 @@ def test_a_bad_token_or_expert_stays_with_its_own():
     assert torch.equal(y[~uses], clean[~uses]) and not y[uses].isfinite().any()
 
 
+@pytest.mark.parametrize("T", [3, 12, 40])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_bad_down_weights_reach_only_the_tokens_of_their_expert(T, bad):
+    H, E, k, I = 256, 8, 2, 128
+    x, (wr, wgu, wd) = rnd(T, H, seed=24), weights(H, E, I, 25)
+    clean, idx, _ = ops.moe_layer_decode(x, wr, wgu, wd, k, return_routing=True)
+    e = int(idx[0, 0])
+    wd[e, 3:, ::5] = bad
+    y = ops.moe_layer_decode(x, wr, wgu, wd, k)
+    touched = (idx == e).any(1)
+    assert torch.equal(y[~touched], clean[~touched]) and torch.equal(y[:, :3], clean[:, :3])
+    assert not y[touched][:, 3:].isfinite().any()
+
+
 def test_residual_in_place_and_other_stream_and_graph():
     T, H, E, k, I = 4, 512, 16, 4, 128
     x, (wr, wgu, wd) = rnd(T, H, seed=24), weights(H, E, I, 25)
