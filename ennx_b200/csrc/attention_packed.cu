@@ -87,6 +87,24 @@ __device__ __forceinline__ bool elect_one() {  // one lane of the (converged) wa
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
   return p != 0;
 }
+// Takes over a block of this grid that has not started: the answer, 16 bytes,
+// completes on `bar`.  After an answer of "none" it must not be asked again.
+__device__ __forceinline__ void request_block(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int answered_block(const uint4* answer) {  // its blockIdx.x, -1: none
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 a, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}"
+      : "=r"(x) : "r"(smem_u32(answer)) : "memory");
+  return x;
+}
 __device__ __forceinline__ float low(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float high(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 // 2^x of a pair on the FMA units: x = n + f with n the nearest integer (left in
@@ -133,11 +151,18 @@ struct Operands {
   long long ldq, ldk, ldv, ldo;
 };
 
+// A work item: the grid index whose head and rows it takes, -1 behind the
+// last, and the first rows of the sequences that hold its tiles' first rows.
+struct Item {
+  int index, first[2];
+};
 struct Bars {
-  uint64_t q_full, kv_full[2], kv_free[2], s_full[2], p_full[2][2] /*[tile][half of the keys]*/, o_done[2];
+  uint4 next;  // what the request for another item answered
+  uint64_t next_full, item_full[2], item_free[2];
+  uint64_t q_full, q_free, kv_full[2], kv_free[2], s_full[2], p_full[2][2] /*[tile][half of the keys]*/, o_done[2];
+  Item item[2];
   uint32_t tmem_base;
   int abort_flag;
-  int first[2];  // first_row of both tiles' first rows
 };
 static_assert(sizeof(Bars) <= 256, "barrier block must fit the reserved 256 bytes");
 
@@ -192,23 +217,35 @@ __global__ void __launch_bounds__(THREADS, 1)
   Bars& bar = *reinterpret_cast<Bars*>(sV + 2 * TILE);
 
   // Later rows first, all heads of a block of rows next to one another: the
-  // last blocks to start are then the packing's first rows, which see few keys
-  // whatever the lengths are (with heads outside blocks of any cost
+  // last items to start are then the packing's first rows, which see few keys
+  // whatever the lengths are (with heads outside items of any cost
   // start last: ragged 16384 tokens 254 us, so 210), and the heads that
   // share a cache head share its tiles in L2.
-  const int qb = (int)((gridDim.x - 1 - blockIdx.x) / heads);
-  const int h = (int)((gridDim.x - 1 - blockIdx.x) % heads), kvh = h / group;
-  const int q0 = qb * 2 * BQ;
+  const int items = (int)gridDim.x;
+  auto row_of = [&](int index) { return (items - 1 - index) / heads * (2 * BQ); };
+  auto head_of = [&](int index) { return (items - 1 - index) % heads; };
   const int end = pk.end();
-  if (q0 >= end) {  // block-uniform: rows behind the last sequence stay as they are
+  if (row_of((int)blockIdx.x) >= end) {  // block-uniform: rows behind the last sequence stay as they are
     wait_previous();
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto load_q = [&](int index) {
+    const int q0 = row_of(index), h = head_of(index), nq = q0 + BQ < end ? 2 : 1;
+    mbar_arrive_expect_tx(&bar.q_full, nq * TILE);
+    for (int x = 0; x < nq; ++x) {
+      tma_load_2d(sQ + x * TILE, &tmQ, &bar.q_full, h * D, q0 + x * BQ);
+      tma_load_2d(sQ + x * TILE + SUB, &tmQ, &bar.q_full, h * D + 64, q0 + x * BQ);
+    }
+  };
 
   if (threadIdx.x == 0) {
+    mbar_init(&bar.next_full, 1);
     mbar_init(&bar.q_full, 1);
+    mbar_init(&bar.q_free, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.item_full[i], 1);
+      mbar_init(&bar.item_free[i], 1 + SOFTMAX_WARPS);
       mbar_init(&bar.kv_full[i], 1);
       mbar_init(&bar.kv_free[i], 1);
       mbar_init(&bar.s_full[i], 1);
@@ -220,15 +257,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     fence_barrier_init();
     fence_proxy_async();
     wait_previous();
-    const int nq = q0 + BQ < end ? 2 : 1;
-    mbar_arrive_expect_tx(&bar.q_full, nq * TILE);
-    for (int x = 0; x < nq; ++x) {
-      tma_load_2d(sQ + x * TILE, &tmQ, &bar.q_full, h * D, q0 + x * BQ);
-      tma_load_2d(sQ + x * TILE + SUB, &tmQ, &bar.q_full, h * D + 64, q0 + x * BQ);
-    }
+    load_q((int)blockIdx.x);
   }
   if (warp == 1) { tmem_alloc(&bar.tmem_base, 512); tmem_relinquish(); }
-  if (threadIdx.x >= 64 && threadIdx.x < 66) bar.first[threadIdx.x - 64] = pk.first_row(q0 + ((int)threadIdx.x - 64) * BQ);
+  if (threadIdx.x >= 64 && threadIdx.x < 66) {
+    const int x = (int)threadIdx.x - 64;
+    bar.item[0].first[x] = pk.first_row(row_of((int)blockIdx.x) + x * BQ);
+    bar.item[0].index = (int)blockIdx.x;
+  }
   wait_previous();  // q and k are rotated; what stands above reads neither
   tc_fence_before();
   __syncthreads();
@@ -237,33 +273,91 @@ __global__ void __launch_bounds__(THREADS, 1)
   volatile int* abort_flag = &bar.abort_flag;
   // key tiles on the 128-row grid, numbered from the one that holds A's first
   // key: tile x uses [js[x], je[x]), its diagonal tile last; B may be empty
-  const int kt0 = bar.first[0] / BKV;
-  const bool two = q0 + BQ < end;
-  const int js[2] = {0, two ? max(0, bar.first[1] / BKV - kt0) : 0};
-  const int je[2] = {q0 / BKV + 1 - kt0, two ? q0 / BKV + 2 - kt0 : 0};
-  const int nt = two ? je[1] : je[0];
+  struct Tiles {
+    int q0, h, kt0, js[2], je[2], nt;
+  };
+  auto tiles_of = [&](const Item& it) {
+    Tiles w;
+    w.q0 = row_of(it.index);
+    w.h = head_of(it.index);
+    w.kt0 = it.first[0] / BKV;
+    const bool two = w.q0 + BQ < end;
+    w.js[0] = 0;
+    w.js[1] = two ? max(0, it.first[1] / BKV - w.kt0) : 0;
+    w.je[0] = w.q0 < end ? w.q0 / BKV + 1 - w.kt0 : 0;
+    w.je[1] = two ? w.q0 / BKV + 2 - w.kt0 : 0;
+    w.nt = two ? w.je[1] : w.je[0];
+    return w;
+  };
+  // by a whole warp, the same answer in every lane
+  auto warp_wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, err)) != 0; };
+  // the n-th item of this block, by a whole warp; index -1: no more
+  auto take_item = [&](int n) {
+    Item it{-1, {0, 0}};
+    if (__any_sync(0xffffffffu, *abort_flag) || !warp_wait(&bar.item_full[n & 1], (n >> 1) & 1)) return it;
+    it = bar.item[n & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar.item_free[n & 1]);
+    return it;
+  };
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS));
   if (warp == 0) {
     if (lane == 0) {
-      int issued = 0;
-      for (int j = 0; j < nt && !*abort_flag; ++j) {
-        const int s = j & 1;
-        if (!mbar_wait(&bar.kv_free[s], ((j >> 1) & 1) ^ 1u, err)) { *abort_flag = 1; break; }
-        mbar_arrive_expect_tx(&bar.kv_full[s], 2 * TILE);
-        const int krow = (kt0 + j) * BKV;
-        uint8_t* k = sK + s * TILE;
-        uint8_t* v = sV + s * TILE;
-        tma_load_2d(k, &tmK, &bar.kv_full[s], kvh * D, krow);
-        tma_load_2d(k + SUB, &tmK, &bar.kv_full[s], kvh * D + 64, krow);
-        tma_load_2d(v, &tmV, &bar.kv_full[s], kvh * D, krow);
-        tma_load_2d(v + SUB, &tmV, &bar.kv_full[s], kvh * D + 64, krow);
-        issued = j + 1;
+      int tiles = 0, loads = 1, asked = 0;  // K/V tiles, Q loads and requests so far
+      bool ok = true;
+      Item it = bar.item[0];
+      mbar_arrive(&bar.item_full[0]);
+      for (int n = 0;; ++n) {
+        const Tiles w = tiles_of(it);
+        const int kvh = w.h / group;
+        auto ask = [&] {
+          fence_proxy_async();  // the answer before has been read
+          mbar_arrive_expect_tx(&bar.next_full, sizeof(uint4));
+          request_block(&bar.next, &bar.next_full);
+          ++asked;
+        };
+        if (n > 0 && w.nt > 0) {
+          ok = mbar_wait(&bar.q_free, (loads & 1) ^ 1, err);
+          if (!ok) break;
+          load_q(it.index);
+          ++loads;
+        }
+        for (int j = 0; j < w.nt; ++j, ++tiles) {
+          // late, so that blocks with little left take what is left
+          if (j == w.nt - 1) ask();
+          const int s = tiles & 1;
+          ok = !*abort_flag && mbar_wait(&bar.kv_free[s], ((tiles >> 1) & 1) ^ 1u, err);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bar.kv_full[s], 2 * TILE);
+          const int krow = (w.kt0 + j) * BKV;
+          uint8_t* k = sK + s * TILE;
+          uint8_t* v = sV + s * TILE;
+          tma_load_2d(k, &tmK, &bar.kv_full[s], kvh * D, krow);
+          tma_load_2d(k + SUB, &tmK, &bar.kv_full[s], kvh * D + 64, krow);
+          tma_load_2d(v, &tmV, &bar.kv_full[s], kvh * D, krow);
+          tma_load_2d(v + SUB, &tmV, &bar.kv_full[s], kvh * D + 64, krow);
+        }
+        if (!ok) break;
+        if (w.nt == 0) ask();
+        ok = mbar_wait(&bar.next_full, n & 1, err);
+        if (!ok) break;
+        it.index = answered_block(&bar.next);
+        if (it.index >= 0)
+          for (int x = 0; x < 2; ++x) it.first[x] = pk.first_row(row_of(it.index) + x * BQ);
+        const int m = n + 1;
+        ok = mbar_wait(&bar.item_free[m & 1], ((m >> 1) & 1) ^ 1, err);
+        if (!ok) break;
+        bar.item[m & 1] = it;
+        mbar_arrive(&bar.item_full[m & 1]);
+        if (it.index < 0) break;
       }
-      if (issued < nt) {  // giving up: no copy may land after the block has gone
-        mbar_wait(&bar.q_full, 0, err);
-        for (int j = max(0, issued - 2); j < issued; ++j) mbar_wait(&bar.kv_full[j & 1], (j >> 1) & 1, err);
+      if (!ok) {  // giving up: no copy may land after the block has gone
+        *abort_flag = 1;
+        mbar_wait(&bar.q_full, (loads - 1) & 1, err);
+        for (int i = max(0, tiles - 2); i < tiles; ++i) mbar_wait(&bar.kv_full[i & 1], (i >> 1) & 1, err);
+        if (asked > 0) mbar_wait(&bar.next_full, (asked - 1) & 1, err);
       }
     }
   } else if (warp == 1) {
@@ -279,10 +373,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       kd[i] = smem_desc_sw128(smem_u32(sK + i * TILE));
       vd[i] = smem_desc_sw128_mn(smem_u32(sV + i * TILE), SUB);
     }
+    int tiles = 0, loads = 0, p_seen[2] = {0, 0}, s_left = 0;  // K/V tiles, items and P tiles so far, S of this item
+    bool ok = true;
     auto s_mma = [&](int x, int j) -> bool {  // S_X = Q_X K(j)^T
-      if (!mbar_wait(&bar.kv_full[j & 1], (j >> 1) & 1, err)) return false;
+      const int at = tiles + j;
+      if (!warp_wait(&bar.kv_full[at & 1], (at >> 1) & 1)) return false;
       tc_fence_after();
-      const uint64_t a = x ? qd[1] : qd[0], b = j & 1 ? kd[1] : kd[0];
+      const uint64_t a = x ? qd[1] : qd[0], b = at & 1 ? kd[1] : kd[0];
+      --s_left;
       if (elected) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -290,39 +388,50 @@ __global__ void __launch_bounds__(THREADS, 1)
           umma_f16(tmem + x * 256, a + off, b + off, IDESC_QK, kk != 0);
         }
         umma_commit(&bar.s_full[x]);
+        if (s_left == 0) umma_commit(&bar.q_free);
       }
       __syncwarp();
       return true;
     };
-    bool ok = mbar_wait(&bar.q_full, 0, err);
-    for (int x = 0; ok && x < 2; ++x)
-      if (je[x] > 0 && js[x] == 0) ok = s_mma(x, 0);
-    for (int j = 0; ok && j < nt && !*abort_flag; ++j) {
-      const int last_user = j < je[1] && j >= js[1] ? 1 : 0;
-      const uint64_t b = j & 1 ? vd[1] : vd[0];
+    for (int n = 0; ok; ++n) {
+    const Item it = take_item(n);
+    if (it.index < 0) break;
+    const Tiles w = tiles_of(it);
+    if (w.nt == 0) continue;
+    s_left = w.je[0] - w.js[0] + w.je[1] - w.js[1];
+    ok = warp_wait(&bar.q_full, loads++ & 1);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (ok && w.je[x] > 0 && w.js[x] == 0) ok = s_mma(x, 0);
+    for (int j = 0; ok && j < w.nt && !__any_sync(0xffffffffu, *abort_flag); ++j) {
+      const int last_user = j < w.je[1] && j >= w.js[1] ? 1 : 0, at = tiles + j;
+      const uint64_t b = at & 1 ? vd[1] : vd[0];
+#pragma unroll
       for (int x = 0; x < 2; ++x) {
-        if (j >= je[x]) continue;
-        if (j >= js[x]) {
+        if (!ok || j >= w.je[x]) continue;
+        if (j >= w.js[x]) {
           // O_X += P_X(j) V(j), P_X in tensor memory over the first 64 columns of S_X
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (!mbar_wait(&bar.p_full[x][half], (j - js[x]) & 1, err)) { ok = false; break; }
+            if (ok) ok = warp_wait(&bar.p_full[x][half], p_seen[x] & 1);
             tc_fence_after();
-            if (elected) {
+            if (ok && elected) {
 #pragma unroll
               for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, b + kk * 128, IDESC_PV, j != js[x] || kk != 0);
+                umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, b + kk * 128, IDESC_PV, j != w.js[x] || kk != 0);
               if (half == 1) {
                 umma_commit(&bar.o_done[x]);
-                if (x == last_user) umma_commit(&bar.kv_free[j & 1]);
+                if (x == last_user) umma_commit(&bar.kv_free[at & 1]);
               }
             }
             __syncwarp();
           }
-          if (!ok) break;
+          ++p_seen[x];
         }
-        if (j + 1 >= js[x] && j + 1 < je[x] && !s_mma(x, j + 1)) { ok = false; break; }
+        if (ok && j + 1 >= w.js[x] && j + 1 < w.je[x]) ok = s_mma(x, j + 1);
       }
+    }
+    tiles += w.nt;
     }
     if (!ok) *abort_flag = 1;
   }
@@ -331,24 +440,30 @@ __global__ void __launch_bounds__(THREADS, 1)
     // softmax: tile x, TMEM lane quarter q = warp % 4, a thread per row
     const int x = (warp - 4) >> 2;
     const int q = warp & 3;
-    const int qx0 = q0 + x * BQ;
-    const int qpos = qx0 + q * 32 + lane;
     const uint32_t s_col = tmem + ((uint32_t)(q * 32) << 16) + x * 256;  // S_X (P_X over its first 64 columns)
     const uint32_t o_col = s_col + 128;                                   // O_X
-    const int steps = je[x] - js[x];
+    int seen = 0;  // S tiles of the items before
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+    const Item it = take_item(n);
+    if (it.index < 0) break;
+    const Tiles w = tiles_of(it);
+    const int steps = w.je[x] - w.js[x], h = w.h, kvh = h / group;
+    if (steps == 0) continue;
+    const int qx0 = w.q0 + x * BQ;
+    const int qpos = qx0 + q * 32 + lane;
     const int lo = pk.first_row(qpos);
     const int max_lo = __reduce_max_sync(0xffffffffu, lo);
     float m = -INFINITY, l = 0.0f;
-    bool ok = true;
     for (int j = 0; j < steps; ++j) {
-      ok = !*abort_flag && mbar_wait(&bar.s_full[x], j & 1, err);
+      ok = !*abort_flag && mbar_wait(&bar.s_full[x], (seen + j) & 1, err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
-      const int k0 = (kt0 + js[x] + j) * BKV;
+      const int k0 = (w.kt0 + w.js[x] + j) * BKV;
       uint32_t v[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, v[c]);
@@ -424,8 +539,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       l = l * alpha + (low(both) + high(both));
       m = m_use;
     }
-    if (steps > 0 && ok) {
-      if (mbar_wait(&bar.o_done[x], (steps - 1) & 1, err)) {
+    seen += steps;
+    if (ok) {
+      ok = warp_wait(&bar.o_done[x], (seen - 1) & 1);
+      if (ok) {
         tc_fence_after();
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const bool mine = qpos >= pk.begin() && qpos < end;
@@ -460,6 +577,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       } else {
         *abort_flag = 1;
       }
+    }
     }
   }
   tc_fence_before();
