@@ -15,19 +15,32 @@
 // One CTA = two 128-row query tiles (A: rows q0..q0+127, B: q0+128..q0+255)
 // of one query head, key/value tiles of 128 keys on the same 128-row grid,
 // shared by both.  Tensor memory: S_A | O_A | S_B | O_B, 128 fp32 columns
-// each.  Warp roles: 0 TMA producer (two-slot K/V ring, no multicast); 1 one
+// each.  Warp roles: 0 TMA producer (two slots of K and of V); 1 one
 // thread issues tcgen05.mma (S = Q K^T; O += P V with P from tensor memory);
 // 4..11 softmax, four warps per query tile, a thread per row, statistics in
 // fp32, P rounded to bf16 (at most 2^-8 relative, random in sign, below the
 // rounding of the bf16 output).
 //
 // A key tile costs each query tile 1024 clocks of tensor work and, at 16 exp2 a
-// clock, 1024 clocks of the exponential unit, and with one query tile's products
-// running under the other's softmax neither may take longer.  So three eighths
-// of the exponentials are a cubic on the FMA units instead (`exp2_cubic`), P is
-// handed over in two halves so that its product starts under the second half,
-// and no two threads share a row (two per row and an exchange of maxima under
-// a barrier: 16384 tokens 1.19 ms).
+// clock, 1024 clocks of the exponential unit; one query tile's products run
+// under the other's softmax.  What bounds the loop is the chain of one query
+// tile, S -> softmax (2100 clocks) -> O += P V -> next S, 3700 clocks of which
+// 2048 are the two tiles' products.  P is handed over in two halves so that its
+// product starts under the second half, and no two threads share a row (two
+// per row and an exchange of maxima under a barrier: 16384 tokens 1.19 ms for
+// 1.04 then).  S in halves of 64 keys, one ahead of the other, breaks the
+// chain, but a 128 x 64 x 16 product lasts 48 clocks instead of 32 and both
+// softmaxes then compete for issue slots: 0.92 ms for 0.87.  A part of the
+// exponentials as a polynomial on the FMA units changed nothing.
+//
+// A block takes over the next item of the grid that has not started
+// (clusterlaunchcontrol), as late as its last key tile: barriers and tensor
+// memory are set up once and the next Q and K arrive while the last softmax
+// runs (ragged 16384 tokens 210 -> 203 us).
+//
+// Measured: one prompt of 16384 tokens, 16 heads on 4: 0.83 ms, 1320 TFLOP/s
+// (0.98 ms at the power limit); 12 ragged prompts of 16384 tokens 197 us, 860
+// TFLOP/s of visible scores.
 //
 // Masked places may hold anything: masked scores are replaced, not added to,
 // but a masked V row still meets P = 0 in the MMA and an infinity or NaN there
@@ -52,7 +65,8 @@ constexpr int SOFTMAX_WARPS = 8;
 constexpr int FEW_REGS = 56, MANY_REGS = 224;
 constexpr int THREADS = 128 + 32 * SOFTMAX_WARPS;
 static_assert(FEW_REGS + 2 * MANY_REGS <= 3 * 168 && THREADS == 384, "registers of the block");
-constexpr int SMEM = 6 * TILE /*Q_A, Q_B, 2 K, 2 V*/ + 1024 + 256;
+constexpr int BARS = 320;
+constexpr int SMEM = 6 * TILE /*Q_A, Q_B, 2 K, 2 V*/ + 1024 + BARS;
 constexpr uint32_t IDESC_QK = idesc_bf16_f32(128, 128);
 constexpr uint32_t IDESC_PV = idesc_bf16_f32(128, 128) | (1u << 16);  // B (V) MN-major
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the max grows by > 2^8
@@ -105,26 +119,13 @@ __device__ __forceinline__ int answered_block(const uint4* answer) {  // its blo
       : "=r"(x) : "r"(smem_u32(answer)) : "memory");
   return x;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float low(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float high(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-// 2^x of a pair on the FMA units: x = n + f with n the nearest integer (left in
-// the low bits by adding 1.5 * 2^23), |f| <= 1/2; 2^f by the cubic of least
-// largest relative error, 7.5e-5, found by the exchange algorithm (P is rounded
-// to bf16 next, 4e-3); then n is added to the exponent.  Below 2^-126 the result
-// stays there instead of going to 0, so masked scores take ex2.
-__device__ __forceinline__ uint64_t exp2_cubic(uint64_t x) {
-  const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f), minus = pack_f32x2(-12582912.0f, -12582912.0f);
-  const uint64_t negone = pack_f32x2(-1.0f, -1.0f);
-  x = pack_f32x2(fmaxf(low(x), -126.0f), fmaxf(high(x), -126.0f));
-  const uint64_t t = add_f32x2(x, magic), f = fma_f32x2(add_f32x2(t, minus), negone, x);
-  uint64_t y = fma_f32x2(f, pack_f32x2(0.05517166852951050f, 0.05517166852951050f),
-                         pack_f32x2(0.24261112511157990f, 0.24261112511157990f));
-  y = fma_f32x2(y, f, pack_f32x2(0.69326096773147583f, 0.69326096773147583f));
-  y = fma_f32x2(y, f, pack_f32x2(0.99992805719375610f, 0.99992805719375610f));
-  const uint32_t lo = ((uint32_t)t << 23) + (uint32_t)y, hi = ((uint32_t)(t >> 32) << 23) + (uint32_t)(y >> 32);
-  return ((uint64_t)hi << 32) | lo;
-}
-
 // Packed rows: [begin, end) belong to sequences, clamped to the rows there are.
 struct Packing {
   const int* cu;
@@ -159,12 +160,12 @@ struct Item {
 struct Bars {
   uint4 next;  // what the request for another item answered
   uint64_t next_full, item_full[2], item_free[2];
-  uint64_t q_full, q_free, kv_full[2], kv_free[2], s_full[2], p_full[2][2] /*[tile][half of the keys]*/, o_done[2];
+  uint64_t q_full, q_free, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2][2] /*[tile][half of the keys]*/, o_done[2];
   Item item[2];
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(Bars) <= 256, "barrier block must fit the reserved 256 bytes");
+static_assert(sizeof(Bars) <= BARS, "the barriers fit their place");
 
 // Output of one (row, head), by one warp, reading visible keys only; every sum
 // in fp32.
@@ -202,7 +203,6 @@ __device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int
 
 struct True { static constexpr bool value = true; };
 struct False { static constexpr bool value = false; };
-constexpr int kCubicOf8 = 3;  // of 8 pairs of exponentials, on the FMA units
 
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     wait_previous();
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // from lane 0, so that the compiler knows it to be the same in a warp
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto load_q = [&](int index) {
     const int q0 = row_of(index), h = head_of(index), nq = q0 + BQ < end ? 2 : 1;
     mbar_arrive_expect_tx(&bar.q_full, nq * TILE);
@@ -246,8 +247,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.item_full[i], 1);
       mbar_init(&bar.item_free[i], 1 + SOFTMAX_WARPS);
-      mbar_init(&bar.kv_full[i], 1);
-      mbar_init(&bar.kv_free[i], 1);
+      mbar_init(&bar.k_full[i], 1);
+      mbar_init(&bar.k_free[i], 1);
+      mbar_init(&bar.v_full[i], 1);
+      mbar_init(&bar.v_free[i], 1);
       mbar_init(&bar.s_full[i], 1);
       mbar_init(&bar.p_full[i][0], 4);
       mbar_init(&bar.p_full[i][1], 4);
@@ -298,6 +301,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     it = bar.item[n & 1];
     __syncwarp();
     if (lane == 0) mbar_arrive(&bar.item_free[n & 1]);
+    it.index = __shfl_sync(0xffffffffu, it.index, 0);  // (see `warp`)
+    it.first[0] = __shfl_sync(0xffffffffu, it.first[0], 0);
+    it.first[1] = __shfl_sync(0xffffffffu, it.first[1], 0);
     return it;
   };
 
@@ -305,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS));
   if (warp == 0) {
     if (lane == 0) {
-      int tiles = 0, loads = 1, asked = 0;  // K/V tiles, Q loads and requests so far
+      int tiles = 0, k_tiles = 0, loads = 1, asked = 0;  // V and K tiles, Q loads and requests so far
       bool ok = true;
       Item it = bar.item[0];
       mbar_arrive(&bar.item_full[0]);
@@ -328,16 +334,21 @@ __global__ void __launch_bounds__(THREADS, 1)
           // late, so that blocks with little left take what is left
           if (j == w.nt - 1) ask();
           const int s = tiles & 1;
-          ok = !*abort_flag && mbar_wait(&bar.kv_free[s], ((tiles >> 1) & 1) ^ 1u, err);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&bar.kv_full[s], 2 * TILE);
           const int krow = (w.kt0 + j) * BKV;
+          const uint32_t empty = ((tiles >> 1) & 1) ^ 1u;
           uint8_t* k = sK + s * TILE;
           uint8_t* v = sV + s * TILE;
-          tma_load_2d(k, &tmK, &bar.kv_full[s], kvh * D, krow);
-          tma_load_2d(k + SUB, &tmK, &bar.kv_full[s], kvh * D + 64, krow);
-          tma_load_2d(v, &tmV, &bar.kv_full[s], kvh * D, krow);
-          tma_load_2d(v + SUB, &tmV, &bar.kv_full[s], kvh * D + 64, krow);
+          ok = !*abort_flag && mbar_wait(&bar.k_free[s], empty, err);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bar.k_full[s], TILE);
+          tma_load_2d(k, &tmK, &bar.k_full[s], kvh * D, krow);
+          tma_load_2d(k + SUB, &tmK, &bar.k_full[s], kvh * D + 64, krow);
+          ++k_tiles;
+          ok = mbar_wait(&bar.v_free[s], empty, err);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bar.v_full[s], TILE);
+          tma_load_2d(v, &tmV, &bar.v_full[s], kvh * D, krow);
+          tma_load_2d(v + SUB, &tmV, &bar.v_full[s], kvh * D + 64, krow);
         }
         if (!ok) break;
         if (w.nt == 0) ask();
@@ -356,82 +367,79 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) {  // giving up: no copy may land after the block has gone
         *abort_flag = 1;
         mbar_wait(&bar.q_full, (loads - 1) & 1, err);
-        for (int i = max(0, tiles - 2); i < tiles; ++i) mbar_wait(&bar.kv_full[i & 1], (i >> 1) & 1, err);
+        for (int i = max(0, k_tiles - 2); i < k_tiles; ++i) mbar_wait(&bar.k_full[i & 1], (i >> 1) & 1, err);
+        for (int i = max(0, tiles - 2); i < tiles; ++i) mbar_wait(&bar.v_full[i & 1], (i >> 1) & 1, err);
         if (asked > 0) mbar_wait(&bar.next_full, (asked - 1) & 1, err);
       }
     }
   } else if (warp == 1) {
     // The whole warp runs the loop, one elected lane issues: descriptors then
-    // stay in uniform registers.  Built per product by a lone lane, they made
-    // an instruction every 110 clocks, which a 128 x 128 x 16 product does not
-    // last (64).
+    // stay in uniform registers.
     const bool elected = elect_one();
-    uint64_t qd[2], kd[2], vd[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      qd[i] = smem_desc_sw128(smem_u32(sQ + i * TILE));
-      kd[i] = smem_desc_sw128(smem_u32(sK + i * TILE));
-      vd[i] = smem_desc_sw128_mn(smem_u32(sV + i * TILE), SUB);
-    }
-    int tiles = 0, loads = 0, p_seen[2] = {0, 0}, s_left = 0;  // K/V tiles, items and P tiles so far, S of this item
+    const uint64_t qd = smem_desc_sw128(smem_u32(sQ));
+    const uint64_t kd = smem_desc_sw128(smem_u32(sK)), vd = smem_desc_sw128_mn(smem_u32(sV), SUB);
+    int tiles = 0, loads = 0, p_seen[2] = {0, 0}, k_seen = 0;  // key tiles, items and P tiles so far; K waited for
     bool ok = true;
-    auto s_mma = [&](int x, int j) -> bool {  // S_X = Q_X K(j)^T
-      const int at = tiles + j;
-      if (!warp_wait(&bar.kv_full[at & 1], (at >> 1) & 1)) return false;
-      tc_fence_after();
-      const uint64_t a = x ? qd[1] : qd[0], b = at & 1 ? kd[1] : kd[0];
-      --s_left;
-      if (elected) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t off = ((kk >> 2) * SUB + (kk & 3) * 32) >> 4;
-          umma_f16(tmem + x * 256, a + off, b + off, IDESC_QK, kk != 0);
-        }
-        umma_commit(&bar.s_full[x]);
-        if (s_left == 0) umma_commit(&bar.q_free);
-      }
-      __syncwarp();
-      return true;
-    };
     for (int n = 0; ok; ++n) {
-    const Item it = take_item(n);
-    if (it.index < 0) break;
-    const Tiles w = tiles_of(it);
-    if (w.nt == 0) continue;
-    s_left = w.je[0] - w.js[0] + w.je[1] - w.js[1];
-    ok = warp_wait(&bar.q_full, loads++ & 1);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (ok && w.je[x] > 0 && w.js[x] == 0) ok = s_mma(x, 0);
-    for (int j = 0; ok && j < w.nt && !__any_sync(0xffffffffu, *abort_flag); ++j) {
-      const int last_user = j < w.je[1] && j >= w.js[1] ? 1 : 0, at = tiles + j;
-      const uint64_t b = at & 1 ? vd[1] : vd[0];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (!ok || j >= w.je[x]) continue;
-        if (j >= w.js[x]) {
-          // O_X += P_X(j) V(j), P_X in tensor memory over the first 64 columns of S_X
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (ok) ok = warp_wait(&bar.p_full[x][half], p_seen[x] & 1);
-            tc_fence_after();
-            if (ok && elected) {
-#pragma unroll
-              for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, b + kk * 128, IDESC_PV, j != w.js[x] || kk != 0);
-              if (half == 1) {
-                umma_commit(&bar.o_done[x]);
-                if (x == last_user) umma_commit(&bar.kv_free[at & 1]);
-              }
-            }
-            __syncwarp();
-          }
-          ++p_seen[x];
+      const Item it = take_item(n);
+      if (it.index < 0) break;
+      const Tiles w = tiles_of(it);
+      if (w.nt == 0) continue;
+      ok = warp_wait(&bar.q_full, loads++ & 1);
+      auto s_mma = [&](int x, int j) {  // S_X = Q_X K(j)^T
+        const int at = tiles + j;
+        if (at >= k_seen) {
+          k_seen = at + 1;
+          ok = ok && warp_wait(&bar.k_full[at & 1], (at >> 1) & 1);
         }
-        if (ok && j + 1 >= w.js[x] && j + 1 < w.je[x]) ok = s_mma(x, j + 1);
+        tc_fence_after();
+        const uint64_t a = qd + (x * TILE >> 4), b = kd + ((at & 1) * TILE >> 4);
+        const bool last_user = x == 1 || j < w.js[1] || j >= w.je[1];
+        if (ok && elected) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off = ((kk >> 2) * SUB + (kk & 3) * 32) >> 4;
+            umma_f16(tmem + x * 256, a + off, b + off, IDESC_QK, kk != 0);
+          }
+          umma_commit(&bar.s_full[x]);
+          if (last_user) umma_commit(&bar.k_free[at & 1]);
+          if (last_user && j == w.nt - 1) umma_commit(&bar.q_free);
+        }
+        __syncwarp();
+      };
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (w.je[x] > 0 && w.js[x] == 0) s_mma(x, 0);
+      for (int j = 0; ok && j < w.nt && !__any_sync(0xffffffffu, *abort_flag); ++j) {
+        const int at = tiles + j;
+        const uint64_t b = vd + ((at & 1) * TILE >> 4);
+        ok = warp_wait(&bar.v_full[at & 1], (at >> 1) & 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (j >= w.js[x] && j < w.je[x]) {
+            // O_X += P_X(j) V(j), P_X in tensor memory over the first 64 columns of S_X
+            const bool last_user = x == 1 || j < w.js[1] || j >= w.je[1];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && warp_wait(&bar.p_full[x][half], p_seen[x] & 1);
+              tc_fence_after();
+              if (ok && elected) {
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                  umma_f16_ts(tmem + x * 256 + 128, tmem + x * 256 + kk * 8, b + kk * 128, IDESC_PV, j != w.js[x] || kk != 0);
+                if (half == 1) {
+                  umma_commit(&bar.o_done[x]);
+                  if (last_user) umma_commit(&bar.v_free[at & 1]);
+                }
+              }
+              __syncwarp();
+            }
+            ++p_seen[x];
+          }
+          if (ok && j + 1 >= w.js[x] && j + 1 < w.je[x]) s_mma(x, j + 1);
+        }
       }
-    }
-    tiles += w.nt;
+      tiles += w.nt;
     }
     if (!ok) *abort_flag = 1;
   }
@@ -453,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int qx0 = w.q0 + x * BQ;
     const int qpos = qx0 + q * 32 + lane;
     const int lo = pk.first_row(qpos);
-    const int max_lo = __reduce_max_sync(0xffffffffu, lo);
+    const int max_lo = __reduce_max_sync(0xffffffffu, lo), min_lo = __reduce_min_sync(0xffffffffu, lo);
     float m = -INFINITY, l = 0.0f;
     for (int j = 0; j < steps; ++j) {
       ok = !*abort_flag && mbar_wait(&bar.s_full[x], (seen + j) & 1, err);
@@ -469,14 +477,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, v[c]);
       tmem_ld_wait();
       // warp-uniform: some key lies outside some row's [lo, row]
-      const bool masked = k0 + BKV - 1 > qx0 + q * 32 || k0 < max_lo;
+      const int row0 = qx0 + q * 32;
+      const bool masked = k0 + BKV - 1 > row0 || k0 < max_lo;
+      uint32_t blank = 0;  // a bit per 32 keys that no row of the warp sees
       if (masked) {
-        const int a = lo - k0, b = qpos - k0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          const int kc = k0 + c * 32, a = lo - kc, b = qpos - kc;
+          if (kc > row0 + 31 || kc + 31 < min_lo) {
+            blank |= 1u << c;
+          } else if (kc + 31 > row0 || kc < max_lo) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c * 32 + i < a || c * 32 + i > b) v[c][i] = 0xff800000u;  // -inf
+            for (int i = 0; i < 32; ++i)
+              if (i < a || i > b) v[c][i] = 0xff800000u;  // -inf
+          }
+        }
       }
       // row max of the raw scores (the positive scale commutes with max)
       float top[4];
@@ -485,8 +500,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         top[c] = __uint_as_float(v[c][0]);
 #pragma unroll
         for (int i = 1; i + 1 < 32; i += 2)
-          top[c] = fmaxf(top[c], fmaxf(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])));
+          top[c] = max3(top[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
         top[c] = fmaxf(top[c], __uint_as_float(v[c][31]));
+      }
+      if (blank) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (blank >> c & 1u) top[c] = -INFINITY;
       }
       const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale_log2);
       const bool rescale = m == -INFINITY ? true : (m_new > m + kRescaleThreshold);
@@ -508,20 +528,24 @@ __global__ void __launch_bounds__(THREADS, 1)
       const float nm = m_use == -INFINITY ? 0.0f : -m_use;
       const uint64_t c2 = pack_f32x2(scale_log2, scale_log2), nm2 = pack_f32x2(nm, nm);
       uint64_t sum[2] = {0ull, 0ull};
-      auto half_p = [&](int half, auto cubic) {
+      auto put_half = [&](int half, auto blanks) {  // without the test where nothing is masked
         uint32_t pk2[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) {
+          if (decltype(blanks)::value && (blank >> (2 * half + c) & 1u)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk2[16 * c + i] = 0u;
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const uint32_t* s2 = &v[2 * half + c][2 * i];
             const uint64_t t = fma_f32x2(((uint64_t)s2[1] << 32) | s2[0], c2, nm2);
-            uint64_t e;
-            if (decltype(cubic)::value && i % 8 < kCubicOf8) e = exp2_cubic(t);
-            else e = pack_f32x2(ex2(low(t)), ex2(high(t)));
+            const uint64_t e = pack_f32x2(ex2(low(t)), ex2(high(t)));
             sum[i & 1] = add_f32x2(sum[i & 1], e);
             pk2[16 * c + i] = pack_bf16x2(low(e), high(e));
           }
+        }
         tmem_st32(s_col + half * 32, pk2);
         tmem_st_wait();
         tc_fence_before();
@@ -529,11 +553,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(&bar.p_full[x][half]);
       };
       if (masked) {
-        half_p(0, False{});
-        half_p(1, False{});
+        put_half(0, True{});
+        put_half(1, True{});
       } else {
-        half_p(0, True{});
-        half_p(1, True{});
+        put_half(0, False{});
+        put_half(1, False{});
       }
       const uint64_t both = add_f32x2(sum[0], sum[1]);
       l = l * alpha + (low(both) + high(both));
