@@ -26,8 +26,8 @@
 // output) goes to the workspace in fp32 and a second kernel joins the partials
 // in order.  (Runs of blocks, with a merge of their warps and an empty ring at
 // the end of each sequence, took 40 us instead of 32 on 32 ragged sequences
-// of up to 4096 keys.)  Small caches take one block per head instead, whose
-// warps share the keys and merge once, and no second kernel.
+// of up to 4096 keys.)  Shorter caches take a block per head, or a cluster of up
+// to 8, whose warps share the keys and meet once, and no second kernel.
 #include "kernels.cuh"
 #include "serve.cuh"
 
@@ -96,6 +96,16 @@ __device__ __forceinline__ uint32_t take_hi(float& x, float& y) {
   x -= __uint_as_float(hi << 16);
   y -= __uint_as_float(hi & 0xffff0000u);
   return hi;
+}
+__device__ __forceinline__ uint32_t cluster_ctas() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ float2 lds_cluster(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
 }
 // 16-byte chunk `c` of row `r` in a tile of 256-byte rows
 __device__ __forceinline__ uint32_t at(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) << 4)); }
@@ -346,25 +356,28 @@ __device__ __forceinline__ const uint16_t* head_base(const uint16_t* cache, long
   return cache + (long long)b * seq_stride + (long long)h * head_stride;
 }
 
-// Small caches: one block per (sequence, cache head, head block); its warps
-// take the steps in turn and are merged at the end.
+// Short caches: one block, or a cluster of up to 8, per (sequence, cache head,
+// block of query heads); the warps take the steps in turn, are merged per block
+// and then over distributed shared memory, row by row.
 template <int kRows>
 __global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __grid_constant__ Args a,
                                                                        const __grid_constant__ RopeTable table) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ double inv[64];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster_ctarank(), cluster = (int)cluster_ctas();
   if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = rope_inv(table, threadIdx.x);
   __syncthreads();
   uint8_t* mine = smem + warp * kWarpRing;
   const uint32_t ring = smem_u32(mine), lo_parts = smem_u32(smem) + kWarps * kWarpRing + warp * kLoBytes;
-  const int per_seq = a.hkv * a.blocks, b = blockIdx.x / per_seq, len = seq_len(a, b), steps = head_steps(len);
+  const int seg = (int)blockIdx.x / cluster, per_seq = a.hkv * a.blocks, b = seg / per_seq;
+  const int len = seq_len(a, b), steps = head_steps(len);
   Head<kRows> s;
-  s.place(a, b, blockIdx.x % per_seq, len);
+  s.place(a, b, seg % per_seq, len);
   const uint16_t *kbase = head_base(a.c.k, a.c.kb, a.c.kh, b, s.h), *vbase = head_base(a.c.v, a.c.vb, a.c.vh, b, s.h);
-  const int n = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 4, ..
+  const int first = rank * kWarps + warp, stride = cluster * kWarps;  // steps first, first + stride, ..
+  const int n = steps > first ? (steps - first + stride - 1) / stride : 0;
   auto fetch = [&](int i) {
-    if (i < n) copy_step(a, kbase, vbase, (warp + i * kWarps) * kStep, len, ring + i % kStages * kStageBytes, lane);
+    if (i < n) copy_step(a, kbase, vbase, (first + i * stride) * kStep, len, ring + i % kStages * kStageBytes, lane);
     cp_commit();
   };
 #pragma unroll
@@ -374,33 +387,78 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __g
     cp_wait<kStages - 2>();
     __syncwarp();            // the stage is there, and all lanes have read the one before it,
     fetch(i + kStages - 1);  // which is filled again while this one is used
-    const int key0 = (warp + i * kWarps) * kStep, p = len - 1 - key0;
+    const int key0 = (first + i * stride) * kStep, p = len - 1 - key0;
     if (a.knew && p >= 0 && p < kStep) s.append(a, mine + i % kStages * kStageBytes, p, lane);
     s.step(a, ring + i % kStages * kStageBytes, lo_parts, key0, lane);
   }
   cp_wait<0>();
   s.close();
-  __syncthreads();  // every ring is drained: the merge buffer may overlay them
+  __syncthreads();  // every ring is drained: the merge buffers may overlay them
   float* merge = reinterpret_cast<float*>(smem);  // [warp][row][kPart]
+  float* joined = merge + kWarps * 16 * kPart;        // [row][kPart], of this block
+  static_assert((kWarps + 1) * 16 * kPart * 4 <= kWarps * kWarpRing, "the merge buffers overlay the rings");
   s.put_partial(merge + warp * 16 * kPart, lane);
   __syncthreads();
+  auto put = [&](int row, const float (&y)[4], float sum) {
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    *reinterpret_cast<uint2*>(a.o + (long long)b * a.ldo + (long long)(s.hq0 + row) * D + lane * 4) =
+        make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
+  };
   for (int row = warp; row < s.rows; row += kWarps) {
-    float mx = -INFINITY, sum = 0.0f, f[kWarps], y[4] = {};
+    float mx = -INFINITY, sum = 0.0f, y[4] = {};
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, merge[(w * 16 + row) * kPart + D]);
     const float ref = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* part = merge + (w * 16 + row) * kPart;
-      f[w] = ex2(part[D] - ref);
-      sum += f[w] * part[D + 1];
+      const float f = ex2(part[D] - ref);
+      sum += f * part[D + 1];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += f[w] * part[lane * 4 + e];
+      for (int e = 0; e < 4; ++e) y[e] += f * part[lane * 4 + e];
     }
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    *reinterpret_cast<uint2*>(a.o + (long long)b * a.ldo + (long long)(s.hq0 + row) * D + lane * 4) =
-        make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
+    if (cluster == 1) {
+      put(row, y, sum);
+    } else {
+      float* to = joined + row * kPart;
+      *reinterpret_cast<float2*>(to + lane * 4) = make_float2(y[0], y[1]);
+      *reinterpret_cast<float2*>(to + lane * 4 + 2) = make_float2(y[2], y[3]);
+      if (lane == 0) *reinterpret_cast<float2*>(to + D) = make_float2(mx, sum);
+    }
   }
+  if (cluster == 1) return;
+  cluster_sync();
+  for (int row = rank + cluster * warp; row < s.rows; row += stride) {
+    float2 ml = make_float2(-INFINITY, 0.0f), u[8], v[8];
+    if (lane < cluster) ml = lds_cluster(mapa_shared(joined + row * kPart + D, lane));
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < cluster) {
+        const uint32_t from = mapa_shared(joined + row * kPart + lane * 4, c);
+        u[c] = lds_cluster(from);
+        v[c] = lds_cluster(from + 8);
+      }
+    float mx = ml.x;
+#pragma unroll
+    for (int off = 4; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));  // lanes 0 .. 7
+    mx = __shfl_sync(0xffffffffu, mx, 0);
+    const float f = ex2(ml.x - (mx == -INFINITY ? 0.0f : mx));
+    float sum = f * ml.y, y[4] = {};
+#pragma unroll
+    for (int off = 4; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    sum = __shfl_sync(0xffffffffu, sum, 0);
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < cluster) {
+        const float fc = __shfl_sync(0xffffffffu, f, c);
+        y[0] += fc * u[c].x;
+        y[1] += fc * u[c].y;
+        y[2] += fc * v[c].x;
+        y[3] += fc * v[c].y;
+      }
+    put(row, y, sum);
+  }
+  cluster_sync();  // no block leaves while its rows are being read
 }
 
 // Any cache: every warp an equal run of all steps.
@@ -613,26 +671,73 @@ __global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_const
   a.o[(long long)b * a.ldo + (long long)(h * a.group + g0 + row) * D + d] = f32_to_bf16_rne(v * inv);
 }
 
-// Caches of up to this many tokens are not split.  A block per head against a
-// split and its join (16 query heads on 4 cache heads): 64 keys 3.8 and 7.8 us,
-// 512 keys 7.8 and 11.3, 1024 keys 12.1 and 11.5; 64 sequences of 1024 keys 24
-// and 31.
-constexpr int kWholeRoom = 1024;
-
 // query heads per block of rows: 8 leave room for the lo parts in the tile,
 // more heads share one reading of the cache by 16
 int block_rows(int group) { return group <= 8 ? 8 : 16; }
 
 int split_grid() { return kPerSm * sm_count(); }
 
+int64_t segments(int64_t batch, int hq, int hkv) {
+  const int group = hq / hkv, rows = block_rows(group);
+  return batch * hkv * ((group + rows - 1) / rows);
+}
+
+// Blocks of a head: one for each 128 tokens of room, 8 at most and two per SM
+// over all heads; a single one up to 256 tokens, where a cluster's start and
+// meeting cost more (64 keys 3.8 us, 5.2 in a cluster; 300 keys 6.1 and 5.2;
+// 4096 keys 37 and 9.5).  0: the cache is split over the device.  That is for
+// rooms of more than 2048 tokens per block, where the longest sequence alone
+// would last longer than a split and its second kernel (one sequence of 16 query
+// heads on 4: 4096 keys 9.5 us and 17.4 split, 8192 keys 13.7 and 18.8, 16384
+// keys 22.9 and 20.9; 64 heads with 4096 keys 25 and 32; 32 ragged sequences of
+// up to 4096 keys 29.9 and 32.5).  The lengths are on the device, so the room
+// decides: one long sequence among empty ones takes up to 21 us instead of 11.
+int whole_cluster(int64_t segs, int room) {
+  int n = 1;
+  while (n < 8 && n * segs <= sm_count() && room > 256 && room > 128 * n) n *= 2;
+  return room <= 2048 * n ? n : 0;
+}
+
 template <int kRows>
-int32_t launch(const Args& a, const RopeTable& table, bool split, int64_t segs, int dev, cudaStream_t s) {
-  static SharedMemorySetup setup[2];
-  const auto kernel = split ? token_split_kernel<kRows> : token_whole_kernel<kRows>;
-  ENNX_TRY(allow_shared_memory(setup[split], dev, kernel, kSmem));
-  kernel<<<split ? (unsigned)split_grid() : (unsigned)segs, kThreads, kSmem, s>>>(a, table);
+int32_t launch_whole(const Args& a, const RopeTable& table, int64_t segs, int cluster, int dev, cudaStream_t s) {
+  static SharedMemorySetup setup;
+  ENNX_TRY(allow_shared_memory(setup, dev, token_whole_kernel<kRows>, kSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(segs * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute together;
+  together.id = cudaLaunchAttributeClusterDimension;
+  together.val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = &together;
+  cfg.numAttrs = 1;
+  ENNX_CUDA(cudaLaunchKernelEx(&cfg, token_whole_kernel<kRows>, a, table), "token attention");
   ENNX_LAUNCH_CHECK("token attention");
   return ENNX_B200_OK;
+}
+template <int kRows>
+int32_t launch_split(const Args& a, const RopeTable& table, int64_t segs, int dev, cudaStream_t s) {
+  static SharedMemorySetup setup;
+  ENNX_TRY(allow_shared_memory(setup, dev, token_split_kernel<kRows>, kSmem));
+  token_split_kernel<kRows><<<(unsigned)split_grid(), kThreads, kSmem, s>>>(a, table);
+  ENNX_LAUNCH_CHECK("token attention");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)segs, (unsigned)(a.group < kRows ? a.group : kRows));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  ENNX_CUDA(cudaLaunchKernelEx(&cfg, token_join_kernel, a, split_grid() * kWarps, kRows), "token attention join");
+  ENNX_LAUNCH_CHECK("token attention join");
+  return ENNX_B200_OK;
+}
+template <int kRows>
+int32_t launch(const Args& a, const RopeTable& table, int64_t segs, int cluster, int dev, cudaStream_t s) {
+  return cluster ? launch_whole<kRows>(a, table, segs, cluster, dev, s) : launch_split<kRows>(a, table, segs, dev, s);
 }
 
 }  // namespace
@@ -643,10 +748,10 @@ using namespace ennx;
 extern "C" {
 
 size_t ennx_b200_gqa_attention_decode_workspace_size(int32_t batch, int32_t room, int32_t hq, int32_t hkv) {
-  if (batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || room <= kWholeRoom) return 0;
-  const int rows = block_rows(hq / hkv);
-  const size_t segs = (size_t)batch * hkv * ((hq / hkv + rows - 1) / rows);
-  return (segs + (size_t)split_grid() * kWarps) * rows * kPart * sizeof(float);
+  if (batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv) return 0;
+  const int64_t segs = segments(batch, hq, hkv);
+  if (whole_cluster(segs, room)) return 0;
+  return ((size_t)segs + (size_t)split_grid() * kWarps) * block_rows(hq / hkv) * kPart * sizeof(float);
 }
 
 int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, float rope_theta, void* workspace,
@@ -677,7 +782,7 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
   if (p->k && (shared(p->k_seq, p->k_token, p->k_head) || shared(p->v_seq, p->v_token, p->v_head)))
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: a cache that takes k and v cannot have strides of 0");
   const int group = p->hq / p->hkv, rows = block_rows(group), blocks = (group + rows - 1) / rows;
-  const int64_t segs = (int64_t)p->batch * p->hkv * blocks;
+  const int64_t segs = segments(p->batch, p->hq, p->hkv);
   if (segs > 0x7fffffffLL - 65536) return set_error(ENNX_B200_UNSUPPORTED, "attention_decode: too many heads");
   const size_t need = ennx_b200_gqa_attention_decode_workspace_size(p->batch, p->room, p->hq, p->hkv);
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u)))
@@ -691,20 +796,8 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
   int dev = 0;
   int* status = nullptr;
   ENNX_TRY(serving_device(&dev, &status));
-  ENNX_TRY(rows == 8 ? launch<8>(a, table, need != 0, segs, dev, s) : launch<16>(a, table, need != 0, segs, dev, s));
-  if (!need) return ENNX_B200_OK;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)segs, (unsigned)(group < rows ? group : rows));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  ENNX_CUDA(cudaLaunchKernelEx(&cfg, token_join_kernel, a, split_grid() * kWarps, rows), "token attention join");
-  ENNX_LAUNCH_CHECK("token attention join");
-  return ENNX_B200_OK;
+  const int cluster = whole_cluster(segs, p->room);
+  return rows == 8 ? launch<8>(a, table, segs, cluster, dev, s) : launch<16>(a, table, segs, cluster, dev, s);
 }
 
 }  // extern "C"

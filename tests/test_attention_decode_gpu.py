@@ -56,12 +56,15 @@ def check(got, q, kc, vc, lengths, theta=0.0):
         assert err.max() <= 0, (b, n, float(err.max()))
 
 
-# rooms of at most 1024 take one block per head, larger ones are split over the device
+# a room that fits a cluster of blocks per head, 2048 tokens each, is not split over the device
 CASES = [
     (16, [1], 1, 1), (16, [16], 4, 1), (64, [17, 0, 63, 64], 4, 2), (300, [65, 299, 300], 16, 4),
     (1024, [1024, 1000, 1, 0, 129], 8, 2), (1025, [1025], 4, 4), (2048, [1, 0, 2048, 64, 65, 2047, 0], 16, 4),
     (5000, [4999, 3, 0, 0, 127, 128, 129], 16, 1), (40000, [40000], 4, 2), (3000, [2999], 17, 1), (1500, [1400, 20], 64, 2),
     (1100, [0, 0, 0], 4, 2), (2000, [11] * 200, 2, 1),
+    (200, [200, 77, 0], 24, 2), (500, [500, 31, 256, 257], 9, 3), (9000, [8999, 1, 4097], 32, 2), (1300, [1300, 3] * 25, 16, 2),
+    (20000, [19999, 3, 0, 0, 127, 128, 129], 16, 1), (17000, [1, 0, 16999, 64, 65, 2047, 0], 16, 4), (16385, [16385], 4, 4),
+    (17000, [2999], 17, 1), (17000, [1400, 20], 64, 2), (17000, [0, 0, 0], 4, 2), (2100, [11, 2100] * 100, 2, 1),
 ]
 
 
@@ -118,7 +121,7 @@ def test_new_token_without_rope_and_out_with_a_stride():
     assert (wide[:, 4 * D:] == 5.0).all()
 
 
-@pytest.mark.parametrize("room,hq", [(300, 4), (3000, 4), (3000, 40)])
+@pytest.mark.parametrize("room,hq", [(200, 4), (300, 4), (3000, 4), (3000, 40), (17000, 4), (17000, 40)])
 def test_out_may_be_the_queries(room, hq):
     kc, vc, q = rnd(3, room, 2, D, seed=50), rnd(3, room, 2, D, seed=51), rnd(3, hq, D, seed=52)
     want, ln = q.clone(), i32([room, 0, 77])
@@ -173,7 +176,7 @@ def test_lengths_outside_the_room_are_taken_as_the_nearest():
     check(o, q, kc, vc, [40, 0, 40])
 
 
-@pytest.mark.parametrize("room", [512, 4096])
+@pytest.mark.parametrize("room", [256, 512, 4096, 17000])
 def test_non_finite_values_that_are_seen(room):
     kc, vc, q = rnd(2, room, 2, D, seed=25), rnd(2, room, 2, D, seed=26), rnd(2, 4, D, seed=27).abs()
     vc[0, 100, 0, 7] = math.inf
@@ -185,7 +188,7 @@ def test_non_finite_values_that_are_seen(room):
     assert torch.equal(~o.isfinite(), bad)
 
 
-@pytest.mark.parametrize("room", [256, 3000])
+@pytest.mark.parametrize("room", [256, 3000, 17000])
 def test_two_graphs_interleaved_with_growing_lengths(room):
     kc, vc = torch.zeros(2, 2, room, 2, D, dtype=torch.bfloat16, device="cuda").unbind(0)
     q, k, v, ln = rnd(2, 4, D, seed=28), rnd(2, 2, D, seed=29), rnd(2, 2, D, seed=30), i32([100, 200])
@@ -209,8 +212,9 @@ def test_two_graphs_interleaved_with_growing_lengths(room):
         check(outs[step & 1], q, kc, vc, [101 + step, 201 + step], 1e6)
 
 
-def test_same_inputs_same_bits():
-    kc, vc, q = rnd(3, 5000, 4, D, seed=33), rnd(3, 5000, 4, D, seed=34), rnd(3, 16, D, seed=35)
+@pytest.mark.parametrize("room", [5000, 17000])
+def test_same_inputs_same_bits(room):
+    kc, vc, q = rnd(3, room, 4, D, seed=33), rnd(3, room, 4, D, seed=34), rnd(3, 16, D, seed=35)
     ln = i32([5000, 1234, 77])
     a = ops.gqa_attention_decode(q, kc, vc, ln, rope_theta=0.0)
     assert torch.equal(a, ops.gqa_attention_decode(q, kc, vc, ln, rope_theta=0.0))

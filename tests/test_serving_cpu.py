@@ -43,7 +43,7 @@ def test_packed_attention_refuses_on_the_host():
 def test_decode_attention_refuses_on_the_host():
     def call(theta=0.0, workspace=P(256), size=1 << 30, **over):
         f = dict(q=256, ld_q=512, k=256, ld_k=256, v=256, ld_v=256, k_cache=256, k_seq=8192, k_token=256, k_head=128,
-                 v_cache=256, v_seq=8192, v_token=256, v_head=128, lengths=256, o=256, ld_o=512, batch=2, room=2048,
+                 v_cache=256, v_seq=8192, v_token=256, v_head=128, lengths=256, o=256, ld_o=512, batch=2, room=1 << 20,
                  hq=4, hkv=2)
         f.update(over)
         return ("ennx_b200_gqa_attention_decode", ctypes.byref(_abi.DecodeAttention(**f)), theta, workspace, size, None)

@@ -60,7 +60,7 @@ class Layer:
         return h, fused, o, a, mid, m, idx, gate, y
 
 
-@pytest.mark.parametrize("room", [400, 1500])  # one block per head; split over the device
+@pytest.mark.parametrize("room", [400, 1500, 17000])  # clusters of blocks per head; split over the device
 def test_prompt_then_tokens(room):
     hidden, lengths = 512, [130, 0, 33, 300, 1]
     layer = Layer(hidden, 4, 2, 8, 3, 128, lengths, room)
