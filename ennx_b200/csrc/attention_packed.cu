@@ -44,8 +44,9 @@
 //
 // Masked places may hold anything: masked scores are replaced, not added to,
 // but a masked V row still meets P = 0 in the MMA and an infinity or NaN there
-// makes 0 * inf = NaN.  A non-finite output is therefore recomputed by
-// `careful_row`, which reads visible keys only.
+// makes 0 * inf = NaN.  Rows behind the last sequence are cleared in shared
+// memory; a non-finite output is recomputed by `careful_row`, which reads
+// visible keys only.
 #include "kernels.cuh"
 #include "serve.cuh"
 
@@ -414,6 +415,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int at = tiles + j;
         const uint64_t b = vd + ((at & 1) * TILE >> 4);
         ok = warp_wait(&bar.v_full[at & 1], (at >> 1) & 1);
+        // rows behind the last sequence may hold anything, their P is 0 and 0
+        // has to come out: cleared here, a row being 128 bytes of each sub-tile
+        const int live = end - (w.kt0 + j) * BKV;
+        if (ok && live < BKV) {
+          const uint32_t v = smem_u32(sV + (at & 1) * TILE);
+          for (int i = live * 8 + lane; i < BKV * 8; i += 32) {
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(v + i * 16), "r"(0) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(v + SUB + i * 16), "r"(0) : "memory");
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (j >= w.js[x] && j < w.je[x]) {

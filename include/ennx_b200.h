@@ -279,8 +279,8 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, 
  * in elements.  Cache strides (multiples of 8) are free, so [batch, room,
  * heads, 128] and [batch, heads, room, 128] both fit; the caches, q and o are
  * 16-byte aligned, ld_q and ld_o multiples of 8.  Caches that take k and v
- * share no rows between sequences or heads; k and v lie outside them.  o may
- * be q itself and overlaps nothing else.  workspace (device,
+ * share no rows between sequences, heads or each other, and k and v lie outside
+ * them.  o may be q itself and overlaps nothing else.  workspace (device,
  * 16-byte aligned) >= ennx_b200_gqa_attention_decode_workspace_size(...)
  * bytes, which is 0 for small rooms; calls that may overlap need one each. */
 typedef struct {

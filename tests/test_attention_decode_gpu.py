@@ -212,6 +212,21 @@ def test_two_graphs_interleaved_with_growing_lengths(room):
         check(outs[step & 1], q, kc, vc, [101 + step, 201 + step], 1e6)
 
 
+@pytest.mark.parametrize("room", [700, 17000])
+def test_two_streams_at_once(room):
+    kc, vc, q = rnd(5, room, 4, D, seed=60), rnd(5, room, 4, D, seed=61), rnd(5, 16, D, seed=62)
+    ln, streams = i32([room, 3, 0, 400, 650]), [torch.cuda.Stream() for _ in range(3)]
+    want = ops.gqa_attention_decode(q, kc, vc, ln)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ops.gqa_attention_decode(q, kc, vc, ln))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 @pytest.mark.parametrize("room", [5000, 17000])
 def test_same_inputs_same_bits(room):
     kc, vc, q = rnd(3, room, 4, D, seed=33), rnd(3, room, 4, D, seed=34), rnd(3, 16, D, seed=35)

@@ -166,6 +166,42 @@ def test_replayed_graph_with_other_lengths_and_a_side_stream():
         close(out[:n], reference(q[:n], k[:n], v[:n], lengths), vmax)
 
 
+def test_captured_with_the_rotation_and_many_items():
+    # more blocks than the device holds at once, q and k rotated in front, fresh operands at every replay
+    lengths, hq, hkv = [1500, 1, 700, 0, 1647, 252], 16, 4
+    rows = sum(lengths)
+    q, k, v = rnd(rows, hq, D, seed=30), rnd(rows, hkv, D, seed=31), rnd(rows, hkv, D, seed=32)
+    qs, ks, cu = q.clone(), k.clone(), starts(lengths)
+    want = ops.gqa_attention_packed(qs, ks, v, cu)
+    assert ((want.double() - reference(qs, ks, v, lengths)).abs() <= 1.001 * 2.0 ** -8 * 2 * float(v.float().abs().max())).all()
+    graph, q1, k1 = torch.cuda.CUDAGraph(), torch.empty_like(q), torch.empty_like(k)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        q1.copy_(q)
+        k1.copy_(k)
+        got = ops.gqa_attention_packed(q1, k1, v, cu)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(got, want) and torch.equal(q1, qs) and torch.equal(k1, ks)
+
+
+def test_two_streams_at_once():
+    lengths = [900, 37, 2200]
+    rows, one, two = sum(lengths), torch.cuda.Stream(), torch.cuda.Stream()
+    q, k, v = rnd(rows, 16, D, seed=33), rnd(rows, 4, D, seed=34), rnd(rows, 4, D, seed=35)
+    cu = starts(lengths)
+    want = ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for s in (one, two):
+            with torch.cuda.stream(s):
+                outs.append(ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_same_inputs_same_bits():
     lengths = [900, 124]
     q, k, v = rnd(1024, 8, D, seed=20), rnd(1024, 2, D, seed=21), rnd(1024, 2, D, seed=22)

@@ -59,13 +59,17 @@ def test_decode_attention_refuses_on_the_host():
     assert "negative" in refused(*call(k_seq=-8192))
     assert "multiple of 8" in refused(*call(v_token=260))
     assert "aligned" in refused(*call(k_cache=260))
+    assert "must be apart" in refused(*call())
     assert "strides of 0" in refused(*call(k_seq=0))
+    many = dict(batch=1 << 20, hq=1 << 8, hkv=1 << 8, room=(1 << 31) - 1, k=0, v=0, ld_q=1 << 15, ld_o=1 << 15)
+    assert "too many" in refused(*call(**many), status=_abi.UNSUPPORTED)
     assert "strides of 0" in refused(*call(v_head=0))
     assert "strides of 0" in refused(*call(v_token=0))
     assert "workspace" in refused(*call(k=0, v=0, k_seq=0, workspace=None))  # caches that are only read may share
-    assert "workspace" in refused(*call(workspace=None))
-    assert "workspace" in refused(*call(size=1000))
-    assert "workspace" in refused(*call(workspace=P(260)))
+    apart = dict(v_cache=1 << 40)
+    assert "workspace" in refused(*call(workspace=None, **apart))
+    assert "workspace" in refused(*call(size=1000, **apart))
+    assert "workspace" in refused(*call(workspace=P(260), **apart))
     assert getattr(_abi.lib(), "ennx_b200_gqa_attention_decode")(*call(batch=0)[1:]) == _abi.OK
     q = torch.zeros(2, 4, 128, dtype=BF16)
     c = torch.zeros(2, 8, 2, 128, dtype=BF16)
