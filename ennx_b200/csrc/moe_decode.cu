@@ -20,8 +20,8 @@
 // Products run on m16n8k16 with weight rows as the 16 rows and tokens as the
 // 8 columns; each warp streams its own weight tiles through a ring of bulk
 // copies, a row (512 bytes) each: copying with a 16-byte instruction per lane
-// instead took 6 times the instructions and was bound by them (64 tokens 212
-// us).  k is permuted the same way in both operands so that a lane's fragments
+// instead took 6 times the instructions and was bound by them (the
+// layer for 64 tokens 212 us).  k is permuted the same way in both operands so that a lane's fragments
 // are 16 contiguous bytes.
 #include "kernels.cuh"
 #include "serve.cuh"
@@ -229,13 +229,15 @@ struct Plan {
   int active;                    // experts that some token picked
   uint8_t expert[kExperts];      // active expert a
   uint16_t first[kExperts + 1];  // its first slot; slots run expert by expert, token by token
+  uint16_t groups[kExperts + 1];  // groups of tokens of the active experts before it
   uint16_t slot[kTokens * kTopK];  // t * kTopK + r of a slot
-  int scan[kWarps][2];
+  uint16_t scan[kWarps][3];
   __device__ __forceinline__ int token(int i) const { return slot[i] / kTopK; }
   __device__ __forceinline__ float gate(int i) const { return gates[slot[i]]; }
 };
 
 // by every thread of a block; those behind the first kThreads only keep step
+template <int kGroup>  // tokens of a group
 __device__ __forceinline__ void make_plan(const Layer& p, Plan& s) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool works = threadIdx.x < kThreads;
@@ -258,25 +260,33 @@ __device__ __forceinline__ void make_plan(const Layer& p, Plan& s) {
   }
   __syncthreads();
   const int n = works ? __popc(s.takers[threadIdx.x][0]) + __popc(s.takers[threadIdx.x][1]) : 0;
-  int slots = n, actives = n > 0;
+  const int own = (n + kGroup - 1) / kGroup;
+  int slots = n, actives = n > 0, groups = own;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, slots, off), b = __shfl_up_sync(0xffffffffu, actives, off);
-    if (lane >= off) { slots += a; actives += b; }
+    const int c = __shfl_up_sync(0xffffffffu, groups, off);
+    if (lane >= off) { slots += a; actives += b; groups += c; }
   }
-  if (works && lane == 31) { s.scan[warp][0] = slots; s.scan[warp][1] = actives; }
+  if (works && lane == 31) {
+    s.scan[warp][0] = (uint16_t)slots;
+    s.scan[warp][1] = (uint16_t)actives;
+    s.scan[warp][2] = (uint16_t)groups;
+  }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWarps - 1; ++w)
-    if (w < warp) { slots += s.scan[w][0]; actives += s.scan[w][1]; }
+    if (w < warp) { slots += s.scan[w][0]; actives += s.scan[w][1]; groups += s.scan[w][2]; }
   if (works) s.start[threadIdx.x] = (uint16_t)(slots - n);
   if (threadIdx.x == kThreads - 1) {
     s.active = actives;
     s.first[actives] = (uint16_t)slots;
+    s.groups[actives] = (uint16_t)groups;
   }
   if (n > 0) {
     s.expert[actives - 1] = (uint8_t)threadIdx.x;
     s.first[actives - 1] = (uint16_t)(slots - n);
+    s.groups[actives - 1] = (uint16_t)(groups - own);
   }
   __syncthreads();
 #pragma unroll
@@ -291,8 +301,10 @@ __device__ __forceinline__ void make_plan(const Layer& p, Plan& s) {
 }
 
 // ---------------------------------------------------------------------------
-// gate/up: a block takes an equal run of the (picked expert, column) list.  A
-// tile is 8 columns (8 gate rows and their 8 up rows) x all k, the k split
+// gate/up: a block takes an equal run of the (picked expert, column) list, an
+// expert's columns counted once per group of its tokens (counted once, a block
+// of an expert with 17 tokens or more took twice as long as the others: the
+// layer for 64 tokens with one such expert 193 us, now 136).  A tile is 8 columns (8 gate rows and their 8 up rows) x all k, the k split
 // over the warps; kN blocks of 8 tokens at a time stay in registers.
 // ---------------------------------------------------------------------------
 template <int kN>
@@ -313,12 +325,33 @@ __global__ void __launch_bounds__(kThreads, 1) token_gate_up_kernel(const __grid
   ring.init(sh.ring[warp][0], sh.full[warp], tile_bytes(16), lane);
   wait_previous();
   launch_dependents();
-  make_plan(p, s);
-  const long long columns = (long long)s.active * p.width;
-  const long long begin = columns * blockIdx.x / gridDim.x, end = columns * (blockIdx.x + 1) / gridDim.x;
+  constexpr bool kOneGroup = kN == 1;  // at most 8 tokens: every expert has one
+  make_plan<kN * 8>(p, s);
+  const long long units = (long long)(kOneGroup ? s.active : s.groups[s.active]) * p.width;
+  const long long begin = units * blockIdx.x / gridDim.x, end = units * (blockIdx.x + 1) / gridDim.x;
   if (begin >= end) return;
-  const int a_first = (int)(begin / p.width), a_last = (int)((end - 1) / p.width);
-  const int c_first = (int)(begin - (long long)a_first * p.width), c_last = (int)(end - (long long)a_last * p.width);
+  // expert and column of a place in the list
+  auto find = [&](int group) {  // the expert that holds a group
+    if constexpr (kOneGroup) return group;
+    int lo = 0, hi = s.active;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (s.groups[mid] <= group) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  auto column = [&](long long at, int a) {
+    if constexpr (kOneGroup) return (int)(at - (long long)a * p.width);
+    return (int)(at - (long long)s.groups[a] * p.width) / (s.groups[a + 1] - s.groups[a]);
+  };
+  const int a_first = find((int)(begin / p.width)), c_first = column(begin, a_first);
+  int a_last = find((int)((end - 1) / p.width)), c_last = column(end, a_last);
+  if (c_last == 0 && a_last > a_first) {  // the first column of the last expert is the next block's
+    --a_last;
+    c_last = p.width;
+  }
+  if (a_first == a_last && c_first >= c_last) return;
   const int chunks = p.hidden / kChunk, passes = (chunks + kWarps * kTileChunks - 1) / (kWarps * kTileChunks);
   const int per = ((chunks + passes - 1) / passes + kWarps - 1) / kWarps;  // chunks of a warp in a pass
 
@@ -491,7 +524,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) token_down_kernel(const __gri
   // the router grid has finished (every gate/up block waited for it before it
   // let this grid start), so the routing and the first weights can be fetched
   // while the gate/up products are still running
-  make_plan(p, s);
+  make_plan<kN * 8>(p, s);
   const int chunks = p.width / kChunk, passes = (chunks + kPassChunks - 1) / kPassChunks;
   const int row_begin = (int)((long long)p.hidden * blockIdx.x / gridDim.x);
   const int row_end = (int)((long long)p.hidden * (blockIdx.x + 1) / gridDim.x);

@@ -103,6 +103,21 @@ def test_all_tokens_pick_the_same_experts():
     check(y, x, wgu, wd, ridx, rgate)
 
 
+@pytest.mark.parametrize("T,E,k,I", [(64, 16, 2, 640), (64, 40, 4, 128), (17, 12, 1, 256), (49, 9, 3, 384)])
+def test_uneven_routing(T, E, k, I):
+    """Experts from one token to nearly all, so groups of tokens from one to four side by side."""
+    H = 256
+    x, (wr, wgu, wd) = rnd(T, H, seed=27), weights(H, E, I, 28)
+    pull = rnd(1, H, seed=31)
+    x = (x.float() + pull.float() * torch.linspace(0, 2, T, device="cuda")[:, None]).to(torch.bfloat16)
+    wr[E // 2] += pull[0] / 8
+    wr[E - 1] += pull[0] / 16
+    y, idx, gate = ops.moe_layer_decode(x, wr, wgu, wd, k, return_routing=True)
+    ridx, rgate = routing(x, wr, k)
+    assert torch.equal(idx.long(), ridx)
+    check(y, x, wgu, wd, ridx, rgate)
+
+
 @pytest.mark.parametrize("E,k", [(16, 8), (200, 8), (8, 8), (33, 1)])
 def test_ties_keep_the_lower_index(E, k):
     H, I = 256, 128
