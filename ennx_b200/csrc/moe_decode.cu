@@ -20,9 +20,9 @@
 // Products run on m16n8k16 with weight rows as the 16 rows and tokens as the
 // 8 columns; each warp streams its own weight tiles through a ring of bulk
 // copies, a row (512 bytes) each: copying with a 16-byte instruction per lane
-// instead took 6 times the instructions and was bound by them (the
-// layer for 64 tokens 212 us).  k is permuted the same way in both operands so that a lane's fragments
-// are 16 contiguous bytes.
+// instead took 6 times the instructions and was bound by them (the layer for 64
+// tokens 212 us).  k is permuted the same way in both operands so that a lane's
+// fragments are 16 contiguous bytes.
 #include "kernels.cuh"
 #include "serve.cuh"
 
