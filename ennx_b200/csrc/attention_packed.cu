@@ -169,38 +169,66 @@ struct Bars {
 static_assert(sizeof(Bars) <= BARS, "the barriers fit their place");
 
 // Output of one (row, head), by one warp, reading visible keys only; every sum
-// in fp32.
+// in fp32.  Keys come four at a time, their loads together.
 __device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int h, int kvh, float scale_log2, int lane) {
+  constexpr int kKeys = 4;
+  auto two = [](uint32_t w, float& a, float& b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+  };
   const uint2 qw = *reinterpret_cast<const uint2*>(t.q + (long long)row * t.ldq + h * D + lane * 4);
-  const uint32_t qp[2] = {qw.x, qw.y};
-  float m = -INFINITY, l = 0.0f, a[4] = {};
-  for (int j = lo; j <= row; ++j) {
-    const uint2 kw = *reinterpret_cast<const uint2*>(t.k + (long long)j * t.ldk + kvh * D + lane * 4);
-    const uint2 vw = *reinterpret_cast<const uint2*>(t.v + (long long)j * t.ldv + kvh * D + lane * 4);
-    const uint32_t kp[2] = {kw.x, kw.y}, vp[2] = {vw.x, vw.y};
-    float s = 0.0f;
+  float q[4], m = -INFINITY, l = 0.0f, a[4] = {};
+  two(qw.x, q[0], q[1]);
+  two(qw.y, q[2], q[3]);
+  for (int j0 = lo; j0 <= row; j0 += kKeys) {
+    uint2 kw[kKeys], vw[kKeys];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      s = fmaf(__uint_as_float(qp[i] << 16), __uint_as_float(kp[i] << 16), s);
-      s = fmaf(__uint_as_float(qp[i] & 0xffff0000u), __uint_as_float(kp[i] & 0xffff0000u), s);
+    for (int u = 0; u < kKeys; ++u) {
+      const long long j = min(j0 + u, row);  // those behind the row are left out below
+      kw[u] = *reinterpret_cast<const uint2*>(t.k + j * t.ldk + kvh * D + lane * 4);
+      vw[u] = *reinterpret_cast<const uint2*>(t.v + j * t.ldv + kvh * D + lane * 4);
+    }
+    float s[kKeys], v[kKeys][4], mn = m, more = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kKeys; ++u) {
+      float k[4];
+      two(kw[u].x, k[0], k[1]);
+      two(kw[u].y, k[2], k[3]);
+      two(vw[u].x, v[u][0], v[u][1]);
+      two(vw[u].y, v[u][2], v[u][3]);
+      s[u] = fmaf(q[3], k[3], fmaf(q[2], k[2], fmaf(q[1], k[1], q[0] * k[0])));
     }
 #pragma unroll
-    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= scale_log2;
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = ex2(m - ref), p = ex2(s - ref);
-    l = l * alpha + p;
+    for (int off = 16; off; off >>= 1)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      a[2 * i] = a[2 * i] * alpha + p * __uint_as_float(vp[i] << 16);
-      a[2 * i + 1] = a[2 * i + 1] * alpha + p * __uint_as_float(vp[i] & 0xffff0000u);
+      for (int u = 0; u < kKeys; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], off);
+#pragma unroll
+    for (int u = 0; u < kKeys; ++u) {
+      s[u] = j0 + u <= row ? s[u] * scale_log2 : -INFINITY;
+      mn = fmaxf(mn, s[u]);
     }
+    const float ref = mn == -INFINITY ? 0.0f : mn, alpha = ex2(m - ref);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] *= alpha;
+#pragma unroll
+    for (int u = 0; u < kKeys; ++u)
+      if (j0 + u <= row) {
+        const float p = ex2(s[u] - ref);
+        more += p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = fmaf(p, v[u][i], a[i]);
+      }
+    l = l * alpha + more;
     m = mn;
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   *reinterpret_cast<uint2*>(t.o + (long long)row * t.ldo + h * D + lane * 4) =
       make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
 }
+
+// All roles wait while rows are recomputed, which lasts long in long sequences
+// (256 rows of 131072 keys 0.7 s): waits are bounded by a minute here.
+constexpr unsigned long long kItemLimitNs = 60000000000ull;
 
 struct True { static constexpr bool value = true; };
 struct False { static constexpr bool value = false; };
@@ -293,8 +321,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     w.nt = two ? w.je[1] : w.je[0];
     return w;
   };
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    return mbar_wait(b, parity, err, kItemLimitNs);
+  };
   // by a whole warp, the same answer in every lane
-  auto warp_wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, err)) != 0; };
+  auto warp_wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
   // the n-th item of this block, by a whole warp; index -1: no more
   auto take_item = [&](int n) {
     Item it{-1, {0, 0}};
@@ -326,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           ++asked;
         };
         if (n > 0 && w.nt > 0) {
-          ok = mbar_wait(&bar.q_free, (loads & 1) ^ 1, err);
+          ok = wait(&bar.q_free, (loads & 1) ^ 1);
           if (!ok) break;
           load_q(it.index);
           ++loads;
@@ -339,13 +370,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t empty = ((tiles >> 1) & 1) ^ 1u;
           uint8_t* k = sK + s * TILE;
           uint8_t* v = sV + s * TILE;
-          ok = !*abort_flag && mbar_wait(&bar.k_free[s], empty, err);
+          ok = !*abort_flag && wait(&bar.k_free[s], empty);
           if (!ok) break;
           mbar_arrive_expect_tx(&bar.k_full[s], TILE);
           tma_load_2d(k, &tmK, &bar.k_full[s], kvh * D, krow);
           tma_load_2d(k + SUB, &tmK, &bar.k_full[s], kvh * D + 64, krow);
           ++k_tiles;
-          ok = mbar_wait(&bar.v_free[s], empty, err);
+          ok = wait(&bar.v_free[s], empty);
           if (!ok) break;
           mbar_arrive_expect_tx(&bar.v_full[s], TILE);
           tma_load_2d(v, &tmV, &bar.v_full[s], kvh * D, krow);
@@ -353,13 +384,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (!ok) break;
         if (w.nt == 0) ask();
-        ok = mbar_wait(&bar.next_full, n & 1, err);
+        ok = wait(&bar.next_full, n & 1);
         if (!ok) break;
         it.index = answered_block(&bar.next);
         if (it.index >= 0)
           for (int x = 0; x < 2; ++x) it.first[x] = pk.first_row(row_of(it.index) + x * BQ);
         const int m = n + 1;
-        ok = mbar_wait(&bar.item_free[m & 1], ((m >> 1) & 1) ^ 1, err);
+        ok = wait(&bar.item_free[m & 1], ((m >> 1) & 1) ^ 1);
         if (!ok) break;
         bar.item[m & 1] = it;
         mbar_arrive(&bar.item_full[m & 1]);
@@ -367,10 +398,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok) {  // giving up: no copy may land after the block has gone
         *abort_flag = 1;
-        mbar_wait(&bar.q_full, (loads - 1) & 1, err);
-        for (int i = max(0, k_tiles - 2); i < k_tiles; ++i) mbar_wait(&bar.k_full[i & 1], (i >> 1) & 1, err);
-        for (int i = max(0, tiles - 2); i < tiles; ++i) mbar_wait(&bar.v_full[i & 1], (i >> 1) & 1, err);
-        if (asked > 0) mbar_wait(&bar.next_full, (asked - 1) & 1, err);
+        wait(&bar.q_full, (loads - 1) & 1);
+        for (int i = max(0, k_tiles - 2); i < k_tiles; ++i) wait(&bar.k_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, tiles - 2); i < tiles; ++i) wait(&bar.v_full[i & 1], (i >> 1) & 1);
+        if (asked > 0) wait(&bar.next_full, (asked - 1) & 1);
       }
     }
   } else if (warp == 1) {
@@ -477,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int max_lo = __reduce_max_sync(0xffffffffu, lo), min_lo = __reduce_min_sync(0xffffffffu, lo);
     float m = -INFINITY, l = 0.0f;
     for (int j = 0; j < steps; ++j) {
-      ok = !*abort_flag && mbar_wait(&bar.s_full[x], (seen + j) & 1, err);
+      ok = !*abort_flag && wait(&bar.s_full[x], (seen + j) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         *abort_flag = 1;

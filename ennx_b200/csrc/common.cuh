@@ -191,13 +191,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 
 // Returns false (and records a timeout) if the phase does not complete in time.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err,
+                                          unsigned long long limit_ns = kWaitLimitNs) {
   uint32_t a = smem_u32(bar);
   if (mbar_try_wait(a, parity)) return true;
   unsigned long long t0 = globaltimer();
   for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(a, parity)) return true;
-    if ((it & 255u) == 0 && globaltimer() - t0 > kWaitLimitNs) {
+    if ((it & 255u) == 0 && globaltimer() - t0 > limit_ns) {
       if (err) atomicExch(err, ENNX_B200_TIMEOUT);
       return false;
     }
