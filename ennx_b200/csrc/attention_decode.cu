@@ -64,6 +64,7 @@ struct Args {
   float scale_log2;
   int rotate;
   float* partial;
+  int longest_first;  // blocks take the sequences in the order of their lengths
 };
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) { return min(a.room, max(0, __ldg(a.lengths + b))); }
@@ -365,11 +366,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __g
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ double inv[64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster_ctarank(), cluster = (int)cluster_ctas();
+  const int seg = (int)blockIdx.x / cluster, per_seq = a.hkv * a.blocks;
+  __shared__ int sequence;
   if (a.rotate && threadIdx.x < 64) inv[threadIdx.x] = rope_inv(table, threadIdx.x);
+  if (a.longest_first && (int)threadIdx.x < a.batch) {  // the sequence whose place by length is this one
+    const int i = (int)threadIdx.x, own = seq_len(a, i);
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < a.batch; ++j) {
+      const int other = seq_len(a, j);
+      place += other > own || (other == own && j < i);
+    }
+    if (place == seg / per_seq) sequence = i;
+  }
   __syncthreads();
   uint8_t* mine = smem + warp * kWarpRing;
   const uint32_t ring = smem_u32(mine), lo_parts = smem_u32(smem) + kWarps * kWarpRing + warp * kLoBytes;
-  const int seg = (int)blockIdx.x / cluster, per_seq = a.hkv * a.blocks, b = seg / per_seq;
+  // (in bounds even where lengths that change under the call left no sequence in this place)
+  const int b = a.longest_first ? (int)min((uint32_t)sequence, (uint32_t)a.batch - 1u) : seg / per_seq;
   const int len = seq_len(a, b), steps = head_steps(len);
   Head<kRows> s;
   s.place(a, b, seg % per_seq, len);
@@ -683,19 +697,29 @@ int64_t segments(int64_t batch, int hq, int hkv) {
 }
 
 // Blocks of a head: one for each 128 tokens of room, 8 at most and two per SM
-// over all heads; a single one up to 256 tokens, where a cluster's start and
-// meeting cost more (64 keys 3.8 us, 5.2 in a cluster; 300 keys 6.1 and 5.2;
-// 4096 keys 37 and 9.5).  0: the cache is split over the device.  That is for
-// rooms of more than 2048 tokens per block, where the longest sequence alone
-// would last longer than a split and its second kernel (one sequence of 16 query
-// heads on 4: 4096 keys 9.5 us and 17.4 split, 8192 keys 13.7 and 18.8, 16384
-// keys 22.9 and 20.9; 64 heads with 4096 keys 25 and 32; 32 ragged sequences of
-// up to 4096 keys 29.9 and 32.5).  The lengths are on the device, so the room
-// decides: one long sequence among empty ones takes up to 21 us instead of 11.
+// over all heads (some more in rooms of more than 2048 tokens per block); a
+// single one up to 256 tokens, where a cluster's start and meeting cost more (64
+// keys 3.8 us, 5.2 in a cluster; 300 keys 6.1 and 5.2; 4096 keys 37 and 9.5).  0:
+// the cache is split over the device.  That is for rooms of more than 2048
+// tokens per block, where the longest sequence alone would last longer than a
+// split and its second kernel (one sequence of 16 query heads on 4: 4096 keys 9.5
+// us and 17.4 split, 8192 keys 13.7 and 18.8, 16384 keys 22.9 and 20.9; 64 heads
+// with 4096 keys 25 and 32; 32 ragged sequences of up to 4096 keys 28 and 32, 24
+// of up to 8192 32 and 38).  The lengths are on the device, so the room decides:
+// one long sequence among empty ones takes up to 21 us instead of 11.
 int whole_cluster(int64_t segs, int room) {
   int n = 1;
-  while (n < 8 && n * segs <= sm_count() && room > 256 && room > 128 * n) n *= 2;
+  while (n < 8 && room > 256 && room > 128 * n &&
+         (n * segs <= sm_count() || (n * segs <= 2 * sm_count() && room > 2048 * n)))
+    n *= 2;
   return room <= 2048 * n ? n : 0;
+}
+// With more blocks than SMs the longest sequences start first (32 ragged
+// sequences of up to 4096 keys 30.1 -> 28.3 us, 24 of up to 8192 with two blocks
+// each 47 -> 42; sequences of one length lose 0.4 us), where a thread per
+// sequence can find the order.
+bool longest_first(int64_t segs, int cluster, int batch) {
+  return segs * cluster > sm_count() && batch > 1 && batch <= kThreads;
 }
 
 template <int kRows>
@@ -792,15 +816,15 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u)))
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: a 16-byte aligned workspace of %zu bytes required",
                      need);
+  const int cluster = whole_cluster(segs, p->room);
   const Args a{p->q, p->k, p->v, p->o, p->ld_q, p->ld_k, p->ld_v, p->ld_o,
                {p->k_cache, p->v_cache, p->k_seq, p->k_token, p->k_head, p->v_seq, p->v_token, p->v_head},
                p->lengths, p->batch, p->room, p->hkv, group, blocks, 1.4426950408889634f / sqrtf((float)D),
-               rope_theta > 0.0f, (float*)workspace};
+               rope_theta > 0.0f, (float*)workspace, longest_first(segs, cluster, p->batch)};
   const RopeTable& table = rope_table(rope_theta > 0.0f ? rope_theta : 1.0f);
   int dev = 0;
   int* status = nullptr;
   ENNX_TRY(serving_device(&dev, &status));
-  const int cluster = whole_cluster(segs, p->room);
   return rows == 8 ? launch<8>(a, table, segs, cluster, dev, s) : launch<16>(a, table, segs, cluster, dev, s);
 }
 

@@ -282,7 +282,8 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, 
  * share no rows between sequences, heads or each other, and k and v lie outside
  * them.  o may be q itself and overlaps nothing else.  workspace (device,
  * 16-byte aligned) >= ennx_b200_gqa_attention_decode_workspace_size(...)
- * bytes, which is 0 for small rooms; calls that may overlap need one each. */
+ * bytes, which is 0 where the cache is not split; calls that may overlap need
+ * one each. */
 typedef struct {
     const uint16_t* q;            /* [batch][hq][128], rows ld_q apart */
     int64_t ld_q;

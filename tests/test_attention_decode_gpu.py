@@ -63,6 +63,7 @@ CASES = [
     (5000, [4999, 3, 0, 0, 127, 128, 129], 16, 1), (40000, [40000], 4, 2), (3000, [2999], 17, 1), (1500, [1400, 20], 64, 2),
     (1100, [0, 0, 0], 4, 2), (2000, [11] * 200, 2, 1),
     (200, [200, 77, 0], 24, 2), (500, [500, 31, 256, 257], 9, 3), (9000, [8999, 1, 4097], 32, 2), (1300, [1300, 3] * 25, 16, 2),
+    (600, [7, 600, 0, 33, 600, 1] * 20, 8, 4), (9000, [8999, 5, 300, 0, 4097, 9000] * 4, 16, 4), (300, [1, 300] * 70, 4, 4),
     (20000, [19999, 3, 0, 0, 127, 128, 129], 16, 1), (17000, [1, 0, 16999, 64, 65, 2047, 0], 16, 4), (16385, [16385], 4, 4),
     (17000, [2999], 17, 1), (17000, [1400, 20], 64, 2), (17000, [0, 0, 0], 4, 2), (2100, [11, 2100] * 100, 2, 1),
 ]
