@@ -408,5 +408,8 @@ int32_t make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, ui
 // swizzle_bytes: 0 (none), 32, 64 or 128
 int32_t make_tmap_2d_bf16_sw(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                              uint64_t row_stride_elems, uint32_t box_inner, uint32_t box_outer, int swizzle_bytes);
+// any element type; extents and boxes in elements
+int32_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                     uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle_bytes);
 
 }  // namespace ennx

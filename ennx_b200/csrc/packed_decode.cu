@@ -104,29 +104,40 @@ struct Split {
   int along, row_warps;  // together all warps of a block
   int passes;            // slices per warp on k
   int tiles;             // row tiles of 16
+  int* status;
 };
 
-// One stage of a warp's ring: 16 code rows, then (scale, bias) pairs.  A flush
-// is kFlush products of 16 columns under one scale; lane t of a row takes
+// How a stage is filled.  kAny: rows at any address, 16-byte granules by cp.async
+// and reads shifted into place.  kTiles: rows start on 16 bytes, a warp's codes of
+// a tile come by one TMA copy.  kAllTiles: so do scales and biases, a group per
+// flush, and one more warp copies for the block (int4, 4 tokens on 151936 rows:
+// 48 us, 51 with copies by the warps themselves).
+enum Fill { kAny, kTiles, kAllTiles };
+
+// One stage of a warp's ring: 16 code rows, and their scales and biases.  A
+// flush is kFlush products of 16 columns under one scale; lane t of a row takes
 // 4 * kFlush consecutive columns of it, one shared-memory read.
-template <int kBits, int kFlush, bool kMoved>
+template <int kBits, int kFlush, bool kMoved, int kFill>
 struct Stage {
   static constexpr int kSlice = Shape<kMoved>::kSlice, kRowBytes = kSlice * kBits / 8;
-  // rows of a fragment read lie on different banks (an 8-lane phase covers
-  // whole rows, each kFlush * 2 * kBits bytes), and a row that starts inside
-  // a 16-byte granule still fits
-  static constexpr int kPitch = kRowBytes + kFlush * 2 * kBits;
+  // kAny: rows of a fragment read lie on different banks (an 8-lane phase
+  // covers whole rows, each kFlush * 2 * kBits bytes), and a row that starts
+  // inside a 16-byte granule still fits.  TMA: 128-byte rows, the 16-byte
+  // chunks of row r exchanged by r & 7.
+  static constexpr int kPitch = kFill == kAny ? kRowBytes + kFlush * 2 * kBits : 128;
   static constexpr int kPieces = kRowBytes / 16 + 1;
   static constexpr int kFlushes = kSlice / 16 / kFlush;
-  static constexpr int kBytes = 16 * kPitch + 16 * kFlushes * 8;
+  static constexpr int kCode = 16 * (kFill == kAny ? kPitch : kRowBytes);
+  static constexpr int kScale = 16 * kFlushes * 8;  // (scale, bias) pairs; kAllTiles: scales, then biases
   // depth: as many as leave 16 warps on an SM (80 to 100 KB in flight)
   static constexpr int kDepth = kBits == 8 ? 2 : 3;
 };
-// ring, then sums of x, then the joins
-template <int kBits, int kN, int kFlush, bool kMoved>
+// rings of codes, rings of scales, sums of x, joins
+template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
 constexpr int smem_bytes() {
-  using S = Stage<kBits, kFlush, kMoved>;
-  return Shape<kMoved>::kWarps * (S::kDepth * S::kBytes + S::kFlushes * 8 * kN * 4 + 2 * kN * 32 * 16);
+  using S = Stage<kBits, kFlush, kMoved, kFill>;
+  return (kFill == kAny ? 0 : 1024) +
+         Shape<kMoved>::kWarps * (S::kDepth * (S::kCode + S::kScale) + S::kFlushes * 8 * kN * 4 + 2 * kN * 32 * 16);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -157,6 +168,12 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t lo, uint32_t hi) {
   return pack_bf16x2(__uint_as_float(0x4b000000u | lo) - 8388608.0f, __uint_as_float(0x4b000000u | hi) - 8388608.0f);
 }
 
+// box of a tensor map to shared memory, completing on `bar`
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                   dst), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y)
+               : "memory");
+}
 // (v & 0x000f000f) | 0x43004300 in one logic instruction: written out, it
 // became two, and logic instructions are what the unpacking is made of
 __device__ __forceinline__ uint32_t nibbles_under_128(uint32_t v) {
@@ -200,21 +217,84 @@ __device__ __forceinline__ uint4 activation_pairs(uint4 v) {  // columns (0,1) (
                     __byte_perm(v.y, v.w, 0x7632));
 }
 
-// kN: blocks of 8 tokens.  kAligned: rows start on 16 bytes and the slice ends
-// on a granule, so copies need no per-row arithmetic and reads no shifting.
-template <int kBits, int kN, int kFlush, bool kMoved, bool kAligned>
-__global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBlocks)
-    packed_tiles_kernel(const __grid_constant__ Product p, const __grid_constant__ Split sp) {
-  using S = Stage<kBits, kFlush, kMoved>;
+struct Maps {
+  CUtensorMap codes, scales, biases;  // of rows of bytes and of floats
+};
+
+// kAllTiles: one more warp copies for all
+template <bool kMoved, int kFill>
+constexpr int block_threads() { return 32 * (Shape<kMoved>::kWarps + (kFill == kAllTiles)); }
+
+// kN: blocks of 8 tokens
+template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
+__global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>::kBlocks)
+    packed_tiles_kernel(const __grid_constant__ Product p, const __grid_constant__ Split sp, const __grid_constant__ Maps maps) {
+  using S = Stage<kBits, kFlush, kMoved, kFill>;
   constexpr int kSlice = S::kSlice, kSliceChunks = Shape<kMoved>::kChunks, kWarps = Shape<kMoved>::kWarps;
   constexpr int kFlushes = S::kFlushes, kStages = S::kDepth, kRuns = kFlush / 2;  // runs of 8 columns of a lane in a flush
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(16) uint8_t raw_smem[];
+  uint8_t* smem = raw_smem + (kFill == kAny ? 0u : (1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
+  __shared__ uint64_t bars[kWarps][kStages];  // kAllTiles: of all warps, full in row 0 and free in row 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  // A lane's rows of the tile are row_g and row_g + 8.  Of 16 lanes that read 8
+  // bytes (or 8 that read 16) in one go the exchanged chunks then differ.
+  constexpr int kLane = kRuns * kBits;  // bytes of a lane in a flush
+  const int row_g = kFill == kAny ? g : kLane == 16 ? g >> 1 | (g & 1) << 2 : (g & 3) << 1 | g >> 2;
   const int wk = warp % sp.along, wr = warp / sp.along;
-  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * S::kBytes;
+  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * S::kCode;
+  const uint32_t scale_ring = base + kWarps * kStages * S::kCode + warp * kStages * S::kScale;
+  uint64_t* full = bars[kFill == kAllTiles ? 0 : warp];
+  uint64_t* free_ = bars[1];
+  if constexpr (kFill == kTiles) {
+    if (lane < kStages) mbar_init(full + lane, 1);
+    fence_barrier_init();
+    fence_proxy_async();
+    __syncwarp();
+  }
+  if constexpr (kFill == kAllTiles) {
+    if (threadIdx.x < kStages) {
+      mbar_init(full + threadIdx.x, 1);
+      mbar_init(free_ + threadIdx.x, kWarps);
+      fence_barrier_init();
+      fence_proxy_async();
+    }
+    __syncthreads();
+    if (warp == kWarps) {
+      // Stages of the whole block: a box of codes per warp, a box of scales and
+      // one of biases per row tile.  (Copies by the warps themselves, cp.async
+      // or boxes, cost each some 600 of a tile's 2300 clocks.)
+      const int item = lane - kWarps;  // of scales and biases
+      const int my_wr = lane < kWarps ? lane / sp.along : item >> 1;
+      int n = 0;
+      bool ok = true;
+      for (int tile0 = (int)blockIdx.x * sp.row_warps; ok && tile0 < sp.tiles; tile0 += (int)gridDim.x * sp.row_warps)
+        for (int pass = 0; ok && pass < sp.passes; ++pass, ++n) {
+          const int at = n % kStages, live = min(sp.row_warps, sp.tiles - tile0);
+          ok = __all_sync(0xffffffffu, mbar_wait(free_ + at, ((n / kStages) & 1) ^ 1, sp.status)) != 0;
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(full + at, live * sp.along * (S::kCode + S::kScale));
+          __syncwarp();
+          const int row = (tile0 + my_wr) * 16;
+          if (lane < kWarps && my_wr < live) {
+            const int first = (pass * sp.along + lane % sp.along) * S::kRowBytes;
+#pragma unroll
+            for (int i = 0; i < S::kRowBytes / 128; ++i)
+              copy_box(base + (at * kWarps + lane) * S::kCode + i * 2048, &maps.codes, full + at, first + 128 * i, row);
+          } else if (item >= 0 && item < 2 * live) {
+            copy_box(base + kWarps * kStages * S::kCode + at * kWarps * S::kScale + (item & 1) * (kWarps * S::kScale / 2) +
+                         my_wr * sp.along * (S::kScale / 2),
+                     item & 1 ? &maps.biases : &maps.scales, full + at, pass * sp.along * S::kFlushes, row);
+          }
+        }
+      // no copy may land behind the block, whose other warps skip their waits once one has given up
+      for (int i = max(0, n - kStages); i < n; ++i) mbar_wait(full + i % kStages, (i / kStages) & 1, sp.status);
+      return;
+    }
+  }
   // sums of x over each flush of this warp's slice, per token
-  float* xsum = reinterpret_cast<float*>(smem + kWarps * kStages * S::kBytes) + warp * kFlushes * 8 * kN;
-  float4* red = reinterpret_cast<float4*>(smem + kWarps * (kStages * S::kBytes + kFlushes * 8 * kN * 4));
+  constexpr int kRings = kWarps * kStages * (S::kCode + S::kScale);
+  float* xsum = reinterpret_cast<float*>(smem + kRings) + warp * kFlushes * 8 * kN;
+  float4* red = reinterpret_cast<float4*>(smem + kRings + kWarps * kFlushes * 8 * kN * 4);
   const uint32_t width = (uint32_t)p.d.input_width, rows = (uint32_t)p.d.output_width, groups = (uint32_t)p.d.groups;
   const uint32_t row_bytes = (uint32_t)p.d.row_bytes;
   const bool wide_x = width % 8 == 0 && ((uintptr_t)p.x & 15u) == 0;
@@ -223,72 +303,64 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
   int tile = (int)blockIdx.x * sp.row_warps + wr;
   auto slice0 = [&](int pass) { return (uint32_t)(pass * sp.along + wk) * kSlice; };
 
-  // What a lane copies of a tile: codes at row `code_row` (aligned rows: every
-  // kCopyRows further down), scale and bias of row `scale_row` and every
-  // kScaleRows further down.  Pointers run from tile to tile.
-  constexpr int kLanes = S::kRowBytes / 16, kCopyRows = 32 / kLanes, kScaleRows = 32 / kFlushes;
-  const uint32_t code_row = lane / kLanes, scale_row = lane / kFlushes, scale_col = lane % kFlushes * (kFlush * 16);
+  // Scale and bias that a lane copies of a tile: at row `scale_row` and every
+  // kScaleRows further down.  Offsets run from tile to tile.
+  constexpr int kScaleRows = 32 / kFlushes;
+  const uint32_t scale_row = lane / kFlushes, scale_col = lane % kFlushes * (kFlush * 16);
   auto group_of = [&](int pass) { return min((slice0(pass) + scale_col) / p.d.group_size, groups - 1u); };
   uint32_t f_group = group_of(0), f_row = (uint32_t)tile * 16;
-  const uint8_t* f_code = p.w + (uint64_t)(f_row + code_row) * row_bytes + 16 * (lane % kLanes);
   uint64_t f_scale = (uint64_t)(f_row + scale_row) * groups;
-  const uint64_t code_step = (uint64_t)(16 * stride) * row_bytes, scale_step = (uint64_t)(16 * stride) * groups;
-  int f_tile = tile, f_pass = 0;
-  uint32_t f_stage = ring;
+  const uint64_t scale_step = (uint64_t)(16 * stride) * groups;
+  int f_tile = tile, f_pass = 0, f_stage = 0, fetched = 0;
   auto fetch = [&] {
+    if constexpr (kFill == kAllTiles) return;
     if (f_tile < sp.tiles) {
-      const uint32_t dst = f_stage, c0 = slice0(f_pass), first = c0 * kBits / 8;
-      const bool whole = f_row + 16 <= rows;
-      if constexpr (kAligned) {
-        if (first + 16 * (lane % kLanes) < row_bytes) {
-          const uint8_t* src = f_code + first;
-          const uint32_t to = dst + code_row * S::kPitch + 16 * (lane % kLanes);
-          if (whole) {
+      const uint32_t dst = ring + f_stage * S::kCode, sdst = scale_ring + f_stage * S::kScale;
+      const uint32_t c0 = slice0(f_pass), first = c0 * kBits / 8;
+      if constexpr (kFill == kAny) {
+        if (c0 < width) {
+          // 16-byte granules that hold a byte of the slice, none behind the row's last
+          const uint32_t last = min(row_bytes, first + S::kRowBytes);
 #pragma unroll
-            for (int i = 0; i < 16 / kCopyRows; ++i)
-              cp_async16(to + i * kCopyRows * S::kPitch, src + (uint64_t)(i * kCopyRows) * row_bytes);
-          } else {
-            for (int i = 0; i < 16 / kCopyRows; ++i)
-              if (f_row + code_row + i * kCopyRows < rows)
-                cp_async16(to + i * kCopyRows * S::kPitch, src + (uint64_t)(i * kCopyRows) * row_bytes);
+          for (int i = lane; i < 16 * S::kPieces; i += 32) {
+            const int r = i / S::kPieces, c = i % S::kPieces;
+            const uint32_t row = f_row + r;
+            if (row < rows) {
+              const uint8_t* start = p.w + (uint64_t)row * row_bytes + first;
+              const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
+              if (src < start + (last - first)) cp_async16(dst + r * S::kPitch + 16 * c, src);
+            }
           }
         }
-      } else if (c0 < width) {
-        // 16-byte granules that hold a byte of the slice, none behind the row's last
-        const uint32_t last = min(row_bytes, first + S::kRowBytes);
+      } else if (lane == 0) {  // what lies outside the matrix arrives as zeros
+        uint64_t* bar = full + f_stage;
+        mbar_arrive_expect_tx(bar, S::kCode);
 #pragma unroll
-        for (int i = lane; i < 16 * S::kPieces; i += 32) {
-          const int r = i / S::kPieces, c = i % S::kPieces;
-          const uint32_t row = f_row + r;
-          if (row < rows) {
-            const uint8_t* start = p.w + (uint64_t)row * row_bytes + first;
-            const uint8_t* src = reinterpret_cast<const uint8_t*>((uintptr_t)start & ~(uintptr_t)15) + 16 * c;
-            if (src < start + (last - first)) cp_async16(dst + r * S::kPitch + 16 * c, src);
-          }
+        for (int i = 0; i < S::kRowBytes / 128; ++i) copy_box(dst + i * 2048, &maps.codes, bar, (int)first + 128 * i, (int)f_row);
+      }
+      if constexpr (kFill != kAllTiles) {
+        // scales behind the last column are 0, which takes their columns out
+        if (sp.passes > 1) f_group = group_of(f_pass);
+        const bool inside = c0 + scale_col < width, whole = f_row + 16 <= rows;
+        const float *sc = p.sc + f_scale + f_group, *bi = p.bi + f_scale + f_group;
+#pragma unroll
+        for (int i = 0; i < 16 / kScaleRows; ++i) {
+          const bool ok = inside && (whole || f_row + scale_row + i * kScaleRows < rows);
+          const uint64_t down = ok ? (uint64_t)(i * kScaleRows) * groups : 0;
+          cp_async4(sdst + lane * 8 + i * 256, ok ? sc + down : p.sc, ok);
+          cp_async4(sdst + lane * 8 + i * 256 + 4, ok ? bi + down : p.bi, ok);
         }
       }
-      // scales behind the last column are 0, which takes their columns out
-      if (sp.passes > 1) f_group = group_of(f_pass);
-      const bool inside = c0 + scale_col < width;
-      const float *sc = p.sc + f_scale + f_group, *bi = p.bi + f_scale + f_group;
-      const uint32_t sdst = dst + 16 * S::kPitch + lane * 8;
-#pragma unroll
-      for (int i = 0; i < 16 / kScaleRows; ++i) {
-        const bool ok = inside && (whole || f_row + scale_row + i * kScaleRows < rows);
-        const uint64_t down = ok ? (uint64_t)(i * kScaleRows) * groups : 0;
-        cp_async4(sdst + i * 256, ok ? sc + down : p.sc, ok);
-        cp_async4(sdst + i * 256 + 4, ok ? bi + down : p.bi, ok);
-      }
+      ++fetched;
       if (++f_pass == sp.passes) {
         f_pass = 0;
         f_tile += stride;
         f_row += 16 * stride;
-        f_code += code_step;
         f_scale += scale_step;
       }
     }
-    f_stage = f_stage + S::kBytes == ring + kStages * S::kBytes ? ring : f_stage + S::kBytes;
-    cp_commit();
+    f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
+    if constexpr (kFill != kAllTiles) cp_commit();
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
@@ -338,39 +410,69 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
   };
   if (sp.passes == 1) load_x(0);
 
-  uint32_t st = ring;
-  for (int done = 0; tile < sp.tiles; ++done) {
+  int stage = 0, used = 0;
+  bool bad = false;  // a wait gave up: later ones are not tried again, the results are void
+  for (int done = 0; tile - (kFill == kAllTiles ? wr : 0) < sp.tiles; ++done) {
+    if (kFill == kAllTiles && tile >= sp.tiles) {  // a stage without a tile for this warp
+      for (int pass = 0; pass < sp.passes; ++pass, ++used) {
+        if (!bad) bad = !mbar_wait(full + stage, (used / kStages) & 1, sp.status);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(free_ + stage);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+      }
+      tile += stride;
+      continue;
+    }
     float out[kN][4] = {};
     for (int pass = 0; pass < sp.passes; ++pass) {
       if (sp.passes > 1) load_x(pass);
-      cp_wait<kStages - 2>();
+      if constexpr (kFill != kAllTiles) cp_wait<kStages - 2>();
+      if constexpr (kFill != kAny)
+        if (!bad) bad = !mbar_wait(full + stage, (used / kStages) & 1, sp.status);
+      ++used;
       __syncwarp();  // the stage is there, and all lanes have read the one before it,
       fetch();       // which is filled again while this one is used
       const uint32_t c0 = slice0(pass);
       {
+        // (kAllTiles: rings of the block, scales of the tile's slices side by side)
+        const uint32_t st = kFill == kAllTiles ? base + (stage * kWarps + warp) * S::kCode : ring + stage * S::kCode;
+        const uint32_t scales = kFill == kAllTiles ? base + kWarps * kStages * S::kCode + stage * kWarps * S::kScale +
+                                                         wr * sp.along * (S::kScale / 2) + wk * kFlushes * 4
+                                                   : scale_ring + stage * S::kScale;
         uint32_t addr[2], element[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t row = (uint32_t)tile * 16 + g + 8 * h;
-          const uint32_t skew =
-              kAligned ? 0u : (uint32_t)((uintptr_t)(p.w + (uint64_t)row * row_bytes) + c0 * kBits / 8) & 15u;
-          addr[h] = st + (g + 8 * h) * S::kPitch + skew + t * (kRuns * kBits);
+          const uint32_t r = row_g + 8 * h, row = (uint32_t)tile * 16 + r;
+          if constexpr (kFill == kAny) {
+            const uint32_t skew = (uint32_t)((uintptr_t)(p.w + (uint64_t)row * row_bytes) + c0 * kBits / 8) & 15u;
+            addr[h] = st + r * S::kPitch + skew + t * kLane;
+          } else {
+            addr[h] = st + r * 128 + ((uint32_t)(t * kLane) ^ (r & 7) << 4);
+          }
           element[h] = (uint32_t)p.d.element_offset + row * width + c0 + t * (8 * kRuns);
         }
+        uint32_t group4[4][4];  // kAllTiles: scales and biases of rows row_g and row_g + 8 in four flushes
 #pragma unroll
         for (int f = 0; f < kFlushes; ++f) {
           float acc[kN][4] = {};
-          constexpr int kWords = kRuns * kBits / 4;  // of a lane's columns in a flush
+          constexpr int kWords = kLane / 4;  // of a lane's columns in a flush
           uint32_t w[2][kWords];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t at = addr[h] + f * (4 * kRuns * kBits);
-            if constexpr (kAligned) {
-              lds_words<kWords>(at, w[h]);
-            } else {
+            constexpr int kFlushBytes = 4 * kLane;
+            if constexpr (kFill == kAny) {
 #pragma unroll
-              for (int i = 0; i < kWords; ++i) w[h][i] = word_at(at + 4 * i);
+              for (int i = 0; i < kWords; ++i) w[h][i] = word_at(addr[h] + f * kFlushBytes + 4 * i);
+            } else {
+              lds_words<kWords>((addr[h] ^ (f * kFlushBytes & 127)) + f * kFlushBytes / 128 * 2048, w[h]);
             }
+          }
+          if constexpr (kFill == kAllTiles) {
+            if (f % 4 == 0)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                lds_words<4>(scales + (i & 1) * (kWarps * S::kScale / 2) + ((row_g + 8 * (i >> 1)) * kFlushes * sp.along + f) * 4,
+                             group4[i]);
           }
 #pragma unroll
           for (int i = 0; i < kRuns; ++i) {
@@ -386,10 +488,15 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
             }
           }
           {
-            const uint32_t sa = st + 16 * S::kPitch + (g * kFlushes + f) * 8;
-            uint32_t u[2], v[2];  // (scale, bias) of rows g and g + 8
-            lds_words<2>(sa, u);
-            lds_words<2>(sa + 64 * kFlushes, v);
+            uint32_t u[2], v[2];  // (scale, bias) of rows row_g and row_g + 8
+            if constexpr (kFill == kAllTiles) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) { u[i] = group4[i][f % 4]; v[i] = group4[2 + i][f % 4]; }
+            } else {
+              const uint32_t sa = scales + (row_g * kFlushes + f) * 8;
+              lds_words<2>(sa, u);
+              lds_words<2>(sa + 64 * kFlushes, v);
+            }
             const float s0 = __uint_as_float(u[0]), b0 = __uint_as_float(u[1]);
             const float s1 = __uint_as_float(v[0]), b1 = __uint_as_float(v[1]);
 #pragma unroll
@@ -405,7 +512,11 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
           }
         }
       }
-      st = st + S::kBytes == ring + kStages * S::kBytes ? ring : st + S::kBytes;
+      if constexpr (kFill == kAllTiles) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(free_ + stage);
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
     if (sp.along > 1) {
       // one barrier a tile: the other buffer is written again only after the
@@ -430,18 +541,20 @@ __global__ void __launch_bounds__(32 * Shape<kMoved>::kWarps, Shape<kMoved>::kBl
       if (sp.along == 1 || wk == n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t row = (uint32_t)tile * 16 + g + 8 * (j >> 1);
+          const uint32_t row = (uint32_t)tile * 16 + row_g + 8 * (j >> 1);
           const int tok = n * 8 + 2 * t + (j & 1);
           if (row < rows && tok < p.tokens) p.out[(uint64_t)tok * rows + row] = f32_to_bf16_rne(out[n][j]);
         }
     tile += stride;
   }
-  cp_wait<0>();
+  if constexpr (kFill != kAllTiles) cp_wait<0>();
+  if (kFill == kTiles && bad)  // no copy may land behind the block
+    for (int i = max(0, fetched - kStages); i < fetched; ++i) mbar_wait(full + i % kStages, (i / kStages) & 1, sp.status);
 }
 
-template <int kBits, int kN, int kFlush, bool kMoved, bool kAligned>
+template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
-  const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved, kAligned>;
+  const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved, kFill>;
   Split sp;
   constexpr int kSlice = Shape<kMoved>::kSlice, kWarps = Shape<kMoved>::kWarps;
   const int slices = (int)((p.d.input_width + kSlice - 1) / kSlice);
@@ -450,24 +563,36 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   sp.row_warps = kWarps / sp.along;
   sp.passes = (slices + sp.along - 1) / sp.along;
   sp.tiles = (int)((p.d.output_width + 15) / 16);
-  constexpr int smem = smem_bytes<kBits, kN, kFlush, kMoved>();
-  static_assert(Shape<kMoved>::kBlocks * (smem + 1024) <= 228 * 1024 && smem <= 227 * 1024, "blocks of an SM");
+  constexpr int smem = smem_bytes<kBits, kN, kFlush, kMoved, kFill>();
+  static_assert(Shape<kMoved>::kBlocks * (smem + 2048) <= 228 * 1024 && smem <= 226 * 1024, "blocks of an SM");
   static SharedMemorySetup setup;
   int dev = 0;
-  int* status = nullptr;
-  ENNX_TRY(serving_device(&dev, &status));
+  ENNX_TRY(serving_device(&dev, &sp.status));
   ENNX_TRY(allow_shared_memory(setup, dev, kernel, smem));
+  Maps maps{};
+  if constexpr (kFill != kAny)
+    ENNX_TRY(make_tmap_2d(&maps.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.d.row_bytes, p.d.output_width, p.d.row_bytes, 128, 16,
+                          128));
+  if constexpr (kFill == kAllTiles) {
+    constexpr uint32_t kGroups = kSlice / 16 / kFlush;
+    for (int i = 0; i < 2; ++i)
+      ENNX_TRY(make_tmap_2d(i ? &maps.biases : &maps.scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, i ? p.bi : p.sc, p.d.groups,
+                            p.d.output_width, p.d.groups * 4, kGroups * sp.along, 16, 0));
+  }
   const int blocks = (sp.tiles + sp.row_warps - 1) / sp.row_warps, cap = Shape<kMoved>::kBlocks * sm_count();
-  kernel<<<(unsigned)(blocks < cap ? blocks : cap), 32 * kWarps, smem, s>>>(p, sp);
+  kernel<<<(unsigned)(blocks < cap ? blocks : cap), block_threads<kMoved, kFill>(), smem, s>>>(p, sp, maps);
   ENNX_LAUNCH_CHECK("packed tiles");
   return ENNX_B200_OK;
 }
 template <int kBits, int kN, int kFlush>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
+  const auto on_16 = [](const void* base, uint64_t row_bytes) { return ((uintptr_t)base & 15u) == 0 && row_bytes % 16 == 0; };
   // moved codes spend their time on the hash: one variant for any alignment
-  if (p.seed.enabled) return launch_tiles<kBits, kN, kFlush, true, false>(p, s);
-  if (p.d.row_bytes % 16 == 0 && ((uintptr_t)p.w & 15u) == 0) return launch_tiles<kBits, kN, kFlush, false, true>(p, s);
-  return launch_tiles<kBits, kN, kFlush, false, false>(p, s);
+  if (p.seed.enabled) return launch_tiles<kBits, kN, kFlush, true, kAny>(p, s);
+  if (!on_16(p.w, p.d.row_bytes)) return launch_tiles<kBits, kN, kFlush, false, kAny>(p, s);
+  if (p.d.group_size == 16 * kFlush && on_16(p.sc, p.d.groups * 4) && on_16(p.bi, p.d.groups * 4))
+    return launch_tiles<kBits, kN, kFlush, false, kAllTiles>(p, s);
+  return launch_tiles<kBits, kN, kFlush, false, kTiles>(p, s);
 }
 template <int kBits, int kN>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {

@@ -131,6 +131,12 @@ int32_t make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, ui
 
 int32_t make_tmap_2d_bf16_sw(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                              uint64_t row_stride_elems, uint32_t box_inner, uint32_t box_outer, int swizzle_bytes) {
+  return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, inner, outer, row_stride_elems * 2, box_inner, box_outer,
+                      swizzle_bytes);
+}
+
+int32_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                     uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle_bytes) {
   if (!g_encode) {
     cudaDriverEntryPointQueryResult q;
     void* fn = nullptr;
@@ -140,13 +146,13 @@ int32_t make_tmap_2d_bf16_sw(CUtensorMap* map, const void* base, uint64_t inner,
       return set_error(ENNX_B200_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
     g_encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
   }
-  if (((uintptr_t)base & 15u) != 0 || (row_stride_elems * 2) % 16 != 0)
+  if (((uintptr_t)base & 15u) != 0 || row_stride_bytes % 16 != 0)
     return set_error(ENNX_B200_INVALID_ARGUMENT, "TMA operand must be 16-byte aligned with a 16-byte row stride");
   cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_stride_elems * 2};
+  cuuint64_t strides[1] = {row_stride_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+  CUresult r = g_encode(map, type, 2, const_cast<void*>(base), dims, strides, box,
                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                         : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
