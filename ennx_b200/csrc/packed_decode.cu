@@ -12,7 +12,7 @@
 // Bound: HBM, half a byte or a byte per weight and 8 bytes per group.  Weight
 // rows are the 16 rows of m16n8k16, tokens the 8 columns.  A warp owns 256
 // columns of k: its activations stay in registers for all rows, its codes
-// stream through a cp.async ring; the warps of a row tile are joined through
+// stream through a ring in shared memory; the warps of a row tile are joined through
 // shared memory.  Narrow matrices put fewer warps on k and more on rows.  Rows
 // may start at any byte: the ring holds the 16-byte granules that cover them
 // (each holds at least one byte of the row) and reads are shifted into place.
@@ -105,14 +105,16 @@ struct Split {
   int passes;            // slices per warp on k
   int tiles;             // row tiles of 16
   int* status;
+  int shift;   // kWideTiles: a group lasts 1 << shift flushes
 };
 
 // How a stage is filled.  kAny: rows at any address, 16-byte granules by cp.async
 // and reads shifted into place.  kTiles: rows start on 16 bytes, a warp's codes of
-// a tile come by one TMA copy.  kAllTiles: so do scales and biases, a group per
-// flush, and one more warp copies for the block (int4, 4 tokens on 151936 rows:
-// 48 us, 51 with copies by the warps themselves).
-enum Fill { kAny, kTiles, kAllTiles };
+// a tile come by one TMA copy.  kAllTiles: so do scales and biases (kWideTiles:
+// groups of several flushes), and one more
+// warp copies for the block (int4, 4 tokens on 151936 rows, groups of 64: kAny 69
+// us, copies by the warps themselves 51, by one warp 48; groups of 128: kTiles 56).
+enum Fill { kAny, kTiles, kAllTiles, kWideTiles };
 
 // One stage of a warp's ring: 16 code rows, and their scales and biases.  A
 // flush is kFlush products of 16 columns under one scale; lane t of a row takes
@@ -223,7 +225,7 @@ struct Maps {
 
 // kAllTiles: one more warp copies for all
 template <bool kMoved, int kFill>
-constexpr int block_threads() { return 32 * (Shape<kMoved>::kWarps + (kFill == kAllTiles)); }
+constexpr int block_threads() { return 32 * (Shape<kMoved>::kWarps + (kFill >= kAllTiles)); }
 
 // kN: blocks of 8 tokens
 template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
@@ -241,9 +243,10 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
   constexpr int kLane = kRuns * kBits;  // bytes of a lane in a flush
   const int row_g = kFill == kAny ? g : kLane == 16 ? g >> 1 | (g & 1) << 2 : (g & 3) << 1 | g >> 2;
   const int wk = warp % sp.along, wr = warp / sp.along;
+  const int shift = kFill == kWideTiles ? sp.shift : 0;
   const uint32_t base = smem_u32(smem), ring = base + warp * kStages * S::kCode;
   const uint32_t scale_ring = base + kWarps * kStages * S::kCode + warp * kStages * S::kScale;
-  uint64_t* full = bars[kFill == kAllTiles ? 0 : warp];
+  uint64_t* full = bars[kFill >= kAllTiles ? 0 : warp];
   uint64_t* free_ = bars[1];
   if constexpr (kFill == kTiles) {
     if (lane < kStages) mbar_init(full + lane, 1);
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
     fence_proxy_async();
     __syncwarp();
   }
-  if constexpr (kFill == kAllTiles) {
+  if constexpr (kFill >= kAllTiles) {
     if (threadIdx.x < kStages) {
       mbar_init(full + threadIdx.x, 1);
       mbar_init(free_ + threadIdx.x, kWarps);
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
           const int at = n % kStages, live = min(sp.row_warps, sp.tiles - tile0);
           ok = __all_sync(0xffffffffu, mbar_wait(free_ + at, ((n / kStages) & 1) ^ 1, sp.status)) != 0;
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(full + at, live * sp.along * (S::kCode + S::kScale));
+          if (lane == 0) mbar_arrive_expect_tx(full + at, live * (sp.along * S::kCode + (sp.along * S::kScale >> shift)));
           __syncwarp();
           const int row = (tile0 + my_wr) * 16;
           if (lane < kWarps && my_wr < live) {
@@ -282,8 +285,8 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
               copy_box(base + (at * kWarps + lane) * S::kCode + i * 2048, &maps.codes, full + at, first + 128 * i, row);
           } else if (item >= 0 && item < 2 * live) {
             copy_box(base + kWarps * kStages * S::kCode + at * kWarps * S::kScale + (item & 1) * (kWarps * S::kScale / 2) +
-                         my_wr * sp.along * (S::kScale / 2),
-                     item & 1 ? &maps.biases : &maps.scales, full + at, pass * sp.along * S::kFlushes, row);
+                         (my_wr * sp.along * (S::kScale / 2) >> shift),
+                     item & 1 ? &maps.biases : &maps.scales, full + at, pass * sp.along * S::kFlushes >> shift, row);
           }
         }
       // no copy may land behind the block, whose other warps skip their waits once one has given up
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
   const uint64_t scale_step = (uint64_t)(16 * stride) * groups;
   int f_tile = tile, f_pass = 0, f_stage = 0, fetched = 0;
   auto fetch = [&] {
-    if constexpr (kFill == kAllTiles) return;
+    if constexpr (kFill >= kAllTiles) return;
     if (f_tile < sp.tiles) {
       const uint32_t dst = ring + f_stage * S::kCode, sdst = scale_ring + f_stage * S::kScale;
       const uint32_t c0 = slice0(f_pass), first = c0 * kBits / 8;
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
 #pragma unroll
         for (int i = 0; i < S::kRowBytes / 128; ++i) copy_box(dst + i * 2048, &maps.codes, bar, (int)first + 128 * i, (int)f_row);
       }
-      if constexpr (kFill != kAllTiles) {
+      if constexpr (kFill < kAllTiles) {
         // scales behind the last column are 0, which takes their columns out
         if (sp.passes > 1) f_group = group_of(f_pass);
         const bool inside = c0 + scale_col < width, whole = f_row + 16 <= rows;
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
       }
     }
     f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
-    if constexpr (kFill != kAllTiles) cp_commit();
+    if constexpr (kFill < kAllTiles) cp_commit();
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
@@ -412,8 +415,8 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
 
   int stage = 0, used = 0;
   bool bad = false;  // a wait gave up: later ones are not tried again, the results are void
-  for (int done = 0; tile - (kFill == kAllTiles ? wr : 0) < sp.tiles; ++done) {
-    if (kFill == kAllTiles && tile >= sp.tiles) {  // a stage without a tile for this warp
+  for (int done = 0; tile - (kFill >= kAllTiles ? wr : 0) < sp.tiles; ++done) {
+    if (kFill >= kAllTiles && tile >= sp.tiles) {  // a stage without a tile for this warp
       for (int pass = 0; pass < sp.passes; ++pass, ++used) {
         if (!bad) bad = !mbar_wait(full + stage, (used / kStages) & 1, sp.status);
         __syncwarp();
@@ -426,7 +429,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
     float out[kN][4] = {};
     for (int pass = 0; pass < sp.passes; ++pass) {
       if (sp.passes > 1) load_x(pass);
-      if constexpr (kFill != kAllTiles) cp_wait<kStages - 2>();
+      if constexpr (kFill < kAllTiles) cp_wait<kStages - 2>();
       if constexpr (kFill != kAny)
         if (!bad) bad = !mbar_wait(full + stage, (used / kStages) & 1, sp.status);
       ++used;
@@ -435,9 +438,9 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
       const uint32_t c0 = slice0(pass);
       {
         // (kAllTiles: rings of the block, scales of the tile's slices side by side)
-        const uint32_t st = kFill == kAllTiles ? base + (stage * kWarps + warp) * S::kCode : ring + stage * S::kCode;
-        const uint32_t scales = kFill == kAllTiles ? base + kWarps * kStages * S::kCode + stage * kWarps * S::kScale +
-                                                         wr * sp.along * (S::kScale / 2) + wk * kFlushes * 4
+        const uint32_t st = kFill >= kAllTiles ? base + (stage * kWarps + warp) * S::kCode : ring + stage * S::kCode;
+        const uint32_t scales = kFill >= kAllTiles ? base + kWarps * kStages * S::kCode + stage * kWarps * S::kScale +
+                                                         (wr * sp.along * (S::kScale / 2) >> shift)
                                                    : scale_ring + stage * S::kScale;
         uint32_t addr[2], element[2];
 #pragma unroll
@@ -467,12 +470,14 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
               lds_words<kWords>((addr[h] ^ (f * kFlushBytes & 127)) + f * kFlushBytes / 128 * 2048, w[h]);
             }
           }
-          if constexpr (kFill == kAllTiles) {
-            if (f % 4 == 0)
+          if constexpr (kFill >= kAllTiles) {
+            const int pitch = kFlushes * sp.along >> shift, group = (wk * kFlushes + f) >> shift;
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                lds_words<4>(scales + (i & 1) * (kWarps * S::kScale / 2) + ((row_g + 8 * (i >> 1)) * kFlushes * sp.along + f) * 4,
-                             group4[i]);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t from = scales + (i & 1) * (kWarps * S::kScale / 2) + ((row_g + 8 * (i >> 1)) * pitch + group) * 4;
+              if constexpr (kFill == kWideTiles) group4[i][f % 4] = lds32(from);
+              else if (f % 4 == 0) lds_words<4>(from, group4[i]);
+            }
           }
 #pragma unroll
           for (int i = 0; i < kRuns; ++i) {
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
           }
           {
             uint32_t u[2], v[2];  // (scale, bias) of rows row_g and row_g + 8
-            if constexpr (kFill == kAllTiles) {
+            if constexpr (kFill >= kAllTiles) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) { u[i] = group4[i][f % 4]; v[i] = group4[2 + i][f % 4]; }
             } else {
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
           }
         }
       }
-      if constexpr (kFill == kAllTiles) {
+      if constexpr (kFill >= kAllTiles) {
         __syncwarp();
         if (lane == 0) mbar_arrive(free_ + stage);
       }
@@ -547,7 +552,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
         }
     tile += stride;
   }
-  if constexpr (kFill != kAllTiles) cp_wait<0>();
+  if constexpr (kFill < kAllTiles) cp_wait<0>();
   if (kFill == kTiles && bad)  // no copy may land behind the block
     for (int i = max(0, fetched - kStages); i < fetched; ++i) mbar_wait(full + i % kStages, (i / kStages) & 1, sp.status);
 }
@@ -555,7 +560,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
 template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
   const auto kernel = packed_tiles_kernel<kBits, kN, kFlush, kMoved, kFill>;
-  Split sp;
+  Split sp{};
   constexpr int kSlice = Shape<kMoved>::kSlice, kWarps = Shape<kMoved>::kWarps;
   const int slices = (int)((p.d.input_width + kSlice - 1) / kSlice);
   sp.along = 1;
@@ -573,11 +578,12 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   if constexpr (kFill != kAny)
     ENNX_TRY(make_tmap_2d(&maps.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.d.row_bytes, p.d.output_width, p.d.row_bytes, 128, 16,
                           128));
-  if constexpr (kFill == kAllTiles) {
+  if constexpr (kFill >= kAllTiles) {
     constexpr uint32_t kGroups = kSlice / 16 / kFlush;
+    while (16u * kFlush << sp.shift < p.d.group_size) ++sp.shift;
     for (int i = 0; i < 2; ++i)
       ENNX_TRY(make_tmap_2d(i ? &maps.biases : &maps.scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, i ? p.bi : p.sc, p.d.groups,
-                            p.d.output_width, p.d.groups * 4, kGroups * sp.along, 16, 0));
+                            p.d.output_width, p.d.groups * 4, kGroups * sp.along >> sp.shift, 16, 0));
   }
   const int blocks = (sp.tiles + sp.row_warps - 1) / sp.row_warps, cap = Shape<kMoved>::kBlocks * sm_count();
   kernel<<<(unsigned)(blocks < cap ? blocks : cap), block_threads<kMoved, kFill>(), smem, s>>>(p, sp, maps);
@@ -590,8 +596,16 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   // moved codes spend their time on the hash: one variant for any alignment
   if (p.seed.enabled) return launch_tiles<kBits, kN, kFlush, true, kAny>(p, s);
   if (!on_16(p.w, p.d.row_bytes)) return launch_tiles<kBits, kN, kFlush, false, kAny>(p, s);
-  if (p.d.group_size == 16 * kFlush && on_16(p.sc, p.d.groups * 4) && on_16(p.bi, p.d.groups * 4))
-    return launch_tiles<kBits, kN, kFlush, false, kAllTiles>(p, s);
+  // a power of two of flushes per group, and 16 bytes of a row's scales per copy at least
+  const uint32_t flushes = p.d.group_size / (16 * kFlush);
+  constexpr uint32_t kSlice = Shape<false>::kSlice;
+  uint32_t along = 1;
+  while (along * kSlice < p.d.input_width && along < (uint32_t)Shape<false>::kWarps) along *= 2;
+  const bool groups_fit = p.d.group_size % (16 * kFlush) == 0 && (flushes & (flushes - 1)) == 0 &&
+                          along * kSlice / p.d.group_size % 4 == 0 && along * kSlice >= 4 * p.d.group_size;
+  if (groups_fit && on_16(p.sc, p.d.groups * 4) && on_16(p.bi, p.d.groups * 4))
+    return flushes == 1 ? launch_tiles<kBits, kN, kFlush, false, kAllTiles>(p, s)
+                        : launch_tiles<kBits, kN, kFlush, false, kWideTiles>(p, s);
   return launch_tiles<kBits, kN, kFlush, false, kTiles>(p, s);
 }
 template <int kBits, int kN>
