@@ -111,9 +111,9 @@ struct Split {
 // How a stage is filled.  kAny: rows at any address, 16-byte granules by cp.async
 // and reads shifted into place.  kTiles: rows start on 16 bytes, a warp's codes of
 // a tile come by one TMA copy.  kAllTiles: so do scales and biases (kWideTiles:
-// groups of several flushes), and one more
-// warp copies for the block (int4, 4 tokens on 151936 rows, groups of 64: kAny 69
-// us, copies by the warps themselves 51, by one warp 48; groups of 128: kTiles 56).
+// of groups of several flushes), and one more warp copies for the block (int4, 4
+// tokens on 151936 rows, groups of 64: kAny 69 us, copies by the warps themselves
+// 51, by one warp 47; groups of 128: kTiles 56, kWideTiles 48).
 enum Fill { kAny, kTiles, kAllTiles, kWideTiles };
 
 // One stage of a warp's ring: 16 code rows, and their scales and biases.  A

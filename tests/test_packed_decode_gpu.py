@@ -45,6 +45,7 @@ def check(got, x, w, sc, bi, lin, seed=(0, 0, 0)):
 
 
 SHAPES = [
+    (4096, 40, 128), (8192, 50, 256), (2048, 333, 512), (6144, 21, 64), (4096, 2500, 32), (512, 700, 128),
     (2048, 512, 64), (256, 48, 32), (64, 16, 64), (32, 1, 32), (1, 1, 1), (7, 3, 4), (200, 17, 48), (37, 9, 8), (16, 33, 16),
     (512, 100, 128), (1024, 31, 256), (2048, 40, 2048), (96, 300, 16), (4096, 64, 64), (4160, 24, 32), (8200, 19, 64),
     (2011, 50, 64), (255, 65, 32), (1000, 20, 1000), (2080, 16, 96), (130, 130, 160), (2304, 8, 2000),
