@@ -130,6 +130,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
   constexpr int kHeld = kV >= 32 ? kV / 32 : 1, kRepeat = kV >= 32 ? 1 : 32 / kV;  // values a lane ends with, lanes of a value
   __shared__ float part[kWarps][kV];
   __shared__ float logits[kExperts];
+  cluster_arrive();  // waited for before the first store to another block, which has to have started by then
+  bool met = false;
   launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster_ctarank();
   const int t0 = (int)(blockIdx.x / kCluster) * kT;
@@ -166,6 +168,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
     for (int i = 0; i < kHeld; ++i)
       if (lane % kRepeat == 0) part[warp][lane / kRepeat * kHeld + i] = acc[i];
     __syncthreads();
+    if (!met) {  // block-uniform
+      cluster_wait();
+      met = true;
+    }
     if (threadIdx.x < kV) {
       float v[kWarps];
 #pragma unroll
@@ -176,6 +182,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(&logits[e], (uint32_t)t)), "f"(sum) : "memory");
     }
   }
+  if (!met) cluster_wait();  // a block without experts
   cluster_sync();  // every block has all logits of its token; nothing remote is touched behind it
   const int tok = t0 + rank;
   if (rank >= kT || tok >= p.tokens || warp != 0) return;

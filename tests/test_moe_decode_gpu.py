@@ -229,3 +229,17 @@ def test_refusals():
         call(x, wr, wgu, wd, 2, residual=x[:2])
     with pytest.raises(ValueError, match="CUDA"):
         call(x.cpu(), wr, wgu, wd, 2)
+
+
+@pytest.mark.parametrize("T,H,E,k", [(1, 64, 1, 1), (8, 64, 1, 1), (64, 64, 3, 2), (9, 64, 9, 8)])
+def test_router_whose_blocks_have_next_to_nothing_to_do(T, H, E, k):
+    """A block of the router stores logits into other blocks' shared memory soon
+    after its start here, or has no expert at all and only receives them."""
+    x, (wr, wgu, wd) = rnd(T, H, seed=70), weights(H, E, 128, 71)
+    y, idx, gate = ops.moe_layer_decode(x, wr, wgu, wd, k, return_routing=True)
+    ridx, rgate = routing(x, wr, k)
+    assert torch.equal(idx.long(), ridx)
+    check(y, x, wgu, wd, ridx, rgate)
+    runs = [ops.moe_layer_decode(x, wr, wgu, wd, k, return_routing=True) for _ in range(200)]
+    assert all(torch.equal(a, y) and torch.equal(b, idx) and torch.equal(c, gate) for a, b, c in runs)
+    ops.device_status()
