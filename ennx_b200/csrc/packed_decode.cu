@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
     if constexpr (kFill >= kAllTiles) return;
     if (f_tile < sp.tiles) {
       const uint32_t dst = ring + f_stage * S::kCode, sdst = scale_ring + f_stage * S::kScale;
-      const uint32_t c0 = slice0(f_pass), first = c0 * kBits / 8;
+      const uint32_t c0 = slice0(f_pass), first = c0 / 8 * kBits;  // c0 * kBits may pass 32 bits
       if constexpr (kFill == kAny) {
         if (c0 < width) {
           // 16-byte granules that hold a byte of the slice, none behind the row's last
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
         for (int h = 0; h < 2; ++h) {
           const uint32_t r = row_g + 8 * h, row = (uint32_t)tile * 16 + r;
           if constexpr (kFill == kAny) {
-            const uint32_t skew = (uint32_t)((uintptr_t)(p.w + (uint64_t)row * row_bytes) + c0 * kBits / 8) & 15u;
+            const uint32_t skew = (uint32_t)((uintptr_t)(p.w + (uint64_t)row * row_bytes) + c0 / 8 * kBits) & 15u;
             addr[h] = st + r * S::kPitch + skew + t * kLane;
           } else {
             addr[h] = st + r * 128 + ((uint32_t)(t * kLane) ^ (r & 7) << 4);
