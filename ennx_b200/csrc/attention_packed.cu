@@ -221,7 +221,7 @@ __device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int
     l = l * alpha + more;
     m = mn;
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const float inv = 1.0f / l;  // every visible score -inf: 0 / 0
   *reinterpret_cast<uint2*>(t.o + (long long)row * t.ldo + h * D + lane * 4) =
       make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
 }
@@ -612,7 +612,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       ok = warp_wait(&bar.o_done[x], (seen - 1) & 1);
       if (ok) {
         tc_fence_after();
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        // a row sees itself at least: a sum of 0 means that every visible
+        // score is -inf, and 0 / 0 is what the softmax gives then
+        const float inv = 1.0f / l;
         const bool mine = qpos >= pk.begin() && qpos < end;
         uint16_t* orow = t.o + (long long)qpos * t.ldo + h * D;
         float worst = 0.0f;  // NaN or 0 * inf = NaN where an output is not finite

@@ -259,7 +259,8 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention(uint16_t* q, uint16_t* k, const ui
  * pairing, position = row within its sequence, angles reduced in 64 bits) is
  * applied to q and k IN PLACE first, which then overlap neither one another
  * nor v.  o must not overlap q, k or v.  Softmax statistics in fp32; a
- * non-finite key or value reaches only the rows that see it.  Allocates
+ * non-finite key or value reaches only the rows that see it, and a row whose
+ * visible scores are all -infinity is NaN, as the softmax is.  Allocates
  * nothing. */
 ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uint16_t* k, int64_t ld_k,
                                                      const uint16_t* v, int64_t ld_v, uint16_t* o, int64_t ld_o,

@@ -236,3 +236,22 @@ def test_refusals():
         call(odd, k, v, cu)
     with pytest.raises(ValueError, match="CUDA"):
         call(q.cpu(), k, v, cu)
+
+
+def test_rows_whose_visible_scores_are_all_minus_infinity():
+    """Softmax of nothing but -infinity is NaN; a row that sees one other score is what that score says."""
+    lengths = [40, 300, 7, 129]
+    q, k, v = rnd(476, 4, D, seed=40).abs(), rnd(476, 2, D, seed=41), rnd(476, 2, D, seed=42)
+    k[0, 0, 3] = -math.inf        # the first row of sequence 0 sees nothing else
+    k[40:240, 1, 9] = -math.inf   # rows 0 .. 199 of sequence 1, over a tile's end
+    k[347:, :, 127] = -math.inf   # all of sequence 3
+    o = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    lost = torch.zeros(476, 4, dtype=torch.bool, device="cuda")
+    lost[0, :2] = True
+    lost[40:240, 2:] = True
+    lost[347:] = True
+    ref = reference(q, k, v, lengths)
+    assert torch.equal(ref.isnan(), lost[:, :, None].expand_as(ref))
+    assert torch.equal(o.isnan(), ref.isnan())
+    close(o[~lost], ref[~lost], float(v.float().abs().max()))
+    ops.device_status()
