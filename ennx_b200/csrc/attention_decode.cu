@@ -329,7 +329,7 @@ struct Head {
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (g + 8 * r < rows) {
-        const float inv = l[r] > 0.0f || l[r] != l[r] ? 1.0f / l[r] : 0.0f;
+        const float inv = 1.0f / l[r];  // every score -inf: 0 / 0, as the softmax
         uint16_t* o = a.o + (long long)b * a.ldo + (long long)(hq0 + g + 8 * r) * D + 2 * t;
 #pragma unroll
         for (int nb = 0; nb < 16; ++nb) {
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_whole_kernel(const __g
   s.put_partial(merge + warp * 16 * kPart, lane);
   __syncthreads();
   auto put = [&](int row, const float (&y)[4], float sum) {
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const float inv = len > 0 ? 1.0f / sum : 0.0f;  // every score -inf: 0 / 0, as the softmax
     *reinterpret_cast<uint2*>(a.o + (long long)b * a.ldo + (long long)(s.hq0 + row) * D + lane * 4) =
         make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
   };
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kThreads) token_join_kernel(const __grid_const
     sum += f * joined[w][D + 1];
     v += f * joined[w][d];
   }
-  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  const float inv = parts > 0 ? 1.0f / sum : 0.0f;  // every score -inf: 0 / 0, as the softmax
   a.o[(long long)b * a.ldo + (long long)(h * a.group + g0 + row) * D + d] = f32_to_bf16_rne(v * inv);
 }
 

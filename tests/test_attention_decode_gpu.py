@@ -261,3 +261,21 @@ def test_refusals():
         call(q, pad, vc, ln)
     with pytest.raises(ValueError, match="rope_theta"):
         call(q, kc, vc, ln, rope_theta=math.inf)
+
+
+# a block, a cluster and a split of the device per head; one and several query heads of each kind of tile
+@pytest.mark.parametrize("room,lengths", [(200, [1, 0, 200]), (2000, [1, 0, 1999]), (17000, [1, 0, 16999])])
+@pytest.mark.parametrize("hq", [4, 24])
+@pytest.mark.parametrize("theta", [0.0, 1e6])
+def test_scores_that_are_all_minus_infinity(room, lengths, hq, theta):
+    """Softmax of nothing but -infinity is NaN; an empty sequence stays 0."""
+    kc, vc, q = rnd(3, room, 2, D, seed=70), rnd(3, room, 2, D, seed=71), rnd(3, hq, D, seed=72).abs()
+    if theta:  # pair 63 turns by 1e-6 of a position: its first half keeps its sign
+        q[..., 127] = 0.0
+    kc[:, :, 0, 63] = -math.inf
+    o = ops.gqa_attention_decode(q, kc, vc, i32(lengths), rope_theta=theta)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert (o[b] == 0).all()
+        else:
+            assert o[b, :hq // 2].isnan().all() and o[b, hq // 2:].isfinite().all()
