@@ -14,6 +14,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
+import _attention  # noqa: E402
+
 from ennx_b200 import ops  # noqa: E402
 
 D = 128
@@ -279,3 +281,33 @@ def test_scores_that_are_all_minus_infinity(room, lengths, hq, theta):
             assert (o[b] == 0).all()
         else:
             assert o[b, :hq // 2].isnan().all() and o[b, hq // 2:].isfinite().all()
+
+
+@pytest.mark.parametrize("room,lengths,hq,hkv", [c for c in CASES if sum(c[1])])
+@pytest.mark.parametrize("theta", [0.0, 1e6])
+def test_precision_of_the_two_part_products(room, lengths, hq, hkv, theta):
+    """The bound of queries and weights carried as hi + lo: narrow enough that
+    the lo parts, the rotation and the new token have to be there
+    (test_attention_bounds_cpu.py plants those mistakes)."""
+    batch = len(lengths)
+    kc, vc = rnd(batch, room, hkv, D, seed=80), rnd(batch, room, hkv, D, seed=81)
+    q, k, v = rnd(batch, hq, D, seed=82), rnd(batch, hkv, D, seed=83), rnd(batch, hkv, D, seed=84)
+    o = ops.gqa_attention_decode(q, kc, vc, i32(lengths), k=k, v=v, rope_theta=theta)
+    assert _attention.excess(o, q, kc, vc, lengths, theta) <= 0
+
+
+@pytest.mark.parametrize("room,lengths,hq,hkv", [c for c in CASES if sum(c[1])])
+def test_keys_that_carry_the_weight(room, lengths, hq, hkv):
+    """Some thirty keys per sequence, the first, the new one and at least one in
+    every part of a split, with nearly all the weight: none may be lost."""
+    batch, theta, group = len(lengths), 1e6, hq // hkv
+    kc, vc = rnd(batch, room, hkv, D, seed=85), rnd(batch, room, hkv, D, seed=86)
+    q, k, v = rnd(batch, hq, D, seed=87), rnd(batch, hkv, D, seed=88), rnd(batch, hkv, D, seed=89)
+    for b, n in enumerate(lengths):
+        if n:
+            _attention.lift(q[b], kc[b, :n], _attention.heavy_keys(n), n - 1, theta)
+            for h in range(hkv):  # turned like q, so along it
+                x = q[b, h * group].double()
+                k[b, h] = (x * ((math.log(n) + 2) * math.sqrt(D) / float(x @ x))).to(k.dtype)
+    o = ops.gqa_attention_decode(q, kc, vc, i32(lengths), k=k, v=v, rope_theta=theta)
+    assert _attention.excess(o, q, kc, vc, lengths, theta) <= 0

@@ -10,6 +10,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
+import _attention  # noqa: E402
 import test_attention_decode_gpu as cached  # noqa: E402
 import test_attention_packed_gpu as prompts  # noqa: E402
 import test_moe_decode_gpu as moe  # noqa: E402
@@ -128,4 +129,30 @@ def test_replayed_steps_are_the_eager_ones():
     assert torch.equal(layers[0].lengths, layers[1].lengths)
     for one, other in ((layers[0].kc, layers[1].kc), (layers[0].vc, layers[1].vc)):
         assert torch.equal(one.view(torch.int16), other.view(torch.int16))
+    ops.device_status()
+
+
+@pytest.mark.parametrize("room", [400, 1500, 17000])
+def test_token_steps_hold_the_bound_of_two_part_products(room):
+    """The cache attention of a layer's steps, as narrow as its arithmetic allows:
+    eagerly, then from a replayed graph whose lengths have grown."""
+    hidden, lengths = 256, [130, 0, 33, 300, 1]
+    layer = Layer(hidden, 4, 2, 8, 2, 128, lengths, room)
+    layer.prompt(rnd(sum(lengths), hidden, seed=20), lengths)
+    x, stream = rnd(len(lengths), hidden, seed=21), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        _, fused, o, *_ = layer.token(x)
+        now = [n + 1 for n in lengths]
+        assert _attention.excess(o, layer.split(fused)[0], layer.kc, layer.vc, now, THETA) <= 0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            _, fused, o, *_ = layer.token(x)
+        for step in range(3):
+            x.copy_(rnd(len(lengths), hidden, seed=22 + step))
+            graph.replay()
+            now = [n + 1 for n in now]
+            assert layer.lengths.tolist() == now
+            assert _attention.excess(o, layer.split(fused)[0], layer.kc, layer.vc, now, THETA) <= 0
+    torch.cuda.current_stream().wait_stream(stream)
     ops.device_status()
