@@ -222,7 +222,7 @@ struct Head {
   __device__ __forceinline__ void step(const Args& a, uint32_t sk, uint32_t lo_parts, int key0, int lane) {
     const int t = lane & 3;
     const uint32_t sv = sk + kStep * 256;
-    float s[2][4] = {};
+    float s[2][4] = {}, lo[2][4] = {};  // lo: of the lo parts, kRows 16 (kRows 8 has them in rows 8 .. 15 of s)
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
       uint32_t kf[4];
@@ -232,8 +232,8 @@ struct Head {
       if (kRows == 16 && a.rotate) {
         uint32_t ql[4];
         ldsm4(lo_parts + at(lane & 15, 2 * kk + (lane >> 4)), ql);
-        mma(s[0], ql, kf[0], kf[1]);
-        mma(s[1], ql, kf[2], kf[3]);
+        mma(lo[0], ql, kf[0], kf[1]);
+        mma(lo[1], ql, kf[2], kf[3]);
       }
     }
     float alpha[R], ref[R], pr[R][4];  // pr[.]: keys 2t, 2t + 1 of both blocks of 8
@@ -244,7 +244,10 @@ struct Head {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int nb = j >> 1, e = j & 1;
-        const float v = kRows == 8 ? s[nb][e] + s[nb][2 + e] : s[nb][2 * r + e];
+        // an infinite score is what the hi parts say: the lo parts of the same
+        // factors may be 0 or of the other sign, and the sum NaN then
+        const float hi = s[nb][2 * r + e], rest = kRows == 8 ? s[nb][2 + e] : lo[nb][2 * r + e];
+        const float v = fabsf(hi) == INFINITY ? hi : hi + rest;
         pr[r][j] = key0 + nb * 8 + 2 * t + e < len ? v * a.scale_log2 : -INFINITY;
         top = fmaxf(top, pr[r][j]);
       }

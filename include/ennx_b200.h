@@ -275,8 +275,10 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, 
  * position p if rope_theta > 0; q, rotated likewise but left as it is, attends
  * to rows 0 .. p.  Without k and v the caches already hold row p.  lengths[b]
  * = 0: nothing is written to the caches and o is 0.  Rows behind p may hold
- * anything; an infinity or NaN in row p or before makes the outputs it enters
- * non-finite (NaN where their limit would be an infinity).  All bf16; strides
+ * anything.  An infinite key counts as its score does (none but -infinity:
+ * NaN, as the softmax); an infinity or NaN in a value of row p or before, or a
+ * NaN in a key, makes the outputs it enters non-finite (NaN where their limit
+ * would be an infinity).  All bf16; strides
  * in elements.  Cache strides (multiples of 8) are free, so [batch, room,
  * heads, 128] and [batch, heads, room, 128] both fit; the caches, q and o are
  * 16-byte aligned, ld_q and ld_o multiples of 8.  Caches that take k and v

@@ -311,3 +311,21 @@ def test_keys_that_carry_the_weight(room, lengths, hq, hkv):
                 k[b, h] = (x * ((math.log(n) + 2) * math.sqrt(D) / float(x @ x))).to(k.dtype)
     o = ops.gqa_attention_decode(q, kc, vc, i32(lengths), k=k, v=v, rope_theta=theta)
     assert _attention.excess(o, q, kc, vc, lengths, theta) <= 0
+
+
+@pytest.mark.parametrize("room,lengths", [(200, [70, 0, 200]), (2000, [17, 0, 1999]), (17000, [3, 0, 16999])])
+@pytest.mark.parametrize("hq", [4, 24])
+@pytest.mark.parametrize("theta", [0.0, 1e6])
+def test_a_key_of_minus_infinite_score_has_weight_zero(room, lengths, hq, theta):
+    kc, vc, q = rnd(3, room, 2, D, seed=73), rnd(3, room, 2, D, seed=74), rnd(3, hq, D, seed=75).abs()
+    if theta:  # pair 63 turns by 1e-6 of a position: its first half keeps its sign
+        q[..., 127] = 0.0
+    keep = torch.ones(room, dtype=torch.bool, device="cuda")
+    for j in (0, 16, 150, 1700, 16990):
+        if j < room:
+            kc[:, j, :, 63], keep[j] = -math.inf, False
+    o = ops.gqa_attention_decode(q, kc, vc, i32(lengths), rope_theta=theta)
+    for b, n in enumerate(lengths):
+        live = keep[:n]
+        ref = _attention.definition(q[b], kc[b, :n][live], vc[b, :n][live], n - 1, theta) if n else (0.0, 0.0)
+        assert _attention.beyond(o[b], *ref) <= 0
