@@ -741,6 +741,18 @@ extern "C" int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uin
   if ((ld_q | ld_k | ld_v | ld_o) % 8 || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15u))
     return set_error(ENNX_B200_INVALID_ARGUMENT,
                      "attention_packed: operands must be 16-byte aligned with strides of a multiple of 8");
+  const auto memory = [&](const uint16_t* p, int64_t ld, int heads) {
+    return Memory::rows(p, rows, ld * 2, (int64_t)heads * D * 2);
+  };
+  const Memory mq = memory(q, ld_q, hq), mk = memory(k, ld_k, hkv), mv = memory(v, ld_v, hkv), mo = memory(o, ld_o, hq);
+  const Memory mcu = Memory::bytes(cu_seqlens, ((int64_t)num_seqs + 1) * 4);
+  for (const Memory& m : {mq, mk, mv, mcu})
+    if (share_bytes(mo, m))
+      return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: o must not overlap q, k, v or cu_seqlens");
+  if (rope_theta > 0.0f && (share_bytes(mq, mk) || share_bytes(mq, mv) || share_bytes(mk, mv) || share_bytes(mq, mcu) ||
+                            share_bytes(mk, mcu)))
+    return set_error(ENNX_B200_INVALID_ARGUMENT,
+                     "attention_packed: q and k are rotated in place and cannot overlap one another, v or cu_seqlens");
   int dev = 0;
   int* err = nullptr;
   ENNX_TRY(serving_device(&dev, &err));

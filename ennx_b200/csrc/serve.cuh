@@ -4,6 +4,7 @@
 
 #include <mutex>
 
+#include "apart.cuh"
 #include "common.cuh"
 
 namespace ennx {

@@ -222,7 +222,8 @@ def gqa_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     [sequences + 1] on the device: sequence s owns rows cu_seqlens[s] ..
     cu_seqlens[s+1] - 1.  q and k are rotated in place when rope_theta > 0.
     Rows behind the last sequence are left as they are (undefined when out is
-    None)."""
+    None).  out shares no memory with q, k or v (other columns of one buffer are
+    fine)."""
     return _abi.serving().gqa_attention_packed(q, k, v, cu_seqlens, rope_theta, out)
 
 

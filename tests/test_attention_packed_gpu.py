@@ -255,3 +255,21 @@ def test_rows_whose_visible_scores_are_all_minus_infinity():
     assert torch.equal(o.isnan(), ref.isnan())
     close(o[~lost], ref[~lost], float(v.float().abs().max()))
     ops.device_status()
+
+
+def test_out_that_shares_memory_is_refused_and_columns_beside_are_not():
+    hq, hkv, rows = 4, 2, 300
+    buf = rnd(rows, (2 * hq + 2 * hkv) * D, seed=50)
+    q, k, v, o = (t.unflatten(1, (-1, D)) for t in buf.split([hq * D, hkv * D, hkv * D, hq * D], 1))
+    cu, call = starts([100, 200]), ops.gqa_attention_packed
+    want = call(q.clone(), k.clone(), v.clone(), cu)
+    for out in (q, buf[:, D:(hq + 1) * D].unflatten(1, (-1, D)), buf[:, 2 * hkv * D:(2 * hkv + hq) * D].unflatten(1, (-1, D))):
+        with pytest.raises(ValueError, match="must not overlap"):
+            call(q, k, v, cu, out=out)
+    with pytest.raises(ValueError, match="in place"):
+        call(q, k, buf[:, (hq + 1) * D:(hq + 1 + hkv) * D].unflatten(1, (-1, D)), cu)
+    # the same memory twice is fine where nothing is written to it
+    call(q, k, k, cu, rope_theta=0.0)
+    call(q, q[:, :hkv], k, cu, rope_theta=0.0)
+    assert call(q, k, v, cu, out=o) is o
+    assert torch.equal(o, want)

@@ -122,3 +122,16 @@ def test_packed_linear_decode_refuses_on_the_host():
     with pytest.raises(ValueError, match="CUDA"):
         ops.packed_linear_decode(torch.zeros(2, 64, dtype=BF16), torch.zeros(256, dtype=torch.uint8), torch.zeros(16),
                                  torch.zeros(16), lin)
+
+
+def test_packed_attention_refuses_memory_that_is_shared():
+    def call(q=1 << 40, k=(1 << 40) + 1024, v=(1 << 40) + 1536, o=1 << 41, cu=1 << 42, ld=1024, ldo=512, theta=0.0, rows=8):
+        return ("ennx_b200_gqa_attention_packed", P(q), ld, P(k), ld, P(v), ld, P(o), ldo, P(cu), 1, rows, 4, 2, theta, None)
+
+    for over in (dict(o=1 << 40, ldo=1024), dict(o=(1 << 40) + 512), dict(o=(1 << 40) + 1536, ldo=1024),
+                 dict(o=(1 << 40) - 7 * 1024, ldo=512), dict(cu=(1 << 41) + 1020), dict(o=(1 << 40) + 1024, ldo=1024),
+                 dict(o=(1 << 40) + 7 * 2048 + 2032)):
+        assert "must not overlap" in refused(*call(**over))
+    for over in (dict(k=(1 << 40) + 1008), dict(v=(1 << 40) + 2048), dict(v=(1 << 40) + 1520), dict(k=1 << 40),
+                 dict(cu=(1 << 40) + 2044)):
+        assert "in place" in refused(*call(theta=1e6, **over))
