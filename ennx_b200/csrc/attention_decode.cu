@@ -819,6 +819,31 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u)))
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: a 16-byte aligned workspace of %zu bytes required",
                      need);
+  const auto rows_at = [&](const uint16_t* at, int64_t ld, int heads) {
+    return Memory::rows(at, p->batch, ld * 2, (int64_t)heads * D * 2);
+  };
+  const auto cache_at = [&](const uint16_t* at, int64_t seq, int64_t token, int64_t head) {
+    return Memory{at, D * 2, {p->batch, p->room, p->hkv}, {seq * 2, token * 2, head * 2}};
+  };
+  const Memory mq = rows_at(p->q, p->ld_q, p->hq), mo = rows_at(p->o, p->ld_o, p->hq);
+  const Memory mk = rows_at(p->k, p->ld_k, p->hkv), mv = rows_at(p->v, p->ld_v, p->hkv);
+  const Memory kc = cache_at(p->k_cache, p->k_seq, p->k_token, p->k_head);
+  const Memory vc = cache_at(p->v_cache, p->v_seq, p->v_token, p->v_head), ml = Memory::bytes(p->lengths, (int64_t)p->batch * 4);
+  const bool in_place = p->o == p->q && (p->ld_o == p->ld_q || p->batch == 1);
+  if (!in_place && share_bytes(mo, mq))
+    return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: o must be q itself or not overlap it");
+  for (const Memory& m : {mk, mv, kc, vc, ml})
+    if (share_bytes(mo, m))
+      return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: o must not overlap k, v, the caches or lengths");
+  if (p->k) {
+    if (shares_own_bytes(kc) || shares_own_bytes(vc))
+      return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: rows of a cache that takes k and v must not overlap");
+    if (share_bytes(kc, vc))
+      return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: k_cache and v_cache that take k and v must be apart");
+    for (const Memory& m : {mq, mk, mv, ml})
+      if (share_bytes(kc, m) || share_bytes(vc, m))
+        return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: caches that take k and v must not overlap q, k, v or lengths");
+  }
   const int cluster = whole_cluster(segs, p->room);
   const Args a{p->q, p->k, p->v, p->o, p->ld_q, p->ld_k, p->ld_v, p->ld_o,
                {p->k_cache, p->v_cache, p->k_seq, p->k_token, p->k_head, p->v_seq, p->v_token, p->v_head},

@@ -238,7 +238,8 @@ def gqa_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     strides; lengths int32 [batch] on the device, tokens with the new one; k/v
     bf16 [batch, Hkv, 128], the new token's key and value, written to cache row
     lengths - 1 (None: the caches hold them).  rope_theta > 0 rotates q (not in
-    place) and k to position lengths - 1."""
+    place) and k to position lengths - 1.  out may be q itself; otherwise what is
+    written shares no memory with what is read."""
     return _abi.serving().gqa_attention_decode(q, k_cache, v_cache, lengths, k, v, rope_theta, out)
 
 

@@ -329,3 +329,34 @@ def test_a_key_of_minus_infinite_score_has_weight_zero(room, lengths, hq, theta)
         live = keep[:n]
         ref = _attention.definition(q[b], kc[b, :n][live], vc[b, :n][live], n - 1, theta) if n else (0.0, 0.0)
         assert _attention.beyond(o[b], *ref) <= 0
+
+
+def test_memory_that_is_shared_is_refused_and_views_of_one_buffer_are_not():
+    batch, room, hq, hkv = 3, 300, 4, 2
+    call, ln = ops.gqa_attention_decode, i32([300, 0, 77])
+    buf = rnd(batch, (2 * hq + 2 * hkv) * D, seed=90)
+    q, k, v, o = (t.unflatten(1, (-1, D)) for t in buf.split([hq * D, hkv * D, hkv * D, hq * D], 1))
+    apart = [rnd(batch, room, hkv, D, seed=91 + i) for i in range(2)]
+    want = call(q.clone(), *(c.clone() for c in apart), ln, k=k.clone(), v=v.clone())
+    # keys and values side by side in one tensor, by token and by head
+    for kv in (torch.stack(apart, 2).unbind(2), torch.stack(apart, 3).unbind(3),
+               [c.transpose(1, 2) for c in torch.stack([c.transpose(1, 2) for c in apart], 3).unbind(3)]):
+        assert call(q, *kv, ln, k=k, v=v, out=o) is o
+        assert torch.equal(o, want)
+    kc, vc = apart
+    for out in (buf[:, D:(hq + 1) * D].unflatten(1, (-1, D)), q[:, :2]):
+        with pytest.raises(ValueError, match="q itself|shape of q"):
+            call(q, kc, vc, ln, k=k, v=v, out=out)
+    for out in (kc[0, :batch * 2].view(batch, hq, D), buf[:, 2 * hkv * D:4 * hkv * D].unflatten(1, (-1, D))):
+        with pytest.raises(ValueError, match="o must not overlap"):
+            call(q, kc, vc, ln, k=k, v=v, out=out)
+    with pytest.raises(ValueError, match="must be apart"):
+        whole = torch.cat([kc, vc], 1)
+        call(q, whole[:, :room], whole[:, 1:room + 1], ln, k=k, v=v)
+    with pytest.raises(ValueError, match="rows of a cache"):
+        call(q, torch.as_strided(kc, (batch, room, hkv, D), (room * D, D, 64, 1)), vc, ln, k=k, v=v)
+    with pytest.raises(ValueError, match="caches that take"):
+        call(q, kc, vc, ln, k=kc[:, 5], v=v)
+    # caches that are only read may be anything
+    assert call(q, kc, kc, ln).isfinite().all()
+    ops.device_status()

@@ -135,3 +135,27 @@ def test_packed_attention_refuses_memory_that_is_shared():
     for over in (dict(k=(1 << 40) + 1008), dict(v=(1 << 40) + 2048), dict(v=(1 << 40) + 1520), dict(k=1 << 40),
                  dict(cu=(1 << 40) + 2044)):
         assert "in place" in refused(*call(theta=1e6, **over))
+
+
+def test_decode_attention_refuses_memory_that_is_shared():
+    base = 1 << 40
+
+    def call(**over):
+        f = dict(q=base, ld_q=1024, k=base + 1024, ld_k=1024, v=base + 1536, ld_v=1024, k_cache=1 << 41, k_seq=8192,
+                 k_token=256, k_head=128, v_cache=1 << 42, v_seq=8192, v_token=256, v_head=128, lengths=1 << 43, o=1 << 44,
+                 ld_o=512, batch=4, room=32, hq=4, hkv=2)
+        f.update(over)
+        return ("ennx_b200_gqa_attention_decode", ctypes.byref(_abi.DecodeAttention(**f)), 0.0, None, 0, None)
+
+    for over in (dict(o=base + 16, ld_o=1024), dict(o=base), dict(o=base - 2048, ld_o=1024), dict(o=base + 512)):
+        assert "q itself" in refused(*call(**over))
+    reads = dict(k=0, v=0)
+    for over in (dict(o=base + 1024, ld_o=1024), dict(o=(1 << 41) + 8192), dict(o=(1 << 42) + 4 * 8192 * 2 - 16),
+                 dict(o=(1 << 43) - 1024 * 3 - 1008), dict(o=(1 << 41) + 8192, **reads)):
+        assert "o must not overlap" in refused(*call(**over))
+    for over in (dict(k_head=120), dict(k_token=64, k_head=32 * 64, k_seq=2 * 32 * 64), dict(v_seq=8192 - 128)):
+        assert "rows of a cache" in refused(*call(**over))
+    for over in (dict(v_cache=(1 << 41) + 256), dict(v_cache=(1 << 41) + 8192 * 2 - 16)):
+        assert "must be apart" in refused(*call(**over))
+    for over in (dict(k_cache=base + 2048), dict(v_cache=base + 1024), dict(k_cache=(1 << 43) - 8192)):
+        assert "caches that take" in refused(*call(**over))
