@@ -787,6 +787,21 @@ int32_t ennx_b200_moe_layer_decode(const uint16_t* x, const uint16_t* w_router, 
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u))
     return set_error(ENNX_B200_INVALID_ARGUMENT, "moe_layer_decode: a 16-byte aligned workspace of %zu bytes required",
                      need);
+  const int64_t row = (int64_t)hidden * 2, picks = tokens * top_k;
+  const Memory read[] = {Memory::bytes(x, tokens * row), Memory::bytes(w_router, experts * row),
+                         Memory::bytes(w_gate_up, experts * row * 2 * expert_width),
+                         Memory::bytes(w_down, experts * row * expert_width), Memory::bytes(residual, tokens * row)};
+  const Memory written[] = {Memory::bytes(y, tokens * row), Memory::bytes(index, picks * 4), Memory::bytes(gate, picks * 4),
+                            Memory::bytes(workspace, (int64_t)need)};
+  for (const Memory& w : written) {
+    for (const Memory& r : read)
+      if (share_bytes(w, r) && !(w.base == y && r.base == residual && y == residual))
+        return set_error(ENNX_B200_INVALID_ARGUMENT,
+                         "moe_layer_decode: outputs and workspace must not overlap x or the weights, nor the residual (y may be it)");
+    for (const Memory& other : written)
+      if (&w != &other && share_bytes(w, other))
+        return set_error(ENNX_B200_INVALID_ARGUMENT, "moe_layer_decode: outputs and workspace must not overlap");
+  }
   int dev = 0;
   int* status = nullptr;
   ENNX_TRY(serving_device(&dev, &status));

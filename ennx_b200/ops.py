@@ -198,7 +198,8 @@ def moe_layer_decode(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.T
                      out: torch.Tensor | None = None):
     """``moe_layer`` for at most 64 tokens (see ``ennx_b200_moe_layer_decode``):
     bound by the bytes of the picked experts' weights.  x and residual bf16
-    [tokens, hidden], weights as for ``moe_layer``; all contiguous."""
+    [tokens, hidden], weights as for ``moe_layer``; all contiguous.  out may be
+    the residual itself and shares no memory with anything else."""
     return _abi.serving().moe_layer_decode(x, w_router, w_gate_up, w_down, top_k, residual, return_routing, out)
 
 

@@ -243,3 +243,18 @@ def test_router_whose_blocks_have_next_to_nothing_to_do(T, H, E, k):
     runs = [ops.moe_layer_decode(x, wr, wgu, wd, k, return_routing=True) for _ in range(200)]
     assert all(torch.equal(a, y) and torch.equal(b, idx) and torch.equal(c, gate) for a, b, c in runs)
     ops.device_status()
+
+
+def test_out_that_shares_memory_is_refused():
+    T, H, E, k, I = 4, 256, 8, 2, 128
+    buf, (wr, wgu, wd) = rnd(5 * T, H, seed=80), weights(H, E, I, 81)
+    x, res, call = buf[:T], buf[T:2 * T], ops.moe_layer_decode
+    for out in (x, buf[1:T + 1], wr[:T], wgu[0, :T]):
+        with pytest.raises(ValueError, match="must not overlap"):
+            call(x, wr, wgu, wd, k, residual=res, out=out)
+    with pytest.raises(ValueError, match="must not overlap"):
+        call(x, wr, wgu, wd, k, residual=res, out=buf[T + 1:2 * T + 1])
+    want = call(x, wr, wgu, wd, k, residual=res)
+    assert torch.equal(call(x, wr, wgu, wd, k, residual=res, out=buf[2 * T:3 * T]), want)
+    assert torch.equal(call(x, wr, wgu, wd, k, residual=x), call(x, wr, wgu, wd, k, residual=x.clone()))
+    assert torch.equal(call(x, wr, wgu, wd, k, residual=res, out=res), want)

@@ -159,3 +159,19 @@ def test_decode_attention_refuses_memory_that_is_shared():
         assert "must be apart" in refused(*call(**over))
     for over in (dict(k_cache=base + 2048), dict(v_cache=base + 1024), dict(k_cache=(1 << 43) - 8192)):
         assert "caches that take" in refused(*call(**over))
+
+
+def test_moe_layer_decode_refuses_memory_that_is_shared():
+    far = [1 << (40 + i) for i in range(9)]
+
+    def call(x=far[0], wr=far[1], wgu=far[2], wd=far[3], res=far[4], y=far[5], index=far[6], gate=far[7], ws=far[8]):
+        p = [P(a) for a in (x, wr, wgu, wd)]
+        return ("ennx_b200_moe_layer_decode", *p, 3, 256, 8, 2, 128, P(res), P(y), P(index), P(gate), P(ws), 1 << 20, None)
+
+    size = 3 * 256 * 2
+    for over in (dict(y=far[0]), dict(y=far[0] + size - 2), dict(y=far[1] + 8 * 512 - 2), dict(y=far[2] + 8 * 256 * 512 - 2),
+                 dict(y=far[3] + 8 * 256 * 256 - 2), dict(y=far[4] + 2), dict(y=far[4] - size + 2), dict(index=far[0]),
+                 dict(gate=far[4] + 8), dict(ws=far[3] + 16), dict(ws=far[0] - 16)):
+        assert "must not overlap x" in refused(*call(**over))
+    for over in (dict(index=far[5]), dict(gate=far[6] + 20), dict(ws=far[7] - 16), dict(y=far[8])):
+        assert "workspace must not overlap" in refused(*call(**over))
