@@ -639,6 +639,12 @@ extern "C" int32_t ennx_b200_packed_linear_decode(const uint16_t* x, int64_t tok
   p.w = weights + p.d.byte_offset;
   p.sc = scales + p.d.scale_offset;
   p.bi = biases + p.d.bias_offset;
+  const Memory written = Memory::bytes(out, tokens * (int64_t)p.d.output_width * 2);
+  const int64_t codes = (int64_t)(p.d.output_width * p.d.row_bytes), groups = (int64_t)(p.d.output_width * p.d.groups) * 4;
+  for (const Memory& read : {Memory::bytes(x, tokens * (int64_t)p.d.input_width * 2), Memory::bytes(p.w, codes),
+                             Memory::bytes(p.sc, groups), Memory::bytes(p.bi, groups)})
+    if (share_bytes(written, read))
+      return set_error(ENNX_B200_INVALID_ARGUMENT, "packed linear decode: out must not overlap x, the codes, scales or biases");
   p.out = out;
   p.seed = seed;
   p.tokens = (int)tokens;

@@ -159,7 +159,8 @@ def packed_linear_decode(x: torch.Tensor, weights: torch.Tensor, scales: torch.T
                          out: torch.Tensor | None = None) -> torch.Tensor:
     """``packed_linear`` for at most 16 tokens, straight from the codes (see
     ``ennx_b200_packed_linear_decode``): any widths and group size, weights not
-    rounded to bf16.  The arenas must hold the whole linear."""
+    rounded to bf16.  The arenas must hold the whole linear; out shares no memory
+    with what is read."""
     return _abi.serving().packed_linear_decode(x, weights, scales, biases, linear, seed, out)
 
 

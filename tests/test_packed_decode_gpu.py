@@ -181,3 +181,16 @@ def test_columns_whose_bits_pass_32_bits(bits, inp, group, offset, moved):
     xt = x[0, -tail:].double()
     ref, size = codes @ xt * 0.5, codes @ xt.abs() * 0.5
     assert ((got - ref).abs() <= 1.001 * 2.0 ** -8 * ref.abs() + 2.0 ** -14 * size).all()
+
+
+def test_out_that_shares_memory_is_refused():
+    w, sc, bi, lin = make(64, 64, 4, 32, 40, offsets=(256, 64, 64))
+    x, call = x_of(4, 64, 41), ops.packed_linear_decode
+    both = torch.cat([x, x])
+    for out in (x, w[256:768].view(torch.bfloat16).view(4, 64), sc[64:192].view(torch.bfloat16).view(4, 64),
+                bi[64:192].view(torch.bfloat16).view(4, 64)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            call(x, w, sc, bi, lin, out=out)
+    with pytest.raises(ValueError, match="must not overlap"):
+        call(both[:4], w, sc, bi, lin, out=both[3:7])
+    assert torch.equal(call(both[:4], w, sc, bi, lin, out=both[4:]), call(x, w, sc, bi, lin))

@@ -175,3 +175,17 @@ def test_moe_layer_decode_refuses_memory_that_is_shared():
         assert "must not overlap x" in refused(*call(**over))
     for over in (dict(index=far[5]), dict(gate=far[6] + 20), dict(ws=far[7] - 16), dict(y=far[8])):
         assert "workspace must not overlap" in refused(*call(**over))
+
+
+def test_packed_linear_decode_refuses_memory_that_is_shared():
+    far = [1 << (40 + i) for i in range(5)]
+    lin = _abi.PackedLinear(64, 16, 32, 100, 8, 4, 32, 0, 0, 0)  # codes 8 x 50 bytes, scales and biases 8 x 4 floats
+
+    def call(x=far[0], w=far[1], sc=far[2], bi=far[3], out=far[4]):
+        return ("ennx_b200_packed_linear_decode", P(x), 3, P(w), P(sc), P(bi), ctypes.byref(lin),
+                _abi.PerturbSeed(0, 0, 0), P(out), None)
+
+    size = 3 * 8 * 2
+    for out in (far[0], far[0] + 3 * 200 - 2, far[0] - size + 2, far[1] + 64 + 398, far[1] + 64 - size + 2,
+                far[2] + 64 + 126, far[2] + 64 - size + 2, far[3] + 128 + 126, far[3] + 128 - size + 2):
+        assert "must not overlap" in refused(*call(out=out))
