@@ -812,8 +812,8 @@ int32_t ennx_b200_gqa_attention_decode(const ennx_b200_decode_attention* p, floa
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_decode: k_cache and v_cache that take k and v must be apart");
   const int group = p->hq / p->hkv, rows = block_rows(group), blocks = (group + rows - 1) / rows;
   const int64_t segs = segments(p->batch, p->hq, p->hkv);
-  // a warp's run is counted in 32 bits
-  if (segs > 0x7fffffffLL - 65536 || segs * (p->room / kStep + 1 + kHeadCost) / ((int64_t)split_grid() * kWarps) > 0x7fffff00LL)
+  // a warp's run and the columns of a row are counted in 32 bits
+  if (p->hq > 0x7fffffff / D || segs > 0x7fffffffLL - 65536 || segs * (p->room / kStep + 1 + kHeadCost) / ((int64_t)split_grid() * kWarps) > 0x7fffff00LL)
     return set_error(ENNX_B200_UNSUPPORTED, "attention_decode: too many heads");
   const size_t need = ennx_b200_gqa_attention_decode_workspace_size(p->batch, p->room, p->hq, p->hkv);
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u)))

@@ -734,7 +734,8 @@ extern "C" int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uin
   if (!q || !k || !v || !o) return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: null argument");
   if (rope_theta > 0.0f && (q == k || q == v || k == v))
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: q and k are rotated in place and cannot be shared");
-  if (rows > 0x7fffff00LL || (rows + 2 * BQ - 1) / (2 * BQ) * hq > 0x7fffffffLL)
+  // columns of a row are counted in 32 bits
+  if (rows > 0x7fffff00LL || hq > 0x7fffffff / D || (rows + 2 * BQ - 1) / (2 * BQ) * hq > 0x7fffffffLL)
     return set_error(ENNX_B200_UNSUPPORTED, "attention_packed: too many rows or heads");
   if (ld_q < (int64_t)hq * D || ld_o < (int64_t)hq * D || ld_k < (int64_t)hkv * D || ld_v < (int64_t)hkv * D)
     return set_error(ENNX_B200_INVALID_ARGUMENT, "attention_packed: a row stride is shorter than its heads");

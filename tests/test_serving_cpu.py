@@ -189,3 +189,14 @@ def test_packed_linear_decode_refuses_memory_that_is_shared():
     for out in (far[0], far[0] + 3 * 200 - 2, far[0] - size + 2, far[1] + 64 + 398, far[1] + 64 - size + 2,
                 far[2] + 64 + 126, far[2] + 64 - size + 2, far[3] + 128 + 126, far[3] + 128 - size + 2):
         assert "must not overlap" in refused(*call(out=out))
+
+
+def test_heads_whose_columns_pass_32_bits_are_refused():
+    heads, far = 1 << 24, [P(1 << (40 + i)) for i in range(7)]
+    assert "too many" in refused("ennx_b200_gqa_attention_packed", far[0], heads * 128, far[1], 128, far[2], 128, far[3],
+                                 heads * 128, far[4], 1, 1, heads, 1, 0.0, None, status=_abi.UNSUPPORTED)
+    p = _abi.DecodeAttention(q=1 << 40, ld_q=heads * 128, k=1 << 41, ld_k=heads * 128, v=1 << 42, ld_v=heads * 128,
+                             k_cache=1 << 43, k_seq=0, k_token=0, k_head=128, v_cache=1 << 44, v_seq=0, v_token=0,
+                             v_head=128, lengths=1 << 45, o=1 << 46, ld_o=heads * 128, batch=1, room=1, hq=heads, hkv=heads)
+    assert "too many" in refused("ennx_b200_gqa_attention_decode", ctypes.byref(p), 0.0, None, 0, None,
+                                 status=_abi.UNSUPPORTED)
