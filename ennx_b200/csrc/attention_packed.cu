@@ -45,8 +45,8 @@
 // Masked places may hold anything: masked scores are replaced, not added to,
 // but a masked V row still meets P = 0 in the MMA and an infinity or NaN there
 // makes 0 * inf = NaN.  Rows behind the last sequence are cleared in shared
-// memory; a non-finite output is recomputed by `careful_row`, which reads
-// visible keys only.
+// memory; a non-finite output whose scores are numbers is recomputed by
+// `careful_row`, which reads visible keys only.
 #include "kernels.cuh"
 #include "serve.cuh"
 
@@ -637,7 +637,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                            pack_bf16x2(f[8 * g + 6], f[8 * g + 7]));
           }
         }
-        uint32_t redo = __ballot_sync(0xffffffffu, mine && worst != worst);
+        // A masked score adds exactly 0 to the sum, so a sum of NaN comes from a
+        // visible one: that row is NaN throughout, as it stands (and where the
+        // sum is 0).  What is left are values.
+        uint32_t redo = __ballot_sync(0xffffffffu, mine && worst != worst && l > 0.0f);
         __syncwarp();
         while (redo) {
           const int src = __ffs(redo) - 1;

@@ -273,3 +273,37 @@ def test_out_that_shares_memory_is_refused_and_columns_beside_are_not():
     call(q, q[:, :hkv], k, cu, rope_theta=0.0)
     assert call(q, k, v, cu, out=o) is o
     assert torch.equal(o, want)
+
+
+def lasts(call, runs=3):
+    """Milliseconds of a call, the best of some runs."""
+    best = math.inf
+    for _ in range(runs):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+def test_bad_keys_at_the_start_of_a_long_prompt_cost_no_recomputation():
+    rows, hq, hkv = 16384, 16, 4
+    q, k, v, cu = rnd(rows, hq, D, seed=60), rnd(rows, hkv, D, seed=61), rnd(rows, hkv, D, seed=62), starts([rows])
+
+    def call():
+        return ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0)
+
+    want = call()
+    clean = lasts(call)
+    for bad in (math.nan, math.inf):
+        k[0, :2, 3] = bad
+        o = call()
+        if bad != bad:
+            assert o[:, :8].isnan().all()
+        else:  # a score of -infinity leaves its row as the others have it, one of +infinity makes it NaN
+            assert torch.equal(o[:, :8].isnan(), (q[:, :8, 3] > 0)[..., None].expand(-1, -1, D) | (torch.arange(rows, device="cuda") == 0)[:, None, None])
+        assert torch.equal(o[:, 8:], want[:, 8:])
+        assert lasts(call) < 4 * clean
+    ops.device_status()
