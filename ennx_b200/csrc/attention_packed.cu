@@ -45,8 +45,11 @@
 // Masked places may hold anything: masked scores are replaced, not added to,
 // but a masked V row still meets P = 0 in the MMA and an infinity or NaN there
 // makes 0 * inf = NaN.  Rows behind the last sequence are cleared in shared
-// memory; a non-finite output whose scores are numbers is recomputed by
-// `careful_row`, which reads visible keys only.
+// memory; a non-finite output whose scores are numbers, and which no visible
+// value explains, is recomputed by `careful_row`, which reads visible keys only.
+// That is slow, 0.15 us a key and row with 32 rows one after the other (16384
+// tokens whose last value is infinite 77 ms), but falls to the rows of the tiles
+// that hold a bad value only.
 #include "kernels.cuh"
 #include "serve.cuh"
 
@@ -224,6 +227,110 @@ __device__ __noinline__ void careful_row(const Operands& t, int row, int lo, int
   const float inv = 1.0f / l;  // every visible score -inf: 0 / 0
   *reinterpret_cast<uint2*>(t.o + (long long)row * t.ldo + h * D + lane * 4) =
       make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
+}
+
+// A set of the columns of a head, a bit each.
+struct Columns {
+  uint32_t w[4];
+  __device__ __forceinline__ void add(const Columns& o, bool where) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] |= where ? o.w[i] : 0u;
+  }
+};
+// the set that byte b of a lane of 16, columns 8 * lane .. 8 * lane + 7, makes with the 15 beside it
+__device__ __forceinline__ Columns columns_of(uint32_t b, int first_lane) {
+  Columns c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c.w[i] = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c.w[i] |= __shfl_sync(0xffffffffu, b, first_lane + 4 * i + j) << (8 * j);
+  }
+  return c;
+}
+
+// Do outputs `bad` of a lane's row, whose scores are numbers, have to be
+// recomputed?  The warp reads the values of keys [from, to), which its tiles
+// covered, once for its 32 rows; the row sees those in [lo, row].  A visible NaN
+// makes its column NaN and a visible infinity makes it what it is; a masked one
+// (which met a weight of 0) makes it NaN wrongly.  A column without either is
+// recomputed too: its sum passed the range of fp32.  (Without this look every
+// row that saw an infinity for real was recomputed: 16384 tokens of 16 heads
+// behind one of them 278 ms, now 3.2.)
+__device__ __forceinline__ bool has_to_be_redone(const Operands& t, Columns bad, int row, int lo, int from, int to, int kvh,
+                                              int lane) {
+  constexpr int kLoads = 8, kKeys = 2 * kLoads;  // two keys a load, 16 lanes each
+  Columns seen{}, seen_nan{}, masked{};
+  const uint16_t* v = t.v + kvh * D + (lane & 15) * 8;
+  for (int j0 = from; j0 < to; j0 += kKeys) {
+    uint4 x[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const long long j = min(j0 + 2 * u + (lane >> 4), to - 1);
+      x[u] = *reinterpret_cast<const uint4*>(v + j * t.ldv);
+    }
+    uint32_t any = 0u;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= __vcmpeq2(w[i] & 0x7f807f80u, 0x7f807f80u);
+    }
+    if (!__any_sync(0xffffffffu, any != 0u)) continue;
+#pragma unroll 1
+    for (int u = 0; u < kLoads; ++u) {
+      const long long j = min(j0 + 2 * u + (lane >> 4), to - 1);
+      const uint4 y = *reinterpret_cast<const uint4*>(v + j * t.ldv);
+      const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+      uint32_t wild = 0u, nan = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t b = w[i] >> (16 * e) & 0x7fffu;
+          wild |= (b >= 0x7f80u ? 1u : 0u) << (2 * i + e);
+          nan |= (b > 0x7f80u ? 1u : 0u) << (2 * i + e);
+        }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int key = min(j0 + 2 * u + half, to - 1);
+        const bool visible = key >= lo && key <= row;
+        const Columns cw = columns_of(wild, 16 * half), cn = columns_of(nan, 16 * half);
+        seen.add(cw, visible);
+        seen_nan.add(cn, visible);
+        masked.add(cw, !visible);
+      }
+    }
+  }
+  uint32_t redo = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) redo |= bad.w[i] & ~seen_nan.w[i] & (masked.w[i] | ~seen.w[i]);
+  return redo != 0u;
+}
+
+// A warp's rows whose outputs are not finite although their scores are numbers
+// (`wild`); those outputs stand in global memory and, times 1 / inv, at o_col.
+__device__ __noinline__ void repair_rows(const Operands& t, uint32_t o_col, float inv, bool wild, int row, int lo, int from,
+                                         int to, int h, int kvh, float scale_log2) {
+  const int lane = threadIdx.x & 31;
+  Columns bad;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t ov[32];
+    tmem_ld32(o_col + c * 32, ov);
+    tmem_ld_wait();
+    bad.w[c] = 0u;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) bad.w[c] |= (isfinite(__uint_as_float(ov[i]) * inv) ? 0u : 1u) << i;
+  }
+  const bool again = has_to_be_redone(t, bad, row, lo, from, to, kvh, lane);
+  uint32_t redo = __ballot_sync(0xffffffffu, wild && again);
+  __syncwarp();  // the rows' first outputs are written
+  while (redo) {
+    const int src = __ffs(redo) - 1;
+    redo &= redo - 1;
+    careful_row(t, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, lo, src), h, kvh, scale_log2, lane);
+  }
 }
 
 // All roles wait while rows are recomputed, which lasts long in long sequences
@@ -640,13 +747,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         // A masked score adds exactly 0 to the sum, so a sum of NaN comes from a
         // visible one: that row is NaN throughout, as it stands (and where the
         // sum is 0).  What is left are values.
-        uint32_t redo = __ballot_sync(0xffffffffu, mine && worst != worst && l > 0.0f);
-        __syncwarp();
-        while (redo) {
-          const int src = __ffs(redo) - 1;
-          redo &= redo - 1;
-          careful_row(t, qx0 + q * 32 + src, __shfl_sync(0xffffffffu, lo, src), h, kvh, scale_log2, lane);
-        }
+        const bool wild = mine && worst != worst && l > 0.0f;
+        if (__any_sync(0xffffffffu, wild))
+          repair_rows(t, o_col, inv, wild, qpos, lo, (w.kt0 + w.js[x]) * BKV, min(end, qx0 + BQ), h, kvh, scale_log2);
       } else {
         *abort_flag = 1;
       }

@@ -260,8 +260,9 @@ ENNX_B200_API int32_t ennx_b200_gqa_attention(uint16_t* q, uint16_t* k, const ui
  * applied to q and k IN PLACE first, which then overlap neither one another
  * nor v.  o must not overlap q, k or v.  Softmax statistics in fp32; a
  * non-finite key or value reaches only the rows that see it, and a row whose
- * visible scores are all -infinity is NaN, as the softmax is.  Allocates
- * nothing. */
+ * visible scores are all -infinity is NaN, as the softmax is.  An infinity or
+ * NaN in v costs time: rows less than 128 before it are computed a second time,
+ * key by key (some 5 us per key of their sequence).  Allocates nothing. */
 ENNX_B200_API int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uint16_t* k, int64_t ld_k,
                                                      const uint16_t* v, int64_t ld_v, uint16_t* o, int64_t ld_o,
                                                      const int32_t* cu_seqlens, int32_t num_seqs, int64_t rows,

@@ -307,3 +307,64 @@ def test_bad_keys_at_the_start_of_a_long_prompt_cost_no_recomputation():
         assert torch.equal(o[:, 8:], want[:, 8:])
         assert lasts(call) < 4 * clean
     ops.device_status()
+
+
+def test_bad_values_at_the_start_of_a_long_prompt_cost_no_recomputation():
+    rows, hq, hkv = 16384, 16, 4
+    q, k, v, cu = rnd(rows, hq, D, seed=63), rnd(rows, hkv, D, seed=64), rnd(rows, hkv, D, seed=65), starts([rows])
+
+    def call():
+        return ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0)
+
+    want = call()
+    clean = lasts(call)
+    v[0, 0, 5], v[0, 1, 6], v[1000, 3] = math.nan, math.inf, math.nan
+    o = call()
+    assert o[:, :4, 5].isnan().all() and (o[:, 4:8, 6] == math.inf).all() and o[1000:, 12:].isnan().all()
+    same = torch.ones_like(o, dtype=torch.bool)
+    same[:, :4, 5] = same[:, 4:8, 6] = same[896:, 12:] = False
+    assert torch.equal(o[same], want[same])
+    # the rows of its tile before the bad one are recomputed, with weights of fp32
+    assert ((o[896:1000, 12:].double() - want[896:1000, 12:].double()).abs() <= 4 * 2.0 ** -8 * 5).all()
+    assert lasts(call) < 20 * clean
+    ops.device_status()
+
+
+@pytest.mark.parametrize("many", [3, 60])
+def test_bad_values_anywhere(many):
+    """Infinities and NaN at random places: each reaches its column of the rows that see it, and nothing else."""
+    lengths, hq, hkv = [5, 130, 0, 1, 300, 77, 513], 4, 2
+    rows = sum(lengths)
+    q, k, v = rnd(rows, hq, D, seed=66), rnd(rows, hkv, D, seed=67), rnd(rows, hkv, D, seed=68)
+    g = torch.Generator().manual_seed(69)
+    sign = torch.zeros(3, rows, hkv, D, dtype=torch.bool, device="cuda")  # +inf, -inf, NaN
+    for _ in range(many):
+        at = [int(torch.randint(n, (1,), generator=g)) for n in (3, rows, hkv, D)]
+        sign[tuple(at)] = True
+    finite = v.masked_fill(sign.any(0), 0.0)
+    for s, value in zip(sign, (math.inf, -math.inf, math.nan)):
+        v[s] = value
+    seq = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths)).cuda()
+    visible = ((seq[:, None] == seq) & (torch.arange(rows).cuda()[:, None] >= torch.arange(rows).cuda())).float()
+    kinds = torch.stack([v == math.inf, v == -math.inf, v.isnan()])
+    sees = (torch.einsum("ij,cjhd->cihd", visible, kinds.float()) > 0).repeat_interleave(hq // hkv, 2)
+    nan = sees[2] | (sees[0] & sees[1])
+    o = ops.gqa_attention_packed(q, k, v, starts(lengths), rope_theta=0.0)
+    assert torch.equal(o.isnan(), nan)
+    assert torch.equal(o == math.inf, sees[0] & ~nan) and torch.equal(o == -math.inf, sees[1] & ~nan)
+    clean = ~sees.any(0)
+    err = (o.double() - reference(q, k, finite, lengths)).abs()[clean]
+    # a weight of a value that counts as 0 here is part of the sum in both
+    assert float(err.max()) <= 1.001 * 2.0 ** -8 * 2 * float(finite.float().abs().max())
+    ops.device_status()
+
+
+def test_values_near_the_end_of_the_range():
+    # the second score is 7 doublings above the first, within the lazy rescale's 8: the product with a weight of 2^7 is no number
+    q, k, v = (torch.zeros(2, 1, D, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    q[:, 0, 0], k[1, 0, 0] = 7.0, 7.0 * math.log(2) * math.sqrt(D) / 7.0
+    v[:, 0, 3], v[:, 0, 4] = 1e37, -1e37
+    v[:, 0, 5] = 1.0
+    o = ops.gqa_attention_packed(q, k, v, starts([2]), rope_theta=0.0)
+    ref = reference(q, k, v, [2])
+    assert ((o.double() - ref).abs() <= 2.01 * 2.0 ** -8 * ref.abs()).all()
