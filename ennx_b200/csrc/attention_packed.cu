@@ -333,9 +333,10 @@ __device__ __noinline__ void repair_rows(const Operands& t, uint32_t o_col, floa
   }
 }
 
-// All roles wait while rows are recomputed, which lasts long in long sequences
-// (256 rows of 131072 keys 0.7 s): waits are bounded by a minute here.
-constexpr unsigned long long kItemLimitNs = 60000000000ull;
+// All roles wait while rows are recomputed, 5.6 us per key of a sequence for
+// the 32 rows of a warp (131072 keys 0.74 s).  So waits are bounded by the usual
+// limit and nearly four times that for the longest sequence there can be.
+unsigned long long wait_limit_ns(int64_t rows) { return kWaitLimitNs + 20000ull * (unsigned long long)rows; }
 
 struct True { static constexpr bool value = true; };
 struct False { static constexpr bool value = false; };
@@ -343,7 +344,7 @@ struct False { static constexpr bool value = false; };
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Operands t, Packing pk,
-                            int heads, int group, float scale_log2, int* err) {
+                            int heads, int group, float scale_log2, unsigned long long limit_ns, int* err) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* base = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     return w;
   };
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    return mbar_wait(b, parity, err, kItemLimitNs);
+    return mbar_wait(b, parity, err, limit_ns);
   };
   // by a whole warp, the same answer in every lane
   auto warp_wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
@@ -888,7 +889,7 @@ extern "C" int32_t ennx_b200_gqa_attention_packed(uint16_t* q, int64_t ld_q, uin
   cfg.attrs = &early;
   cfg.numAttrs = rope_theta > 0.0f ? 1 : 0;
   ENNX_CUDA(cudaLaunchKernelEx(&cfg, prompt_attention_kernel, tq, tk, tv, t, pk, hq, hq / hkv,
-                               1.4426950408889634f / sqrtf((float)D), err), "packed attention");
+                               1.4426950408889634f / sqrtf((float)D), wait_limit_ns(rows), err), "packed attention");
   ENNX_LAUNCH_CHECK("packed attention");
   return ENNX_B200_OK;
 }

@@ -368,3 +368,18 @@ def test_values_near_the_end_of_the_range():
     o = ops.gqa_attention_packed(q, k, v, starts([2]), rope_theta=0.0)
     ref = reference(q, k, v, [2])
     assert ((o.double() - ref).abs() <= 2.01 * 2.0 ** -8 * ref.abs()).all()
+
+
+def test_a_long_recomputation_ends_before_the_waits_for_it():
+    """A bad last value: the rows of its tile walk the whole prompt one after
+    another while every other role waits (3 s at 50000 rows; the walk takes 0.3)."""
+    rows = 50000
+    q, k, v, cu = rnd(rows, 2, D, seed=70), rnd(rows, 1, D, seed=71), rnd(rows, 1, D, seed=72), starts([rows])
+    want = ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0)
+    v[-1, 0, 9] = math.nan
+    o = ops.gqa_attention_packed(q, k, v, cu, rope_theta=0.0)
+    ops.device_status()
+    assert o[-1, :, 9].isnan().all() and o[:-1].isfinite().all()
+    first = (rows - 1) // 128 * 128
+    assert torch.equal(o[:first], want[:first])
+    assert ((o[first:-1].double() - want[first:-1].double()).abs() <= 4 * 2.0 ** -8 * 5).all()
