@@ -3,7 +3,9 @@
 ``python -m ennx_b200.build`` (or ``__graft_entry__.build()``) compiles every
 ``csrc/*.cu`` with nvcc for ``sm_100a`` and links one shared library exporting
 the C ABI declared in ``include/ennx_b200.h``, then ``csrc/bindings.cpp`` into
-the extension module of the serving operators.  Objects are cached under
+the extension module of the serving operators.  The library needs nvcc alone;
+without torch or its C++ headers the module is left out, with a note, and the
+serving operators are reached through the C ABI only.  Objects are cached under
 ``_build/`` and rebuilt when a source or header is newer.
 """
 from __future__ import annotations
@@ -11,6 +13,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -47,17 +50,22 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def _build_bindings() -> None:
-    """The torch extension module over the library (host code only)."""
+    """The torch extension module over the library (host code only), where torch can be built against."""
+    try:
+        import torch
+    except ImportError:
+        print("no torch here: the module of the serving operators is not built", file=sys.stderr)
+        return
+    root, python = Path(torch.__file__).parent, Path(sysconfig.get_paths()["include"])
+    if not (root / "include" / "ATen" / "ATen.h").exists() or not (python / "Python.h").exists():
+        print("no C++ headers of torch and Python here: the module of the serving operators is not built", file=sys.stderr)
+        return
     src = CSRC / "bindings.cpp"
     newest = max(p.stat().st_mtime for p in [src, *_headers()])
     if BINDINGS.exists() and BINDINGS.stat().st_mtime >= newest:
         return
-    import sysconfig
-
-    import torch
-    root = Path(torch.__file__).parent
     inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", ROOT / "include",
-           Path(NVCC).parents[1] / "include", Path(sysconfig.get_paths()["include"])]
+           Path(NVCC).parents[1] / "include", python]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{p}" for p in inc],
            str(src), "-o", str(BINDINGS), f"-L{LIB.parent}", "-lennx_b200", "-Wl,-rpath,$ORIGIN",
