@@ -253,11 +253,20 @@ def serving():
     if _serving is None:
         import importlib.machinery
         import importlib.util
+        import json
 
         import torch  # noqa: F401  (the module links against torch's libraries)
         path = LIB_PATH.with_name("ennx_b200_serving.so")
         if not path.exists():
             raise EnnxB200Error(CUDA_ERROR, f"{path} is missing: run `python -m ennx_b200.build`")
+        stamp = path.with_suffix(".key")
+        if stamp.exists():
+            from .build import bindings_key
+            made = json.loads(stamp.read_text())
+            for what, here in bindings_key().items():
+                if made.get(what) != here:
+                    raise EnnxB200Error(CUDA_ERROR, f"{path} was built for {what} {made.get(what)}, this is {here}: run "
+                                                    "`python -m ennx_b200.build`")
         lib()
         loader = importlib.machinery.ExtensionFileLoader("ennx_b200_serving", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("ennx_b200_serving", loader))

@@ -6,10 +6,12 @@ the C ABI declared in ``include/ennx_b200.h``, then ``csrc/bindings.cpp`` into
 the extension module of the serving operators.  The library needs nvcc alone;
 without torch or its C++ headers the module is left out, with a note, and the
 serving operators are reached through the C ABI only.  Objects are cached under
-``_build/`` and rebuilt when a source or header is newer.
+``_build/`` and rebuilt when a source or header is newer, the module also when
+torch, Python or its command are others than the ones kept beside it.
 """
 from __future__ import annotations
 
+import json
 import os
 import subprocess
 import sys
@@ -49,6 +51,12 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def bindings_key() -> dict[str, str]:
+    """What the extension module's binary interface hangs on, kept beside it."""
+    import torch
+    return {"torch": torch.__version__, "python": str(sysconfig.get_config_var("SOABI"))}
+
+
 def _build_bindings() -> None:
     """The torch extension module over the library (host code only), where torch can be built against."""
     try:
@@ -61,18 +69,26 @@ def _build_bindings() -> None:
         print("no C++ headers of torch and Python here: the module of the serving operators is not built", file=sys.stderr)
         return
     src = CSRC / "bindings.cpp"
-    newest = max(p.stat().st_mtime for p in [src, *_headers()])
-    if BINDINGS.exists() and BINDINGS.stat().st_mtime >= newest:
-        return
-    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", ROOT / "include",
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", "include",
            Path(NVCC).parents[1] / "include", python]
+    made = BINDINGS.with_suffix(".new")
+    # run in ROOT, whose place does not matter: relative paths within it
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{p}" for p in inc],
-           str(src), "-o", str(BINDINGS), f"-L{LIB.parent}", "-lennx_b200", "-Wl,-rpath,$ORIGIN",
+           str(src.relative_to(ROOT)), "-L" + str(LIB.parent.relative_to(ROOT)), "-lennx_b200", "-Wl,-rpath,$ORIGIN",
            f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    key = json.dumps({**bindings_key(), "command": cmd}, indent=1)
+    stamp = BINDINGS.with_suffix(".key")
+    newest = max(p.stat().st_mtime for p in [src, *_headers()])
+    if BINDINGS.exists() and BINDINGS.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == key:
+        return
+    stamp.unlink(missing_ok=True)
+    r = subprocess.run([*cmd, "-o", str(made)], capture_output=True, text=True, cwd=ROOT)
     if r.returncode != 0:
+        made.unlink(missing_ok=True)
         raise RuntimeError(f"g++ failed for bindings.cpp:\n{r.stdout}\n{r.stderr}")
+    made.replace(BINDINGS)
+    stamp.write_text(key)
 
 
 def build(verbose: bool = False) -> Path:
