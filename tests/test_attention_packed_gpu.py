@@ -383,3 +383,19 @@ def test_a_long_recomputation_ends_before_the_waits_for_it():
     first = (rows - 1) // 128 * 128
     assert torch.equal(o[:first], want[:first])
     assert ((o[first:-1].double() - want[first:-1].double()).abs() <= 4 * 2.0 ** -8 * 5).all()
+
+
+@pytest.mark.parametrize("lengths", [[0] * 300 + [70, 0, 129] + [0] * 300, [0] * 40 + [1] + [0] * 40, [0] * 500])
+def test_many_empty_sequences_at_both_ends_with_the_rotation(lengths):
+    rows = sum(lengths) + 9
+    q, k, v = rnd(rows, 4, D, seed=73), rnd(rows, 2, D, seed=74), rnd(rows, 2, D, seed=75)
+    q0, k0, out = q.clone(), k.clone(), torch.full((rows, 4, D), 3.0, dtype=torch.bfloat16, device="cuda")
+    live = sum(lengths)
+    ops.gqa_attention_packed(q, k, v, starts(lengths), out=out)
+    assert (out[live:] == 3.0).all() and torch.equal(q[live:], q0[live:]) and torch.equal(k[live:], k0[live:])
+    if live:
+        for got, before in ((q, q0), (k, k0)):
+            ref = turned(before[:live], lengths, 1e6)
+            assert ((got[:live].double() - ref).abs() <= 1.01 * 2.0 ** -8 * ref.abs() + 1e-5).all()
+        close(out[:live], reference(q[:live], k[:live], v[:live], lengths), float(v.float().abs().max()))
+    ops.device_status()
