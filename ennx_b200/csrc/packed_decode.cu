@@ -109,12 +109,13 @@ struct Split {
 };
 
 // How a stage is filled.  kAny: rows at any address, 16-byte granules by cp.async
-// and reads shifted into place.  kTiles: rows start on 16 bytes, a warp's codes of
-// a tile come by one TMA copy.  kAllTiles: so do scales and biases (kWideTiles:
-// of groups of several flushes), and one more warp copies for the block (int4, 4
-// tokens on 151936 rows, groups of 64: kAny 69 us, copies by the warps themselves
-// 51, by one warp 47; groups of 128: kTiles 56, kWideTiles 48).
-enum Fill { kAny, kTiles, kAllTiles, kWideTiles };
+// and reads shifted into place.  The others want rows that start on 16 bytes.
+// kRows: 16-byte pieces by cp.async, without arithmetic per row.  kTiles: a warp's
+// codes of a tile come by one TMA copy.  kAllTiles: so do scales and biases
+// (kWideTiles: of groups of several flushes), and one more warp copies for the
+// block (int4, 4 tokens on 151936 rows, groups of 64: kAny 69 us, kRows 55,
+// kAllTiles 51; groups of 128: kRows 55, kWideTiles 51).
+enum Fill { kAny, kRows, kTiles, kAllTiles, kWideTiles };
 
 // One stage of a warp's ring: 16 code rows, and their scales and biases.  A
 // flush is kFlush products of 16 columns under one scale; lane t of a row takes
@@ -122,15 +123,19 @@ enum Fill { kAny, kTiles, kAllTiles, kWideTiles };
 template <int kBits, int kFlush, bool kMoved, int kFill>
 struct Stage {
   static constexpr int kSlice = Shape<kMoved>::kSlice, kRowBytes = kSlice * kBits / 8;
-  // kAny: rows of a fragment read lie on different banks (an 8-lane phase
+  static constexpr bool kBoxes = kFill >= kTiles;  // copied by TMA
+  // cp.async: rows of a fragment read lie on different banks (an 8-lane phase
   // covers whole rows, each kFlush * 2 * kBits bytes), and a row that starts
   // inside a 16-byte granule still fits.  TMA: 128-byte rows, the 16-byte
   // chunks of row r exchanged by r & 7.
-  static constexpr int kPitch = kFill == kAny ? kRowBytes + kFlush * 2 * kBits : 128;
+  static constexpr int kPitch = kBoxes ? 128 : kRowBytes + kFlush * 2 * kBits;
   static constexpr int kPieces = kRowBytes / 16 + 1;
   static constexpr int kFlushes = kSlice / 16 / kFlush;
-  static constexpr int kCode = 16 * (kFill == kAny ? kPitch : kRowBytes);
+  static constexpr int kCode = 16 * (kBoxes ? kRowBytes : kPitch);
   static constexpr int kScale = 16 * kFlushes * 8;  // (scale, bias) pairs; kAllTiles: scales, then biases
+  // from one stage of a warp to the next: cp.async keeps a stage's scales behind
+  // its codes, boxes have a ring of their own for them
+  static constexpr int kCodeStep = kBoxes ? kCode : kCode + kScale;
   // depth: as many as leave 16 warps on an SM (80 to 100 KB in flight)
   static constexpr int kDepth = kBits == 8 ? 2 : 3;
 };
@@ -138,7 +143,7 @@ struct Stage {
 template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
 constexpr int smem_bytes() {
   using S = Stage<kBits, kFlush, kMoved, kFill>;
-  return (kFill == kAny ? 0 : 1024) +
+  return (S::kBoxes ? 1024 : 0) +
          Shape<kMoved>::kWarps * (S::kDepth * (S::kCode + S::kScale) + S::kFlushes * 8 * kN * 4 + 2 * kN * 32 * 16);
 }
 
@@ -219,9 +224,14 @@ __device__ __forceinline__ uint4 activation_pairs(uint4 v) {  // columns (0,1) (
                     __byte_perm(v.y, v.w, 0x7632));
 }
 
+// Tensor maps of rows of bytes and of floats.  Fills without boxes get none: a
+// launch pays for its parameters (three unused maps: 0.15 us).
+template <bool kBoxes>
 struct Maps {
-  CUtensorMap codes, scales, biases;  // of rows of bytes and of floats
+  CUtensorMap codes, scales, biases;
 };
+template <>
+struct Maps<false> {};
 
 // kAllTiles: one more warp copies for all
 template <bool kMoved, int kFill>
@@ -230,22 +240,23 @@ constexpr int block_threads() { return 32 * (Shape<kMoved>::kWarps + (kFill >= k
 // kN: blocks of 8 tokens
 template <int kBits, int kN, int kFlush, bool kMoved, int kFill>
 __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>::kBlocks)
-    packed_tiles_kernel(const __grid_constant__ Product p, const __grid_constant__ Split sp, const __grid_constant__ Maps maps) {
+    packed_tiles_kernel(const __grid_constant__ Product p, const __grid_constant__ Split sp,
+                        const __grid_constant__ Maps<(kFill >= kTiles)> maps) {
   using S = Stage<kBits, kFlush, kMoved, kFill>;
   constexpr int kSlice = S::kSlice, kSliceChunks = Shape<kMoved>::kChunks, kWarps = Shape<kMoved>::kWarps;
   constexpr int kFlushes = S::kFlushes, kStages = S::kDepth, kRuns = kFlush / 2;  // runs of 8 columns of a lane in a flush
   extern __shared__ __align__(16) uint8_t raw_smem[];
-  uint8_t* smem = raw_smem + (kFill == kAny ? 0u : (1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
+  uint8_t* smem = raw_smem + (S::kBoxes ? (1024u - (smem_u32(raw_smem) & 1023u)) & 1023u : 0u);
   __shared__ uint64_t bars[kWarps][kStages];  // kAllTiles: of all warps, full in row 0 and free in row 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   // A lane's rows of the tile are row_g and row_g + 8.  Of 16 lanes that read 8
   // bytes (or 8 that read 16) in one go the exchanged chunks then differ.
   constexpr int kLane = kRuns * kBits;  // bytes of a lane in a flush
-  const int row_g = kFill == kAny ? g : kLane == 16 ? g >> 1 | (g & 1) << 2 : (g & 3) << 1 | g >> 2;
+  const int row_g = !S::kBoxes ? g : kLane == 16 ? g >> 1 | (g & 1) << 2 : (g & 3) << 1 | g >> 2;
   const int wk = warp % sp.along, wr = warp / sp.along;
   const int shift = kFill == kWideTiles ? sp.shift : 0;
-  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * S::kCode;
-  const uint32_t scale_ring = base + kWarps * kStages * S::kCode + warp * kStages * S::kScale;
+  const uint32_t base = smem_u32(smem), ring = base + warp * kStages * S::kCodeStep;
+  const uint32_t scale_ring = S::kBoxes ? base + kWarps * kStages * S::kCode + warp * kStages * S::kScale : ring + S::kCode;
   uint64_t* full = bars[kFill >= kAllTiles ? 0 : warp];
   uint64_t* free_ = bars[1];
   if constexpr (kFill == kTiles) {
@@ -314,11 +325,17 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
   uint32_t f_group = group_of(0), f_row = (uint32_t)tile * 16;
   uint64_t f_scale = (uint64_t)(f_row + scale_row) * groups;
   const uint64_t scale_step = (uint64_t)(16 * stride) * groups;
+  // kRows: a lane's piece of row `code_row` and of every kCopyRows further down
+  constexpr int kLanes = S::kRowBytes / 16, kCopyRows = 32 / kLanes;
+  const uint32_t code_row = lane / kLanes, code_at = 16 * (lane % kLanes);
+  const uint8_t* f_code = p.w + (uint64_t)(f_row + code_row) * row_bytes + code_at;
+  const uint64_t code_step = (uint64_t)(16 * stride) * row_bytes;
   int f_tile = tile, f_pass = 0, f_stage = 0, fetched = 0;
+  uint32_t f_at = ring;  // without boxes: the stage's address (from the number it takes registers that spill)
   auto fetch = [&] {
     if constexpr (kFill >= kAllTiles) return;
     if (f_tile < sp.tiles) {
-      const uint32_t dst = ring + f_stage * S::kCode, sdst = scale_ring + f_stage * S::kScale;
+      const uint32_t dst = S::kBoxes ? ring + f_stage * S::kCode : f_at, sdst = S::kBoxes ? scale_ring + f_stage * S::kScale : f_at + S::kCode;
       const uint32_t c0 = slice0(f_pass), first = c0 / 8 * kBits;  // c0 * kBits may pass 32 bits
       if constexpr (kFill == kAny) {
         if (c0 < width) {
@@ -335,11 +352,27 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
             }
           }
         }
-      } else if (lane == 0) {  // what lies outside the matrix arrives as zeros
-        uint64_t* bar = full + f_stage;
-        mbar_arrive_expect_tx(bar, S::kCode);
+      } else if constexpr (kFill == kRows) {
+        if (first + code_at < row_bytes) {
+          const uint8_t* src = f_code + first;
+          const uint32_t to = dst + code_row * S::kPitch + code_at;
+          if (f_row + 16 <= rows) {
 #pragma unroll
-        for (int i = 0; i < S::kRowBytes / 128; ++i) copy_box(dst + i * 2048, &maps.codes, bar, (int)first + 128 * i, (int)f_row);
+            for (int i = 0; i < 16 / kCopyRows; ++i)
+              cp_async16(to + i * kCopyRows * S::kPitch, src + (uint64_t)(i * kCopyRows) * row_bytes);
+          } else {
+            for (int i = 0; i < 16 / kCopyRows; ++i)
+              if (f_row + code_row + i * kCopyRows < rows)
+                cp_async16(to + i * kCopyRows * S::kPitch, src + (uint64_t)(i * kCopyRows) * row_bytes);
+          }
+        }
+      } else if constexpr (kFill == kTiles) {
+        if (lane == 0) {  // what lies outside the matrix arrives as zeros
+          uint64_t* bar = full + f_stage;
+          mbar_arrive_expect_tx(bar, S::kCode);
+#pragma unroll
+          for (int i = 0; i < S::kRowBytes / 128; ++i) copy_box(dst + i * 2048, &maps.codes, bar, (int)first + 128 * i, (int)f_row);
+        }
       }
       if constexpr (kFill < kAllTiles) {
         // scales behind the last column are 0, which takes their columns out
@@ -360,9 +393,11 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
         f_tile += stride;
         f_row += 16 * stride;
         f_scale += scale_step;
+        f_code += code_step;
       }
     }
     f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
+    f_at = f_at + S::kCodeStep == ring + kStages * S::kCodeStep ? ring : f_at + S::kCodeStep;
     if constexpr (kFill < kAllTiles) cp_commit();
   };
 #pragma unroll
@@ -414,6 +449,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
   if (sp.passes == 1) load_x(0);
 
   int stage = 0, used = 0;
+  uint32_t at = ring;  // without boxes: the stage's address
   bool bad = false;  // a wait gave up: later ones are not tried again, the results are void
   for (int done = 0; tile - (kFill >= kAllTiles ? wr : 0) < sp.tiles; ++done) {
     if (kFill >= kAllTiles && tile >= sp.tiles) {  // a stage without a tile for this warp
@@ -430,7 +466,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
     for (int pass = 0; pass < sp.passes; ++pass) {
       if (sp.passes > 1) load_x(pass);
       if constexpr (kFill < kAllTiles) cp_wait<kStages - 2>();
-      if constexpr (kFill != kAny)
+      if constexpr (S::kBoxes)
         if (!bad) bad = !mbar_wait(full + stage, (used / kStages) & 1, sp.status);
       ++used;
       __syncwarp();  // the stage is there, and all lanes have read the one before it,
@@ -438,10 +474,10 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
       const uint32_t c0 = slice0(pass);
       {
         // (kAllTiles: rings of the block, scales of the tile's slices side by side)
-        const uint32_t st = kFill >= kAllTiles ? base + (stage * kWarps + warp) * S::kCode : ring + stage * S::kCode;
+        const uint32_t st = kFill >= kAllTiles ? base + (stage * kWarps + warp) * S::kCode : S::kBoxes ? ring + stage * S::kCode : at;
         const uint32_t scales = kFill >= kAllTiles ? base + kWarps * kStages * S::kCode + stage * kWarps * S::kScale +
                                                          (wr * sp.along * (S::kScale / 2) >> shift)
-                                                   : scale_ring + stage * S::kScale;
+                                                   : S::kBoxes ? scale_ring + stage * S::kScale : at + S::kCode;
         uint32_t addr[2], element[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -449,6 +485,8 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
           if constexpr (kFill == kAny) {
             const uint32_t skew = (uint32_t)((uintptr_t)(p.w + (uint64_t)row * row_bytes) + c0 / 8 * kBits) & 15u;
             addr[h] = st + r * S::kPitch + skew + t * kLane;
+          } else if constexpr (kFill == kRows) {
+            addr[h] = st + r * S::kPitch + t * kLane;
           } else {
             addr[h] = st + r * 128 + ((uint32_t)(t * kLane) ^ (r & 7) << 4);
           }
@@ -466,6 +504,8 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
             if constexpr (kFill == kAny) {
 #pragma unroll
               for (int i = 0; i < kWords; ++i) w[h][i] = word_at(addr[h] + f * kFlushBytes + 4 * i);
+            } else if constexpr (kFill == kRows) {
+              lds_words<kWords>(addr[h] + f * kFlushBytes, w[h]);
             } else {
               lds_words<kWords>((addr[h] ^ (f * kFlushBytes & 127)) + f * kFlushBytes / 128 * 2048, w[h]);
             }
@@ -522,6 +562,7 @@ __global__ void __launch_bounds__(block_threads<kMoved, kFill>(), Shape<kMoved>:
         if (lane == 0) mbar_arrive(free_ + stage);
       }
       stage = stage + 1 == kStages ? 0 : stage + 1;
+      at = at + S::kCodeStep == ring + kStages * S::kCodeStep ? ring : at + S::kCodeStep;
     }
     if (sp.along > 1) {
       // one barrier a tile: the other buffer is written again only after the
@@ -574,8 +615,8 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   int dev = 0;
   ENNX_TRY(serving_device(&dev, &sp.status));
   ENNX_TRY(allow_shared_memory(setup, dev, kernel, smem));
-  Maps maps{};
-  if constexpr (kFill != kAny)
+  Maps<(kFill >= kTiles)> maps{};
+  if constexpr (kFill >= kTiles)
     ENNX_TRY(make_tmap_2d(&maps.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.d.row_bytes, p.d.output_width, p.d.row_bytes, 128, 16,
                           128));
   if constexpr (kFill >= kAllTiles) {
@@ -596,17 +637,31 @@ int32_t launch_tiles(const Product& p, cudaStream_t s) {
   // moved codes spend their time on the hash: one variant for any alignment
   if (p.seed.enabled) return launch_tiles<kBits, kN, kFlush, true, kAny>(p, s);
   if (!on_16(p.w, p.d.row_bytes)) return launch_tiles<kBits, kN, kFlush, false, kAny>(p, s);
-  // a power of two of flushes per group, and 16 bytes of a row's scales per copy at least
-  const uint32_t flushes = p.d.group_size / (16 * kFlush);
-  constexpr uint32_t kSlice = Shape<false>::kSlice;
-  uint32_t along = 1;
-  while (along * kSlice < p.d.input_width && along < (uint32_t)Shape<false>::kWarps) along *= 2;
-  const bool groups_fit = p.d.group_size % (16 * kFlush) == 0 && (flushes & (flushes - 1)) == 0 &&
-                          along * kSlice / p.d.group_size % 4 == 0 && along * kSlice >= 4 * p.d.group_size;
-  if (groups_fit && on_16(p.sc, p.d.groups * 4) && on_16(p.bi, p.d.groups * 4))
-    return flushes == 1 ? launch_tiles<kBits, kN, kFlush, false, kAllTiles>(p, s)
-                        : launch_tiles<kBits, kN, kFlush, false, kWideTiles>(p, s);
-  return launch_tiles<kBits, kN, kFlush, false, kTiles>(p, s);
+  // One warp copies for the block up to 8 tokens (figures at kAllTiles).  From 9
+  // on a thread holds 64 registers of activations, and with the 96 that the ninth
+  // warp leaves it the products spill (16 tokens, by one warp and kRows: int4,
+  // groups of 32, 151936 rows 110 and 98 us, 16384 x 4096 64 and 54, 2048 x 2048
+  // 9.0 and 7.8; groups of 64 80 and 75, 46 and 42, 7.4 and 5.6).  int8 blocks that
+  // have one tile gain nothing from copies ahead: from a block per SM on (4
+  // tokens, groups of 64, 2048 columns, by one warp and kRows: 512 rows 3.9 and
+  // 3.75 us, 2048 rows 4.7 and 4.6; 4096 rows 6.2 and 6.5, 151936 rows 86 and 89).
+  if constexpr (kN == 1) {
+    // a power of two of flushes per group, and 16 bytes of a row's scales per copy at least
+    const uint32_t flushes = p.d.group_size / (16 * kFlush);
+    constexpr uint32_t kSlice = Shape<false>::kSlice, kWarps = Shape<false>::kWarps;
+    uint32_t along = 1;
+    while (along * kSlice < p.d.input_width && along < kWarps) along *= 2;
+    const bool groups_fit = p.d.group_size % (16 * kFlush) == 0 && (flushes & (flushes - 1)) == 0 &&
+                            along * kSlice / p.d.group_size % 4 == 0 && along * kSlice >= 4 * p.d.group_size;
+    const bool enough = kBits == 4 || p.d.output_width > (uint64_t)sm_count() * (16 * (kWarps / along));
+    if (enough && groups_fit && on_16(p.sc, p.d.groups * 4) && on_16(p.bi, p.d.groups * 4))
+      return flushes == 1 ? launch_tiles<kBits, kN, kFlush, false, kAllTiles>(p, s)
+                          : launch_tiles<kBits, kN, kFlush, false, kWideTiles>(p, s);
+  }
+  // (16 tokens, groups of 64, boxes of a warp's own and kRows: 151936 rows 117 and
+  // 129 us, 16384 x 4096 45.1 and 45.8, 2048 x 2048 6.3 and 6.05; the others spill more)
+  if constexpr (kN == 2 && kBits == 8 && kFlush == 4) return launch_tiles<kBits, kN, kFlush, false, kTiles>(p, s);
+  else return launch_tiles<kBits, kN, kFlush, false, kRows>(p, s);
 }
 template <int kBits, int kN>
 int32_t launch_tiles(const Product& p, cudaStream_t s) {
