@@ -538,7 +538,8 @@ ENNX_B200_API int32_t ennx_b200_packed_linear_bf16(const uint16_t* x, int64_t to
  * once -- ennx_b200_packed_linear_bf16 rounds every weight to bf16 first.  Any
  * widths, group size and arena alignment (x and out 2-byte, scales and biases
  * 4-byte aligned); x bf16 [tokens, input_width] and out [tokens, output_width]
- * contiguous, out apart from all that is read.  tokens == 0 does nothing. */
+ * contiguous, out apart from all that is read.  A non-finite activation makes
+ * its own token non-finite (NaN or an infinity).  tokens == 0 does nothing. */
 ENNX_B200_API int32_t ennx_b200_packed_linear_decode(const uint16_t* x, int64_t tokens, const uint8_t* weights,
                                                      const float* scales, const float* biases,
                                                      const ennx_b200_packed_linear* linear,

@@ -151,15 +151,16 @@ def test_rows_of_zero_codes_without_bias_give_zero(inp, group):
     assert (y[:, 5:40] == 0).all() and (y[:, :5] != 0).any()
 
 
-@pytest.mark.parametrize("bits,inp,group,offset,moved", [
-    (8, (1 << 29) + 1056, 96, 0, False),   # codes copied as tiles
-    (8, (1 << 29) + 1024, 64, 0, False),   # scales too
-    (8, (1 << 29) + 1053, 96, 3, False),   # rows at any byte
-    (8, (1 << 29) + 1056, 96, 0, True),
-    (4, (1 << 30) + 1056, 96, 0, False),
-    (4, (1 << 30) + 1050, 96, 5, False),
+@pytest.mark.parametrize("bits,inp,group,offset,moved,tokens", [
+    (8, (1 << 29) + 1056, 96, 0, False, 1),   # codes copied row by row
+    (8, (1 << 29) + 1024, 64, 0, False, 9),   # as boxes, by each warp
+    (4, (1 << 30) + 1024, 64, 0, False, 1),   # by one warp, scales too
+    (8, (1 << 29) + 1053, 96, 3, False, 1),   # rows at any byte
+    (8, (1 << 29) + 1056, 96, 0, True, 1),
+    (4, (1 << 30) + 1056, 96, 0, False, 1),
+    (4, (1 << 30) + 1050, 96, 5, False, 1),
 ])
-def test_columns_whose_bits_pass_32_bits(bits, inp, group, offset, moved):
+def test_columns_whose_bits_pass_32_bits(bits, inp, group, offset, moved, tokens):
     """Rows of more than 2^32 bits: only the last columns have an activation, the
     first ones hold other codes than the last."""
     rows, tail = 2, 1000
@@ -170,15 +171,16 @@ def test_columns_whose_bits_pass_32_bits(bits, inp, group, offset, moved):
                                                                            generator=g, dtype=torch.uint8)
     sc, bi = torch.full((rows * groups,), 0.5, device="cuda"), torch.zeros(rows * groups, device="cuda")
     lin = _abi.PackedLinear(offset, 0, 0, inp, rows, bits, group, 7, 1, 1 << 31)
-    x = torch.zeros(1, inp, dtype=torch.bfloat16, device="cuda")
-    x[0, -tail:] = x_of(1, tail, 31)[0]
+    x = torch.zeros(tokens, inp, dtype=torch.bfloat16, device="cuda")
+    x[-1, -tail:] = x_of(1, tail, 31)[0]
     seed = (0x9E37, 0x51ED27, int(moved))
     codes = ops.packed_dequantize(w, torch.ones_like(sc), bi, lin, seed, dtype=torch.float32)[:, -tail:].double()
     if not moved:  # the dequantised codes are those of the arena
         end = w[offset:].view(rows, row_bytes)[:, -tail * bits // 8:].long()
         assert torch.equal(codes, (end if bits == 8 else torch.stack([end & 15, end >> 4], 2).flatten(1)).double())
-    got = ops.packed_linear_decode(x, w, sc, bi, lin, seed)[0].double()
-    xt = x[0, -tail:].double()
+    out = ops.packed_linear_decode(x, w, sc, bi, lin, seed)
+    assert (out[:-1] == 0).all()
+    got, xt = out[-1].double(), x[-1, -tail:].double()
     ref, size = codes @ xt * 0.5, codes @ xt.abs() * 0.5
     assert ((got - ref).abs() <= 1.001 * 2.0 ** -8 * ref.abs() + 2.0 ** -14 * size).all()
 
