@@ -71,7 +71,7 @@ def _build_bindings() -> None:
     src = CSRC / "bindings.cpp"
     inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", "include",
            Path(NVCC).parents[1] / "include", python]
-    made = BINDINGS.with_suffix(".new")
+    made = BINDINGS.with_suffix(f".new{os.getpid()}")  # renamed when whole: ranks may build at once
     # run in ROOT, whose place does not matter: relative paths within it
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{p}" for p in inc],

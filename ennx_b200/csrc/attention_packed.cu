@@ -38,9 +38,9 @@
 // memory are set up once and the next Q and K arrive while the last softmax
 // runs (ragged 16384 tokens 210 -> 203 us).
 //
-// Measured: one prompt of 16384 tokens, 16 heads on 4: 0.83 ms, 1320 TFLOP/s
-// (0.98 ms at the power limit); 12 ragged prompts of 16384 tokens 197 us, 860
-// TFLOP/s of visible scores.
+// Measured in a stream of calls: one prompt of 16384 tokens, 16 heads on 4: 0.99
+// ms, 1110 TFLOP/s at the power limit (0.87 ms in single calls after a pause); 12
+// ragged prompts of 16384 tokens 221 us, 765 TFLOP/s of visible scores.
 //
 // Masked places may hold anything: masked scores are replaced, not added to,
 // but a masked V row still meets P = 0 in the MMA and an infinity or NaN there

@@ -1,5 +1,9 @@
 // serve.cuh -- helpers shared by the serving operators (packed-prompt and
 // single-token attention, few-token MoE, few-token packed products).
+//
+// Times in the comments of these kernels compare two forms of one kernel, most
+// of them as the best of five replays of a graph; a stream of calls over changing
+// inputs runs 5 to 15 % longer.
 #pragma once
 
 #include <mutex>
