@@ -399,3 +399,21 @@ def test_many_empty_sequences_at_both_ends_with_the_rotation(lengths):
             assert ((got[:live].double() - ref).abs() <= 1.01 * 2.0 ** -8 * ref.abs() + 1e-5).all()
         close(out[:live], reference(q[:live], k[:live], v[:live], lengths), float(v.float().abs().max()))
     ops.device_status()
+
+
+def test_offsets_past_32_bits():
+    hq, hkv, n = 16, 4, 997
+    count = (1 << 31) // (n * hq * D) + 20  # 2.2e9 elements of q and of the output
+    rows = n * count
+    g = torch.Generator(device="cuda").manual_seed(80)
+    q, k, v = (torch.randn(rows, h, D, generator=g, device="cuda", dtype=torch.bfloat16) for h in (hq, hkv, hkv))
+    last = slice(rows - 3 * n, rows)
+    rq, rk = (turned(x[last], [n] * 3, 1e6) for x in (q, k))
+    o = ops.gqa_attention_packed(q, k, v, starts([n] * count))
+    for got, ref in ((q[last], rq), (k[last], rk)):
+        assert ((got.double() - ref).abs() <= 1.01 * 2.0 ** -8 * ref.abs() + 1e-5).all()
+    close(o[last], reference(q[last], k[last], v[last], [n] * 3), float(v[last].float().abs().max()))
+    v[-40, 1, 7] = math.nan  # and where rows are computed again
+    o = ops.gqa_attention_packed(q, k, v, starts([n] * count), rope_theta=0.0)
+    assert o[-40:, 4:8, 7].isnan().all() and int((~o[last].isfinite()).sum()) == 40 * 4
+    ops.device_status()

@@ -258,3 +258,17 @@ def test_out_that_shares_memory_is_refused():
     assert torch.equal(call(x, wr, wgu, wd, k, residual=res, out=buf[2 * T:3 * T]), want)
     assert torch.equal(call(x, wr, wgu, wd, k, residual=x), call(x, wr, wgu, wd, k, residual=x.clone()))
     assert torch.equal(call(x, wr, wgu, wd, k, residual=res, out=res), want)
+
+
+@pytest.mark.parametrize("T", [2, 20])
+def test_weight_offsets_past_32_bits(T):
+    H, E, k, I = 8192, 160, 2, 1024  # 2.7e9 elements of gate and up, 1.3e9 of down
+    g = torch.Generator(device="cuda").manual_seed(90)
+    wgu = torch.randn(E, 2 * I, H, generator=g, device="cuda", dtype=torch.bfloat16).mul_(H ** -0.5)
+    wd = torch.randn(E, H, I, generator=g, device="cuda", dtype=torch.bfloat16).mul_(I ** -0.5)
+    x, wr = rnd(T, H, seed=91), rnd(E, H, seed=92, std=1.5 / H ** 0.5)
+    wr[E - 1] = wr[E - 1] + x[0] / 32  # the last expert is picked
+    y, idx, _ = ops.moe_layer_decode(x, wr, wgu, wd, k, return_routing=True)
+    ridx, rgate = routing(x, wr, k)
+    assert torch.equal(idx.long(), ridx) and int(ridx.max()) == E - 1
+    check(y, x, wgu, wd, ridx, rgate)

@@ -196,3 +196,23 @@ def test_out_that_shares_memory_is_refused():
     with pytest.raises(ValueError, match="must not overlap"):
         call(both[:4], w, sc, bi, lin, out=both[3:7])
     assert torch.equal(call(both[:4], w, sc, bi, lin, out=both[4:]), call(x, w, sc, bi, lin))
+
+
+@pytest.mark.parametrize("bits,group,tokens,moved,skew", [(8, 64, 3, False, 0), (8, 32, 11, False, 0), (8, 64, 16, False, 0),
+                                                          (4, 64, 2, False, 0), (4, 32, 16, False, 0), (8, 64, 2, False, 1),
+                                                          (8, 64, 4, True, 0), (8, 16, 1, False, 0)])
+def test_rows_whose_offsets_pass_32_bits(bits, group, tokens, moved, skew):
+    inp, last = 2048, 40
+    row_bytes, groups = inp * bits // 8, inp // group
+    rows = (1 << 32) // row_bytes + 100
+    g = torch.Generator(device="cuda").manual_seed(50)
+    w = torch.randint(0, 256, (skew + rows * row_bytes,), generator=g, device="cuda", dtype=torch.uint8)
+    sc = torch.rand(rows * groups, generator=g, device="cuda") * 1e-3
+    bi = -sc * (1 << (bits - 1))
+    x, seed = x_of(tokens, inp, 51), (3, 4, int(moved))
+    whole = _abi.PackedLinear(skew, 0, 0, inp, rows, bits, group, 0, 1, 1 << 30)
+    got = ops.packed_linear_decode(x, w, sc, bi, whole, seed)
+    for first in (0, rows - last):  # rows of the large linear are those of a small one at their place
+        part = _abi.PackedLinear(skew + first * row_bytes, first * groups, first * groups, inp, last, bits, group,
+                                 first * inp % 2 ** 32, 1, 1 << 30)
+        check(got[:, first:first + last], x, w, sc, bi, part, seed)
